@@ -202,6 +202,7 @@ def _run_adamw(s, case):
         F = _package()
         F.adamw_step(s["params"], s["grads"], s["first"], s["second"], s["step"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY)
         first, second = (s["first"], s["second"]) if case["bits"] == 32 else F.adamw_state_values(s["first"], s["second"])
+        first, second = ([t.view(p.shape) for t, p in zip(ts, s["params"])] for ts in (first, second))
         return {"params": s["params"], "first": first, "second": second}
     s["step"] += 1
     t = s["step"].double()
