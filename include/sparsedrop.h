@@ -55,7 +55,8 @@ enum sd_status {
   SD_ERR_RUNTIME = 3      /* HIP launch or runtime failure */
 };
 
-enum sd_dtype { SD_F16 = 0, SD_BF16 = 1 };
+/* SD_F32: only in the calls that name it */
+enum sd_dtype { SD_F16 = 0, SD_BF16 = 1, SD_F32 = 2 };
 
 /* activations the GEMM epilogues can apply; GELU is the exact (erf) form, torch.nn.GELU's default */
 enum sd_act { SD_ACT_NONE = 0, SD_ACT_RELU = 1, SD_ACT_GELU = 2 };
@@ -603,6 +604,79 @@ int sd_conv2d_taps_dw(const void* x_rows, int64_t x_ld, const void* dy_rows, int
                       int64_t h, int64_t w, int64_t k_out, int64_t r, int64_t s, int64_t pad_h, int64_t pad_w, int64_t stride_h,
                       int64_t stride_w, int64_t dil_h, int64_t dil_w, float scale, int dtype, void* workspace,
                       int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (f) products in 8 bits with a scale for each block of 128
+ *
+ * A matrix [rows, cols] in 8 bits: e4m3 codes, row-major, on 16 bytes with a pitch that is a multiple of 16 and holds
+ * whole 128-blocks (columns behind the last are zeros), and a power of two for each block of 1 x 128 or 128 x 128, as
+ * the byte exponent + 127 (e8m0).  The scale is the least one with which the block's largest finite magnitude stays within 448;
+ * 127 for a block of zeros, 0 at least.  Values are rounded to nearest, halves to the even code; what is not finite becomes NaN.
+ * Scales of 1 x 128 blocks that a product reads lie 128-block by 128-block: scale of (row, block k) at [k * ld + row].
+ *
+ * The calls that make matrices for themselves hold them in one buffer each, of sd_fp8_matrix_bytes bytes on 16 bytes: pass it on as
+ * it was filled.  square: blocks of 128 x 128.
+ *
+ * sd_fp8_quantize / sd_fp8_dequantize: one matrix (f16, bf16 or f32; block_rows 1 or 128) to codes and scales and back.
+ * sd_fp8_gemm: C = A . B^T of two of them, fp32 sums, rounded once to dtype (f16 or bf16); workspace optional (a split reduction).
+ * sd_fp8_linear: Y = X . W^T for X in 16 bits, which is quantized in 1 x 128 blocks, and weights in 128 x 128 blocks.
+ *   At most 16 rows run in one launch that reads each weight once and needs no workspace.
+ * sd_fp8_dropout_matmul_forward: Y = s (keep (.) X) W^T with X in 1 x 128 and W in 128 x 128 blocks; mask given, or drawn as
+ *   sd_random_lists draws it and stored to mask_out [ceil(M/bs), ceil(K/bs)].  Dropped blocks are neither quantized nor multiplied.
+ *   XT (a [K, M] matrix) and WT (a square [K, N] one), each NULL where its gradient is not wanted, receive what the backward reads: X in blocks along the tokens,
+ *   for dW sums over them, and W turned.  block_size: multiples of 128 (SD_ERR_UNSUPPORTED otherwise).
+ * sd_fp8_dropout_matmul_backward: dX = s (dY W) (.) keep (zeros in dropped blocks) from WT and / or dW = s dY^T (keep (.) X) from XT, dY
+ *   quantized in blocks along the features for the one and along the tokens for the other.
+ * Workspaces: as many bytes as the .._workspace_bytes functions say, on 16 bytes, and of one call at a time.
+ * ------------------------------------------------------------------------------------------- */
+int64_t sd_fp8_matrix_bytes(int64_t rows, int64_t cols, int square);
+int sd_fp8_quantize(const void* x, int64_t x_stride_r, int64_t x_stride_c, int64_t rows, int64_t cols, int dtype,
+                    int64_t block_rows, void* data, int64_t data_ld, uint8_t* scales, int64_t scales_stride_r,
+                    int64_t scales_stride_k, void* stream);
+int sd_fp8_dequantize(const void* data, int64_t data_ld, const uint8_t* scales, int64_t scales_stride_r, int64_t scales_stride_k,
+                      int64_t block_rows, int64_t rows, int64_t cols, void* out, int64_t out_ld, int dtype, void* stream);
+int64_t sd_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int sd_fp8_gemm(const void* A, int64_t lda, const uint8_t* A_scales, int64_t A_scales_ld, const void* B, int64_t ldb,
+                const uint8_t* B_scales, int64_t B_scales_stride_r, int64_t B_scales_stride_k, int64_t B_block_rows, void* C,
+                int64_t c_stride_r, int64_t c_stride_c, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                int64_t workspace_bytes, void* stream);
+int64_t sd_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int sd_fp8_linear(const void* X, int64_t ldx, const void* W, int64_t ldw, const uint8_t* W_scales, int64_t W_scales_stride_r,
+                  int64_t W_scales_stride_k, void* Y, int64_t ldy, int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int64_t sd_fp8_dropout_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int backward);
+int sd_fp8_dropout_matmul_forward(const void* X, int64_t x_stride_r, int64_t x_stride_c, const void* W, int64_t w_stride_r,
+                                  int64_t w_stride_c, void* Y, int64_t y_stride_r, int64_t y_stride_c, const uint8_t* mask,
+                                  int64_t mask_stride_r, int64_t mask_stride_c, uint64_t* rng_state, uint64_t seed, uint64_t offset,
+                                  double p, uint8_t* mask_out, void* XT, void* WT, int64_t M, int64_t N, int64_t K,
+                                  int64_t block_size, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dy_stride_r, int64_t dy_stride_c, const uint8_t* mask,
+                                   int64_t mask_stride_r, int64_t mask_stride_c, void* XT, void* WT, void* dX, int64_t dx_stride_r,
+                                   int64_t dx_stride_c, void* dW, int64_t dw_stride_r, int64_t dw_stride_c, int64_t M, int64_t N,
+                                   int64_t K, int64_t block_size, double p, int dtype, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (g) AdamW over many tensors
+ *
+ *   t = *step + 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ *
+ * count tensors of one dtype (f16, bf16 or f32, gradients alike), each of numels[i] elements without gaps; the arrays of pointers and sizes
+ * are HOST arrays, read before the call returns.  state_bits 32: exp_avgs and exp_avg_sqs are floats.  8: codes, a byte an element, and
+ * a power of two (exponent + 127) for each 128 elements in the scales: the first average e4m3, the second without a sign, five bits of exponent
+ * (bias 15) and three of mantissa.  Both are rounded at random, up with the probability that the value's place between two codes says; the
+ * random bits are a function of t and the element's index.  Zeros are codes 0 with scales 127.
+ * step: device memory; with `advance` the call moves it on when all is done (its upper half is scratch meanwhile), so a
+ * captured graph counts its replays.  lr_at: a float in device memory that replaces lr, or NULL.
+ * sd_adamw_state_values: averages in 8 bits (second[i]: the second one) as floats.
+ * ------------------------------------------------------------------------------------------- */
+int sd_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                  uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales, const int64_t* numels, int64_t* step,
+                  const float* lr_at, double lr, double beta1, double beta2, double eps, double weight_decay, int dtype,
+                  int state_bits, int advance, void* stream);
+int sd_adamw_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* values,
+                          const int64_t* numels, const int32_t* second, void* stream);
 
 #ifdef __cplusplus
 }

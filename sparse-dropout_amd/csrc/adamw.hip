@@ -1,0 +1,383 @@
+// AdamW over many tensors in few launches, the two averages held in 32 or in 8 bits.
+//
+//   m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+//   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// Bound by the bytes of parameters, gradients and averages: 28 an element in 32 bits throughout, 16 with averages in 8.  Tensors of any
+// number go by tables of kTensors in the launch's arguments, a workgroup takes runs of elements off the whole of them.
+//
+// Averages in 8 bits have a power of two for each block of 128 elements.  The first is e4m3; the second, which has no sign, has five
+// bits of exponent and three of mantissa, so that 2^34 lies between its least and its largest number: a second average that is small
+// in its block must not come out as zero, for its element would then move by m / eps.  An average moves by (1 - beta) of the way a
+// step, a thousandth for the second, which is less than half of the 2^-3 between two numbers: rounded to nearest it would never move.
+// So it is rounded at random, up with the probability that its place between the two numbers says, and stays right on average.  The random
+// bits are a function of step and element alone: equal runs have equal states.  The averages are computed in 64 bits before that,
+// since whether a value lies below or above its random border must not depend on how the compiler orders 32-bit arithmetic.
+#include "fp8.h"
+
+#include <cfloat>
+
+namespace sd {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTensors = 56;
+constexpr int kPer = 8;                    // elements of a thread at a time
+constexpr int kChunk = kThreads * kPer;    // of a workgroup: whole 128-blocks
+
+struct AdamTensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  uint8_t *ms, *vs;
+  int64_t n;
+};
+struct AdamTable {
+  AdamTensor tensor[kTensors];
+  uint32_t first[kTensors + 1];  // chunk of the launch that a tensor begins at
+  int32_t n;
+  int64_t* step;
+  int32_t last;  // of the call's launches: moves the step on
+  const float* lr_at;
+  double lr, beta1, beta2, eps, decay;
+};
+static_assert(sizeof(AdamTable) <= 4096, "a launch's arguments");
+
+struct F32 {
+  typedef float elem;
+  static constexpr int id = kF32;
+  __device__ static inline float to_float(float v) { return v; }
+  __device__ static inline float from_float(float v) { return v; }
+};
+
+template <typename T>
+struct Elem {
+  typedef uint16_t type;
+};
+template <>
+struct Elem<F32> {
+  typedef float type;
+};
+
+// base^t by squaring; its relative error grows with t as t * 2^-53
+__device__ inline double power(double base, uint32_t t) {
+  double r = 1.0;
+  for (; t; t >>= 1) {
+    if (t & 1) r *= base;
+    base *= base;
+  }
+  return r;
+}
+
+// M. O'Neill's permuted congruential generator, 32 bits, output function RXS-M-XS, one step behind x
+__device__ inline uint32_t mixed(uint32_t x) {
+  const uint32_t s = x * 747796405u + 2891336453u;
+  const uint32_t w = ((s >> ((s >> 28) + 4)) ^ s) * 277803737u;
+  return (w >> 22) ^ w;
+}
+
+template <typename E>
+__device__ inline void load_run(const E* src, int left, float (&out)[kPer]);
+template <>
+__device__ inline void load_run<float>(const float* src, int left, float (&out)[kPer]) {
+  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+  if (left >= kPer) {
+    const f32x4 a = *reinterpret_cast<const f32x4_any*>(src), b = *reinterpret_cast<const f32x4_any*>(src + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[i] = a[i];
+      out[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[i] = i < left ? src[i] : 0.f;
+  }
+}
+template <typename T>
+__device__ inline void load_typed(const void* src, int64_t at, int left, float (&out)[kPer]) {
+  if constexpr (T::id == kF32) {
+    load_run<float>(static_cast<const float*>(src) + at, left, out);
+  } else {
+    const uint16_t* s = static_cast<const uint16_t*>(src) + at;
+    if (left >= kPer) {
+      const u32x4 w = *reinterpret_cast<const u32x4_any*>(s);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) out[i] = T::to_float((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) out[i] = i < left ? T::to_float(s[i]) : 0.f;
+    }
+  }
+}
+template <typename T>
+__device__ inline void store_typed(void* dst, int64_t at, int left, const float (&v)[kPer]) {
+  if constexpr (T::id == kF32) {
+    typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+    float* d = static_cast<float*>(dst) + at;
+    if (left >= kPer) {
+      *reinterpret_cast<f32x4_any*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4_any*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < left) d[i] = v[i];
+    }
+  } else {
+    uint16_t* d = static_cast<uint16_t*>(dst) + at;
+    if (left >= kPer) {
+      *reinterpret_cast<u32x4_any*>(d) = u32x4{T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7])};
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < left) d[i] = T::from_float(v[i]);
+    }
+  }
+}
+// eight codes
+typedef u32x2 __attribute__((aligned(1))) u32x2_any;
+__device__ inline u32x2 load_codes(const uint8_t* src, int left) {
+  if (left >= kPer) return *reinterpret_cast<const u32x2_any*>(src);
+  u32x2 w = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (i < left) w[i / 4] |= (uint32_t)src[i] << (8 * (i % 4));
+  return w;
+}
+__device__ inline void store_codes(uint8_t* dst, int left, u32x2 w) {
+  if (left >= kPer) {
+    *reinterpret_cast<u32x2_any*>(dst) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < left) dst[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+// ---- the two formats ------------------------------------------------------------------------------------------------------
+// 8 bits of a magnitude: exponent behind the bias, three bits of mantissa.  LIMIT20: the upper 20 bits of the largest number's mantissa,
+// TOP its exponent.
+struct First {
+  static constexpr int bias = 7, least = -6, top = 8;
+  static constexpr uint32_t limit20 = 0xC0000u;  // 448 = 1.75 * 2^8
+  static constexpr uint32_t infinite = 0x7f, nan = 0x7f;  // (e4m3 has no infinity)
+  __device__ static inline float decode(u32x2 w, int i) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const int word = (int)w[i / 4];
+    const f32x2 pair = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(word, true) : __builtin_amdgcn_cvt_pk_f32_fp8(word, false);
+    return pair[i & 1];
+  }
+};
+struct Second {
+  static constexpr int bias = 15, least = -14, top = 15;
+  static constexpr uint32_t limit20 = 0xE0000u;  // 61440 = 1.875 * 2^15
+  static constexpr uint32_t infinite = 0xf8, nan = 0xff;
+  __device__ static inline float decode(u32x2 w, int i) {  // an fp16 without its sign and its last seven bits
+    return F16::to_float((uint16_t)(((w[i / 4] >> (8 * (i % 4))) & 0xffu) << 7));
+  }
+};
+
+// What decides a block's scale, as a number that grows with the magnitude: the upper half of its 64 bits, with the lower half's
+// being other than zero in the last.  0 for what is not finite in 32 bits.
+__device__ inline uint32_t magnitude_word(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x) & 0x7fffffffffffffffull;
+  const uint32_t hi = (uint32_t)(b >> 32), w = hi | ((uint32_t)b != 0u ? 1u : 0u);
+  return w < ((1023u + 128u) << 20) ? w : 0u;
+}
+// the byte of the least power of two with which `word` stays within the largest number
+template <typename Format>
+__device__ inline uint32_t scale_byte(uint32_t word) {
+  const int e = (int)(word >> 20) - 1023 - Format::top + ((word & 0xfffffu) > Format::limit20 ? 1 : 0) + 127;
+  return word == 0u ? 127u : (uint32_t)(e < 0 ? 0 : e);
+}
+// |x| / 2^(byte - 127) rounded down after random / 2^16 of the distance to the next number was added
+template <typename Format>
+__device__ inline uint32_t encode(double x, uint32_t byte, uint32_t random) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t hi = (uint32_t)(b >> 32) & 0x7fffffffu;
+  if (hi >= (1023u + 128u) << 20) return hi > 0x7ff00000u || (hi == 0x7ff00000u && (uint32_t)b) ? Format::nan : Format::infinite;
+  const int scaled = (int)hi - (((int)byte - 127) << 20);
+  const int exponent = (scaled >> 20) - 1023;
+  if (exponent >= Format::least) return (((uint32_t)scaled + (random << 1)) >> 17) - ((1023u - Format::bias) << 3);
+  // below the least normal number: whole steps of 2^(least - 3), and 2^16 parts of one
+  const double parts = __builtin_ldexp(fabs(x), 19 - Format::least - ((int)byte - 127));
+  return ((uint32_t)parts + random) >> 16;
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
+  const uint32_t t = (uint32_t)(*reinterpret_cast<const volatile uint32_t*>(a.step)) + 1u;
+  const double lr = a.lr_at ? (double)*a.lr_at : a.lr;
+  const float by = (float)(lr / (1.0 - power(a.beta1, t))), root = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
+  const float keep = (float)(1.0 - lr * a.decay), eps = (float)a.eps;
+  const uint32_t chunks = a.first[a.n];
+  int which = 0;
+  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    while (chunk >= a.first[which + 1]) ++which;
+    const AdamTensor& x = a.tensor[which];
+    const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + threadIdx.x * kPer;
+    const int64_t rest = x.n - at;
+    const int left = rest < 0 ? 0 : rest > kPer ? kPer : (int)rest;
+    float p[kPer], g[kPer];
+    load_typed<T>(x.p, at, left, p);
+    load_typed<T>(x.g, at, left, g);
+    if constexpr (BITS == 32) {
+      float m[kPer], v[kPer];
+      load_run<float>(static_cast<const float*>(x.m) + at, left, m);
+      load_run<float>(static_cast<const float*>(x.v) + at, left, v);
+      const float b1 = (float)a.beta1, c1 = (float)(1.0 - a.beta1), b2 = (float)a.beta2, c2 = (float)(1.0 - a.beta2);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        m[i] = m[i] * b1 + g[i] * c1;
+        v[i] = v[i] * b2 + (g[i] * g[i]) * c2;
+        p[i] = p[i] * keep - by * (m[i] / (sqrtf(v[i]) * root + eps));
+      }
+      store_typed<F32>(x.m, at, left, m);
+      store_typed<F32>(x.v, at, left, v);
+    } else {
+      const int64_t block = at / 128;
+      uint8_t *const mc = static_cast<uint8_t*>(x.m) + at, *const vc = static_cast<uint8_t*>(x.v) + at;
+      u32x2 mw = load_codes(mc, left), vw = load_codes(vc, left);
+      const float ms = fp8_power(left ? x.ms[block] : 127u), vs = fp8_power(left ? x.vs[block] : 127u);
+      double m[kPer], v[kPer];
+      uint32_t m_most = 0, v_most = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const double gd = (double)g[i];
+        m[i] = (double)(First::decode(mw, i) * ms) * a.beta1 + gd * (1.0 - a.beta1);
+        v[i] = (double)(Second::decode(vw, i) * vs) * a.beta2 + (gd * gd) * (1.0 - a.beta2);
+        m_most = max(m_most, magnitude_word(m[i]));
+        v_most = max(v_most, magnitude_word(v[i]));
+        const float mf = (float)m[i], vf = (float)v[i];
+        p[i] = p[i] * keep - by * (mf / (sqrtf(vf) * root + eps));
+      }
+      // sixteen lanes hold a block (those behind the tensor's end hold zeros)
+      const uint32_t mb = scale_byte<First>(max_of_row16(m_most)), vb = scale_byte<Second>(max_of_row16(v_most));
+      const uint32_t key = t * 0x9E3779B1u + (uint32_t)at;
+      mw = u32x2{0u, 0u};
+      vw = u32x2{0u, 0u};
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t random = mixed(key + i);
+        const uint32_t sign = (uint32_t)(__builtin_bit_cast(uint64_t, m[i]) >> 56) & 0x80u;
+        const uint32_t mq = encode<First>(m[i], mb, random >> 16) | sign, vq = encode<Second>(v[i], vb, random & 0xffffu);
+        mw[i / 4] |= mq << (8 * (i % 4));
+        vw[i / 4] |= vq << (8 * (i % 4));
+      }
+      store_codes(mc, left, mw);
+      store_codes(vc, left, vw);
+      if ((threadIdx.x & 15) == 0 && left) {
+        x.ms[block] = (uint8_t)mb;
+        x.vs[block] = (uint8_t)vb;
+      }
+    }
+    store_typed<T>(x.p, at, left, p);
+  }
+  // The step moves on when every workgroup has read it: the one that is done last writes it.  Its upper half counts them meanwhile.
+  if (a.last) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t* const arrivals = reinterpret_cast<uint32_t*>(a.step) + 1;
+      if (atomicAdd(arrivals, 1u) == gridDim.x - 1) {
+        *arrivals = 0u;
+        *reinterpret_cast<uint32_t*>(a.step) = t;
+      }
+    }
+  }
+}
+
+struct ValueTensor {
+  const uint8_t *codes, *scales;
+  float* out;
+  int64_t n;
+  int32_t second;
+};
+struct ValueTable {
+  ValueTensor tensor[kTensors];
+  uint32_t first[kTensors + 1];
+  int32_t n;
+};
+static_assert(sizeof(ValueTable) <= 4096, "a launch's arguments");
+
+// averages in 8 bits -> their values in 32
+__global__ __launch_bounds__(kThreads) void state_values_kernel(ValueTable a) {
+  const uint32_t chunks = a.first[a.n];
+  int which = 0;
+  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    while (chunk >= a.first[which + 1]) ++which;
+    const ValueTensor& x = a.tensor[which];
+    const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + threadIdx.x * kPer, rest = x.n - at;
+    if (rest <= 0) continue;
+    const int left = rest > kPer ? kPer : (int)rest;
+    const u32x2 w = load_codes(x.codes + at, left);
+    const float s = fp8_power(x.scales[at / 128]);
+    float v[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = (x.second ? Second::decode(w, i) : First::decode(w, i)) * s;
+    store_typed<F32>(x.out, at, left, v);
+  }
+}
+
+// workgroups: as many as are resident, each through several chunks
+unsigned grid_of(uint32_t chunks) { return chunks < 2048 ? chunks : 2048; }
+
+}  // namespace
+
+int launch_adamw(int count, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* ms, uint8_t* const* vs,
+                 const int64_t* n, int64_t* step, const float* lr_at, double lr, double beta1, double beta2, double eps, double decay,
+                 int dtype, int bits, bool moves_on, hipStream_t stream) {
+  AdamTable a = {};
+  a.step = step;
+  a.lr_at = lr_at;
+  a.lr = lr;
+  a.beta1 = beta1;
+  a.beta2 = beta2;
+  a.eps = eps;
+  a.decay = decay;
+  auto* kernel = bits == 8 ? (dtype == kF32 ? &adamw_kernel<F32, 8> : dtype == SD_BF16 ? &adamw_kernel<BF16, 8> : &adamw_kernel<F16, 8>)
+                           : (dtype == kF32 ? &adamw_kernel<F32, 32> : dtype == SD_BF16 ? &adamw_kernel<BF16, 32> : &adamw_kernel<F16, 32>);
+  for (int i = 0; i < count || (i == 0 && moves_on);) {
+    a.n = 0;
+    a.first[0] = 0;
+    int64_t chunks = 0;
+    for (; i < count && a.n < kTensors; ++i) {
+      const int64_t more = ceil_div(n[i], kChunk);
+      if (chunks + more >= (1LL << 31)) break;
+      if (more == 0) continue;
+      a.tensor[a.n] = AdamTensor{p[i], g[i], m[i], v[i], ms ? ms[i] : nullptr, vs ? vs[i] : nullptr, n[i]};
+      chunks += more;
+      a.first[++a.n] = (uint32_t)chunks;
+    }
+    if (i < count && a.n == 0) return fail(SD_ERR_UNSUPPORTED, "adamw_step: a tensor of %lld elements is too large", (long long)n[i]);
+    a.last = moves_on && i == count ? 1 : 0;
+    if (chunks == 0 && !a.last) break;
+    hipLaunchKernelGGL(kernel, dim3(chunks ? grid_of((uint32_t)chunks) : 1), dim3(kThreads), 0, stream, a);
+    if (int rc = check_launch("adamw_step")) return rc;
+    if (i == count) break;
+  }
+  return SD_OK;
+}
+
+int launch_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* out, const int64_t* n,
+                        const int32_t* second, hipStream_t stream) {
+  ValueTable a = {};
+  for (int i = 0; i < count;) {
+    a.n = 0;
+    a.first[0] = 0;
+    int64_t chunks = 0;
+    for (; i < count && a.n < kTensors; ++i) {
+      const int64_t more = ceil_div(n[i], kChunk);
+      if (chunks + more >= (1LL << 31)) break;
+      if (more == 0) continue;
+      a.tensor[a.n] = ValueTensor{codes[i], scales[i], out[i], n[i], second[i]};
+      chunks += more;
+      a.first[++a.n] = (uint32_t)chunks;
+    }
+    if (i < count && a.n == 0) return fail(SD_ERR_UNSUPPORTED, "adamw_state_values: a tensor of %lld elements is too large", (long long)n[i]);
+    if (chunks == 0) break;
+    hipLaunchKernelGGL(&state_values_kernel, dim3(grid_of((uint32_t)chunks)), dim3(kThreads), 0, stream, a);
+    if (int rc = check_launch("adamw_state_values")) return rc;
+  }
+  return SD_OK;
+}
+
+}  // namespace sd

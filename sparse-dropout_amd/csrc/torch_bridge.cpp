@@ -23,6 +23,7 @@
 #include <mutex>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "sparsedrop.h"
@@ -1201,6 +1202,350 @@ Tensor conv2d(const Tensor& input, const Tensor& kernel_in, const OptTensor& mas
   return y;
 }
 
+// ---- products in 8 bits ---------------------------------------------------------------------------------------------------
+// (see functional/fp8_blocks.py for what is computed)
+constexpr int64_t kFp8 = 128;  // columns of a block
+
+int dtype_with_f32(const char* name, const Tensor& t) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name,
+                   " must be float16, bfloat16 or float32 (got ", t.dtype(), ")");
+  return t.scalar_type() == at::kFloat ? SD_F32 : dtype_of(t);
+}
+
+// codes [rows, whole 128-blocks] and scales, a row each or a row for 128 rows, as fp8_quantize gives them
+struct Fp8Codes {
+  Tensor data, scales;
+  int64_t rows, nk;
+  bool square;
+  Fp8Codes(const char* name, const Tensor& data_, const Tensor& scales_) : data(data_), scales(scales_) {
+    TORCH_CHECK_VALUE(data.is_cuda() && scales.device() == data.device(), name, ": codes and scales must be on the same GPU (got ",
+                      data.device(), " and ", scales.device(), ")");
+    TORCH_CHECK_TYPE(data.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kFloat8_e8m0fnu, name,
+                     ": codes must be float8_e4m3fn and scales float8_e8m0fnu (got ", data.dtype(), " and ", scales.dtype(), ")");
+    TORCH_CHECK_VALUE(data.dim() == 2 && scales.dim() == 2, name, ": codes and scales must be 2D");
+    TORCH_CHECK_VALUE(data.size(1) % kFp8 == 0, name, ": codes are filled up to whole blocks of 128 columns (got ", data.size(1), ")");
+    rows = data.size(0);
+    nk = data.size(1) / kFp8;
+    square = scales.size(0) != rows;
+    TORCH_CHECK_VALUE(scales.size(1) == nk && (!square || scales.size(0) == ceil_div(rows, kFp8)), name, ": scales ", scales.sizes(),
+                      " are not those of codes ", data.sizes());
+    const bool rows_apart = rows <= 1 || (data.stride(0) >= data.size(1) && data.stride(0) % 16 == 0);
+    if (!(data.size(1) == 0 || data.stride(1) == 1) || !rows_apart || reinterpret_cast<uintptr_t>(data.data_ptr()) % 16) data = data.contiguous();
+  }
+  const void* codes() const { return data.data_ptr(); }
+  int64_t ld() const { return rows <= 1 ? data.size(1) : data.stride(0); }
+  const uint8_t* s() const { return static_cast<const uint8_t*>(scales.data_ptr()); }
+  // (strides over an extent of one are arbitrary; 0 over more is an expanded tensor, which reads alike)
+  int64_t s_r() const { return std::max<int64_t>(scales.stride(0), 1); }
+  int64_t s_k() const { return std::max<int64_t>(scales.stride(1), 1); }
+  int64_t block_rows() const { return square ? kFp8 : 1; }
+  void no_expanded_scales() {
+    for (int64_t d = 0; d < 2; ++d)
+      if (scales.size(d) > 1 && scales.stride(d) == 0) scales = scales.contiguous();
+  }
+  // scales of rows laid out 128-block by 128-block, as the products read them
+  void lay_out_rows() {
+    const int64_t ld = ceil_div(rows, 16) * 16;
+    const bool fits = (rows <= 1 || scales.stride(0) == 1) && (nk <= 1 || (scales.stride(1) >= rows && scales.stride(1) % 4 == 0));
+    if (fits && reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 == 0) return;
+    Tensor laid = at::empty({nk, ld}, scales.options().dtype(at::kByte)).narrow(1, 0, rows).t();
+    laid.copy_(scales.view(at::kByte));
+    scales = laid.view(at::kFloat8_e8m0fnu);
+  }
+  int64_t row_ld() const { return nk <= 1 ? ceil_div(rows, 4) * 4 : scales.stride(1); }
+};
+
+std::tuple<Tensor, Tensor> fp8_quantize(const Tensor& x_, int64_t block_rows) {
+  TORCH_CHECK_VALUE(x_.is_cuda(), "x must be on the GPU (got ", x_.device(), ")");
+  TORCH_CHECK_VALUE(x_.dim() == 2, "x must be 2D (got ", x_.dim(), "D)");
+  const int dtype = dtype_with_f32("x", x_);
+  at::NoGradGuard no_grad;
+  const Tensor x = as_matrix(x_);
+  const int64_t rows = x.size(0), cols = x.size(1), nk = ceil_div(cols, kFp8), ld = ceil_div(rows, 16) * 16;
+  Tensor data = at::empty({rows, nk * kFp8}, x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scales = block_rows == 1 ? at::empty({nk, ld}, x.options().dtype(at::kFloat8_e8m0fnu)).t().narrow(0, 0, rows)
+                                  : at::empty({ceil_div(rows, kFp8), nk}, x.options().dtype(at::kFloat8_e8m0fnu));
+  if (rows == 0 || cols == 0) return {data, scales};
+  const Mat xm(x);
+  c10::DeviceGuard guard(x.device());
+  check(sd_fp8_quantize(MAT(xm), rows, cols, dtype, block_rows, data.data_ptr(), nk * kFp8, static_cast<uint8_t*>(scales.data_ptr()),
+                        block_rows == 1 ? 1 : nk, block_rows == 1 ? ld : 1, stream_of(x)),
+        "sd_fp8_quantize");
+  return {data, scales};
+}
+
+Tensor fp8_dequantize(const Tensor& data, const Tensor& scales, std::optional<int64_t> cols_, at::ScalarType dtype) {
+  Fp8Codes q("data", data, scales);
+  q.no_expanded_scales();
+  const int64_t cols = cols_.value_or(data.size(1));
+  TORCH_CHECK_VALUE(cols >= 0 && ceil_div(cols, kFp8) == q.nk, "cols ", cols, " are not those of codes ", data.sizes());
+  Tensor out = at::empty({q.rows, cols}, data.options().dtype(dtype));
+  const int code = dtype_with_f32("dtype", out);
+  if (out.numel() == 0) return out;
+  c10::DeviceGuard guard(data.device());
+  check(sd_fp8_dequantize(q.codes(), q.ld(), q.s(), q.s_r(), q.s_k(), q.block_rows(), q.rows, cols, out.data_ptr(), cols, code, stream_of(data)),
+        "sd_fp8_dequantize");
+  return out;
+}
+
+Tensor fp8_gemm(const Tensor& a_, const Tensor& a_scales, const Tensor& b_, const Tensor& b_scales, at::ScalarType dtype) {
+  Fp8Codes a("A", a_, a_scales), b("B", b_, b_scales);
+  TORCH_CHECK_VALUE(a.data.device() == b.data.device(), "A and B must be on the same device");
+  TORCH_CHECK_VALUE(a.nk == b.nk, "reduction dims differ: A ", a_.sizes(), ", B ", b_.sizes());
+  TORCH_CHECK_TYPE(dtype == at::kHalf || dtype == at::kBFloat16, "the result must be float16 or bfloat16 (got ", dtype, ")");
+  TORCH_CHECK_NOT_IMPLEMENTED(!a.square, "A must have a scale for each 1 x 128 block (128 x 128 ones are taken for B)");
+  const int64_t M = a.rows, N = b.rows, K = a.nk * kFp8;
+  Tensor c = at::empty({M, N}, a_.options().dtype(dtype));
+  if (c.numel() == 0) return c;
+  if (K == 0) return c.zero_();
+  a.lay_out_rows();
+  if (b.square) b.no_expanded_scales();
+  else b.lay_out_rows();
+  Scratch ws(c, sd_fp8_gemm_workspace_bytes(M, N, K));
+  c10::DeviceGuard guard(c.device());
+  check(sd_fp8_gemm(a.codes(), a.ld(), a.s(), a.row_ld(), b.codes(), b.ld(), b.s(), b.square ? b.s_r() : 1, b.square ? b.s_k() : b.row_ld(),
+                    b.block_rows(), c.data_ptr(), N, 1, M, N, K, dtype_of(c), ws.ptr, ws.bytes, stream_of(c)),
+        "sd_fp8_gemm");
+  return c;
+}
+
+Tensor fp8_linear(const Tensor& input, const Tensor& data, const Tensor& scales) {
+  TORCH_CHECK_VALUE(input.dim() == 2, "input must be [M, K] (got ", input.dim(), "D)");
+  TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && input.requires_grad()),
+                              "the product with kept 8-bit weights has no gradient: call it under torch.no_grad()");
+  Tensor x = autocast(input);
+  check_operand("input", x);
+  refuse_forward_mode(std::array<Tensor, 1>{x});
+  Fp8Codes w("weight", data, scales);
+  const int64_t M = x.size(0), K = x.size(1), N = w.rows;
+  TORCH_CHECK_VALUE(data.device() == x.device(), "input and weights must be on the same device");
+  TORCH_CHECK_VALUE(ceil_div(K, kFp8) == w.nk, "reduction dims differ: input ", x.sizes(), ", codes ", data.sizes());
+  TORCH_CHECK_NOT_IMPLEMENTED(w.square || N <= 1, "weights must have a scale for each 128 x 128 block");
+  Tensor y = at::empty({M, N}, x.options());
+  if (y.numel() == 0) return y;
+  if (K == 0) return y.zero_();
+  w.no_expanded_scales();
+  x = as_matrix(x);
+  if (!row_major(x)) x = x.contiguous();
+  Scratch ws(x, ceil_div(sd_fp8_linear_workspace_bytes(M, N, K), 4) * 4);
+  const Mat xm(x);
+  c10::DeviceGuard guard(x.device());
+  check(sd_fp8_linear(xm.ptr, xm.sr, w.codes(), w.ld(), w.s(), w.s_r(), w.s_k(), y.data_ptr(), N, M, N, K, dtype_of(x), ws.ptr, ws.bytes,
+                      stream_of(x)),
+        "sd_fp8_linear");
+  return y;
+}
+
+struct Fp8LinearBackward : Node {
+  Saved xt, wt, mask;  // X and W as the backward reads them, in 8 bits; each only where its gradient is wanted
+  at::TensorOptions options;
+  int64_t M = 0, N = 0, K = 0, bs = 0;
+  double p = 0;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    at::NoGradGuard no_grad;
+    variable_list out(2);
+    const Tensor x = xt.get(), w = wt.get(), m = mask.get();
+    const bool need_dx = task_should_compute_output(0) && w.defined(), need_dw = task_should_compute_output(1) && x.defined();
+    TORCH_CHECK(m.defined(), "Trying to backward through the graph a second time, or after its saved tensors were freed");
+    if (!need_dx && !need_dw) return out;
+    if (need_dx) out[0] = at::empty({M, K}, options);
+    if (need_dw) out[1] = at::empty({N, K}, options);
+    if (N == 0 || !grads[0].defined()) {
+      for (Tensor& t : out)
+        if (t.defined()) t.zero_();
+      return out;
+    }
+    TORCH_CHECK_VALUE(grads[0].dim() == 2 && grads[0].size(0) == M && grads[0].size(1) == N && grads[0].device() == m.device(),
+                      "dy must be a [", M, ", ", N, "] tensor on ", m.device());
+    const Tensor dy = as_matrix(grads[0].scalar_type() == c10::typeMetaToScalarType(options.dtype()) ? grads[0] : grads[0].to(options.dtype()));
+    const Scratch ws(m, ceil_div(sd_fp8_dropout_matmul_workspace_bytes(M, N, K, 1), 4) * 4);
+    const Tensor mc = check_mask(m, ceil_div(M, bs), ceil_div(K, bs), m), xc = x.defined() ? x.contiguous() : x, wc = w.defined() ? w.contiguous() : w;
+    const MaskArg ma(mc);
+    Mat dxm, dwm;
+    if (need_dx) dxm = Mat(out[0]);
+    if (need_dw) dwm = Mat(out[1]);
+    const Mat gm(dy);
+    c10::DeviceGuard guard(m.device());
+    check(sd_fp8_dropout_matmul_backward(MAT(gm), ma.ptr, ma.sr, ma.sc, need_dw ? xc.data_ptr() : nullptr, need_dx ? wc.data_ptr() : nullptr,
+                                         MAT(dxm), MAT(dwm), M, N, K, bs, p, dtype_of(dy), ws.ptr, ws.bytes, stream_of(m)),
+          "sd_fp8_dropout_matmul_backward");
+    return out;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    xt.drop();
+    wt.drop();
+    mask.drop();
+  }
+  std::string name() const override { return "BlockwiseDropoutMatmulFP8Backward"; }
+};
+
+Tensor linear_fp8(const Tensor& input, const Tensor& weight, const OptTensor& mask, int64_t bs, double p,
+                  std::optional<uint64_t> seed, const OptTensor& state) {
+  TORCH_CHECK_VALUE(input.dim() == 2 && weight.dim() == 2, "input must be [M, K] and weight [N, K]");
+  const Tensor x = as_matrix(autocast(input)), w = as_matrix(autocast(weight));
+  refuse_forward_mode(std::array<Tensor, 2>{x, w});
+  check_pair(x, w);
+  check_p(p);
+  TORCH_CHECK_NOT_IMPLEMENTED(bs % kFp8 == 0, "block_size ", bs, ": products in 8 bits take multiples of 128");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0), mb = ceil_div(M, bs), kb = ceil_div(K, bs);
+  TORCH_CHECK_VALUE(mb > 0 && kb > 0, "mask must be non-empty");
+  const bool record = records(std::array<Tensor, 2>{x, w});
+  Tensor y, xt, wt, drop;
+  {
+    NoRecord guard;
+    const Draw draw{mask, seed, state};
+    MaskArg given;
+    if (mask) {
+      drop = check_mask(*mask, mb, kb, x);
+      given = MaskArg(drop);
+    } else {
+      drop = at::empty({mb, kb}, x.options().dtype(at::kBool));
+    }
+    const auto bytes = x.options().dtype(at::kByte);
+    if (record && w.requires_grad()) xt = at::empty({sd_fp8_matrix_bytes(K, M, 0)}, bytes);
+    if (record && x.requires_grad()) wt = at::empty({sd_fp8_matrix_bytes(K, N, 1)}, bytes);
+    y = new_matrix(x, M, N);
+    const Scratch ws(x, ceil_div(sd_fp8_dropout_matmul_workspace_bytes(M, N, K, 0), 4) * 4);
+    const Mat xm(x), wm(w), ym(y);
+    c10::DeviceGuard device(x.device());
+    check(sd_fp8_dropout_matmul_forward(MAT(xm), MAT(wm), MAT(ym), given.ptr, given.sr, given.sc, draw.state_ptr(), seed.value_or(0), 0, p,
+                                        mask ? nullptr : static_cast<uint8_t*>(drop.data_ptr()), xt.defined() ? xt.data_ptr() : nullptr,
+                                        wt.defined() ? wt.data_ptr() : nullptr, M, N, K, bs, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
+          "sd_fp8_dropout_matmul_forward");
+  }
+  if (record) {
+    auto node = make_node<Fp8LinearBackward>({x, w});
+    node->xt.keep(xt);
+    node->wt.keep(wt);
+    node->mask.keep(drop);
+    node->options = x.options();
+    node->M = M;
+    node->N = N;
+    node->K = K;
+    node->bs = bs;
+    node->p = p;
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+// ---- AdamW ----------------------------------------------------------------------------------------------------------------
+// (see functional/adamw.py for what is computed)
+// Launches write parameters and averages behind autograd's back: their versions say so.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& avgs,
+                const std::vector<Tensor>& sqs, const std::vector<Tensor>& avg_scales, const std::vector<Tensor>& sq_scales,
+                const Tensor& step, const OptTensor& lr_at, double lr, double beta1, double beta2, double eps, double decay) {
+  at::NoGradGuard no_grad;
+  const size_t n = params.size();
+  const bool in8 = !avg_scales.empty() || !sq_scales.empty();
+  TORCH_CHECK_VALUE(grads.size() == n && avgs.size() == n && sqs.size() == n && (!in8 || (avg_scales.size() == n && sq_scales.size() == n)),
+                    "one gradient and both averages are needed for each of ", n, " parameters");
+  TORCH_CHECK_VALUE(step.is_cuda() && step.scalar_type() == at::kLong && step.numel() == 1, "step must be one int64 on the GPU (got ",
+                    step.sizes(), " ", step.dtype(), " on ", step.device(), ")");
+  TORCH_CHECK_VALUE(!lr_at || (lr_at->device() == step.device() && lr_at->scalar_type() == at::kFloat && lr_at->numel() == 1),
+                    "a learning rate in a tensor must be one float32 on ", step.device());
+  std::vector<Tensor> keep;  // gradients laid out here
+  struct Group {
+    std::vector<void*> p, m, v;
+    std::vector<const void*> g;
+    std::vector<uint8_t*> ms, vs;
+    std::vector<int64_t> n;
+  } groups[3];
+  std::unordered_set<void*> seen;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &m = avgs[i], &v = sqs[i];
+    Tensor g = grads[i];
+    TORCH_CHECK_VALUE(p.device() == step.device() && g.device() == step.device() && m.device() == step.device() && v.device() == step.device(),
+                      "parameter ", i, ", its gradient and averages must be on ", step.device(), " like the step");
+    TORCH_CHECK_VALUE(g.layout() == at::kStrided && p.layout() == at::kStrided, "parameter ", i, ": sparse parameters and gradients are not taken");
+    const int code = dtype_with_f32("a parameter", p);
+    TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "parameter ", i, " is ", p.dtype(), " and its gradient ", g.dtype());
+    TORCH_CHECK_VALUE(g.sizes() == p.sizes(), "parameter ", i, " is ", p.sizes(), " and its gradient ", g.sizes());
+    TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "parameter ", i, " must fill its memory (strides ", p.strides(), ")");
+    const int64_t size = p.numel();
+    if (in8) {
+      const Tensor &a = avg_scales[i], &b = sq_scales[i];
+      const bool fit = m.scalar_type() == at::kByte && v.scalar_type() == at::kByte && a.scalar_type() == at::kByte && b.scalar_type() == at::kByte &&
+                       m.numel() == size && v.numel() == size && a.numel() == ceil_div(size, kFp8) && b.numel() == a.numel() && m.is_contiguous() &&
+                       v.is_contiguous() && a.is_contiguous() && b.is_contiguous() && a.device() == step.device() && b.device() == step.device();
+      TORCH_CHECK_VALUE(fit, "parameter ", i, ": averages in 8 bits are ", size, " contiguous uint8 codes and ", ceil_div(size, kFp8),
+                        " uint8 scales on ", step.device());
+    } else {
+      TORCH_CHECK_VALUE(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat && m.sizes() == p.sizes() && v.sizes() == p.sizes() &&
+                            m.strides() == p.strides() && v.strides() == p.strides(),
+                        "parameter ", i, ": averages in 32 bits must be float32 tensors laid out like it (", p.sizes(), ", strides ", p.strides(), ")");
+    }
+    if (size == 0) continue;
+    for (void* at : {p.data_ptr(), m.data_ptr(), v.data_ptr()})
+      TORCH_CHECK_VALUE(seen.insert(at).second, "parameter ", i, " or an average of it was given twice");
+    if (g.strides() != p.strides() || g.is_neg() || g.is_conj()) {
+      Tensor like = at::empty_like(p);
+      like.copy_(g);
+      keep.push_back(like);
+      g = like;
+    }
+    Group& to = groups[code];
+    to.p.push_back(p.data_ptr());
+    to.g.push_back(g.data_ptr());
+    to.m.push_back(m.data_ptr());
+    to.v.push_back(v.data_ptr());
+    if (in8) {
+      to.ms.push_back(static_cast<uint8_t*>(avg_scales[i].data_ptr()));
+      to.vs.push_back(static_cast<uint8_t*>(sq_scales[i].data_ptr()));
+    }
+    to.n.push_back(size);
+  }
+  int last = 0;
+  for (int i = 0; i < 3; ++i)
+    if (!groups[i].n.empty()) last = i;
+  c10::DeviceGuard guard(step.device());
+  for (int i = 0; i < 3; ++i) {
+    Group& to = groups[i];
+    if (to.n.empty() && i != last) continue;
+    check(sd_adamw_step((int)to.n.size(), to.p.data(), to.g.data(), to.m.data(), to.v.data(), to.ms.data(), to.vs.data(), to.n.data(),
+                        static_cast<int64_t*>(step.data_ptr()), lr_at ? static_cast<const float*>(lr_at->data_ptr()) : nullptr, lr, beta1,
+                        beta2, eps, decay, i, in8 ? 8 : 32, i == last ? 1 : 0, stream_of(step)),
+          "sd_adamw_step");
+  }
+  for (const auto* list : {&params, &avgs, &sqs, &avg_scales, &sq_scales})
+    for (const Tensor& t : *list) written(t);
+  written(step);
+}
+
+std::vector<Tensor> adamw_state_values(const std::vector<Tensor>& codes, const std::vector<Tensor>& scales, const std::vector<int>& second) {
+  at::NoGradGuard no_grad;
+  TORCH_CHECK_VALUE(codes.size() == scales.size() && codes.size() == second.size(), "codes and scales are needed for every average");
+  std::vector<Tensor> out;
+  std::vector<const uint8_t*> c, s;
+  std::vector<float*> o;
+  std::vector<int64_t> n;
+  std::vector<int32_t> kind;
+  for (size_t i = 0; i < codes.size(); ++i) {
+    const Tensor &q = codes[i], &b = scales[i];
+    TORCH_CHECK_VALUE(q.is_cuda() && q.device() == codes[0].device() && b.device() == q.device(), "averages must be on one GPU");
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kByte && b.scalar_type() == at::kByte && q.is_contiguous() && b.is_contiguous() &&
+                          b.numel() == ceil_div(q.numel(), kFp8),
+                      "averages in 8 bits are contiguous uint8 codes and a uint8 scale for each 128 of them");
+    out.push_back(at::empty(q.sizes(), q.options().dtype(at::kFloat)));
+    if (q.numel() == 0) continue;
+    c.push_back(static_cast<const uint8_t*>(q.data_ptr()));
+    s.push_back(static_cast<const uint8_t*>(b.data_ptr()));
+    o.push_back(static_cast<float*>(out.back().data_ptr()));
+    n.push_back(q.numel());
+    kind.push_back(second[i]);
+  }
+  if (c.empty()) return out;
+  c10::DeviceGuard guard(codes[0].device());
+  check(sd_adamw_state_values((int)c.size(), c.data(), s.data(), o.data(), n.data(), kind.data(), stream_of(codes[0])), "sd_adamw_state_values");
+  return out;
+}
+
 std::array<int, 3> conv_routes() { return {last_routes[0].load(), last_routes[1].load(), last_routes[2].load()}; }
 
 }  // namespace
@@ -1213,4 +1558,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mlp", torch::wrap_pybind_function(mlp));
   m.def("conv2d", torch::wrap_pybind_function(conv2d));
   m.def("conv_routes", &conv_routes);
+  m.def("fp8_quantize", torch::wrap_pybind_function(fp8_quantize));
+  m.def("fp8_dequantize", torch::wrap_pybind_function(fp8_dequantize));
+  m.def("fp8_gemm", torch::wrap_pybind_function(fp8_gemm));
+  m.def("fp8_linear", torch::wrap_pybind_function(fp8_linear));
+  m.def("linear_fp8", torch::wrap_pybind_function(linear_fp8));
+  m.def("adamw_step", torch::wrap_pybind_function(adamw_step));
+  m.def("adamw_state_values", torch::wrap_pybind_function(adamw_state_values));
 }

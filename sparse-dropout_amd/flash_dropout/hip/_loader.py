@@ -120,6 +120,23 @@ SIGNATURES = {
     "sd_col2im": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
                           *([c_int64] * 12), c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "sd_col2im_kernel": (c_int, [c_int64] * 17),
+    "sd_fp8_matrix_bytes": (c_int64, [c_int64, c_int64, c_int]),
+    "sd_fp8_quantize": (c_int, [*_mat, c_int64, c_int64, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    "sd_fp8_dequantize": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+                                  c_void_p]),
+    "sd_fp8_gemm_workspace_bytes": (c_int64, [c_int64] * 3),
+    "sd_fp8_gemm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, *_mat,
+                            c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "sd_fp8_linear_workspace_bytes": (c_int64, [c_int64] * 3),
+    "sd_fp8_linear": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                              c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "sd_fp8_dropout_matmul_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "sd_fp8_dropout_matmul_forward": (c_int, [*_mat, *_mat, *_mat, *_mat, c_void_p, c_uint64, c_uint64, c_double, c_void_p, c_void_p,
+                                              c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "sd_fp8_dropout_matmul_backward": (c_int, [*_mat, *_mat, c_void_p, c_void_p, *_mat, *_mat, c_int64, c_int64, c_int64, c_int64,
+                                               c_double, c_int, c_void_p, c_int64, c_void_p]),
+    "sd_adamw_step": (c_int, [c_int, *([c_void_p] * 9), c_double, c_double, c_double, c_double, c_double, c_int, c_int, c_int, c_void_p]),
+    "sd_adamw_state_values": (c_int, [c_int, *([c_void_p] * 5), c_void_p]),
 }
 
 

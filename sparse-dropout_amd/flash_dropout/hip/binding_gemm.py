@@ -555,6 +555,12 @@ class GEMM:
                        self._stream(A))
         return C
 
+    def gemm_fp8(self, A: torch.Tensor, A_scales: torch.Tensor, B: torch.Tensor, B_scales: torch.Tensor,
+                 dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """Dense ``A @ B.T`` of matrices in 8 bits (codes and scales as ``flash_dropout.functional.fp8_quantize`` gives them): A in
+        (1, 128) blocks, B in (1, 128) or (128, 128) blocks, fp32 sums, the result in ``dtype``."""
+        return _loader.bridge().fp8_gemm(A, A_scales, B, B_scales, dtype)
+
     # ------------------------------------------------------------------ the autograd function's two calls
     def dropout_matmul_forward(self, x: torch.Tensor, w: torch.Tensor, block_size, p: float,
                                mask: torch.Tensor | None = None, seed: int | None = None):

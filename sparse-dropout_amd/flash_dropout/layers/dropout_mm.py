@@ -15,6 +15,8 @@ _BLOCKWISE = {
     # the reference's backend names keep working and run the HIP kernels
     "blockwise[cuda]": F.cuda_blockwise_dropout_matmul,
     "blockwise[triton]": F.triton_blockwise_dropout_matmul,
+    # products of operands in 8 bits with a scale for each block of 128; block sizes are multiples of 128
+    "blockwise[hip-fp8]": F.hip_blockwise_dropout_matmul_fp8,
 }
 VARIANTS = ("none", "vanilla", *_BLOCKWISE)
 

@@ -1,0 +1,109 @@
+"""``AdamW``: decoupled weight decay, the averages in 32 or in 8 bits (functional/adamw.py has the formulas and the 8-bit format).
+
+The reference leaves optimizers to torch; this is torch's ``AdamW`` for the package's layers, with the same arguments and
+``state_dict`` keys."""
+from __future__ import annotations
+
+import torch
+
+from ..functional.adamw import adamw_empty_state, adamw_state_values, adamw_step
+
+
+class AdamW(torch.optim.Optimizer):
+    """``state_bits``: 32, or 8 (a quarter of the memory and less than that to read and write; a state of a parameter is then
+    ``exp_avg`` and ``exp_avg_sq`` codes with ``exp_avg_scale`` and ``exp_avg_sq_scale``).
+
+    ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  ``step`` of a parameter's state is an int64
+    on the GPU, shared by the parameters that have been updated the same number of times; parameters without a gradient are left out
+    of a step, as torch's optimizers leave them out.  Parameters must be on the GPU, float16, bfloat16 or float32, and fill their memory."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32) -> None:
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError(f"lr must not be negative (got {lr})")
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"betas must be in [0, 1) (got {betas})")
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError(f"eps and weight_decay must not be negative (got {eps}, {weight_decay})")
+        if state_bits not in (8, 32):
+            raise ValueError(f"averages are held in 8 or in 32 bits (got {state_bits})")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def _init_state(self, p: torch.Tensor, bits: int, step: torch.Tensor) -> None:
+        state = self.state[p]
+        state["step"] = step
+        if bits == 8:
+            state["exp_avg"], state["exp_avg_scale"] = adamw_empty_state(p)
+            state["exp_avg_sq"], state["exp_avg_sq_scale"] = adamw_empty_state(p)
+        else:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+
+    @staticmethod
+    def _averages(states, key):
+        return [(s[key], s[key + "_scale"]) if key + "_scale" in s else s[key] for s in states]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            fresh: dict[torch.device, torch.Tensor] = {}
+            together: dict[int, list[torch.Tensor]] = {}  # by the step tensor that the parameters share
+            members: dict[int, int] = {}
+            for p in group["params"]:
+                state = self.state.get(p)
+                if state:
+                    members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
+                if p.grad is None:
+                    continue
+                if not state:
+                    if p.device not in fresh:
+                        fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+                    self._init_state(p, group["state_bits"], fresh[p.device])
+                    state = self.state[p]
+                    members[id(state["step"])] = members.get(id(state["step"]), 0) + 1
+                together.setdefault(id(state["step"]), []).append(p)
+            for key, params in together.items():
+                states = [self.state[p] for p in params]
+                step = states[0]["step"]
+                if len(params) < members[key]:  # the others stay behind, with a count of their own
+                    step = step.clone()
+                    for s in states:
+                        s["step"] = step
+                adamw_step(params, [p.grad for p in params], self._averages(states, "exp_avg"), self._averages(states, "exp_avg_sq"), step,
+                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
+        return loss
+
+    def state_values(self, p: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Both averages of a parameter as float32 tensors of its shape."""
+        s = self.state[p]
+        if "exp_avg_scale" not in s:
+            return s["exp_avg"], s["exp_avg_sq"]
+        (m,), (v,) = adamw_state_values(self._averages([s], "exp_avg"), self._averages([s], "exp_avg_sq"))
+        if p.is_contiguous():
+            return m.view(p.shape), v.view(p.shape)
+        return tuple(torch.as_strided(t, p.shape, p.stride()) for t in (m, v))
+
+    def load_state_dict(self, state_dict) -> None:
+        """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved."""
+        super().load_state_dict(state_dict)
+        numbers = iter([i for g in state_dict["param_groups"] for i in g["params"]])
+        shared: dict[tuple, torch.Tensor] = {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                s = state_dict["state"].get(next(numbers))
+                if not s:
+                    continue
+                state = self.state[p]
+                for key, value in s.items():
+                    if not isinstance(value, torch.Tensor):
+                        state[key] = value
+                        continue
+                    kept = value.detach().to(p.device, copy=True)
+                    if key in ("exp_avg", "exp_avg_sq") and kept.dtype == torch.float32 and kept.stride() != p.stride():
+                        kept = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(kept)
+                    state[key] = kept
+                count = int(state["step"])
+                state["step"] = shared.setdefault((id(group), p.device, count), torch.full((), count, dtype=torch.int64, device=p.device))
