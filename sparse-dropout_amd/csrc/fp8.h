@@ -64,6 +64,8 @@ struct Fp8Gemm {
 };
 enum Fp8Mode { kFp8Dense = 0, kFp8Dsd = 1, kFp8Sdd = 2 };  // the mask is over A's blocks [m, k], or over C's [m, n]
 int launch_fp8_gemm(const Fp8Gemm& g, int mode, int dtype, hipStream_t stream);
+// dX (SDD, B square) and dW (DSD) of a layer, in one launch where neither fills the chip
+int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStream_t stream);
 // scratch that a split reduction wants, 0 for none
 int64_t fp8_gemm_scratch(int64_t M, int64_t N, int64_t K, int mode);
 
@@ -99,6 +101,35 @@ __device__ inline uint32_t pack_fp8(float a, float b, float c, float d) {
   int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
+
+// 16-bit elements, two to a word.  Their magnitudes are 15-bit whole numbers, of which the larger stands for the larger number;
+// from kInfinite on they are not finite.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ inline uint32_t pk_max(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <typename T>
+constexpr uint32_t kInfinite = T::id == SD_BF16 ? 0x7f80u : 0x7c00u;
+// the bits in fp32 of a magnitude
+template <typename T>
+__device__ inline uint32_t size_bits(uint32_t m) {
+  return T::id == SD_BF16 ? m << 16 : __builtin_bit_cast(uint32_t, F16::to_float((uint16_t)m));
+}
+// Two elements over 2^(byte - 127) as codes, in the lower or upper half of a word: the codes that multiplying in fp32 and converting
+// give, for every 16-bit number and scale.  (The instruction looks at the scale's exponent alone, so byte 0 needs no other form.)
+template <typename T, bool HI>
+__device__ inline uint32_t codes_of(uint32_t old, uint32_t pair, uint32_t byte) {
+  const float scale = __builtin_bit_cast(float, byte << 23);
+  s16x2 r;
+  if constexpr (T::id == SD_BF16) r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(s16x2, old), __builtin_bit_cast(bf16x2, pair), scale, HI);
+  else r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s16x2, old), __builtin_bit_cast(f16x2, pair), scale, HI);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
 // the largest of a value over the 16 lanes of a row, in all of them
 __device__ inline uint32_t max_of_row16(uint32_t v) {
   auto turned = [](uint32_t x, auto n) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + decltype(n)::value, 0xf, 0xf, false); };

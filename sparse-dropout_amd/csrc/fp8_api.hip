@@ -145,8 +145,8 @@ int sd_fp8_quantize(const void* x, int64_t sr, int64_t sc, int64_t rows, int64_t
   if (int rc = check_matrix("fp8_quantize", "x", x, sr, sc, rows, cols)) return rc;
   if (rows == 0 || cols == 0) return SD_OK;
   SD_REQUIRE(data != nullptr && scales != nullptr, "fp8_quantize: null pointer");
-  SD_REQUIRE(reinterpret_cast<uintptr_t>(data) % 8 == 0 && data_ld % 8 == 0 && data_ld >= up(cols, kFp8Block),
-             "fp8_quantize: codes must start on 8 bytes and their pitch hold whole 128-blocks (got %lld)", (long long)data_ld);
+  SD_REQUIRE(aligned16(data) && data_ld % 16 == 0 && data_ld >= up(cols, kFp8Block),
+             "fp8_quantize: codes must start on 16 bytes, rows too, and their pitch hold whole 128-blocks (got %lld)", (long long)data_ld);
   SD_REQUIRE(ssr >= 1 && ssk >= 1, "fp8_quantize: scales: strides must be positive");
   QuantJobs js = {};
   js.n = 1;
@@ -340,23 +340,19 @@ int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dysr, int64_t dysc, c
   js.job[0] = quant_job(dY, dysr, dysc, M, N, dX ? dy.form(dyq) : Fp8Form{}, dW ? dyt.form(dytq) : Fp8Form{}, false);
   if (int rc = launch_quantize(js, dtype, (hipStream_t)stream)) return rc;
   const float scale = (float)(1.0 / (1.0 - p));
-  if (dX) {  // dX[m, k] = sum over n of dY[m, n] W[n, k], kept blocks
-    Fp8Gemm g = product(dy, dyq, wt, WT, dX, dxsr, dxsc, M, K, N, scale, nullptr, 0);
-    g.mask = mask;
-    g.msr = msr;
-    g.msc = msc;
-    g.split = (int32_t)(bs / kFp8Block);
-    if (int rc = launch_fp8_gemm(g, kFp8Sdd, dtype, (hipStream_t)stream)) return rc;
-  }
-  if (dW) {  // dW^T[k, n] = sum over m of X[m, k] dY[m, n], kept blocks of X
-    Fp8Gemm g = product(xt, XT, dyt, dytq, dW, dwsc, dwsr, K, N, M, scale, part, fp8_gemm_scratch(K, N, M, kFp8Dsd));
-    g.mask = mask;
-    g.msr = msc;
-    g.msc = msr;
-    g.split = (int32_t)(bs / kFp8Block);
-    if (int rc = launch_fp8_gemm(g, kFp8Dsd, dtype, (hipStream_t)stream)) return rc;
-  }
-  return SD_OK;
+  // dX[m, k] = sum over n of dY[m, n] W[n, k], kept blocks
+  Fp8Gemm gx = product(dy, dyq, wt, WT, dX, dxsr, dxsc, M, K, N, scale, nullptr, 0);
+  gx.mask = mask;
+  gx.msr = msr;
+  gx.msc = msc;
+  // dW^T[k, n] = sum over m of X[m, k] dY[m, n], kept blocks of X
+  Fp8Gemm gw = product(xt, XT, dyt, dytq, dW, dwsc, dwsr, K, N, M, scale, part, fp8_gemm_scratch(K, N, M, kFp8Dsd));
+  gw.mask = mask;
+  gw.msr = msc;
+  gw.msc = msr;
+  gx.split = gw.split = (int32_t)(bs / kFp8Block);
+  if (dX && dW) return launch_fp8_backward(gx, gw, dtype, (hipStream_t)stream);
+  return dX ? launch_fp8_gemm(gx, kFp8Sdd, dtype, (hipStream_t)stream) : launch_fp8_gemm(gw, kFp8Dsd, dtype, (hipStream_t)stream);
 }
 
 int sd_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,

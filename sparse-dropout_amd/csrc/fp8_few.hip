@@ -29,30 +29,41 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(Fp8Few g) {
       wh = *reinterpret_cast<const u32x4*>(w + (int64_t)k * kFp8Block + 64 + 16 * q);
     }
     const int ws = sw[(int64_t)k * g.sw_k];
-    // this lane's 32 elements of row r: 16 q .. + 15 and 64 + 16 q .. + 15 of the block
-    float v[32];
+    // this lane's 32 elements of row r, two to a word: 16 q .. + 15 and 64 + 16 q .. + 15 of the block
+    uint32_t v[16], size[16], most = 0u;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       const int c = k * kFp8Block + (h >> 1) * 64 + 16 * q + (h & 1) * 8, left = has_x ? g.K - c : 0;
       if (left >= 8) {
         const u32x4 e = *reinterpret_cast<const u32x4_any*>(x + c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] = T::to_float((uint16_t)(i & 1 ? e[i / 2] >> 16 : e[i / 2] & 0xffffu));
+        for (int i = 0; i < 4; ++i) v[4 * h + i] = e[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] = i < left ? T::to_float(x[c + i]) : 0.f;
+        for (int i = 0; i < 4; ++i)
+          v[4 * h + i] = (2 * i < left ? x[c + 2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)x[c + 2 * i + 1] << 16 : 0u);
       }
     }
-    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) most = max(most, finite_magnitude(v[i]));
+    for (int i = 0; i < 16; ++i) {
+      size[i] = v[i] & 0x7fff7fffu;
+      most = pk_max(most, size[i]);
+    }
+    most = max(most & 0xffffu, most >> 16);
+    if (most >= kInfinite<T>) {
+      most = 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t lo = size[i] & 0xffffu, hi = size[i] >> 16;
+        most = max(most, max(lo < kInfinite<T> ? lo : 0u, hi < kInfinite<T> ? hi : 0u));
+      }
+    }
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-    const uint32_t xs = fp8_scale_of(most);
-    const float by = fp8_inverse(xs);
+    const uint32_t xs = fp8_scale_of(size_bits<T>(most));
     i32x8 a, b;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (int)pack_fp8(v[4 * i] * by, v[4 * i + 1] * by, v[4 * i + 2] * by, v[4 * i + 3] * by);
+    for (int i = 0; i < 8; ++i) a[i] = (int)codes_of<T, true>(codes_of<T, false>(0u, v[2 * i], xs), v[2 * i + 1], xs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       b[i] = (int)wl[i];

@@ -20,6 +20,8 @@ namespace {
 constexpr int kB = kFp8Block;
 constexpr int kBlockBytes = kB * kB;  // of one 128 x 128 block of codes
 constexpr int kLdsLimit = 160 * 1024;
+constexpr int kCus = 256;
+constexpr int64_t kPairBlocks = 1024;  // workgroups of both gradients up to which they share a launch
 constexpr int kMaxList = 4096;        // 128-blocks that a workgroup's list can hold
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -203,23 +205,22 @@ __device__ inline int make_list(int lo, int hi, uint32_t* list, uint8_t* scratch
 }
 
 // ---- 128 x 128 tiles ------------------------------------------------------------------------------------------------------
-// Four waves of 64 x 64, two stages, two workgroups to a CU: while one waits at its barrier the other's matrix instructions run.
-// Bound by the LDS: 32 KB in and 64 KB out a step for 512 clocks of matrix instructions.
+// Four waves of 64 x 64.  Two stages and two workgroups to a CU: while one waits at its barrier the other's matrix instructions run; bound
+// by the LDS, 32 KB in and 64 KB out a step for 512 clocks of matrix instructions.  Four stages, a workgroup to a CU, where
+// there are no more of them than CUs: then a step costs what is left of a load's latency, of which three steps are on their way.
 constexpr int kMidStage = 2 * kBlockBytes + 2 * 512;  // A block, B block, words of scales of either
-constexpr int kMidList = 2 * kMidStage;
-constexpr int mid_lds(int list) { return kMidList + list * 5 + 16; }
+constexpr int mid_lds(int stages, int list) { return stages * kMidStage + list * 5 + 16; }
 
-template <typename T, int MODE, bool SQUARE>
-__global__ __launch_bounds__(256, 2) void fp8_mid_kernel(Args p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+template <typename T, int MODE, bool SQUARE, int STAGES>
+__device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
   const Fp8Gemm& g = p.g;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   int tm, tn, part;
-  tile_of_split_block<DSD_GROUP_M>((int)blockIdx.x, p.tiles_m, p.tiles_n, p.splits, tm, tn, part);
+  tile_of_split_block<DSD_GROUP_M>(block, p.tiles_m, p.tiles_n, p.splits, tm, tn, part);
   const int64_t m0 = (int64_t)tm * kB, n0 = (int64_t)tn * kB;
   const int lo = part * p.per_split, hi = min(p.nk, lo + p.per_split);
   float* const out_part = p.splits > 1 ? g.part + (int64_t)part * g.M * g.N : nullptr;
-  uint32_t* const list = reinterpret_cast<uint32_t*>(smem + kMidList);
+  uint32_t* const list = reinterpret_cast<uint32_t*>(smem + STAGES * kMidStage);
   int steps = hi - lo;
   if constexpr (MODE == kFp8Dsd) {
     uint8_t* const scratch = reinterpret_cast<uint8_t*>(list + p.per_split);
@@ -230,6 +231,7 @@ __global__ __launch_bounds__(256, 2) void fp8_mid_kernel(Args p) {
   if constexpr (MODE == kFp8Sdd) {
     if (dropped(g, tm, tn)) steps = 0;
   }
+  steps = __builtin_amdgcn_readfirstlane(steps);
   const int wm = wave >> 1, wn = wave & 1;
   BlockLoader la, lb;
   la.init(g.a + m0 * g.lda, g.lda, g.M - m0, lane);
@@ -237,10 +239,11 @@ __global__ __launch_bounds__(256, 2) void fp8_mid_kernel(Args p) {
   const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
   const u32x4 bb = SQUARE ? buffer_over(g.sb + tn * g.sb_r, (int64_t)(p.nk - 1) * g.sb_k + 1) : buffer_over(g.sb + n0, (int64_t)p.nk * g.sb_k - n0);
   const uint32_t lds = lds_address(smem);
+  const int per_step = wave < 2 ? 9 : 8;  // loads of this wave
   auto step_block = [&](int s) { return MODE == kFp8Dsd ? __builtin_amdgcn_readfirstlane((int)(list[s] & 0xffffu)) : lo + s; };
   auto load = [&](int s) {
     const int k = step_block(s);
-    const uint32_t at = lds + (uint32_t)(s & 1) * kMidStage;
+    const uint32_t at = lds + (uint32_t)(s % STAGES) * kMidStage;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       la.load(wave * 4 + q, k, at);
@@ -253,12 +256,12 @@ __global__ __launch_bounds__(256, 2) void fp8_mid_kernel(Args p) {
     }
   };
   f32x4 acc[4][4] = {};
-  if (steps > 0) load(0);
+  for (int s = 0; s < STAGES - 1 && s < steps; ++s) load(s);
   for (int s = 0; s < steps; ++s) {
-    wait_loads();
+    wait_loads_all_but(per_step * min(STAGES - 2, steps - 1 - s));
     barrier();
-    if (s + 1 < steps) load(s + 1);
-    const char* st = smem + (s & 1) * kMidStage;
+    if (s + STAGES - 1 < steps) load(s + STAGES - 1);  // (into the stage of step s - 1, which every wave is done with)
+    const char* st = smem + (s % STAGES) * kMidStage;
     const char* scales = st + 2 * kBlockBytes;
     const int sa = *reinterpret_cast<const int*>(scales + 64 * wm + 4 * (lane & 15));
     int sb = *reinterpret_cast<const int*>(scales + 512 + (SQUARE ? 0 : 64 * wn + 4 * (lane & 15)));
@@ -276,6 +279,20 @@ __global__ __launch_bounds__(256, 2) void fp8_mid_kernel(Args p) {
     wait_reads();  // (before the stage that was read is loaded over, behind the next barrier)
   }
   store_patch<T>(g, m0 + 64 * wm, n0 + 64 * wn, acc, out_part, lane);
+}
+
+template <typename T, int MODE, bool SQUARE, int STAGES>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void fp8_mid_kernel(Args p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  mid_tile<T, MODE, SQUARE, STAGES>(p, (int)blockIdx.x, smem);
+}
+
+// Both gradients of a layer in one launch, the weight gradient's workgroups behind the input gradient's.
+template <typename T, int STAGES>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void fp8_pair_kernel(Args x, Args w, int first_w) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  if ((int)blockIdx.x < first_w) mid_tile<T, kFp8Sdd, true, STAGES>(x, (int)blockIdx.x, smem);
+  else mid_tile<T, kFp8Dsd, false, STAGES>(w, (int)blockIdx.x - first_w, smem);
 }
 
 // C = scale * sum of the parts, in their order
@@ -328,21 +345,59 @@ Plan plan(int64_t M, int64_t N, int64_t K, int mode) {
   return {(int)ceil_div(nk, per), (int)per};
 }
 
-template <typename T, int MODE>
-int launch(const Fp8Gemm& g, const Args& p, hipStream_t stream) {
-  const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  if (blocks >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8 product: %lld tiles are too many for one launch", (long long)blocks);
-  auto* kernel = g.sb_square ? &fp8_mid_kernel<T, MODE, true> : &fp8_mid_kernel<T, MODE, false>;
-  const int lds = mid_lds(MODE == kFp8Dsd ? p.per_split : 0);
+int64_t blocks_of(const Args& p) { return (int64_t)p.tiles_m * p.tiles_n * p.splits; }
+
+template <typename T>
+int launch_sum(const Args& p, hipStream_t stream) {
+  if (p.splits <= 1) return SD_OK;
+  hipLaunchKernelGGL(&fp8_sum_kernel<T>, dim3((unsigned)ceil_div(p.g.M * p.g.N, 1024)), dim3(256), 0, stream, p.g, p.splits);
+  return check_launch("fp8_sum");
+}
+
+template <typename T, int MODE, int STAGES>
+int launch_mid(const Args& p, hipStream_t stream) {
+  auto* kernel = p.g.sb_square ? &fp8_mid_kernel<T, MODE, true, STAGES> : &fp8_mid_kernel<T, MODE, false, STAGES>;
   static std::atomic<bool> configured[2][16] = {};
-  if (int rc = configure(reinterpret_cast<const void*>(kernel), configured[g.sb_square])) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, stream, p);
-  note_kernel("fp8:mid splits=%d", p.splits);
-  if (int rc = check_launch("fp8_gemm")) return rc;
-  if (p.splits > 1) {
-    hipLaunchKernelGGL(&fp8_sum_kernel<T>, dim3((unsigned)ceil_div(g.M * g.N, 1024)), dim3(256), 0, stream, g, p.splits);
-    return check_launch("fp8_sum");
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), configured[p.g.sb_square])) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks_of(p)), dim3(256), mid_lds(STAGES, MODE == kFp8Dsd ? p.per_split : 0), stream, p);
+  note_kernel("fp8:mid stages=%d splits=%d", STAGES, p.splits);
+  return check_launch("fp8_gemm");
+}
+
+// Four stages where every workgroup has a CU to itself and more than two steps
+bool deep(int64_t blocks, const Args& p) { return blocks <= kCus && p.per_split > 2; }
+
+template <typename T, int MODE>
+int launch(const Args& p, hipStream_t stream) {
+  if (blocks_of(p) >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8 product: %lld tiles are too many for one launch", (long long)blocks_of(p));
+  if (int rc = deep(blocks_of(p), p) ? launch_mid<T, MODE, 4>(p, stream) : launch_mid<T, MODE, 2>(p, stream)) return rc;
+  return launch_sum<T>(p, stream);
+}
+
+template <typename T, int STAGES>
+int launch_pair(const Args& x, const Args& w, hipStream_t stream) {
+  auto* kernel = &fp8_pair_kernel<T, STAGES>;
+  static std::atomic<bool> configured[16] = {};
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), configured)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_of(x) + blocks_of(w))), dim3(256), mid_lds(STAGES, w.per_split), stream, x, w, (int)blocks_of(x));
+  note_kernel("fp8:pair stages=%d splits=%d", STAGES, w.splits);
+  if (int rc = check_launch("fp8_pair")) return rc;
+  return launch_sum<T>(w, stream);
+}
+
+int make_args(const Fp8Gemm& g, int mode, Args& p) {
+  p.g = g;
+  const Plan q = plan(g.M, g.N, g.K, mode);
+  p.nk = (int)ceil_div(g.K, kB);
+  p.splits = q.splits;
+  p.per_split = q.per_split;
+  if (p.splits > 1 && (g.part == nullptr || g.part_bytes < (int64_t)p.splits * g.M * g.N * 4)) {
+    if (mode == kFp8Dsd && p.nk > kMaxList) return fail(SD_ERR_INVALID, "fp8 product: a reduction of %d blocks needs its scratch", p.nk);
+    p.splits = 1;
+    p.per_split = p.nk;
   }
+  p.tiles_m = (int)ceil_div(g.M, kB);
+  p.tiles_n = (int)ceil_div(g.N, kB);
   return SD_OK;
 }
 
@@ -357,24 +412,27 @@ int64_t fp8_gemm_scratch(int64_t M, int64_t N, int64_t K, int mode) {
 int launch_fp8_gemm(const Fp8Gemm& g, int mode, int dtype, hipStream_t stream) {
   if (g.M == 0 || g.N == 0) return SD_OK;
   Args p;
-  p.g = g;
-  const Plan q = plan(g.M, g.N, g.K, mode);
-  p.nk = (int)ceil_div(g.K, kB);
-  p.splits = q.splits;
-  p.per_split = q.per_split;
-  if (p.splits > 1 && (g.part == nullptr || g.part_bytes < (int64_t)p.splits * g.M * g.N * 4)) {
-    if (mode == kFp8Dsd && p.nk > kMaxList) return fail(SD_ERR_INVALID, "fp8 product: a reduction of %d blocks needs its scratch", p.nk);
-    p.splits = 1;
-    p.per_split = p.nk;
-  }
-  p.tiles_m = (int)ceil_div(g.M, kB);
-  p.tiles_n = (int)ceil_div(g.N, kB);
+  if (int rc = make_args(g, mode, p)) return rc;
   if (dtype == SD_BF16) {
-    if (mode == kFp8Dense) return launch<BF16, kFp8Dense>(g, p, stream);
-    return mode == kFp8Dsd ? launch<BF16, kFp8Dsd>(g, p, stream) : launch<BF16, kFp8Sdd>(g, p, stream);
+    if (mode == kFp8Dense) return launch<BF16, kFp8Dense>(p, stream);
+    return mode == kFp8Dsd ? launch<BF16, kFp8Dsd>(p, stream) : launch<BF16, kFp8Sdd>(p, stream);
   }
-  if (mode == kFp8Dense) return launch<F16, kFp8Dense>(g, p, stream);
-  return mode == kFp8Dsd ? launch<F16, kFp8Dsd>(g, p, stream) : launch<F16, kFp8Sdd>(g, p, stream);
+  if (mode == kFp8Dense) return launch<F16, kFp8Dense>(p, stream);
+  return mode == kFp8Dsd ? launch<F16, kFp8Dsd>(p, stream) : launch<F16, kFp8Sdd>(p, stream);
+}
+
+int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStream_t stream) {
+  Args x, w;
+  if (int rc = make_args(gx, kFp8Sdd, x)) return rc;
+  if (int rc = make_args(gw, kFp8Dsd, w)) return rc;
+  const int64_t blocks = blocks_of(x) + blocks_of(w);
+  if (!gx.sb_square || gw.sb_square || blocks > kPairBlocks) {
+    if (int rc = launch_fp8_gemm(gx, kFp8Sdd, dtype, stream)) return rc;
+    return launch_fp8_gemm(gw, kFp8Dsd, dtype, stream);
+  }
+  const bool four = deep(blocks, x) || deep(blocks, w);
+  if (dtype == SD_BF16) return four ? launch_pair<BF16, 4>(x, w, stream) : launch_pair<BF16, 2>(x, w, stream);
+  return four ? launch_pair<F16, 4>(x, w, stream) : launch_pair<F16, 2>(x, w, stream);
 }
 
 }  // namespace sd

@@ -2,8 +2,11 @@
 //
 // A training step needs its activations and output gradients twice: with blocks along their rows for the products that sum over
 // features, and with blocks along their columns, transposed, for the weight gradient, which sums over tokens.  Both come out of one
-// read: a workgroup holds a 128 x 128 tile in registers, 8 x 8 elements a thread, takes the largest magnitude along both directions
-// and writes the codes both ways.  Bound by its reads and writes: 2 bytes in and 1 or 2 out per element.
+// read: a workgroup holds a 128 x 128 tile in registers, 4 rows x 8 columns a thread, takes the largest magnitude along both directions
+// and writes the codes both ways, those across turned through LDS so that both are stored in whole 128-byte lines.
+// Bound by its reads and writes, 2 bytes in and 1 or 2 out per element, as long as the arithmetic stays out of the way: magnitudes of
+// 16-bit elements are compared two at a time as whole numbers, and the conversion takes two of them and the scale in one
+// instruction (its results are those of multiplying in fp32 and converting, for every 16-bit number within the range).
 #include "fp8.h"
 
 #include <type_traits>
@@ -11,50 +14,147 @@
 namespace sd {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kRows = 4;           // of a thread, by eight columns
+constexpr int kTurnPitch = 132;    // bytes of a column's codes in LDS: 33 words, so that a wave's words meet a bank twice at most
 
 struct F32 {
   static constexpr int id = kF32;
 };
 
-// eight consecutive elements, zeros where `left` ends
+// Eight elements of a row and what is done with them.  w: two to a word; magnitudes are 15-bit whole numbers, of which the larger
+// stands for the larger number.
 template <typename T>
-__device__ inline void load_eight(const void* src, int64_t at, int left, float (&v)[8]) {
-  if constexpr (T::id == kF32) {
-    typedef f32x4 __attribute__((aligned(4))) f32x4_any;
-    const float* s = static_cast<const float*>(src) + at;
-    if (left >= 8) {
-      const f32x4 a = *reinterpret_cast<const f32x4_any*>(s), b = *reinterpret_cast<const f32x4_any*>(s + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? s[i] : 0.f;
-    }
-  } else {
+struct Eight {
+  uint32_t w[4];
+  __device__ inline void load(const void* src, int64_t at, int left) {
     const uint16_t* s = static_cast<const uint16_t*>(src) + at;
     if (left >= 8) {
-      const u32x4 w = *reinterpret_cast<const u32x4_any*>(s);
+      const u32x4 v = *reinterpret_cast<const u32x4_any*>(s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = T::to_float((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+      for (int i = 0; i < 4; ++i) w[i] = v[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? T::to_float(s[i]) : 0.f;
+      for (int i = 0; i < 4; ++i)
+        w[i] = (2 * i < left ? s[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)s[2 * i + 1] << 16 : 0u);
     }
   }
-}
+  __device__ inline void sizes(uint32_t (&a)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = w[i] & 0x7fff7fffu;
+  }
+};
+// A thread's 4 x 8 elements.
+template <typename T>
+struct Patch {
+  Eight<T> e[kRows];
+  __device__ inline void load(const void* src, int64_t ld, int r0, int c0, int rows, int cols) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) e[i].load(src, (int64_t)(r0 + i) * ld + c0, r0 + i < rows ? cols - c0 : 0);
+  }
+  // the largest finite magnitude of each row, and of the columns two to a word
+  __device__ inline void most(uint32_t (&row)[kRows], uint32_t (&col)[4]) const {
+    uint32_t a[kRows][4], all = 0u;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      e[i].sizes(a[i]);
+      all = pk_max(all, pk_max(pk_max(a[i][0], a[i][1]), pk_max(a[i][2], a[i][3])));
+    }
+    if (max(all & 0xffffu, all >> 16) >= kInfinite<T>) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          if ((a[i][d] & 0xffffu) >= kInfinite<T>) a[i][d] &= 0xffff0000u;
+          if (a[i][d] >> 16 >= kInfinite<T>) a[i][d] &= 0xffffu;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const uint32_t m = pk_max(pk_max(a[i][0], a[i][1]), pk_max(a[i][2], a[i][3]));
+      row[i] = max(m & 0xffffu, m >> 16);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) col[d] = pk_max(pk_max(a[0][d], a[1][d]), pk_max(a[2][d], a[3][d]));
+  }
+  static constexpr int kColWords = 4;
+  __device__ static inline uint32_t merge(uint32_t a, uint32_t b) { return pk_max(a, b); }
+  __device__ static inline uint32_t bits(uint32_t m) { return size_bits<T>(m); }
+  __device__ static inline uint32_t col_bits(const uint32_t (&col)[4], int j) { return size_bits<T>(j & 1 ? col[j / 2] >> 16 : col[j / 2] & 0xffffu); }
+  __device__ inline u32x2 row_codes(int i, uint32_t byte) const {
+    u32x2 q;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) q[h] = codes_of<T, true>(codes_of<T, false>(0u, e[i].w[2 * h], byte), e[i].w[2 * h + 1], byte);
+    return q;
+  }
+  __device__ inline uint32_t col_codes(int j, uint32_t byte) const {  // of the four rows
+    const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+    const int d = j / 2;
+    const uint32_t lo = __builtin_amdgcn_perm(e[1].w[d], e[0].w[d], pick), hi = __builtin_amdgcn_perm(e[3].w[d], e[2].w[d], pick);
+    return codes_of<T, true>(codes_of<T, false>(0u, lo, byte), hi, byte);
+  }
+};
+template <>
+struct Patch<F32> {
+  float v[kRows][8];
+  __device__ inline void load(const void* src, int64_t ld, int r0, int c0, int rows, int cols) {
+    typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const float* s = static_cast<const float*>(src) + (int64_t)(r0 + i) * ld + c0;
+      const int left = r0 + i < rows ? cols - c0 : 0;
+      if (left >= 8) {
+        const f32x4 a = *reinterpret_cast<const f32x4_any*>(s), b = *reinterpret_cast<const f32x4_any*>(s + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[i][j] = a[j];
+          v[i][4 + j] = b[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = j < left ? s[j] : 0.f;
+      }
+    }
+  }
+  static constexpr int kColWords = 8;
+  __device__ inline void most(uint32_t (&row)[kRows], uint32_t (&col)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) col[j] = 0u;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      row[i] = 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = finite_magnitude(v[i][j]);
+        row[i] = max(row[i], a);
+        col[j] = max(col[j], a);
+      }
+    }
+  }
+  __device__ static inline uint32_t merge(uint32_t a, uint32_t b) { return max(a, b); }
+  __device__ static inline uint32_t bits(uint32_t m) { return m; }
+  __device__ static inline uint32_t col_bits(const uint32_t (&col)[8], int j) { return col[j]; }
+  __device__ inline u32x2 row_codes(int i, uint32_t byte) const {
+    const float s = fp8_inverse(byte);
+    return u32x2{pack_fp8(v[i][0] * s, v[i][1] * s, v[i][2] * s, v[i][3] * s), pack_fp8(v[i][4] * s, v[i][5] * s, v[i][6] * s, v[i][7] * s)};
+  }
+  __device__ inline uint32_t col_codes(int j, uint32_t byte) const {
+    const float s = fp8_inverse(byte);
+    return pack_fp8(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s);
+  }
+};
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantJobs js) {
-  __shared__ uint32_t most_of[4][kFp8Block];  // [wave][column], or [wave][0] of a square block
+  constexpr int W = Patch<T>::kColWords;
+  __shared__ __attribute__((aligned(16))) uint32_t most_of[kThreads / 64][16 * W];  // [wave][the columns' words], or [wave][0] of a square block
+  __shared__ uint32_t turned[kFp8Block * kTurnPitch / 4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int which = js.n > 1 && blockIdx.x >= js.job[1].first_block ? 1 : 0;
   const QuantJob& p = js.job[which];
   const uint32_t tile = blockIdx.x - p.first_block;
   const int tr = (int)(tile / p.tiles_c), tc = (int)(tile - (uint32_t)tr * p.tiles_c);
+  const int r0 = tr * kFp8Block + (t >> 4) * kRows, c0 = tc * kFp8Block + (t & 15) * 8;
   bool dropped = false;
   if (p.masked) {
     MaskSrc src = js.mask;
@@ -64,91 +164,88 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantJobs js) {
     if (js.mask_out && t == 0 && si * src.split == i && sj * src.split == j) js.mask_out[(int64_t)si * src.kb + sj] = dropped ? 1 : 0;
   }
   if (!dropped) {  // (uniform)
-    const int r0 = tr * kFp8Block + (t >> 4) * 8, c0 = tc * kFp8Block + (t & 15) * 8;
-    float v[8][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int left = r0 + i < p.rows ? p.cols - c0 : 0;
-      load_eight<T>(p.src, (int64_t)(r0 + i) * p.ld + c0, left, v[i]);
-    }
-    uint32_t row_most[8], col_most[8] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      row_most[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t a = finite_magnitude(v[i][j]);
-        row_most[i] = max(row_most[i], a);
-        col_most[j] = max(col_most[j], a);
-      }
-    }
-    uint32_t row_scale[8], col_scale[8];
+    Patch<T> v;
+    v.load(p.src, p.ld, r0, c0, p.rows, p.cols);
+    uint32_t row_scale[kRows], col_scale[8], row_most[kRows], col_most[W];
+    v.most(row_most, col_most);
     if (p.square) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, row_most[i]);
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+      uint32_t m = max(max(row_most[0], row_most[1]), max(row_most[2], row_most[3]));
+      m = max_of_row16(m);
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
       if (lane == 0) most_of[wave][0] = m;
       __syncthreads();
-      m = max(max(most_of[0][0], most_of[1][0]), max(most_of[2][0], most_of[3][0]));
-      const uint32_t s = fp8_scale_of(m);
+      m = most_of[0][0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) row_scale[i] = col_scale[i] = s;
+      for (int i = 1; i < kThreads / 64; ++i) m = max(m, most_of[i][0]);
+      const uint32_t s = fp8_scale_of(Patch<T>::bits(m));
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) row_scale[i] = s;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) col_scale[j] = s;
     } else {
       if (p.along.data) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) row_scale[i] = fp8_scale_of(max_of_row16(row_most[i]));
+        for (int i = 0; i < kRows; ++i) row_scale[i] = fp8_scale_of(Patch<T>::bits(max_of_row16(row_most[i])));
       }
       if (p.across.data) {  // (uniform)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t m = col_most[j];
-          m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-          m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-          if (lane < 16) most_of[wave][(t & 15) * 8 + j] = m;
+        for (int d = 0; d < W; ++d) {
+          col_most[d] = Patch<T>::merge(col_most[d], (uint32_t)__shfl_xor((int)col_most[d], 16));
+          col_most[d] = Patch<T>::merge(col_most[d], (uint32_t)__shfl_xor((int)col_most[d], 32));
+          if (lane < 16) most_of[wave][lane * W + d] = col_most[d];
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = (t & 15) * 8 + j;
-          col_scale[j] = fp8_scale_of(max(max(most_of[0][c], most_of[1][c]), max(most_of[2][c], most_of[3][c])));
+        for (int d = 0; d < W; ++d) {
+#pragma unroll
+          for (int i = 0; i < kThreads / 64; ++i) col_most[d] = Patch<T>::merge(col_most[d], most_of[i][(t & 15) * W + d]);
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) col_scale[j] = fp8_scale_of(Patch<T>::col_bits(col_most, j));
       }
     }
     if (p.along.data) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r0 + i >= p.rows) continue;
-        const float s = fp8_inverse(row_scale[i]);
-        const u32x2 q = {pack_fp8(v[i][0] * s, v[i][1] * s, v[i][2] * s, v[i][3] * s),
-                         pack_fp8(v[i][4] * s, v[i][5] * s, v[i][6] * s, v[i][7] * s)};
-        *reinterpret_cast<u32x2*>(p.along.data + (int64_t)(r0 + i) * p.along.ld + c0) = q;
-        if ((t & 15) == 0 && !p.square) p.along.scales[(int64_t)(r0 + i) * p.along.s_r + (int64_t)tc * p.along.s_k] = (uint8_t)row_scale[i];
+      for (int i = 0; i < kRows; ++i)
+        if (r0 + i < p.rows) *reinterpret_cast<u32x2*>(p.along.data + (int64_t)(r0 + i) * p.along.ld + c0) = v.row_codes(i, row_scale[i]);
+      if (p.square) {
+        if (t == 0) p.along.scales[(int64_t)tr * p.along.s_r + (int64_t)tc * p.along.s_k] = (uint8_t)row_scale[0];
+      } else if ((t & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (r0 + i < p.rows) p.along.scales[(int64_t)(r0 + i) * p.along.s_r + (int64_t)tc * p.along.s_k] = (uint8_t)row_scale[i];
       }
-      if (p.square && t == 0) p.along.scales[(int64_t)tr * p.along.s_r + (int64_t)tc * p.along.s_k] = (uint8_t)row_scale[0];
     }
     if (p.across.data) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (c0 + j >= p.cols) continue;
-        const float s = fp8_inverse(col_scale[j]);
-        const u32x2 q = {pack_fp8(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s),
-                         pack_fp8(v[4][j] * s, v[5][j] * s, v[6][j] * s, v[7][j] * s)};
-        *reinterpret_cast<u32x2*>(p.across.data + (int64_t)(c0 + j) * p.across.ld + r0) = q;
-        if (t < 16 && !p.square) p.across.scales[(int64_t)(c0 + j) * p.across.s_r + (int64_t)tr * p.across.s_k] = (uint8_t)col_scale[j];
+      for (int j = 0; j < 8; ++j) turned[((t & 15) * 8 + j) * (kTurnPitch / 4) + (t >> 4)] = v.col_codes(j, col_scale[j]);
+      if (p.square) {
+        if (t == 0) p.across.scales[(int64_t)tc * p.across.s_r + (int64_t)tr * p.across.s_k] = (uint8_t)col_scale[0];
+      } else if (t < 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j < p.cols) p.across.scales[(int64_t)(c0 + j) * p.across.s_r + (int64_t)tr * p.across.s_k] = (uint8_t)col_scale[j];
       }
-      if (p.square && t == 0) p.across.scales[(int64_t)tc * p.across.s_r + (int64_t)tr * p.across.s_k] = (uint8_t)col_scale[0];
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = h * 64 + (t >> 3), at = (t & 7) * 4;
+        if (tc * kFp8Block + c >= p.cols) continue;
+        const uint32_t* w = turned + c * (kTurnPitch / 4) + at;
+        *reinterpret_cast<u32x4*>(p.across.data + (int64_t)(tc * kFp8Block + c) * p.across.ld + tr * kFp8Block + at * 4) = u32x4{w[0], w[1], w[2], w[3]};
+      }
     }
   }
   report_in(const_cast<uint64_t*>(js.mask.state), gridDim.x);
 }
 
 // codes and scales -> values, four to a thread.  Bound by what it writes.
+constexpr int kOutThreads = 256;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k,
+__global__ __launch_bounds__(kOutThreads) void dequantize_kernel(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k,
                                                               int square, int64_t rows, int64_t cols, uint32_t quads, void* out, int64_t out_ld) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, r = at / quads, c = (at - r * quads) * 4;
+  const int64_t at = (int64_t)blockIdx.x * kOutThreads + threadIdx.x, r = at / quads, c = (at - r * quads) * 4;
   if (r >= rows) return;
   const uint32_t q = *reinterpret_cast<const uint32_t*>(data + r * ld + c);
   const float s = fp8_power(scales[(square ? r / kFp8Block : r) * s_r + c / kFp8Block * s_k]);
@@ -181,11 +278,11 @@ int launch_quantize(QuantJobs& js, int dtype, hipStream_t stream) {
 
 int launch_dequantize(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k, int square, int64_t rows,
                       int64_t cols, void* out, int64_t out_ld, int dtype, hipStream_t stream) {
-  const int64_t quads = ceil_div(cols, 4), blocks = ceil_div(rows * quads, kThreads);
+  const int64_t quads = ceil_div(cols, 4), blocks = ceil_div(rows * quads, kOutThreads);
   if (blocks == 0) return SD_OK;
   if (blocks >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8_dequantize: %lld x %lld is too large for one launch", (long long)rows, (long long)cols);
   auto* kernel = dtype == kF32 ? &dequantize_kernel<F32> : dtype == SD_BF16 ? &dequantize_kernel<BF16> : &dequantize_kernel<F16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, data, ld, scales, s_r, s_k, square, rows, cols, (uint32_t)quads, out, out_ld);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kOutThreads), 0, stream, data, ld, scales, s_r, s_k, square, rows, cols, (uint32_t)quads, out, out_ld);
   return check_launch("fp8_dequantize");
 }
 
