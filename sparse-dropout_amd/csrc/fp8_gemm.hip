@@ -66,22 +66,24 @@ __device__ inline void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// One 128-row block of an operand on its way into LDS, 1 KB (8 LDS rows) an instruction, 16 in all.
-struct BlockLoader {
-  u32x4 buffer;       // from the block's first row
-  uint32_t even, odd; // a lane's offset in instructions 2 n and 2 n + 1 of a group of eight (see offset())
+// raw buffer over an operand's block of up to 128 rows
+__device__ inline u32x4 block_buffer(const uint8_t* first_row, int64_t ld, int64_t rows) {
+  return buffer_over(first_row, (rows < kB ? rows : kB) * ld);
+}
+// One 128-row block of an operand on its way into LDS, 1 KB (8 LDS rows) an instruction, 16 in all.  LDS row s = 8 q + lane / 8 of a
+// group of 64 holds row 4 (s % 16) + s / 16; the 16-byte chunks of an LDS row are turned by (s / 2) % 8, so that the 16 rows of a
+// fragment read meet no bank twice.
+struct BlockRows {
+  uint32_t even, odd;  // a lane's offset in instructions 2 n and 2 n + 1 of a group of eight
   uint32_t ld;
-  // LDS row s = 8 q + lane / 8 of a group of 64 holds row 4 (s % 16) + s / 16; the 16-byte chunks of an LDS row are turned by
-  // (s / 2) % 8, so that the 16 rows of a fragment read meet no bank twice
-  __device__ inline void init(const uint8_t* base, int64_t ld_, int64_t rows, int lane) {
-    buffer = buffer_over(base, (rows < kB ? rows : kB) * ld_);
+  __device__ inline BlockRows(int64_t ld_, int lane) {
     ld = (uint32_t)ld_;
     const uint32_t r = (uint32_t)lane / 8, p = (uint32_t)lane % 8;
     even = 4 * r * ld + ((p ^ (r / 2)) << 4);
     odd = (4 * r + 32) * ld + ((p ^ (4 + r / 2)) << 4);
   }
   // instruction q (0 .. 15; wave-uniform) of 128-block k
-  __device__ inline void load(int q, int k, uint32_t lds_block) const {
+  __device__ inline void load(u32x4 buffer, int q, int k, uint32_t lds_block) const {
     const uint32_t on = (uint32_t)(64 * (q / 8) + q % 8 / 2) * ld + (uint32_t)k * kB;
     buffer16_to_lds(buffer, (q & 1 ? odd : even) + on, lds_block + (uint32_t)q * 1024);
   }
@@ -106,6 +108,7 @@ struct Args {
   Fp8Gemm g;
   int32_t nk, per_split;  // 128-blocks of the reduction, of one part of it
   int32_t tiles_m, tiles_n, splits;
+  bool big;  // tiles of 256 x 256 instead of 128 x 128
 };
 
 __device__ inline bool dropped(const Fp8Gemm& g, int i, int j) {
@@ -116,87 +119,83 @@ __device__ inline bool dropped(const Fp8Gemm& g, int i, int j) {
   return g.mask[i * g.msr + j * g.msc] != 0;
 }
 
-// The patch of 64 rows (from m0) x 64 columns (from n0) of a wave: sums of row group i and column group j in acc[i][j].
+// The patch of 64 rows (from m0) x 64 columns (from n0) of a wave: sums of row group i and column group j in acc[i][j], scaled and
+// rounded to C, or as they are to a part of a split reduction.  A whole patch is stored by straight code, four or eight elements
+// a lane at a time; one at C's edge element by element.
 template <typename T>
 __device__ inline void store_patch(const Fp8Gemm& g, int64_t m0, int64_t n0, const f32x4 (&acc)[4][4], float* part, int lane) {
+  typedef u32x2 __attribute__((aligned(2))) u32x2_any;
   const int r = lane & 15, q = lane >> 4;
   const bool along_n = g.c_sc == 1;
-  const float scale = part ? 1.f : g.scale;
   const int64_t ld = part ? (along_n ? g.N : g.M) : (along_n ? g.c_sr : g.c_sc);
-  if (along_n) {
-    const int64_t n = n0 + 4 * r;
-    if (n >= g.N) return;
-    const bool whole = n + 4 <= g.N;
+  const bool whole = m0 + 64 <= g.M && n0 + 64 <= g.N && (!part || ld % 4 == 0);
+  if (whole && along_n) {
+    const int64_t at = (m0 + 16 * q) * ld + n0 + 4 * r;
+    if (part) {
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+      for (int v = 0; v < 4; ++v)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + 16 * q + 4 * v + i;
-        if (m >= g.M) continue;
-        const float x[4] = {acc[i][0][v] * scale, acc[i][1][v] * scale, acc[i][2][v] * scale, acc[i][3][v] * scale};
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(part + at + (4 * v + i) * ld) = f32x4{acc[i][0][v], acc[i][1][v], acc[i][2][v], acc[i][3][v]};
+    } else {
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<u32x2_any*>(g.c + at + (4 * v + i) * ld) =
+              u32x2{T::pack2(acc[i][0][v] * g.scale, acc[i][1][v] * g.scale), T::pack2(acc[i][2][v] * g.scale, acc[i][3][v] * g.scale)};
+    }
+  } else if (whole) {  // sixteen rows a lane and column
+    const int64_t at = (n0 + 4 * r) * ld + m0 + 16 * q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = acc[e & 3][j][2 * h + e / 4] * (part ? 1.f : g.scale);
         if (part) {
-          float* dst = part + m * ld + n;
-          if (whole && g.N % 4 == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
-          else
-            for (int j = 0; j < 4; ++j)
-              if (n + j < g.N) dst[j] = x[j];
-        } else {
-          uint16_t* dst = g.c + m * ld + n;
-          typedef u32x2 __attribute__((aligned(2))) u32x2_any;
-          if (whole) *reinterpret_cast<u32x2_any*>(dst) = u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
-          else
-            for (int j = 0; j < 4; ++j)
-              if (n + j < g.N) dst[j] = T::from_float(x[j]);
-        }
-      }
-    return;
-  }
-  const int64_t m = m0 + 16 * q;  // sixteen rows a lane and column
-  if (m >= g.M) return;
-  const bool whole = m + 16 <= g.M;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t n = n0 + 4 * r + j;
-    if (n >= g.N) continue;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = acc[e & 3][j][2 * h + e / 4] * scale;
-      if (part) {
-        float* dst = part + n * ld + m + 8 * h;
-        if (whole && g.M % 4 == 0) {
+          float* dst = part + at + j * ld + 8 * h;
           *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
           *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
         } else {
-          for (int e = 0; e < 8; ++e)
-            if (m + 8 * h + e < g.M) dst[e] = x[e];
+          *reinterpret_cast<u32x4_any*>(g.c + at + j * ld + 8 * h) = u32x4{T::pack2(x[0], x[1]), T::pack2(x[2], x[3]), T::pack2(x[4], x[5]), T::pack2(x[6], x[7])};
         }
-      } else {
-        uint16_t* dst = g.c + n * ld + m + 8 * h;
-        if (whole) *reinterpret_cast<u32x4_any*>(dst) = u32x4{T::pack2(x[0], x[1]), T::pack2(x[2], x[3]), T::pack2(x[4], x[5]), T::pack2(x[6], x[7])};
-        else
-          for (int e = 0; e < 8; ++e)
-            if (m + 8 * h + e < g.M) dst[e] = T::from_float(x[e]);
       }
-    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t m = m0 + 16 * q + 4 * v + i, n = n0 + 4 * r + j, at = along_n ? m * ld + n : n * ld + m;
+          if (m >= g.M || n >= g.N) continue;
+          if (part) part[at] = acc[i][j][v];
+          else g.c[at] = T::from_float(acc[i][j][v] * g.scale);
+        }
   }
 }
 
-// The steps of a workgroup: list[s] = 128-block | flags << 16 of the blocks with any flag set, in order; returns how many.
-// flag(k): bits of what of block k is kept, for k in [lo, hi).  smem: (hi - lo) bytes of scratch.
-template <int THREADS, typename Flag>
+// Entries 128-block | flags << 16 of blocks [lo, hi): in front, in their order, those with any flag set, whose number is
+// returned; ALL: the others from behind.  flag(k): bits of what of block k is kept.  scratch: hi - lo bytes.
+template <int THREADS, bool ALL, typename Flag>
 __device__ inline int make_list(int lo, int hi, uint32_t* list, uint8_t* scratch, int* count, Flag flag) {
   const int t = threadIdx.x, n = hi - lo;
   for (int k = t; k < n; k += THREADS) scratch[k] = (uint8_t)flag(lo + k);
   __syncthreads();
   if (t < 64) {
-    int done = 0;
+    int done = 0, none = 0;
     for (int k0 = 0; k0 < n; k0 += 64) {
-      const uint32_t f = k0 + t < n ? scratch[k0 + t] : 0u;
-      const uint64_t some = __ballot(f != 0u);
-      if (f) list[done + __popcll(some & ((1ull << t) - 1))] = (uint32_t)(lo + k0 + t) | f << 16;
+      const bool in = k0 + t < n;
+      const uint32_t f = in ? scratch[k0 + t] : 0u;
+      const uint64_t some = __ballot(f != 0u), below = (1ull << t) - 1;
+      if (f) list[done + __popcll(some & below)] = (uint32_t)(lo + k0 + t) | f << 16;
       done += __popcll(some);
+      if (ALL) {
+        const uint64_t empty = __ballot(in && f == 0u);
+        if (in && f == 0u) list[n - 1 - none - __popcll(empty & below)] = (uint32_t)(lo + k0 + t);
+        none += __popcll(empty);
+      }
     }
     if (t == 0) *count = done;
   }
@@ -225,7 +224,7 @@ __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
   if constexpr (MODE == kFp8Dsd) {
     uint8_t* const scratch = reinterpret_cast<uint8_t*>(list + p.per_split);
     int* const count = reinterpret_cast<int*>(smem);
-    steps = make_list<256>(lo, hi, list, scratch, count, [&](int k) { return dropped(g, tm, k) ? 0 : 1; });
+    steps = make_list<256, false>(lo, hi, list, scratch, count, [&](int k) { return dropped(g, tm, k) ? 0 : 1; });
     __syncthreads();  // (count lies where the first stage goes)
   }
   if constexpr (MODE == kFp8Sdd) {
@@ -233,9 +232,8 @@ __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
   }
   steps = __builtin_amdgcn_readfirstlane(steps);
   const int wm = wave >> 1, wn = wave & 1;
-  BlockLoader la, lb;
-  la.init(g.a + m0 * g.lda, g.lda, g.M - m0, lane);
-  lb.init(g.b + n0 * g.ldb, g.ldb, g.N - n0, lane);
+  const BlockRows rows_a(g.lda, lane), rows_b(g.ldb, lane);
+  const u32x4 of_a = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_b = block_buffer(g.b + n0 * g.ldb, g.ldb, g.N - n0);
   const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
   const u32x4 bb = SQUARE ? buffer_over(g.sb + tn * g.sb_r, (int64_t)(p.nk - 1) * g.sb_k + 1) : buffer_over(g.sb + n0, (int64_t)p.nk * g.sb_k - n0);
   const uint32_t lds = lds_address(smem);
@@ -246,8 +244,8 @@ __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
     const uint32_t at = lds + (uint32_t)(s % STAGES) * kMidStage;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      la.load(wave * 4 + q, k, at);
-      lb.load(wave * 4 + q, k, at + kBlockBytes);
+      rows_a.load(of_a, wave * 4 + q, k, at);
+      rows_b.load(of_b, wave * 4 + q, k, at + kBlockBytes);
     }
     if (wave == 0) buffer4_to_lds(ba, (uint32_t)((int64_t)k * g.sa_ld) + (lane & 31) * 4, at + 2 * kBlockBytes);
     if (wave == 1) {
@@ -295,6 +293,156 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void fp8_pair_kernel(Args
   else mid_tile<T, kFp8Dsd, false, STAGES>(w, (int)blockIdx.x - first_w, smem);
 }
 
+// ---- 256 x 256 tiles ------------------------------------------------------------------------------------------------------
+// Eight waves of 128 x 64 in two groups of four, one for each of the tile's two row blocks; waves w and w + 4 share a SIMD.  A step of a
+// wave is a memory phase (its share of the coming blocks on its way, then all of the step's fragments into registers) and a compute phase of
+// 32 matrix instructions and nothing else.  A barrier ends each phase, and the second group runs one phase behind the first, so
+// that of each SIMD's two waves one computes while the other reads.  Two stages of 64 KB: reading step s, group 0 loads B of step
+// s + 1 into the other stage, group 1 the second row block of A of step s + 1 there and the first one of step s + 2 into the stage
+// it reads, whose first block group 0 is done with.  A wave waits for its own loads at the end of the compute phase behind.
+//
+// DSD walks the 128-blocks that either row block keeps; a group whose row block drops one skips its phases' work, and the block is not
+// loaded.  SDD takes two of the column blocks that either row of the pair keeps, in their order (behind them those that neither
+// keeps, whose blocks of C come out as zeros); a wave whose block of C is dropped skips its work.
+constexpr int kBigStage = 4 * kBlockBytes;        // A's two blocks, B's two
+constexpr int kBigScales = 2 * kBigStage;         // then 256 bytes of A's scales and 256 of B's for each stage
+constexpr int kBigList = kBigScales + 2 * 512;
+constexpr int big_lds(int list) { return kBigList + list * 5 + 16; }
+
+template <typename T, int MODE, bool SQUARE>
+__global__ __launch_bounds__(512, 2) void fp8_big_kernel(Args p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Fp8Gemm& g = p.g;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = wave >> 2, c = wave & 3;
+  int tm, tn, part;
+  tile_of_split_block<DSD_GROUP_M>((int)blockIdx.x, p.tiles_m, p.tiles_n, p.splits, tm, tn, part);
+  const int lo = part * p.per_split, hi = min(p.nk, lo + p.per_split);
+  float* const out_part = p.splits > 1 ? g.part + (int64_t)part * g.M * g.N : nullptr;
+  uint32_t* const list = reinterpret_cast<uint32_t*>(smem + kBigList);
+  int* const count = reinterpret_cast<int*>(smem + kBigScales);
+  const int row_blocks = (int)((g.M + kB - 1) / kB), col_blocks = (int)((g.N + kB - 1) / kB);
+  auto kept_rows = [&](int j) {  // of column j (SDD) or 128-block j (DSD)
+    return (dropped(g, 2 * tm, j) ? 0u : 1u) | (2 * tm + 1 < row_blocks && !dropped(g, 2 * tm + 1, j) ? 2u : 0u);
+  };
+  int steps = hi - lo, cols[2] = {2 * tn, 2 * tn + 1};
+  uint32_t tiles = 0xfu;  // SDD: bit 2 b + g of row block g, column block b
+  if constexpr (MODE == kFp8Dsd) {
+    steps = make_list<512, false>(lo, hi, list, reinterpret_cast<uint8_t*>(list + p.per_split), count, kept_rows);
+    __syncthreads();  // (count lies where the first scales go)
+  }
+  if constexpr (MODE == kFp8Sdd) {
+    make_list<512, true>(0, col_blocks, list, reinterpret_cast<uint8_t*>(list + col_blocks), count, kept_rows);
+    const uint32_t e0 = list[2 * tn], e1 = 2 * tn + 1 < col_blocks ? list[2 * tn + 1] : (uint32_t)col_blocks;
+    cols[0] = (int)(e0 & 0xffffu);
+    cols[1] = (int)(e1 & 0xffffu);
+    tiles = uniform(e0 >> 16 | e1 >> 16 << 2);
+    if (tiles == 0u) steps = 0;
+    __syncthreads();
+  }
+  steps = __builtin_amdgcn_readfirstlane(steps);
+  const int64_t m0 = (int64_t)tm * 2 * kB, c0 = (int64_t)__builtin_amdgcn_readfirstlane(cols[0]) * kB, c1 = (int64_t)__builtin_amdgcn_readfirstlane(cols[1]) * kB;
+  // group 0 loads B, a column block to two waves; group 1 loads A
+  const int64_t n_mine = c < 2 ? c0 : c1;
+  const BlockRows rows(grp == 0 ? g.ldb : g.lda, lane);
+  const u32x4 of_b = block_buffer(g.b + n_mine * g.ldb, g.ldb, g.N - n_mine);
+  const u32x4 of_a0 = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_a1 = block_buffer(g.a + (m0 + kB) * g.lda, g.lda, g.M - m0 - kB);
+  const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
+  const u32x4 bb = SQUARE ? buffer_over(g.sb, (int64_t)(col_blocks - 1) * g.sb_r + (int64_t)(p.nk - 1) * g.sb_k + 1)
+                          : buffer_over(g.sb + c0, (int64_t)p.nk * g.sb_k - c0);
+  const uint32_t square_at = SQUARE ? (uint32_t)((lane < 32 ? c0 : c1) / kB * g.sb_r) : 0u;
+  const uint32_t lds = lds_address(smem);
+  auto load_b = [&](int s, int k) {
+    const uint32_t at = lds + (uint32_t)(s & 1) * kBigStage + (2 + c / 2) * kBlockBytes, scales = lds + kBigScales + (uint32_t)(s & 1) * 512;
+    if (MODE != kFp8Sdd || (tiles >> (2 * (c / 2)) & 3u)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rows.load(of_b, 8 * (c & 1) + q, k, at);
+    }
+    if (c == 0) buffer4_to_lds(ba, (uint32_t)((int64_t)k * g.sa_ld) + lane * 4, scales);
+    if (c == 1) {
+      if (SQUARE) buffer1_to_lds(bb, square_at + (uint32_t)((int64_t)k * g.sb_k), scales + 256);
+      else buffer4_to_lds(bb, (uint32_t)((int64_t)k * g.sb_k) + lane * 4, scales + 256);
+    }
+  };
+  auto load_a = [&](int row, int s, int k) {
+    const uint32_t at = lds + (uint32_t)(s & 1) * kBigStage + row * kBlockBytes;
+    if (row) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rows.load(of_a1, 4 * c + q, k, at);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rows.load(of_a0, 4 * c + q, k, at);
+    }
+  };
+  auto entry = [&](int s) -> uint32_t {
+    if (MODE == kFp8Dsd) return s < steps ? list[s] : 0u;
+    return (uint32_t)(lo + s) | (MODE == kFp8Sdd ? ((tiles | tiles >> 2) & 3u) : 3u) << 16;
+  };
+  auto flag = [](uint32_t e, int row) { return (e >> 16 >> row & 1u) != 0u; };
+  auto block = [](uint32_t e) { return (int)(e & 0xffffu); };
+
+  f32x4 acc[2][4][4] = {};
+  if (steps > 0) {
+    uint32_t e0 = uniform(entry(0)), e1 = uniform(entry(1)), e2 = uniform(entry(2));
+    const bool works = MODE != kFp8Sdd || (tiles >> (2 * (c / 2) + grp) & 1u);
+    if (grp == 0) {
+      load_b(0, block(e0));
+    } else {
+      if (flag(e0, 0)) load_a(0, 0, block(e0));
+      if (flag(e0, 1)) load_a(1, 0, block(e0));
+      if (steps > 1 && flag(e1, 0)) load_a(0, 1, block(e1));
+    }
+    wait_loads();
+    barrier();
+    if (grp == 1) barrier();
+    for (int s = 0; s < steps; ++s) {
+      // memory phase
+      if (grp == 0) {
+        if (s + 1 < steps) load_b(s + 1, block(e1));
+      } else {
+        if (s + 1 < steps && flag(e1, 1)) load_a(1, s + 1, block(e1));
+        if (s + 2 < steps && flag(e2, 0)) load_a(0, s + 2, block(e2));
+      }
+      const bool on = works && flag(e0, grp);
+      i32x8 fa[8], fb[4];
+      int sa[2], sb;
+      if (on) {
+        const char* st = smem + (s & 1) * kBigStage;
+        const char* scales = smem + kBigScales + (s & 1) * 512;
+        sa[0] = *reinterpret_cast<const int*>(scales + 128 * grp + 4 * (lane & 15));
+        sa[1] = *reinterpret_cast<const int*>(scales + 128 * grp + 64 + 4 * (lane & 15));
+        sb = *reinterpret_cast<const int*>(scales + 256 + (SQUARE ? 128 * (c / 2) : 64 * c + 4 * (lane & 15)));
+        if (SQUARE) sb *= 0x01010101;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fb[j] = read_fragment(st + (2 + c / 2) * kBlockBytes + (c & 1) * 64 * kB, j, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fa[i] = read_fragment(st + grp * kBlockBytes + (i / 4) * 64 * kB, i & 3, lane);
+      }
+      wait_reads();
+      barrier();
+      // compute phase
+      const uint32_t e3 = entry(s + 3);
+      if (on) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[h][i][j] = mfma(fa[4 * h + i], fb[j], acc[h][i][j], sa[h], i, sb, j);
+        __builtin_amdgcn_s_setprio(0);
+      }
+      e0 = e1;
+      e1 = e2;
+      e2 = uniform(e3);
+      wait_loads();
+      if (grp == 0 || s + 1 < steps) barrier();
+    }
+  }
+  const int64_t n_out = n_mine + (c & 1) * 64;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) store_patch<T>(g, m0 + grp * kB + h * 64, n_out, acc[h], out_part, lane);
+}
+
 // C = scale * sum of the parts, in their order
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Gemm g, int splits) {
@@ -332,17 +480,19 @@ int configure(const void* kernel, std::atomic<bool>* done) {
 }
 
 struct Plan {
+  bool big;
   int splits, per_split;
 };
 Plan plan(int64_t M, int64_t N, int64_t K, int mode) {
-  const int64_t nk = ceil_div(K, kB), tiles = ceil_div(M, kB) * ceil_div(N, kB);
+  const int64_t nk = ceil_div(K, kB), tiles = ceil_div(M, kB) * ceil_div(N, kB), big_tiles = ceil_div(M, 2 * kB) * ceil_div(N, 2 * kB);
+  const bool big = big_tiles >= kCus;
   int64_t splits = 1;
-  if (mode != kFp8Sdd) {
+  if (mode != kFp8Sdd && !big) {
     while (tiles * splits < 256 && nk / (splits * 2) >= 4) splits *= 2;
   }
   if (mode == kFp8Dsd && ceil_div(nk, splits) > kMaxList) splits = ceil_div(nk, kMaxList);
   const int64_t per = ceil_div(nk, splits > 0 ? splits : 1);
-  return {(int)ceil_div(nk, per), (int)per};
+  return {big, (int)ceil_div(nk, per), (int)per};
 }
 
 int64_t blocks_of(const Args& p) { return (int64_t)p.tiles_m * p.tiles_n * p.splits; }
@@ -368,7 +518,22 @@ int launch_mid(const Args& p, hipStream_t stream) {
 bool deep(int64_t blocks, const Args& p) { return blocks <= kCus && p.per_split > 2; }
 
 template <typename T, int MODE>
+int launch_big(const Args& p, hipStream_t stream) {
+  auto* kernel = p.g.sb_square ? &fp8_big_kernel<T, MODE, true> : &fp8_big_kernel<T, MODE, false>;
+  static std::atomic<bool> configured[2][16] = {};
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), configured[p.g.sb_square])) return rc;
+  const int list = MODE == kFp8Dsd ? p.per_split : MODE == kFp8Sdd ? (int)ceil_div(p.g.N, kB) : 0;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks_of(p)), dim3(512), big_lds(list), stream, p);
+  note_kernel("fp8:big splits=%d", p.splits);
+  return check_launch("fp8_gemm");
+}
+
+template <typename T, int MODE>
 int launch(const Args& p, hipStream_t stream) {
+  if (p.big) {
+    if (int rc = launch_big<T, MODE>(p, stream)) return rc;
+    return launch_sum<T>(p, stream);
+  }
   if (blocks_of(p) >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8 product: %lld tiles are too many for one launch", (long long)blocks_of(p));
   if (int rc = deep(blocks_of(p), p) ? launch_mid<T, MODE, 4>(p, stream) : launch_mid<T, MODE, 2>(p, stream)) return rc;
   return launch_sum<T>(p, stream);
@@ -391,13 +556,15 @@ int make_args(const Fp8Gemm& g, int mode, Args& p) {
   p.nk = (int)ceil_div(g.K, kB);
   p.splits = q.splits;
   p.per_split = q.per_split;
-  if (p.splits > 1 && (g.part == nullptr || g.part_bytes < (int64_t)p.splits * g.M * g.N * 4)) {
+  if (q.splits > 1 && (g.part == nullptr || g.part_bytes < (int64_t)p.splits * g.M * g.N * 4)) {
     if (mode == kFp8Dsd && p.nk > kMaxList) return fail(SD_ERR_INVALID, "fp8 product: a reduction of %d blocks needs its scratch", p.nk);
     p.splits = 1;
     p.per_split = p.nk;
   }
-  p.tiles_m = (int)ceil_div(g.M, kB);
-  p.tiles_n = (int)ceil_div(g.N, kB);
+  // (SDD on large tiles lists a row pair's column blocks)
+  p.big = q.big && !(mode == kFp8Sdd && (!g.sb_square || ceil_div(g.N, kB) > kMaxList));
+  p.tiles_m = (int)ceil_div(g.M, p.big ? 2 * kB : kB);
+  p.tiles_n = (int)ceil_div(g.N, p.big ? 2 * kB : kB);
   return SD_OK;
 }
 
@@ -426,7 +593,7 @@ int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStre
   if (int rc = make_args(gx, kFp8Sdd, x)) return rc;
   if (int rc = make_args(gw, kFp8Dsd, w)) return rc;
   const int64_t blocks = blocks_of(x) + blocks_of(w);
-  if (!gx.sb_square || gw.sb_square || blocks > kPairBlocks) {
+  if (!gx.sb_square || gw.sb_square || x.big || w.big || blocks > kPairBlocks) {
     if (int rc = launch_fp8_gemm(gx, kFp8Sdd, dtype, stream)) return rc;
     return launch_fp8_gemm(gw, kFp8Dsd, dtype, stream);
   }

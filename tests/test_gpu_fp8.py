@@ -241,7 +241,9 @@ def whole(rows, cols, seed, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-@pytest.mark.parametrize("m,k,n", SHAPES + [(700, 900, 1100), (2600, 1300, 400), (257, 4000, 513)])
+@pytest.mark.parametrize("m,k,n", SHAPES + [(700, 900, 1100), (2600, 1300, 400), (257, 4000, 513),
+                                                       # 256 x 256 tiles for the forward, the input gradient and the weight gradient
+                                                       (4001, 299, 4195), (3970, 4195, 299), (299, 4195, 4001), (4096, 4224, 128)])
 @pytest.mark.parametrize("bs,p", [(128, 0.0), (128, 0.5), (256, 0.5), (384, 0.5)])
 def test_whole_numbers_come_out_exactly(m, k, n, bs, p, dtype):
     dt = DT[dtype]
