@@ -205,10 +205,10 @@ __device__ inline uint32_t encode(double x, uint32_t byte, uint32_t random) {
 
 template <typename T, int BITS>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
-  const uint32_t t = (uint32_t)(*reinterpret_cast<const volatile uint32_t*>(a.step)) + 1u;
-  const double lr = a.lr_at ? (double)*a.lr_at : a.lr;
-  const float by = (float)(lr / (1.0 - power(a.beta1, t))), root = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
-  const float keep = (float)(1.0 - lr * a.decay), eps = (float)a.eps;
+  const uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)*reinterpret_cast<const volatile uint32_t*>(a.step)) + 1u;
+  float by = 0.f, root = 0.f, keep = 0.f;
+  const float eps = (float)a.eps;
+  bool known = false;
   const uint32_t chunks = a.first[a.n];
   int which = 0;
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
@@ -220,10 +220,20 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
     float p[kPer], g[kPer];
     load_typed<T>(x.p, at, left, p);
     load_typed<T>(x.g, at, left, g);
+    // the step's factors, worked out while the first loads are on their way
+    auto factors = [&] {
+      if (known) return;
+      const double lr = a.lr_at ? (double)*a.lr_at : a.lr;
+      by = (float)(lr / (1.0 - power(a.beta1, t)));
+      root = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
+      keep = (float)(1.0 - lr * a.decay);
+      known = true;
+    };
     if constexpr (BITS == 32) {
       float m[kPer], v[kPer];
       load_run<float>(static_cast<const float*>(x.m) + at, left, m);
       load_run<float>(static_cast<const float*>(x.v) + at, left, v);
+      factors();
       const float b1 = (float)a.beta1, c1 = (float)(1.0 - a.beta1), b2 = (float)a.beta2, c2 = (float)(1.0 - a.beta2);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -238,6 +248,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
       uint8_t *const mc = static_cast<uint8_t*>(x.m) + at, *const vc = static_cast<uint8_t*>(x.v) + at;
       u32x2 mw = load_codes(mc, left), vw = load_codes(vc, left);
       const float ms = fp8_power(left ? x.ms[block] : 127u), vs = fp8_power(left ? x.vs[block] : 127u);
+      factors();
       double m[kPer], v[kPer];
       uint32_t m_most = 0, v_most = 0;
 #pragma unroll
@@ -298,22 +309,37 @@ struct ValueTable {
 };
 static_assert(sizeof(ValueTable) <= 4096, "a launch's arguments");
 
-// averages in 8 bits -> their values in 32
+// averages in 8 bits -> their values in 32, four a thread at a time so that a wave's stores are whole lines.  Bound by what it writes.
 __global__ __launch_bounds__(kThreads) void state_values_kernel(ValueTable a) {
   const uint32_t chunks = a.first[a.n];
   int which = 0;
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     while (chunk >= a.first[which + 1]) ++which;
     const ValueTensor& x = a.tensor[which];
-    const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + threadIdx.x * kPer, rest = x.n - at;
-    if (rest <= 0) continue;
-    const int left = rest > kPer ? kPer : (int)rest;
-    const u32x2 w = load_codes(x.codes + at, left);
-    const float s = fp8_power(x.scales[at / 128]);
-    float v[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = (x.second ? Second::decode(w, i) : First::decode(w, i)) * s;
-    store_typed<F32>(x.out, at, left, v);
+    for (int h = 0; h < kPer / 4; ++h) {
+      const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + (h * kThreads + threadIdx.x) * 4, rest = x.n - at;
+      if (rest <= 0) continue;
+      const float s = fp8_power(x.scales[at / 128]);
+      u32x2 w = {0u, 0u};
+      if (rest >= 4) {
+        typedef uint32_t __attribute__((aligned(1))) u32_any;
+        w[0] = *reinterpret_cast<const u32_any*>(x.codes + at);
+      } else {
+        for (int i = 0; i < rest; ++i) w[0] |= (uint32_t)x.codes[at + i] << (8 * i);
+      }
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (x.second ? Second::decode(w, i) : First::decode(w, i)) * s;
+      if (rest >= 4) {
+        typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+        *reinterpret_cast<f32x4_any*>(x.out + at) = f32x4{v[0], v[1], v[2], v[3]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (i < rest) x.out[at + i] = v[i];
+      }
+    }
   }
 }
 

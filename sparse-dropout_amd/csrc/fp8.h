@@ -59,6 +59,7 @@ struct Fp8Gemm {
   const uint8_t* mask;  // null: nothing is dropped; else bytes, one to `split` x `split` blocks of 128
   int64_t msr, msc;
   int32_t split;
+  float keep;        // expected fraction of blocks kept: picks the kernel
   float* part;       // fp32 scratch for a split reduction: [splits][M][N] in C's element order
   int64_t part_bytes;
 };

@@ -114,6 +114,7 @@ Fp8Gemm product(const Packed& a, void* pa, const Packed& b, void* pb, void* c, i
   g.K = K;
   g.scale = scale;
   g.split = 1;
+  g.keep = 1.f;
   g.part = static_cast<float*>(part);
   g.part_bytes = part_bytes;
   return g;
@@ -212,6 +213,7 @@ int sd_fp8_gemm(const void* A, int64_t lda, const uint8_t* SA, int64_t sa_ld, co
   g.K = K;
   g.scale = 1.f;
   g.split = 1;
+  g.keep = 1.f;
   g.part = ws_ok ? static_cast<float*>(workspace) : nullptr;
   g.part_bytes = ws_ok ? workspace_bytes : 0;
   return launch_fp8_gemm(g, kFp8Dense, dtype, (hipStream_t)stream);
@@ -351,6 +353,7 @@ int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dysr, int64_t dysc, c
   gw.msr = msc;
   gw.msc = msr;
   gx.split = gw.split = (int32_t)(bs / kFp8Block);
+  gx.keep = gw.keep = (float)(1.0 - p);
   if (dX && dW) return launch_fp8_backward(gx, gw, dtype, (hipStream_t)stream);
   return dX ? launch_fp8_gemm(gx, kFp8Sdd, dtype, (hipStream_t)stream) : launch_fp8_gemm(gw, kFp8Dsd, dtype, (hipStream_t)stream);
 }

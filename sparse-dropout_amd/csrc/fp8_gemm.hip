@@ -21,6 +21,7 @@ constexpr int kB = kFp8Block;
 constexpr int kBlockBytes = kB * kB;  // of one 128 x 128 block of codes
 constexpr int kLdsLimit = 160 * 1024;
 constexpr int kCus = 256;
+constexpr float kDuoKeep = 0.55f;  // SDD: fraction of blocks kept up to which 128 x 256 tiles of kept blocks are faster than 256 x 256 ones
 constexpr int64_t kPairBlocks = 1024;  // workgroups of both gradients up to which they share a launch
 constexpr int kMaxList = 4096;        // 128-blocks that a workgroup's list can hold
 
@@ -108,7 +109,7 @@ struct Args {
   Fp8Gemm g;
   int32_t nk, per_split;  // 128-blocks of the reduction, of one part of it
   int32_t tiles_m, tiles_n, splits;
-  bool big;  // tiles of 256 x 256 instead of 128 x 128
+  bool big, duo;  // tiles of 256 x 256, of 128 x 256 (SDD) instead of 128 x 128
 };
 
 __device__ inline bool dropped(const Fp8Gemm& g, int i, int j) {
@@ -443,6 +444,115 @@ __global__ __launch_bounds__(512, 2) void fp8_big_kernel(Args p) {
   for (int h = 0; h < 2; ++h) store_patch<T>(g, m0 + grp * kB + h * 64, n_out, acc[h], out_part, lane);
 }
 
+// ---- 128 x 256 tiles of C's kept blocks ------------------------------------------------------------------------------------------
+// SDD where much is dropped: a workgroup takes two kept column blocks of one row block, so none of its work is for blocks that
+// are dropped.  Eight waves of 128 x 64 in two groups of four that take the steps in turn, so that each has half of the reduction; waves w
+// and w + 4, one of either group, share a SIMD.  A phase is a step: while one group reads the step's fragments into registers (and
+// puts the blocks of the step after next on their way into the third stage), the other's matrix instructions run from theirs.  At the end the
+// groups swap halves of their sums through LDS, add and store a half each.
+// dX of 8192^3 at p = 0.5: 321 us, 371 on 256 x 256 tiles; it loads 48 KB for two blocks of C a step, those 64 for up to four.
+// (DSD in this shape, whose row blocks walk the reduction apart from each other and meet in the L2 less: 431 us, 310 on 256 x 256.)
+constexpr int kDuoStage = 3 * kBlockBytes;        // A's block, B's two
+constexpr int kDuoScales = 3 * kDuoStage;         // then 256 bytes of A's scales and 256 of B's for each stage
+constexpr int kDuoList = kDuoScales + 3 * 512;
+constexpr int kDuoMaxList = 2048;
+constexpr int duo_lds(int list) { return kDuoList + list * 5 + 16; }
+static_assert(duo_lds(kDuoMaxList) <= kLdsLimit && 8 * 16 * 1024 <= kDuoScales, "LDS");
+
+template <typename T>
+__global__ __launch_bounds__(512, 2) void fp8_duo_kernel(Args p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Fp8Gemm& g = p.g;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = wave >> 2, c = wave & 3;
+  int tm, tn;
+  tile_of_block<DSD_GROUP_M>((int)blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  uint32_t* const list = reinterpret_cast<uint32_t*>(smem + kDuoList);
+  const int col_blocks = (int)((g.N + kB - 1) / kB), steps_all = p.nk;
+  make_list<512, true>(0, col_blocks, list, reinterpret_cast<uint8_t*>(list + col_blocks), reinterpret_cast<int*>(smem), [&](int j) { return dropped(g, tm, j) ? 0u : 1u; });
+  const uint32_t e0 = list[2 * tn], e1 = 2 * tn + 1 < col_blocks ? list[2 * tn + 1] : (uint32_t)col_blocks;
+  const uint32_t tiles = uniform(e0 >> 16 | e1 >> 16 << 1);  // which of the two are kept
+  const int steps = tiles ? steps_all : 0;
+  const int64_t m0 = (int64_t)tm * kB, c0 = (int64_t)uniform(e0 & 0xffffu) * kB, c1 = (int64_t)uniform(e1 & 0xffffu) * kB;
+  const int64_t n_mine = c < 2 ? c0 : c1;
+  __syncthreads();  // (the count lies where the first stage goes)
+  // a wave loads a quarter of A's block and half of its column block
+  const BlockRows rows_a(g.lda, lane), rows_b(g.ldb, lane);
+  const u32x4 of_a = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_b = block_buffer(g.b + n_mine * g.ldb, g.ldb, g.N - n_mine);
+  const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
+  const u32x4 bb = buffer_over(g.sb, (int64_t)(col_blocks - 1) * g.sb_r + (int64_t)(p.nk - 1) * g.sb_k + 1);
+  const uint32_t square_at = (uint32_t)((lane < 32 ? c0 : c1) / kB * g.sb_r);
+  const uint32_t lds = lds_address(smem);
+  const bool works = (tiles >> (c / 2) & 1u) != 0u;
+  auto load = [&](int k, int stage) {
+    const uint32_t at = lds + (uint32_t)stage * kDuoStage, scales = lds + kDuoScales + (uint32_t)stage * 512;
+    if (works) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rows_b.load(of_b, 8 * (c & 1) + q, k, at + (1 + c / 2) * kBlockBytes);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rows_a.load(of_a, 4 * c + q, k, at);
+    if (c == 0) buffer4_to_lds(ba, (uint32_t)((int64_t)k * g.sa_ld) + (lane & 31) * 4, scales);
+    if (c == 1) buffer1_to_lds(bb, square_at + (uint32_t)((int64_t)k * g.sb_k), scales + 256);
+  };
+
+  f32x4 acc[2][4][4] = {};
+  if (steps > 0) {
+    if (grp < steps) load(grp, grp);
+    wait_loads();
+    barrier();
+    if (grp == 1) barrier();
+    int stage = grp;
+    for (int s = grp; s < steps; s += 2) {
+      // memory phase; the stage after next, which is the one before this, is free
+      const int to = stage == 0 ? 2 : stage - 1;
+      if (s + 2 < steps) load(s + 2, to);
+      i32x8 fa[8], fb[4];
+      int sa[2], sb;
+      const char* st = smem + stage * kDuoStage;
+      const char* scales = smem + kDuoScales + stage * 512;
+      sa[0] = *reinterpret_cast<const int*>(scales + 4 * (lane & 15));
+      sa[1] = *reinterpret_cast<const int*>(scales + 64 + 4 * (lane & 15));
+      sb = *reinterpret_cast<const int*>(scales + 256 + 128 * (c / 2)) * 0x01010101;
+      if (works) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fb[j] = read_fragment(st + (1 + c / 2) * kBlockBytes + (c & 1) * 64 * kB, j, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fa[i] = read_fragment(st + (i / 4) * 64 * kB, i & 3, lane);
+      }
+      wait_reads();
+      barrier();
+      // compute phase
+      if (works) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[h][i][j] = mfma(fa[4 * h + i], fb[j], acc[h][i][j], sa[h], i, sb, j);
+        __builtin_amdgcn_s_setprio(0);
+      }
+      stage = to;
+      wait_loads();
+      if (s + 1 < steps) barrier();
+    }
+    // group 0 gives away the sums of the second 64 rows, group 1 those of the first
+    barrier();
+    f32x4* const mine = reinterpret_cast<f32x4*>(smem) + wave * 16 * 64;
+    const f32x4* const other = reinterpret_cast<const f32x4*>(smem) + (wave ^ 4) * 16 * 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine[(4 * i + j) * 64 + lane] = grp ? acc[0][i][j] : acc[1][i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[0][i][j] = (grp ? acc[1][i][j] : acc[0][i][j]) + other[(4 * i + j) * 64 + lane];
+  }
+  store_patch<T>(g, m0 + grp * 64, n_mine + (c & 1) * 64, acc[0], nullptr, lane);
+}
+
 // C = scale * sum of the parts, in their order
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8Gemm g, int splits) {
@@ -479,6 +589,10 @@ int configure(const void* kernel, std::atomic<bool>* done) {
   return SD_OK;
 }
 
+// How a product is cut up.  256 x 256 tiles where they fill the chip; else 128 x 128 ones, and where there are few of them and the
+// reduction is long, that is cut into parts.  A part costs its fp32 sums, written and read once, and one more launch; what it saves are
+// steps, a microsecond each with two workgroups on a CU and 0.7 with one (128 x 32768 at 256 .. 2048: 6.5, 9.1, 11.9, 17.6 us).
+// 200 x 8192 over 2048 in two parts 19.4 us, in one 15.
 struct Plan {
   bool big;
   int splits, per_split;
@@ -488,7 +602,16 @@ Plan plan(int64_t M, int64_t N, int64_t K, int mode) {
   const bool big = big_tiles >= kCus;
   int64_t splits = 1;
   if (mode != kFp8Sdd && !big) {
-    while (tiles * splits < 256 && nk / (splits * 2) >= 4) splits *= 2;
+    double least = 1e30;
+    for (int64_t s = 1; s <= 16 && (s == 1 || nk / s >= 2); ++s) {
+      const int64_t steps = ceil_div(nk, s), wgs = tiles * ceil_div(nk, steps);
+      const double us = wgs <= kCus ? 0.7 * steps : (double)ceil_div(wgs, 2 * kCus) * (1.0 * steps + 3.0);
+      const double sum = s == 1 ? 0.0 : 4.0 + 8e-6 / 4.0 * (double)(ceil_div(nk, steps) * M * N);
+      if (us + sum < least) {
+        least = us + sum;
+        splits = s;
+      }
+    }
   }
   if (mode == kFp8Dsd && ceil_div(nk, splits) > kMaxList) splits = ceil_div(nk, kMaxList);
   const int64_t per = ceil_div(nk, splits > 0 ? splits : 1);
@@ -528,8 +651,19 @@ int launch_big(const Args& p, hipStream_t stream) {
   return check_launch("fp8_gemm");
 }
 
+template <typename T>
+int launch_duo(const Args& p, hipStream_t stream) {
+  auto* kernel = &fp8_duo_kernel<T>;
+  static std::atomic<bool> configured[16] = {};
+  if (int rc = configure(reinterpret_cast<const void*>(kernel), configured)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks_of(p)), dim3(512), duo_lds((int)ceil_div(p.g.N, kB)), stream, p);
+  note_kernel("fp8:duo");
+  return check_launch("fp8_gemm");
+}
+
 template <typename T, int MODE>
 int launch(const Args& p, hipStream_t stream) {
+  if (p.duo) return launch_duo<T>(p, stream);
   if (p.big) {
     if (int rc = launch_big<T, MODE>(p, stream)) return rc;
     return launch_sum<T>(p, stream);
@@ -563,8 +697,10 @@ int make_args(const Fp8Gemm& g, int mode, Args& p) {
   }
   // (SDD on large tiles lists a row pair's column blocks)
   p.big = q.big && !(mode == kFp8Sdd && (!g.sb_square || ceil_div(g.N, kB) > kMaxList));
+  p.duo = p.big && mode == kFp8Sdd && g.keep <= kDuoKeep && ceil_div(g.N, kB) <= kDuoMaxList;
+  if (p.duo) p.big = false;
   p.tiles_m = (int)ceil_div(g.M, p.big ? 2 * kB : kB);
-  p.tiles_n = (int)ceil_div(g.N, p.big ? 2 * kB : kB);
+  p.tiles_n = (int)ceil_div(g.N, p.big || p.duo ? 2 * kB : kB);
   return SD_OK;
 }
 
@@ -593,7 +729,7 @@ int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStre
   if (int rc = make_args(gx, kFp8Sdd, x)) return rc;
   if (int rc = make_args(gw, kFp8Dsd, w)) return rc;
   const int64_t blocks = blocks_of(x) + blocks_of(w);
-  if (!gx.sb_square || gw.sb_square || x.big || w.big || blocks > kPairBlocks) {
+  if (!gx.sb_square || gw.sb_square || x.big || w.big || x.duo || w.duo || blocks > kPairBlocks) {
     if (int rc = launch_fp8_gemm(gx, kFp8Sdd, dtype, stream)) return rc;
     return launch_fp8_gemm(gw, kFp8Dsd, dtype, stream);
   }
