@@ -620,7 +620,7 @@ int sd_conv2d_taps_dw(const void* x_rows, int64_t x_ld, const void* dy_rows, int
  * sd_fp8_quantize / sd_fp8_dequantize: one matrix (f16, bf16 or f32; block_rows 1 or 128) to codes and scales and back.
  * sd_fp8_gemm: C = A . B^T of two of them, fp32 sums, rounded once to dtype (f16 or bf16); workspace optional (a split reduction).
  * sd_fp8_linear: Y = X . W^T for X in 16 bits, which is quantized in 1 x 128 blocks, and weights in 128 x 128 blocks.
- *   At most 16 rows run in one launch that reads each weight once and needs no workspace.
+ *   Few rows (16, and up to 64 where N K is not large) run in one launch that reads each weight once and needs no workspace.
  * sd_fp8_dropout_matmul_forward: Y = s (keep (.) X) W^T with X in 1 x 128 and W in 128 x 128 blocks; mask given, or drawn as
  *   sd_random_lists draws it and stored to mask_out [ceil(M/bs), ceil(K/bs)].  Dropped blocks are neither quantized nor multiplied.
  *   XT (a [K, M] matrix) and WT (a square [K, N] one), each NULL where its gradient is not wanted, receive what the backward reads: X in blocks along the tokens,

@@ -20,10 +20,10 @@
 namespace sd {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWide = 1024;  // of a workgroup, few and many
 constexpr int kTensors = 56;
 constexpr int kPer = 8;                    // elements of a thread at a time
-constexpr int kChunk = kThreads * kPer;    // of a workgroup: whole 128-blocks
+constexpr int kChunk = kThreads * kPer;    // what the tables count in: whole 128-blocks
 
 struct AdamTensor {
   void* p;
@@ -67,6 +67,13 @@ __device__ inline double power(double base, uint32_t t) {
     base *= base;
   }
   return r;
+}
+
+// a wa + b wb, each product and the sum rounded by itself, as elementary operations round them (see encode_border)
+__device__ inline double weighted(double a, double wa, double b, double wb) {
+#pragma clang fp contract(off)
+  const double x = a * wa, y = b * wb;
+  return x + y;
 }
 
 // M. O'Neill's permuted congruential generator, 32 bits, output function RXS-M-XS, one step behind x
@@ -189,32 +196,58 @@ __device__ inline uint32_t scale_byte(uint32_t word) {
   const int e = (int)(word >> 20) - 1023 - Format::top + ((word & 0xfffffu) > Format::limit20 ? 1 : 0) + 127;
   return word == 0u ? 127u : (uint32_t)(e < 0 ? 0 : e);
 }
-// |x| / 2^(byte - 127) rounded down after random / 2^16 of the distance to the next number was added
+// Where |x| and the random bits make a border but for the last few of 64 bits, the code is what the formula gives in torch, step by step:
+// torch.ldexp multiplies by pow(2, k), which for some k is an ulp below 2^k on this hardware.  (Weights like 0.9 and 0.1 make such sums of
+// one element in 10^7, where 9 m + g is a multiple of ten of its last places; equal formulas have equal states with this.)
 template <typename Format>
-__device__ inline uint32_t encode(double x, uint32_t byte, uint32_t random) {
+__device__ inline uint32_t encode_border(double x, uint32_t byte, uint32_t random, const double* powers) {
+#pragma clang fp contract(off)
+  const double y = fabs(x) * powers[254u - byte];
+  const int exponent = (int)((uint32_t)(__builtin_bit_cast(uint64_t, y) >> 52) & 0x7ffu) - 1023, at = max(exponent, Format::least);
+  const double steps = y * powers[127 + 3 - at], up = (double)random * 0x1p-16;
+  return (uint32_t)(steps + up) + (at > Format::least ? (uint32_t)(at + Format::bias - 1) * 8u : 0u);
+}
+// |x| / 2^(byte - 127) rounded down after random / 2^16 of the distance to the next number was added.  powers[127 + k]: pow(2, k)
+template <typename Format>
+__device__ inline uint32_t encode(double x, uint32_t byte, uint32_t random, const double* powers) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint32_t hi = (uint32_t)(b >> 32) & 0x7fffffffu;
-  if (hi >= (1023u + 128u) << 20) return hi > 0x7ff00000u || (hi == 0x7ff00000u && (uint32_t)b) ? Format::nan : Format::infinite;
+  const uint32_t hi = (uint32_t)(b >> 32) & 0x7fffffffu, lo = (uint32_t)b;
+  if (hi >= (1023u + 128u) << 20) return hi > 0x7ff00000u || (hi == 0x7ff00000u && lo) ? Format::nan : Format::infinite;
   const int scaled = (int)hi - (((int)byte - 127) << 20);
   const int exponent = (scaled >> 20) - 1023;
-  if (exponent >= Format::least) return (((uint32_t)scaled + (random << 1)) >> 17) - ((1023u - Format::bias) << 3);
+  if (exponent >= Format::least) {
+    const uint32_t sum = (uint32_t)scaled + (random << 1), near = lo + 8u;
+    if (near < 16u && ((sum + (near < 8u ? 1u : 0u)) & 0x1ffffu) == 0u) return encode_border<Format>(x, byte, random, powers);
+    return (sum >> 17) - ((1023u - Format::bias) << 3);
+  }
   // below the least normal number: whole steps of 2^(least - 3), and 2^16 parts of one
   const double parts = __builtin_ldexp(fabs(x), 19 - Format::least - ((int)byte - 127));
-  return ((uint32_t)parts + random) >> 16;
+  const uint32_t whole = (uint32_t)parts;
+  const double rest = parts - (double)whole;
+  if ((hi | lo) && (rest < 0x1p-28 || rest > 1.0 - 0x1p-28)) return encode_border<Format>(x, byte, random, powers);
+  return (whole + random) >> 16;
 }
 
-template <typename T, int BITS>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
-  const uint32_t t = (uint32_t)__builtin_amdgcn_readfirstlane((int)*reinterpret_cast<const volatile uint32_t*>(a.step)) + 1u;
+template <typename T, int BITS, int THREADS>
+__global__ __launch_bounds__(THREADS) void adamw_kernel(AdamTable a) {
+  constexpr int PART = THREADS / kThreads;  // chunks that a workgroup takes at a time
+  const int part = PART == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / kThreads), lane = (int)threadIdx.x % kThreads;
+  __shared__ double powers[BITS == 8 ? 256 : 1];
+  if constexpr (BITS == 8) {
+    if (threadIdx.x < 256) powers[threadIdx.x] = pow(2.0, (double)((int)threadIdx.x - 127));
+    __syncthreads();
+  }
   float by = 0.f, root = 0.f, keep = 0.f;
   const float eps = (float)a.eps;
   bool known = false;
+  uint32_t t = 0u, key = 0u;
   const uint32_t chunks = a.first[a.n];
   int which = 0;
-  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    while (chunk >= a.first[which + 1]) ++which;
+  // (with no elements at all one workgroup runs, to move the step on: through an empty piece of an empty tensor)
+  for (uint32_t chunk = blockIdx.x * PART + part; chunk < chunks || !known; chunk += gridDim.x * PART) {
+    while (chunk >= a.first[which + 1] && which + 1 < a.n) ++which;
     const AdamTensor& x = a.tensor[which];
-    const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + threadIdx.x * kPer;
+    const int64_t at = (int64_t)(chunk - a.first[which]) * kChunk + lane * kPer;
     const int64_t rest = x.n - at;
     const int left = rest < 0 ? 0 : rest > kPer ? kPer : (int)rest;
     float p[kPer], g[kPer];
@@ -223,10 +256,12 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
     // the step's factors, worked out while the first loads are on their way
     auto factors = [&] {
       if (known) return;
+      t = (uint32_t)__builtin_amdgcn_readfirstlane((int)*reinterpret_cast<const volatile uint32_t*>(a.step)) + 1u;
       const double lr = a.lr_at ? (double)*a.lr_at : a.lr;
       by = (float)(lr / (1.0 - power(a.beta1, t)));
       root = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));
       keep = (float)(1.0 - lr * a.decay);
+      key = t * 0x9E3779B1u;
       known = true;
     };
     if constexpr (BITS == 32) {
@@ -254,8 +289,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const double gd = (double)g[i];
-        m[i] = (double)(First::decode(mw, i) * ms) * a.beta1 + gd * (1.0 - a.beta1);
-        v[i] = (double)(Second::decode(vw, i) * vs) * a.beta2 + (gd * gd) * (1.0 - a.beta2);
+        m[i] = weighted((double)(First::decode(mw, i) * ms), a.beta1, gd, 1.0 - a.beta1);
+        v[i] = weighted((double)(Second::decode(vw, i) * vs), a.beta2, gd * gd, 1.0 - a.beta2);
         m_most = max(m_most, magnitude_word(m[i]));
         v_most = max(v_most, magnitude_word(v[i]));
         const float mf = (float)m[i], vf = (float)v[i];
@@ -263,14 +298,13 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
       }
       // sixteen lanes hold a block (those behind the tensor's end hold zeros)
       const uint32_t mb = scale_byte<First>(max_of_row16(m_most)), vb = scale_byte<Second>(max_of_row16(v_most));
-      const uint32_t key = t * 0x9E3779B1u + (uint32_t)at;
       mw = u32x2{0u, 0u};
       vw = u32x2{0u, 0u};
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const uint32_t random = mixed(key + i);
+        const uint32_t random = mixed(key + (uint32_t)at + i);
         const uint32_t sign = (uint32_t)(__builtin_bit_cast(uint64_t, m[i]) >> 56) & 0x80u;
-        const uint32_t mq = encode<First>(m[i], mb, random >> 16) | sign, vq = encode<Second>(v[i], vb, random & 0xffffu);
+        const uint32_t mq = encode<First>(m[i], mb, random >> 16, powers) | sign, vq = encode<Second>(v[i], vb, random & 0xffffu, powers);
         mw[i / 4] |= mq << (8 * (i % 4));
         vw[i / 4] |= vq << (8 * (i % 4));
       }
@@ -283,15 +317,14 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamTable a) {
     }
     store_typed<T>(x.p, at, left, p);
   }
-  // The step moves on when every workgroup has read it: the one that is done last writes it.  Its upper half counts them meanwhile.
+  // The step moves on when every workgroup is done with it: the last to report writes it.  Its upper half counts the reports meanwhile, 10 ns
+  // each, one at a time.  (Made at the start they hold up the others' reads of the step: 58 us for 1.9 M parameters, at the end 19.
+  // A launch that moves the step on takes 4 us.)
   if (a.last) {
     __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t* const arrivals = reinterpret_cast<uint32_t*>(a.step) + 1;
-      if (atomicAdd(arrivals, 1u) == gridDim.x - 1) {
-        *arrivals = 0u;
-        *reinterpret_cast<uint32_t*>(a.step) = t;
-      }
+    if (threadIdx.x == 0 && atomicAdd(reinterpret_cast<uint32_t*>(a.step) + 1, 1u) == gridDim.x - 1) {
+      *(reinterpret_cast<uint32_t*>(a.step) + 1) = 0u;
+      *reinterpret_cast<uint32_t*>(a.step) = t;
     }
   }
 }
@@ -346,6 +379,16 @@ __global__ __launch_bounds__(kThreads) void state_values_kernel(ValueTable a) {
 // workgroups: as many as are resident, each through several chunks
 unsigned grid_of(uint32_t chunks) { return chunks < 2048 ? chunks : 2048; }
 
+// Workgroups of 1024 threads where their number matters, for they report one after the other, and not where everything is done at once (too few
+// of them for all CUs) or goes on for long (5 % slower at 168 M parameters).
+template <typename T>
+void launch_table(const AdamTable& a, int bits, uint32_t chunks, hipStream_t stream) {
+  const bool wide = chunks > 512 && chunks <= 8192;
+  const dim3 grid(wide ? (chunks + 3) / 4 < 512 ? (chunks + 3) / 4 : 512 : chunks ? grid_of(chunks) : 1), block(wide ? kWide : kThreads);
+  if (bits == 8) hipLaunchKernelGGL((wide ? &adamw_kernel<T, 8, kWide> : &adamw_kernel<T, 8, kThreads>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((wide ? &adamw_kernel<T, 32, kWide> : &adamw_kernel<T, 32, kThreads>), grid, block, 0, stream, a);
+}
+
 }  // namespace
 
 int launch_adamw(int count, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* ms, uint8_t* const* vs,
@@ -359,8 +402,6 @@ int launch_adamw(int count, void* const* p, const void* const* g, void* const* m
   a.beta2 = beta2;
   a.eps = eps;
   a.decay = decay;
-  auto* kernel = bits == 8 ? (dtype == kF32 ? &adamw_kernel<F32, 8> : dtype == SD_BF16 ? &adamw_kernel<BF16, 8> : &adamw_kernel<F16, 8>)
-                           : (dtype == kF32 ? &adamw_kernel<F32, 32> : dtype == SD_BF16 ? &adamw_kernel<BF16, 32> : &adamw_kernel<F16, 32>);
   for (int i = 0; i < count || (i == 0 && moves_on);) {
     a.n = 0;
     a.first[0] = 0;
@@ -376,7 +417,10 @@ int launch_adamw(int count, void* const* p, const void* const* g, void* const* m
     if (i < count && a.n == 0) return fail(SD_ERR_UNSUPPORTED, "adamw_step: a tensor of %lld elements is too large", (long long)n[i]);
     a.last = moves_on && i == count ? 1 : 0;
     if (chunks == 0 && !a.last) break;
-    hipLaunchKernelGGL(kernel, dim3(chunks ? grid_of((uint32_t)chunks) : 1), dim3(kThreads), 0, stream, a);
+    if (chunks == 0) a.tensor[0] = AdamTensor{};
+    if (dtype == kF32) launch_table<F32>(a, bits, (uint32_t)chunks, stream);
+    else if (dtype == SD_BF16) launch_table<BF16>(a, bits, (uint32_t)chunks, stream);
+    else launch_table<F16>(a, bits, (uint32_t)chunks, stream);
     if (int rc = check_launch("adamw_step")) return rc;
     if (i == count) break;
   }

@@ -71,7 +71,8 @@ int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStre
 int64_t fp8_gemm_scratch(int64_t M, int64_t N, int64_t K, int mode);
 
 // y[m, n] for at most kFp8FewRows rows of x in 16 bits against weights in 8: x is quantized as it is read
-constexpr int kFp8FewRows = 16;
+constexpr int kFp8FewRows = 64;
+bool fp8_few_takes(int64_t M, int64_t N, int64_t K);
 struct Fp8Few {
   const uint16_t* x;
   int64_t ldx;

@@ -221,7 +221,7 @@ int sd_fp8_gemm(const void* A, int64_t lda, const uint8_t* SA, int64_t sa_ld, co
 
 int64_t sd_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 0 || M >= kMaxDim || N >= kMaxDim || K >= kMaxDim) return -1;
-  if (M <= kFp8FewRows) return 0;
+  if (fp8_few_takes(M, N, K)) return 0;
   return Packed(M, K, false).bytes + fp8_gemm_scratch(M, N, K, kFp8Dense);
 }
 
@@ -238,7 +238,7 @@ int sd_fp8_linear(const void* X, int64_t ldx, const void* W, int64_t ldw, const 
   SD_REQUIRE(swr >= 1 && swk >= 1, "fp8_linear: scales: strides must be positive");
   if (int rc = check_reach("fp8_linear", M, K)) return rc;
   if (ceil_div(K, kFp8Block) * swk >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8_linear: too many scales");
-  if (M <= kFp8FewRows) {
+  if (fp8_few_takes(M, N, K)) {
     const Fp8Few f = {static_cast<const uint16_t*>(X), ldx, static_cast<const uint8_t*>(W), ldw, SW, swr, swk, static_cast<uint16_t*>(Y), ldy,
                       (int32_t)M, (int32_t)N, (int32_t)K};
     return launch_fp8_few(f, dtype, (hipStream_t)stream);

@@ -1,9 +1,10 @@
-// y = x . W^T for at most 16 rows of x in 16 bits and weights in 8 bits (fp8.h): the product of serving a few tokens.
+// y = x . W^T for few rows of x in 16 bits and weights in 8 bits (fp8.h): the product of serving a few tokens.
 //
-// Bound by reading the weights, a byte each: nothing else is as large.  So they go from memory straight into the matrix instruction's
-// registers, every byte once, and x, which a launch before would have to bring into 8 bits, is quantized by each workgroup as it reads
-// it (16 rows of x are a few KB out of the L2 for every 128 columns, and the arithmetic hides behind the loads).  A workgroup owns 16
-// outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block w + waves * n, and meet once in LDS.
+// Bound by reading the weights, a byte each, as long as there are few rows.  So they go from memory straight into the matrix
+// instruction's registers, every byte once, and x, which a launch before would have to bring into 8 bits, is quantized by each workgroup as
+// it reads it out of the L2.  A workgroup owns 16 outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block
+// w + waves * n, a few of them on their way at a time, and meet once in LDS.  Rows come in groups of 16, up to four; what a row behind the
+// last or an output behind the last holds is never stored, so their lanes read another's.
 #include "fp8.h"
 
 namespace sd {
@@ -11,90 +12,171 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-template <typename T, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(Fp8Few g) {
-  __shared__ float sums[WAVES][16][17];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16, nk = (g.K + kFp8Block - 1) / kFp8Block;
-  const bool has_w = n0 + r < g.N, has_x = r < g.M;
-  const uint8_t* const w = g.w + (int64_t)(has_w ? n0 + r : 0) * g.ldw;
-  const uint16_t* const x = g.x + (int64_t)(has_x ? r : 0) * g.ldx;
-  const uint8_t* const sw = g.sw + (int64_t)(n0 / kFp8Block) * g.sw_r;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int k = wave; k < nk; k += WAVES) {
-    u32x4 wl = {0u, 0u, 0u, 0u}, wh = wl;
-    if (has_w) {
-      wl = *reinterpret_cast<const u32x4*>(w + (int64_t)k * kFp8Block + 16 * q);
-      wh = *reinterpret_cast<const u32x4*>(w + (int64_t)k * kFp8Block + 64 + 16 * q);
-    }
-    const int ws = sw[(int64_t)k * g.sw_k];
-    // this lane's 32 elements of row r, two to a word: 16 q .. + 15 and 64 + 16 q .. + 15 of the block
-    uint32_t v[16], size[16], most = 0u;
+// This lane's 32 elements of a row in one 128-block, two to a word: 16 q .. + 15 and 64 + 16 q .. + 15.
+struct RowPart {
+  uint32_t v[16];
+  __device__ inline void load(const uint16_t* at) {  // the block's first element plus 16 q
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const int c = k * kFp8Block + (h >> 1) * 64 + 16 * q + (h & 1) * 8, left = has_x ? g.K - c : 0;
-      if (left >= 8) {
-        const u32x4 e = *reinterpret_cast<const u32x4_any*>(x + c);
+      const u32x4 e = *reinterpret_cast<const u32x4_any*>(at + (h >> 1) * 64 + (h & 1) * 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * h + i] = e[i];
-      } else {
+      for (int i = 0; i < 4; ++i) v[4 * h + i] = e[i];
+    }
+  }
+  __device__ inline void load_some(const uint16_t* at, int left) {  // of the block, `left` elements behind `at` are there
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[4 * h + i] = (2 * i < left ? x[c + 2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)x[c + 2 * i + 1] << 16 : 0u);
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = (h >> 1) * 64 + (h & 1) * 8 + 2 * i;
+        v[4 * h + i] = (c < left ? at[c] : 0u) | (c + 1 < left ? (uint32_t)at[c + 1] << 16 : 0u);
       }
-    }
+  }
+  // as codes, with the scale's byte
+  template <typename T>
+  __device__ inline i32x8 codes(int& byte) const {
+    uint32_t most = 0u;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      size[i] = v[i] & 0x7fff7fffu;
-      most = pk_max(most, size[i]);
-    }
+    for (int i = 0; i < 16; ++i) most = pk_max(most, v[i] & 0x7fff7fffu);
     most = max(most & 0xffffu, most >> 16);
     if (most >= kInfinite<T>) {
       most = 0u;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const uint32_t lo = size[i] & 0xffffu, hi = size[i] >> 16;
+        const uint32_t lo = v[i] & 0x7fffu, hi = v[i] >> 16 & 0x7fffu;
         most = max(most, max(lo < kInfinite<T> ? lo : 0u, hi < kInfinite<T> ? hi : 0u));
       }
     }
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-    const uint32_t xs = fp8_scale_of(size_bits<T>(most));
-    i32x8 a, b;
+    const uint32_t s = fp8_scale_of(size_bits<T>(most));
+    byte = (int)s;
+    i32x8 a;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (int)codes_of<T, true>(codes_of<T, false>(0u, v[2 * i], xs), v[2 * i + 1], xs);
+    for (int i = 0; i < 8; ++i) a[i] = (int)codes_of<T, true>(codes_of<T, false>(0u, v[2 * i], s), v[2 * i + 1], s);
+    return a;
+  }
+};
+
+__device__ inline i32x8 load_weights(const uint8_t* at) {  // the block's first code plus 16 q
+  const u32x4 lo = *reinterpret_cast<const u32x4*>(at), hi = *reinterpret_cast<const u32x4*>(at + 64);
+  i32x8 b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      b[i] = (int)wl[i];
-      b[4 + i] = (int)wh[i];
+  for (int i = 0; i < 4; ++i) {
+    b[i] = (int)lo[i];
+    b[4 + i] = (int)hi[i];
+  }
+  return b;
+}
+
+// AHEAD: 128-blocks of a wave on their way together
+template <typename T, int WAVES, int GROUPS, int AHEAD>
+__global__ __launch_bounds__(WAVES * 64, AHEAD == 2 && GROUPS == 1 ? 8 : WAVES / 4) void fp8_few_kernel(Fp8Few g) {
+  __shared__ float sums[WAVES][16][17];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15, q = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16, whole = g.K / kFp8Block, left = g.K - whole * kFp8Block;
+  const uint8_t* const w = g.w + (int64_t)min(n0 + r, g.N - 1) * g.ldw + 16 * q;
+  const uint8_t* const sw = g.sw + (int64_t)(n0 / kFp8Block) * g.sw_r;
+  const uint16_t* x[GROUPS];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) x[i] = g.x + (int64_t)min(16 * i + r, g.M - 1) * g.ldx + 16 * q;
+  f32x4 acc[GROUPS] = {};
+  auto multiply = [&](const RowPart (&p)[GROUPS], const i32x8& b, int ws) {
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      int xs;
+      const i32x8 a = p[i].template codes<T>(xs);
+      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i], 0, 0, 0, xs, 0, ws);
     }
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, (int)xs, 0, ws);
+  };
+  for (int k0 = wave; k0 < whole; k0 += WAVES * AHEAD) {
+    RowPart p[AHEAD][GROUPS];
+    i32x8 b[AHEAD];
+    int ws[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t k = k0 + u * WAVES;
+      if (k < whole) {
+        b[u] = load_weights(w + k * kFp8Block);
+        ws[u] = sw[k * g.sw_k];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) p[u][i].load(x[i] + k * kFp8Block);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (k0 + u * WAVES < whole) multiply(p[u], b[u], ws[u]);
+  }
+  if (left && wave == whole % WAVES) {
+    RowPart p[GROUPS];
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) p[i].load_some(x[i] + (int64_t)whole * kFp8Block, left - 16 * q);
+    multiply(p, load_weights(w + (int64_t)whole * kFp8Block), sw[(int64_t)whole * g.sw_k]);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sums[wave][4 * q + i][r] = acc[i];
-  __syncthreads();
-  if (t < 256) {
-    const int m = t >> 4, n = t & 15;
-    if (m < g.M && n0 + n < g.N) {
-      float sum = 0.f;
+  for (int i = 0; i < GROUPS; ++i) {
+    if (i) __syncthreads();
 #pragma unroll
-      for (int i = 0; i < WAVES; ++i) sum += sums[i][m][n];
-      g.y[(int64_t)m * g.ldy + n0 + n] = T::from_float(sum);
+    for (int e = 0; e < 4; ++e) sums[wave][4 * q + e][r] = acc[i][e];
+    __syncthreads();
+    if (t < 256) {
+      const int row = t >> 4, n = t & 15, m = 16 * i + row;
+      if (m < g.M && n0 + n < g.N) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < WAVES; ++j) sum += sums[j][row][n];
+        g.y[(int64_t)m * g.ldy + n0 + n] = T::from_float(sum);
+      }
     }
+  }
+}
+
+struct FewPlan {
+  int groups;  // of 16 rows
+  bool wide;   // sixteen waves instead of four
+  bool many;   // more workgroups than CUs: two to a CU, with half of the registers
+  double us;
+};
+// Sixteen waves a workgroup where the reduction is long.  The time, from 7 layers between 512^2 and 8192^2 at 1 to 64 rows: 5 us, and for
+// each 128-block of a wave and group of rows 2.1 with sixteen waves (32 rows through 4096^2 12.8 us, 64 22.5), 1 with four (64
+// through 8192 x 2048 20).
+FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
+  FewPlan p;
+  const int64_t nk = ceil_div(K, kFp8Block), wgs = ceil_div(N, 16);
+  p.groups = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  p.wide = nk > 16;
+  p.many = wgs > 256;
+  const int waves = p.wide ? 16 : 4;
+  const double rounds = (double)(wgs * waves) / 4096.0;
+  p.us = 5.0 + (p.wide ? 2.1 : 1.0) * p.groups * (double)ceil_div(nk, waves) * (rounds > 1.0 ? rounds : 1.0);
+  return p;
+}
+
+template <typename T>
+void launch_few(const Fp8Few& g, const FewPlan& p, hipStream_t stream) {
+  const dim3 grid((unsigned)ceil_div(g.N, 16)), block(p.wide ? 1024 : 256);
+  if (p.groups == 1) {
+    auto* kernel = !p.wide ? &fp8_few_kernel<T, 4, 1, 4> : p.many ? &fp8_few_kernel<T, 16, 1, 2> : &fp8_few_kernel<T, 16, 1, 4>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);
+  } else if (p.groups == 2) {
+    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 2, 2> : &fp8_few_kernel<T, 4, 2, 2>), grid, block, 0, stream, g);
+  } else {
+    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 4, 1> : &fp8_few_kernel<T, 4, 4, 1>), grid, block, 0, stream, g);
   }
 }
 
 }  // namespace
 
+// Whether the kernel takes the product: up to 16 rows always; up to 64 where it is expected to take less than quantizing x and 128 x 128
+// tiles do, 15 to 20 us at such sizes.
+bool fp8_few_takes(int64_t M, int64_t N, int64_t K) { return M <= 16 || (M <= kFp8FewRows && few_plan(M, N, K).us <= 15.0); }
+
 int launch_fp8_few(const Fp8Few& g, int dtype, hipStream_t stream) {
   if (g.M == 0 || g.N == 0) return SD_OK;
-  const int nk = (int)ceil_div(g.K, kFp8Block);
-  const bool wide = nk > 16;
-  auto* kernel = dtype == SD_BF16 ? (wide ? &fp8_few_kernel<BF16, 16> : &fp8_few_kernel<BF16, 4>)
-                                  : (wide ? &fp8_few_kernel<F16, 16> : &fp8_few_kernel<F16, 4>);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(g.N, 16)), dim3(wide ? 1024 : 256), 0, stream, g);
-  note_kernel("fp8:few waves=%d", wide ? 16 : 4);
+  const FewPlan p = few_plan(g.M, g.N, g.K);
+  if (dtype == SD_BF16) launch_few<BF16>(g, p, stream);
+  else launch_few<F16>(g, p, stream);
+  note_kernel("fp8:few waves=%d groups=%d", p.wide ? 16 : 4, p.groups);
   return check_launch("fp8_few");
 }
 

@@ -15,6 +15,7 @@ namespace sd {
 namespace {
 
 constexpr int kThreads = 512;
+constexpr uint32_t kDrawingBlocks = 256;  // workgroups up to which they draw the mask themselves
 constexpr int kRows = 4;           // of a thread, by eight columns
 constexpr int kTurnPitch = 132;    // bytes of a column's codes in LDS: 33 words, so that a wave's words meet a bank twice at most
 
@@ -241,6 +242,14 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantJobs js) {
 }
 
 // codes and scales -> values, four to a thread.  Bound by what it writes.
+// A mask drawn by a launch of its own, four entries a thread.
+constexpr int kDrawThreads = 256;
+__global__ __launch_bounds__(kDrawThreads) void draw_mask_kernel(MaskSrc src, int64_t rows, uint8_t* out) {
+  src.resolve();
+  write_mask(src, rows, out, (int64_t)blockIdx.x * kDrawThreads + threadIdx.x, (int64_t)gridDim.x * kDrawThreads);
+  report_in(const_cast<uint64_t*>(src.state), gridDim.x);
+}
+
 constexpr int kOutThreads = 256;
 template <typename T>
 __global__ __launch_bounds__(kOutThreads) void dequantize_kernel(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k,
@@ -271,6 +280,18 @@ int launch_quantize(QuantJobs& js, int dtype, hipStream_t stream) {
     js.blocks += (uint32_t)(ceil_div(p.rows, kFp8Block) * p.tiles_c);
   }
   if (js.blocks == 0) return SD_OK;
+  // Workgroups that draw from the generator's state report one at a time, 10 ns each, so that the last can move it on: beyond some
+  // hundreds of them a launch that draws the mask before takes less.
+  if (js.mask_out && js.mask.state && js.blocks > kDrawingBlocks) {
+    const int64_t groups = ceil_div((int64_t)js.mask.mb * js.mask.kb, 4 * kDrawThreads);
+    hipLaunchKernelGGL(&draw_mask_kernel, dim3((unsigned)(groups < 64 ? groups : 64)), dim3(kDrawThreads), 0, stream, js.mask, (int64_t)js.mask.mb, js.mask_out);
+    if (int rc = check_launch("fp8_draw")) return rc;
+    js.mask.mask = js.mask_out;
+    js.mask.st_row = js.mask.kb;
+    js.mask.st_col = 1;
+    js.mask.state = nullptr;
+    js.mask_out = nullptr;
+  }
   auto* kernel = dtype == kF32 ? &quantize_kernel<F32> : dtype == SD_BF16 ? &quantize_kernel<BF16> : &quantize_kernel<F16>;
   hipLaunchKernelGGL(kernel, dim3(js.blocks), dim3(kThreads), 0, stream, js);
   return check_launch("fp8_quantize");

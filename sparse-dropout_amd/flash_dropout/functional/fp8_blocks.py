@@ -44,7 +44,7 @@ def fp8_dequantize(data: torch.Tensor, scales: torch.Tensor, cols: int | None = 
 @traceable
 def fp8_linear(input: torch.Tensor, data: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """``input @ W.T`` for weights kept in 8 bits: ``data``, ``scales = fp8_quantize(W, (128, 128))``.  ``input`` is [M, K] in float16 or
-    bfloat16 (under autocast: cast to its dtype) and is quantized by the call in (1, 128) blocks; so is the result.  Up to 16 rows run
+    bfloat16 (under autocast: cast to its dtype) and is quantized by the call in (1, 128) blocks; so is the result.  Few rows (16, and up to 64 of small layers) run
     in one launch that reads each weight once.  No gradient: the call is refused where one would be recorded."""
     return _loader.bridge().fp8_linear(input, data, scales)
 

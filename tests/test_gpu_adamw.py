@@ -167,6 +167,14 @@ def test_many_tensors_of_mixed_types_and_a_step_without_any():
         check_param(p[i], before[i], g[i], np.zeros(sizes[i]), np.zeros(sizes[i]), 1, DT[kinds[i]])
     F.adamw_step([], [], [], [], count, **HYPER)
     assert count.item() == 2
+    # a launch's table of tensors with elements, then only tensors without any
+    some = lambda std: [torch.full((5,), std, device="cuda") for _ in range(56)] + [torch.zeros(0, device="cuda") for _ in range(3)]
+    p, g, m, v = some(1.0), some(0.5), some(0.0), some(0.0)
+    count.zero_()
+    F.adamw_step(p, g, m, v, count, lr=0.25, weight_decay=0.0)
+    assert count.item() == 1
+    for t in p[:56]:  # one step of lr against a gradient of one sign
+        assert ((t - 0.75).abs() <= 32 * 2.0 ** -24).all()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -195,6 +203,33 @@ def test_large_tensor():
     want = -(g.double() / (g.double().abs() + 1e-8))  # (the corrected averages of one step are g and g^2)
     assert ((p.double() - want).abs() <= 24 * 2.0 ** -24).all()
     assert ((m.double() - 0.1 * g.double()).abs() <= 4 * 2.0 ** -24 * 0.1 * g.double().abs() + 2.0 ** -149).all()
+
+
+def test_averages_in_8_bits_next_to_a_random_border():
+    """0.9 m + 0.1 g is a multiple of the border's 2^-16 of a step, but for the last bits of 64, wherever 9 m + g is one of ten: either
+    neighbour is right there, and the code is the one that the formula gives in torch, whose ldexp multiplies by pow(2, k)."""
+    n = 128 * 4096
+    gen = torch.Generator().manual_seed(3)
+    m0 = torch.randint(8, 16, (n,), generator=gen).float() * torch.where(torch.rand(n, generator=gen) < 0.5, -1.0, 1.0)
+    g = torch.randint(-200, 200, (n,), generator=gen).float()
+    g = g + (-(9 * m0 + g)) % 5  # (9 m + g) / 10: a whole number of halves
+    m0[::128], g[::128] = 15.0, 5.0
+    m, v = codes_of(m0, "first"), codes_of(torch.zeros(n), "second")
+    assert np.array_equal(np64(F.adamw_state_values([m], [v])[0][0]), np64(m0))
+    F.adamw_step([torch.zeros(n, device="cuda")], [g.cuda()], [m], [v], torch.full((), 6, dtype=torch.int64, device="cuda"), betas=(0.9, 0.99))
+    got, x = np64(F.adamw_state_values([m], [v])[0][0]), 0.9 * np64(m0) + (1 - 0.9) * np64(g)
+    want = O.rounded_state(x, "first", 7)
+    scales = np.repeat(np.exp2(np64(m[1]) - 127), 128)
+    y = torch.from_numpy(np.abs(x)).cuda() * torch.ldexp(torch.ones(n, dtype=torch.float64, device="cuda"), 127 - m[1].int().repeat_interleave(128))
+    at = (torch.frexp(y)[1] - 1).clamp_min(-6)
+    in_torch = np64(torch.floor(torch.ldexp(y, 3 - at) + torch.from_numpy(O.dither(n, 7, "first")).cuda())) * np.exp2(np64(at) - 3) * scales
+    grid = np.exp2(np.floor(np.log2(np.maximum(np.abs(x) / scales, 2.0 ** -6))) - 3)
+    z = np.abs(x) / scales / grid + O.dither(n, 7, "first")
+    border = np.abs(z - np.rint(z)) < 2.0 ** -40
+    assert border.any() and not border.all()
+    assert np.array_equal(got[~border], want[~border])
+    assert np.array_equal(np.abs(got), in_torch)
+    assert (np.abs(got - want) <= grid * scales).all()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
