@@ -669,6 +669,7 @@ int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dy_stride_r, int64_t 
  * random bits are a function of t and the element's index.  Zeros are codes 0 with scales 127.
  * step: device memory; with `advance` the call moves it on when all is done (its upper half is scratch meanwhile), so a
  * captured graph counts its replays.  lr_at: a float in device memory that replaces lr, or NULL.
+ * eps is 0 or lies between 2^-126 and 2^120.
  * sd_adamw_state_values: averages in 8 bits (second[i]: the second one) as floats.
  * ------------------------------------------------------------------------------------------- */
 int sd_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,

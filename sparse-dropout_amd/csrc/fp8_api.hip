@@ -368,7 +368,7 @@ int sd_adamw_step(int count, void* const* params, const void* const* grads, void
   SD_REQUIRE(step != nullptr && reinterpret_cast<uintptr_t>(step) % 8 == 0, "adamw_step: step must be an aligned device pointer");
   SD_REQUIRE(lr_at != nullptr || (lr >= 0.0 && lr <= DBL_MAX), "adamw_step: lr must not be negative (got %g)", lr);
   SD_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: betas must be in [0, 1) (got %g, %g)", beta1, beta2);
-  SD_REQUIRE(eps >= 0.0, "adamw_step: eps must not be negative (got %g)", eps);
+  SD_REQUIRE(eps == 0.0 || (eps >= 0x1p-126 && eps <= 0x1p120), "adamw_step: eps must be 0 or from 2^-126 to 2^120 (got %g)", eps);
   SD_REQUIRE(weight_decay >= 0.0, "adamw_step: weight_decay must not be negative (got %g)", weight_decay);
   for (int i = 0; i < count; ++i) {
     SD_REQUIRE(numels[i] >= 0, "adamw_step: tensor %d: negative size", i);

@@ -22,8 +22,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"lr must not be negative (got {lr})")
         if not all(0 <= b < 1 for b in betas):
             raise ValueError(f"betas must be in [0, 1) (got {betas})")
-        if not eps >= 0 or not weight_decay >= 0:
-            raise ValueError(f"eps and weight_decay must not be negative (got {eps}, {weight_decay})")
+        if not (eps == 0 or 2.0 ** -126 <= eps <= 2.0 ** 120) or not weight_decay >= 0:
+            raise ValueError(f"eps must be 0 or from 2^-126 to 2^120 and weight_decay not negative (got {eps}, {weight_decay})")
         if state_bits not in (8, 32):
             raise ValueError(f"averages are held in 8 or in 32 bits (got {state_bits})")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
