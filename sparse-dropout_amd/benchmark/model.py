@@ -12,7 +12,10 @@ Models are built from ``DropoutMM`` the way the reference's evaluation models ar
            batch 32; eval/llm/model.py:58-66: 1024 -> 4096 -> GELU -> 1024) on its 32x128 = 4096 tokens
 Each is timed with variant "none" (dense), "vanilla" (element dropout + dense), "blockwise[hip]" and
 "blockwise[hip-fused]": the same layers as one autograd function whose GEMM stores apply the activation and
-its derivative (no activation kernels in either direction)."""
+its derivative (no activation kernels in either direction), and "blockwise[hip-fp8]": products of operands in 8 bits, on
+blocks of 128 (or --block-size, where that is a multiple of it).
+
+--optimizer adds an AdamW step with averages in 32 or 8 bits to what is timed."""
 from __future__ import annotations
 
 import argparse
@@ -24,6 +27,7 @@ from torch import nn
 
 import flash_dropout.functional as F
 from flash_dropout.layers import DropoutMM
+from flash_dropout.optim import AdamW
 
 from .utils import FLUSH_BYTES
 
@@ -103,14 +107,23 @@ MODELS = {
 }
 
 
-def time_model(model: nn.Module, x: torch.Tensor, warmup: float, rep: float, graph: bool = False) -> list[float]:
+OPTIMIZERS = {"none": None, "adamw": 32, "adamw-8bit": 8}  # bits of the averages
+
+
+def time_model(model: nn.Module, x: torch.Tensor, warmup: float, rep: float, graph: bool = False,
+               optimizer: torch.optim.Optimizer | None = None) -> list[float]:
     """fwd+bwd milliseconds per repetition, cache flushed before each (benchmark/model.py:119-142).
     With ``graph`` the step is captured once in a HIP graph and replayed: no Python or launch path in the
-    timed region (block-dropout masks still change from replay to replay, they are drawn from device state)."""
+    timed region (block-dropout masks still change from replay to replay, they are drawn from device state).
+    ``optimizer``: its step, from fresh gradients, belongs to the repetition."""
     cache = torch.empty(FLUSH_BYTES, dtype=torch.int8, device="cuda")
 
     def step():
+        if optimizer is not None:
+            optimizer.zero_grad(set_to_none=True)
         model(x).float().square().mean().backward()
+        if optimizer is not None:
+            optimizer.step()
 
     f = step
     if graph:
@@ -153,18 +166,22 @@ def main() -> None:
     ap.add_argument("--block-size", type=int, default=64)
     ap.add_argument("--rep", type=float, default=0.3, help="seconds of timed repetitions per point")
     ap.add_argument("--graph", action="store_true", help="capture the step in a HIP graph and time replays")
+    ap.add_argument("--optimizer", choices=list(OPTIMIZERS), default="none", help="AdamW step after the backward pass, by its averages' bits")
     args = ap.parse_args()
+    bits = OPTIMIZERS[args.optimizer]
     torch.manual_seed(0)
     for name in args.model:
         cls, make_x = MODELS[name]
         x = make_x().cuda().half()
-        print(f"=== {name}  input {tuple(x.shape)}  block_size {args.block_size}{'  (graph replay)' if args.graph else ''}")
+        print(f"=== {name}  input {tuple(x.shape)}  block_size {args.block_size}{'  (graph replay)' if args.graph else ''}"
+              f"{'' if bits is None else f'  with AdamW, averages in {bits} bits'}")
         for variant, ps in (("none", [0.0]), ("vanilla", [0.5]), ("blockwise[hip]", args.p),
-                            ("blockwise[hip-fused]", args.p)):
+                            ("blockwise[hip-fused]", args.p), ("blockwise[hip-fp8]", args.p)):
             for p in ps:
-                model = (fused_variant(name, p, args.block_size) if variant.endswith("fused]")
-                         else cls(variant, p, args.block_size)).cuda().half().train()
-                ts = time_model(model, x, warmup=0.2, rep=args.rep, graph=args.graph)
+                size = 128 if variant.endswith("fp8]") and args.block_size % 128 else args.block_size
+                model = (fused_variant(name, p, size) if variant.endswith("fused]") else cls(variant, p, size)).cuda().half().train()
+                optimizer = None if bits is None else AdamW(model.parameters(), lr=1e-4, state_bits=bits)
+                ts = time_model(model, x, warmup=0.2, rep=args.rep, graph=args.graph, optimizer=optimizer)
                 sem = statistics.stdev(ts) / len(ts) ** 0.5 if len(ts) > 1 else 0.0
                 print(f"{variant:<21} p={p:<4} median {statistics.median(ts):8.4f} ms  "
                       f"mean {statistics.mean(ts):8.4f} +- {1.96 * sem:.4f}  n={len(ts)}")

@@ -1,5 +1,6 @@
 """Single products on model shapes: forward (DSD), dX (SDD) and dW (DSD on transposed views) of a block-dropout linear
-layer at a few drop rates, beside ``torch.matmul`` on the same operands.  L2 flushed before every call, median of 20.
+layer at a few drop rates, beside ``torch.matmul`` on the same operands, and the forward product of operands in 8 bits: with
+both quantized before, and of an input that is quantized by the call, with kept weights.  L2 flushed before every call, median of 20.
 
     python -m benchmark.products                      # the shapes below
     python -m benchmark.products --shape 4096 1024 4096 --p 0 0.5
@@ -12,6 +13,7 @@ import argparse
 
 import torch
 
+import flash_dropout.functional as F
 from flash_dropout.hip import GEMM
 
 # tokens M, output features N, input features K
@@ -63,6 +65,9 @@ def main() -> None:
                                            lambda: torch.matmul(dy.t(), x))]
         print(f"{name:13s} M={M} N={N} K={K}   torch.matmul: forward {t[0]:.0f}  dX {t[1]:.0f}  dW {t[2]:.0f}  sum {sum(t):.0f} us",
               flush=True)
+        xq, wq = F.fp8_quantize(x), F.fp8_quantize(w, (128, 128))
+        t = [median_us(f, flush) for f in (lambda: F.fp8_quantize(x), lambda: ext.gemm_fp8(*xq, *wq, dtype), lambda: F.fp8_linear(x, *wq))]
+        print(f"   8 bits: quantize x {t[0]:.0f}  product {t[1]:.0f}  linear with kept weights {t[2]:.0f} us", flush=True)
         for p in args.p:
             mask = torch.rand(-(-M // 64), -(-K // 64), device="cuda", generator=gen) < p
             lists = ext.build_lists(mask)

@@ -63,8 +63,10 @@ int check_codes(const char* fn, const char* name, const void* data, int64_t ld, 
   SD_REQUIRE(rows == 0 || cols == 0 || (data != nullptr && scales != nullptr), "%s: %s: null pointer", fn, name);
   SD_REQUIRE(aligned16(data) && ld % 16 == 0, "%s: %s: codes must start on 16 bytes, rows too (pitch %lld)", fn, name, (long long)ld);
   SD_REQUIRE(ld >= up(cols, kFp8Block), "%s: %s: a pitch of %lld does not hold %lld columns in whole 128-blocks", fn, name, (long long)ld, (long long)cols);
-  SD_REQUIRE(ld <= kMaxPitch, "%s: %s: a pitch of %lld is too large", fn, name, (long long)ld);
   return SD_OK;
+}
+int check_pitch(const char* fn, int64_t ld) {
+  return ld <= kMaxPitch ? SD_OK : fail(SD_ERR_UNSUPPORTED, "%s: a pitch of %lld is too large (at most %lld)", fn, (long long)ld, (long long)kMaxPitch);
 }
 int check_dtype(const char* fn, int dtype) {
   SD_REQUIRE(dtype == SD_F16 || dtype == SD_BF16, "%s: dtype must be SD_F16 or SD_BF16 (got %d)", fn, dtype);
@@ -182,6 +184,7 @@ int sd_fp8_gemm(const void* A, int64_t lda, const uint8_t* SA, int64_t sa_ld, co
   SD_REQUIRE(b_block_rows == 1 || b_block_rows == kFp8Block, "fp8_gemm: B's blocks are of 1 x 128 or 128 x 128 (got %lld rows)", (long long)b_block_rows);
   if (int rc = check_codes("fp8_gemm", "A", A, lda, SA, M, K)) return rc;
   if (int rc = check_codes("fp8_gemm", "B", B, ldb, SB, N, K)) return rc;
+  if (int rc = check_pitch("fp8_gemm", lda > ldb ? lda : ldb)) return rc;
   if (int rc = check_matrix("fp8_gemm", "C", C, csr, csc, M, N)) return rc;
   if (M == 0 || N == 0) return SD_OK;
   SD_REQUIRE(K > 0, "fp8_gemm: empty reduction");
@@ -232,6 +235,7 @@ int sd_fp8_linear(const void* X, int64_t ldx, const void* W, int64_t ldw, const 
   if (int rc = check_dtype("fp8_linear", dtype)) return rc;
   if (int rc = check_matrix("fp8_linear", "X", X, ldx, 1, M, K)) return rc;
   if (int rc = check_codes("fp8_linear", "W", W, ldw, SW, N, K)) return rc;
+  if (int rc = check_pitch("fp8_linear", ldw)) return rc;
   if (int rc = check_matrix("fp8_linear", "Y", Y, ldy, 1, M, N)) return rc;
   if (M == 0 || N == 0) return SD_OK;
   SD_REQUIRE(K > 0, "fp8_linear: empty reduction");
@@ -370,6 +374,7 @@ int sd_adamw_step(int count, void* const* params, const void* const* grads, void
   SD_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: betas must be in [0, 1) (got %g, %g)", beta1, beta2);
   SD_REQUIRE(eps == 0.0 || (eps >= 0x1p-126 && eps <= 0x1p120), "adamw_step: eps must be 0 or from 2^-126 to 2^120 (got %g)", eps);
   SD_REQUIRE(weight_decay >= 0.0, "adamw_step: weight_decay must not be negative (got %g)", weight_decay);
+  SD_REQUIRE(count == 0 || (params && grads && exp_avgs && exp_avg_sqs && numels), "adamw_step: null array");
   for (int i = 0; i < count; ++i) {
     SD_REQUIRE(numels[i] >= 0, "adamw_step: tensor %d: negative size", i);
     if (numels[i] == 0) continue;
@@ -383,6 +388,7 @@ int sd_adamw_step(int count, void* const* params, const void* const* grads, void
 int sd_adamw_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* values, const int64_t* numels,
                           const int32_t* second, void* stream) {
   SD_REQUIRE(count >= 0, "adamw_state_values: negative count");
+  SD_REQUIRE(count == 0 || (codes && scales && values && numels && second), "adamw_state_values: null array");
   for (int i = 0; i < count; ++i) {
     SD_REQUIRE(numels[i] >= 0, "adamw_state_values: tensor %d: negative size", i);
     SD_REQUIRE(numels[i] == 0 || (codes[i] && scales[i] && values[i]), "adamw_state_values: tensor %d: null pointer", i);

@@ -241,7 +241,6 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantJobs js) {
   report_in(const_cast<uint64_t*>(js.mask.state), gridDim.x);
 }
 
-// codes and scales -> values, four to a thread.  Bound by what it writes.
 // A mask drawn by a launch of its own, four entries a thread.
 constexpr int kDrawThreads = 256;
 __global__ __launch_bounds__(kDrawThreads) void draw_mask_kernel(MaskSrc src, int64_t rows, uint8_t* out) {
@@ -250,35 +249,40 @@ __global__ __launch_bounds__(kDrawThreads) void draw_mask_kernel(MaskSrc src, in
   report_in(const_cast<uint64_t*>(src.state), gridDim.x);
 }
 
+// codes and scales -> values, four to a thread at a time.  Bound by what it writes.
 constexpr int kOutThreads = 256;
+constexpr int64_t kOutBlocks = 1 << 20;
 template <typename T>
 __global__ __launch_bounds__(kOutThreads) void dequantize_kernel(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k,
                                                               int square, int64_t rows, int64_t cols, uint32_t quads, void* out, int64_t out_ld) {
-  const int64_t at = (int64_t)blockIdx.x * kOutThreads + threadIdx.x, r = at / quads, c = (at - r * quads) * 4;
-  if (r >= rows) return;
-  const uint32_t q = *reinterpret_cast<const uint32_t*>(data + r * ld + c);
-  const float s = fp8_power(scales[(square ? r / kFp8Block : r) * s_r + c / kFp8Block * s_k]);
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
-  const float v[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+  for (int64_t at = (int64_t)blockIdx.x * kOutThreads + threadIdx.x; at < rows * quads; at += (int64_t)gridDim.x * kOutThreads) {
+    const int64_t r = at / quads, c = (at - r * quads) * 4;
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(data + r * ld + c);
+    const float s = fp8_power(scales[(square ? r / kFp8Block : r) * s_r + c / kFp8Block * s_k]);
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+    const float v[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (c + i >= cols) break;
-    if constexpr (T::id == kF32) static_cast<float*>(out)[r * out_ld + c + i] = v[i];
-    else static_cast<uint16_t*>(out)[r * out_ld + c + i] = T::from_float(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      if (c + i >= cols) break;
+      if constexpr (T::id == kF32) static_cast<float*>(out)[r * out_ld + c + i] = v[i];
+      else static_cast<uint16_t*>(out)[r * out_ld + c + i] = T::from_float(v[i]);
+    }
   }
 }
 
 }  // namespace
 
 int launch_quantize(QuantJobs& js, int dtype, hipStream_t stream) {
-  js.blocks = 0;
+  int64_t blocks = 0;
   for (int i = 0; i < js.n; ++i) {
     QuantJob& p = js.job[i];
     p.tiles_c = (uint32_t)ceil_div(p.cols, kFp8Block);
-    p.first_block = js.blocks;
-    js.blocks += (uint32_t)(ceil_div(p.rows, kFp8Block) * p.tiles_c);
+    p.first_block = (uint32_t)blocks;
+    blocks += ceil_div(p.rows, kFp8Block) * p.tiles_c;
+    if (blocks * kThreads >= (1LL << 32)) return fail(SD_ERR_UNSUPPORTED, "fp8_quantize: a %d x %d matrix is too large for one launch", p.rows, p.cols);
   }
+  js.blocks = (uint32_t)blocks;
   if (js.blocks == 0) return SD_OK;
   // Workgroups that draw from the generator's state report one at a time, 10 ns each, so that the last can move it on: beyond some
   // hundreds of them a launch that draws the mask before takes less.
@@ -299,9 +303,8 @@ int launch_quantize(QuantJobs& js, int dtype, hipStream_t stream) {
 
 int launch_dequantize(const uint8_t* data, int64_t ld, const uint8_t* scales, int64_t s_r, int64_t s_k, int square, int64_t rows,
                       int64_t cols, void* out, int64_t out_ld, int dtype, hipStream_t stream) {
-  const int64_t quads = ceil_div(cols, 4), blocks = ceil_div(rows * quads, kOutThreads);
+  const int64_t quads = ceil_div(cols, 4), all = ceil_div(rows * quads, kOutThreads), blocks = all < kOutBlocks ? all : kOutBlocks;
   if (blocks == 0) return SD_OK;
-  if (blocks >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8_dequantize: %lld x %lld is too large for one launch", (long long)rows, (long long)cols);
   auto* kernel = dtype == kF32 ? &dequantize_kernel<F32> : dtype == SD_BF16 ? &dequantize_kernel<BF16> : &dequantize_kernel<F16>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kOutThreads), 0, stream, data, ld, scales, s_r, s_k, square, rows, cols, (uint32_t)quads, out, out_ld);
   return check_launch("fp8_dequantize");

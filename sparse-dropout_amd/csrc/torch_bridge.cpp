@@ -1230,7 +1230,8 @@ struct Fp8Codes {
     TORCH_CHECK_VALUE(scales.size(1) == nk && (!square || scales.size(0) == ceil_div(rows, kFp8)), name, ": scales ", scales.sizes(),
                       " are not those of codes ", data.sizes());
     const bool rows_apart = rows <= 1 || (data.stride(0) >= data.size(1) && data.stride(0) % 16 == 0);
-    if (!(data.size(1) == 0 || data.stride(1) == 1) || !rows_apart || reinterpret_cast<uintptr_t>(data.data_ptr()) % 16) data = data.contiguous();
+    if (!(data.size(1) == 0 || data.stride(1) == 1) || !rows_apart || reinterpret_cast<uintptr_t>(data.data_ptr()) % 16)
+      data = data.clone(at::MemoryFormat::Contiguous);
   }
   const void* codes() const { return data.data_ptr(); }
   int64_t ld() const { return rows <= 1 ? data.size(1) : data.stride(0); }
@@ -1311,7 +1312,7 @@ Tensor fp8_gemm(const Tensor& a_, const Tensor& a_scales, const Tensor& b_, cons
 
 Tensor fp8_linear(const Tensor& input, const Tensor& data, const Tensor& scales) {
   TORCH_CHECK_VALUE(input.dim() == 2, "input must be [M, K] (got ", input.dim(), "D)");
-  TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && input.requires_grad()),
+  TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && (input.requires_grad() || data.requires_grad() || scales.requires_grad())),
                               "the product with kept 8-bit weights has no gradient: call it under torch.no_grad()");
   Tensor x = autocast(input);
   check_operand("input", x);

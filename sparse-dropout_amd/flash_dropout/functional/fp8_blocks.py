@@ -23,7 +23,7 @@ import torch
 from ..hip import _loader
 from ..hip.binding_gemm import _block_size
 from .blockwise_dropout_matmul_hip import draw_source
-from .tracing import traceable
+from .tracing import _RecordedPlainCall, traceable
 
 
 def fp8_quantize(x: torch.Tensor, block=(1, 128)) -> tuple[torch.Tensor, torch.Tensor]:
@@ -41,11 +41,11 @@ def fp8_dequantize(data: torch.Tensor, scales: torch.Tensor, cols: int | None = 
     return _loader.bridge().fp8_dequantize(data, scales, cols, dtype)
 
 
-@traceable
+@traceable(recorded=_RecordedPlainCall)
 def fp8_linear(input: torch.Tensor, data: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """``input @ W.T`` for weights kept in 8 bits: ``data``, ``scales = fp8_quantize(W, (128, 128))``.  ``input`` is [M, K] in float16 or
-    bfloat16 (under autocast: cast to its dtype) and is quantized by the call in (1, 128) blocks; so is the result.  Few rows (16, and up to 64 of small layers) run
-    in one launch that reads each weight once.  No gradient: the call is refused where one would be recorded."""
+    bfloat16 (under autocast: cast to its dtype), quantized by the call in (1, 128) blocks; the result has its dtype.  Few rows (16, and up
+    to 64 of small layers) run in one launch.  No gradient: the call is refused where one would be recorded."""
     return _loader.bridge().fp8_linear(input, data, scales)
 
 

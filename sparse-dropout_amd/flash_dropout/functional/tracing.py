@@ -52,8 +52,25 @@ class _RecordedCall(torch.autograd.Function):
         return (None, *(next(grads) if t.requires_grad else None for t in ctx.leaves))
 
 
-def traceable(function):
+class _RecordedPlainCall(torch.autograd.Function):
+    """Of a function without a gradient, which refuses inputs that want one: whether a trace's inputs do is only known when it is
+    differentiated."""
+
+    @staticmethod
+    def forward(ctx, call, *tensors):
+        with torch.autocast("cuda", enabled=False):
+            return call([t.detach() for t in tensors])
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("the traced function has no gradient: call it under torch.no_grad()")
+
+
+def traceable(function=None, *, recorded=_RecordedCall):
     """Makes a function of tensors that calls native code one recorded operation under ``torch.jit.trace``."""
+
+    if function is None:
+        return functools.partial(traceable, recorded=recorded)
 
     @functools.wraps(function)
     def run(*args, **kwargs):
@@ -63,12 +80,12 @@ def traceable(function):
         names, values = list(kwargs), _take([*args, *kwargs.values()], tensors)
         if torch.is_autocast_enabled("cuda"):  # the casts are the trace's own
             dtype = torch.get_autocast_dtype("cuda")
-            tensors = [t.to(dtype) if t.is_floating_point() else t for t in tensors]
+            tensors = [t.to(dtype) if t.is_floating_point() and t.element_size() > 1 else t for t in tensors]  # (8-bit codes stay)
 
         def call(given):
             filled = _put(values, given)
             return function(*filled[:len(args)], **dict(zip(names, filled[len(args):])))
 
-        return _RecordedCall.apply(call, *tensors)
+        return recorded.apply(call, *tensors)
 
     return run

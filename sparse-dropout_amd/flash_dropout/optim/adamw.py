@@ -15,7 +15,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  ``step`` of a parameter's state is an int64
     on the GPU, shared by the parameters that have been updated the same number of times; parameters without a gradient are left out
-    of a step, as torch's optimizers leave them out.  Parameters must be on the GPU, float16, bfloat16 or float32, and fill their memory."""
+    of a step, as torch's optimizers leave them out.  A step can be captured into a graph once one with the same gradients has been
+    taken.  Parameters must be on the GPU, float16, bfloat16 or float32, and fill their memory."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32) -> None:
         if not isinstance(lr, torch.Tensor) and not lr >= 0:
@@ -29,6 +30,8 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
     def _init_state(self, p: torch.Tensor, bits: int, step: torch.Tensor) -> None:
+        if bits not in (8, 32):
+            raise ValueError(f"averages are held in 8 or in 32 bits (got {bits})")
         state = self.state[p]
         state["step"] = step
         if bits == 8:
@@ -37,6 +40,12 @@ class AdamW(torch.optim.Optimizer):
         else:
             state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+
+    @staticmethod
+    def _not_captured(p: torch.Tensor, what: str) -> None:
+        # (a replay would do it again: averages back to zero, a count back to what it was)
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} cannot be captured into a graph: take a step with the same gradients before the capture")
 
     @staticmethod
     def _averages(states, key):
@@ -59,6 +68,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 if not state:
+                    self._not_captured(p, "a parameter's first step")
                     if p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
                     self._init_state(p, group["state_bits"], fresh[p.device])
@@ -69,6 +79,7 @@ class AdamW(torch.optim.Optimizer):
                 states = [self.state[p] for p in params]
                 step = states[0]["step"]
                 if len(params) < members[key]:  # the others stay behind, with a count of their own
+                    self._not_captured(params[0], "the first step without some of the parameters")
                     step = step.clone()
                     for s in states:
                         s["step"] = step

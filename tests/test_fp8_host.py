@@ -1,0 +1,234 @@
+"""What the products in 8 bits and AdamW refuse before anything runs on a GPU, and the sizes that they ask for."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import fp8_oracle as O
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_dropout.hip import _loader
+
+    return _loader.load()
+
+
+FAKE = ctypes.c_void_p(0x1000)
+ODD = ctypes.c_void_p(0x1008)
+INVALID, UNSUPPORTED = 1, 2
+
+
+def refused(lib, rc, code, text):
+    assert rc == code and text in lib.sd_last_error(), (rc, lib.sd_last_error())
+
+
+def test_sizes(lib):
+    # codes with rows of whole 128-blocks, then the scales, to whole 16 bytes
+    assert lib.sd_fp8_matrix_bytes(1, 1, 0) == 128 + 16
+    assert lib.sd_fp8_matrix_bytes(17, 129, 0) == 17 * 256 + 2 * 32
+    assert lib.sd_fp8_matrix_bytes(300, 300, 1) == 300 * 384 + 16
+    assert lib.sd_fp8_matrix_bytes(0, 5, 0) == lib.sd_fp8_matrix_bytes(5, 0, 1) == 0
+    assert lib.sd_fp8_matrix_bytes(70000, 70000, 0) > 2 ** 32
+    for bad in ((-1, 1), (1, -1), (1 << 31, 1), (1, 1 << 31)):
+        assert lib.sd_fp8_matrix_bytes(*bad, 0) == -1
+        assert lib.sd_fp8_gemm_workspace_bytes(*bad, 1) == lib.sd_fp8_linear_workspace_bytes(1, *bad) == -1
+        assert lib.sd_fp8_dropout_matmul_workspace_bytes(*bad, 1, 0) == -1
+    # a few tokens take no workspace, more the input in 8 bits at least
+    assert lib.sd_fp8_linear_workspace_bytes(16, 8192, 8192) == 0
+    assert lib.sd_fp8_linear_workspace_bytes(65, 512, 512) >= lib.sd_fp8_matrix_bytes(65, 512, 0)
+    # a reduction that does not fit a workgroup's list of kept blocks is cut into parts, whose sums are 4 bytes each
+    m, n, k = 128 * 4097, 256, 256
+    assert lib.sd_fp8_dropout_matmul_workspace_bytes(m, n, k, 1) >= lib.sd_fp8_matrix_bytes(m, n, 0) + 2 * 4 * n * k
+
+
+def test_quantizer_refusals(lib):
+    def q(x=FAKE, sr=256, sc=1, rows=10, cols=256, dtype=0, block=1, data=FAKE, ld=256, scales=FAKE, ssr=1, ssk=16):
+        return lib.sd_fp8_quantize(x, sr, sc, rows, cols, dtype, block, data, ld, ctypes.cast(scales, ctypes.c_void_p), ssr, ssk, None)
+
+    refused(lib, q(rows=-1), INVALID, b"negative")
+    refused(lib, q(rows=1 << 31), INVALID, b"too large")
+    refused(lib, q(dtype=3), INVALID, b"dtype")
+    refused(lib, q(block=64), INVALID, b"1 x 128 or 128 x 128")
+    refused(lib, q(x=None), INVALID, b"null pointer")
+    refused(lib, q(sr=512, sc=2), INVALID, b"row or column major")
+    refused(lib, q(sr=100), INVALID, b"row stride")
+    refused(lib, q(data=None), INVALID, b"null pointer")
+    refused(lib, q(data=ODD), INVALID, b"16 bytes")
+    refused(lib, q(ld=264), INVALID, b"16 bytes")
+    refused(lib, q(cols=250, ld=240), INVALID, b"whole 128-blocks")
+    refused(lib, q(ssr=0), INVALID, b"positive")
+    refused(lib, q(rows=1 << 30, cols=1 << 20, sr=1 << 20, ld=1 << 20, ssk=1 << 30), UNSUPPORTED, b"one launch")
+    assert q(rows=0) == 0 and q(cols=0) == 0
+
+    def d(data=FAKE, ld=256, scales=FAKE, block=1, rows=10, cols=256, out=FAKE, out_ld=256, dtype=0):
+        return lib.sd_fp8_dequantize(data, ld, scales, 1, 16, block, rows, cols, out, out_ld, dtype, None)
+
+    refused(lib, d(cols=-1), INVALID, b"negative")
+    refused(lib, d(dtype=9), INVALID, b"dtype")
+    refused(lib, d(block=2), INVALID, b"1 x 128 or 128 x 128")
+    refused(lib, d(data=None), INVALID, b"null pointer")
+    refused(lib, d(data=ODD), INVALID, b"16 bytes")
+    refused(lib, d(ld=128), INVALID, b"does not hold")
+    refused(lib, d(out=None), INVALID, b"null pointer")
+    refused(lib, d(out_ld=255), INVALID, b"row stride")
+    assert d(rows=0) == 0
+
+
+def test_product_refusals(lib):
+    def g(a=FAKE, lda=256, sa=FAKE, sal=16, b=FAKE, ldb=256, sb=FAKE, sbr=2, sbk=1, block=128, c=FAKE, csr=20, csc=1, M=10, N=20, K=256, dtype=0):
+        return lib.sd_fp8_gemm(a, lda, sa, sal, b, ldb, sb, sbr, sbk, block, c, csr, csc, M, N, K, dtype, None, 0, None)
+
+    refused(lib, g(M=-1), INVALID, b"negative")
+    refused(lib, g(dtype=2), INVALID, b"dtype")
+    refused(lib, g(block=32), INVALID, b"1 x 128 or 128 x 128")
+    refused(lib, g(a=None), INVALID, b"null pointer")
+    refused(lib, g(sa=None), INVALID, b"null pointer")
+    refused(lib, g(b=ODD), INVALID, b"16 bytes")
+    refused(lib, g(lda=250), INVALID, b"16 bytes")
+    refused(lib, g(ldb=128), INVALID, b"does not hold")
+    refused(lib, g(csr=19), INVALID, b"row stride")
+    refused(lib, g(K=0), INVALID, b"empty reduction")
+    refused(lib, g(sal=9), INVALID, b"A's scales")
+    refused(lib, g(sal=18), INVALID, b"A's scales")
+    refused(lib, g(sbk=0), INVALID, b"positive")
+    refused(lib, g(block=1, sbr=1, sbk=18), INVALID, b"B's scales")
+    refused(lib, g(block=1, sbr=2, sbk=32), INVALID, b"B's scales")
+    refused(lib, g(lda=(1 << 22) + 128), UNSUPPORTED, b"pitch")
+    refused(lib, g(lda=1 << 22, ldb=1 << 22, K=1 << 22, sal=1 << 16), UNSUPPORTED, b"too many scales")
+    assert g(M=0) == 0 and g(N=0, csr=1) == 0
+
+    def f(x=FAKE, ldx=256, w=FAKE, ldw=256, sw=FAKE, swr=2, swk=1, y=FAKE, ldy=20, M=10, N=20, K=256, dtype=0, ws=None, bytes_=0):
+        return lib.sd_fp8_linear(x, ldx, w, ldw, sw, swr, swk, y, ldy, M, N, K, dtype, ws, bytes_, None)
+
+    refused(lib, f(x=None), INVALID, b"null pointer")
+    refused(lib, f(ldx=255), INVALID, b"row stride")
+    refused(lib, f(w=ODD), INVALID, b"16 bytes")
+    refused(lib, f(ldw=128), INVALID, b"does not hold")
+    refused(lib, f(sw=None), INVALID, b"null pointer")
+    refused(lib, f(ldy=19), INVALID, b"row stride")
+    refused(lib, f(K=0), INVALID, b"empty reduction")
+    refused(lib, f(swk=0), INVALID, b"positive")
+    refused(lib, f(dtype=2), INVALID, b"dtype")
+    refused(lib, f(M=100), INVALID, b"workspace")
+    need = lib.sd_fp8_linear_workspace_bytes(100, 20, 256)
+    refused(lib, f(M=100, ws=FAKE, bytes_=need - 1), INVALID, b"workspace")
+    refused(lib, f(M=100, ws=ODD, bytes_=need), INVALID, b"workspace")
+    refused(lib, f(K=(1 << 22) + 1, ldx=1 << 23, ldw=1 << 23), UNSUPPORTED, b"pitch")
+
+
+def test_layer_refusals(lib):
+    def fwd(x=FAKE, xsr=256, xsc=1, w=FAKE, y=FAKE, ysr=20, mask=FAKE, msr=2, msc=1, state=None, p=0.5, out=None, xt=None, wt=None, M=10, N=20,
+            K=256, bs=128, dtype=0, ws=FAKE, bytes_=1 << 40):
+        return lib.sd_fp8_dropout_matmul_forward(x, xsr, xsc, w, 256, 1, y, ysr, 1, mask, msr, msc, state, 0, 0, p, out, xt, wt, M, N, K, bs, dtype,
+                                                 ws, bytes_, None)
+
+    refused(lib, fwd(M=-5), INVALID, b"negative")
+    refused(lib, fwd(M=0), INVALID, b"empty operand")
+    refused(lib, fwd(dtype=2), INVALID, b"dtype")
+    for p in (-0.1, 1.0, float("nan")):
+        refused(lib, fwd(p=p), INVALID, b"p must be")
+    refused(lib, fwd(bs=0), INVALID, b"positive")
+    refused(lib, fwd(bs=192), UNSUPPORTED, b"multiples of 128")
+    refused(lib, fwd(M=(1 << 22) + 1), UNSUPPORTED, b"too long")
+    refused(lib, fwd(x=None), INVALID, b"null pointer")
+    refused(lib, fwd(xsr=2, xsc=3), INVALID, b"row or column major")
+    refused(lib, fwd(ysr=10), INVALID, b"row stride")
+    refused(lib, fwd(xt=ODD), INVALID, b"16 bytes")
+    refused(lib, fwd(msr=2, msc=3), INVALID, b"row or column major")
+    refused(lib, fwd(mask=None), INVALID, b"mask_out")
+    refused(lib, fwd(mask=None, out=FAKE, state=ctypes.c_void_p(0x1004)), INVALID, b"aligned")
+    need = lib.sd_fp8_dropout_matmul_workspace_bytes(10, 20, 256, 0)
+    refused(lib, fwd(bytes_=need - 1), INVALID, b"workspace")
+    refused(lib, fwd(ws=None), INVALID, b"workspace")
+
+    def bwd(dy=FAKE, mask=FAKE, xt=FAKE, wt=FAKE, dx=FAKE, dw=FAKE, M=10, N=20, K=256, bs=128, p=0.5, ws=FAKE, bytes_=1 << 40):
+        return lib.sd_fp8_dropout_matmul_backward(dy, N, 1, mask, 2, 1, xt, wt, dx, K, 1, dw, K, 1, M, N, K, bs, p, 0, ws, bytes_, None)
+
+    refused(lib, bwd(N=0), INVALID, b"no outputs")
+    refused(lib, bwd(dx=None, dw=None), INVALID, b"neither gradient")
+    refused(lib, bwd(mask=None), INVALID, b"mask")
+    refused(lib, bwd(dy=None), INVALID, b"null pointer")
+    refused(lib, bwd(wt=None), INVALID, b"needs WT")
+    refused(lib, bwd(xt=ODD), INVALID, b"needs XT")
+    refused(lib, bwd(bs=100), UNSUPPORTED, b"multiples of 128")
+    refused(lib, bwd(bytes_=lib.sd_fp8_dropout_matmul_workspace_bytes(10, 20, 256, 1) - 1), INVALID, b"workspace")
+
+
+def test_adamw_refusals(lib):
+    pointers = (ctypes.c_void_p * 1)(0x1000)
+    nothing = (ctypes.c_void_p * 1)(None)
+    sizes = (ctypes.c_int64 * 1)(5)
+
+    def step(count=1, p=pointers, g=pointers, m=pointers, v=pointers, ms=pointers, vs=pointers, n=sizes, at=FAKE, lr_at=None, lr=1e-3, b1=0.9,
+             b2=0.99, eps=1e-8, decay=0.1, dtype=2, bits=8):
+        return lib.sd_adamw_step(count, p, g, m, v, ms, vs, n, at, lr_at, lr, b1, b2, eps, decay, dtype, bits, 1, None)
+
+    refused(lib, step(count=-1), INVALID, b"negative count")
+    refused(lib, step(dtype=3), INVALID, b"dtype")
+    refused(lib, step(bits=16), INVALID, b"8 or in 32 bits")
+    refused(lib, step(at=None), INVALID, b"step")
+    refused(lib, step(at=ctypes.c_void_p(0x1004)), INVALID, b"step")
+    for kw, text in ((dict(lr=-1.0), b"lr"), (dict(lr=float("nan")), b"lr"), (dict(lr=float("inf")), b"lr"), (dict(b1=1.0), b"betas"), (dict(b2=-0.1), b"betas"),
+                     (dict(eps=-1e-8), b"eps"), (dict(eps=1e-39), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(eps=1e37), b"eps"),
+                     (dict(decay=-0.1), b"weight_decay")):
+        refused(lib, step(**kw), INVALID, text)
+    refused(lib, step(n=None), INVALID, b"null array")
+    refused(lib, step(g=None), INVALID, b"null array")
+    refused(lib, step(m=nothing), INVALID, b"null pointer")
+    refused(lib, step(vs=nothing), INVALID, b"scales")
+    refused(lib, step(ms=None), INVALID, b"scales")
+    refused(lib, step(n=(ctypes.c_int64 * 1)(-5)), INVALID, b"negative size")
+    refused(lib, step(n=(ctypes.c_int64 * 1)(1 << 43)), UNSUPPORTED, b"too large")
+    second = (ctypes.c_int32 * 1)(0)
+    values = lambda count=1, c=pointers, n=sizes: lib.sd_adamw_state_values(count, c, pointers, pointers, n, second, None)  # noqa: E731
+    refused(lib, values(count=-1), INVALID, b"negative count")
+    refused(lib, values(c=None), INVALID, b"null array")
+    refused(lib, values(c=nothing), INVALID, b"null pointer")
+    refused(lib, values(n=(ctypes.c_int64 * 1)(-1)), INVALID, b"negative size")
+    assert values(count=0) == 0
+
+
+def test_operands_on_the_cpu_are_refused():
+    import flash_dropout.functional as F
+    from flash_dropout.hip import GEMM
+    from flash_dropout.layers import DropoutMM
+    from flash_dropout.optim import AdamW
+
+    x = torch.zeros(4, 256, dtype=torch.float16)
+    data, scales = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(1, 2).to(torch.float8_e8m0fnu)
+    for call in (lambda: F.fp8_quantize(x), lambda: F.fp8_dequantize(data, scales), lambda: F.fp8_linear(x, data, scales),
+                 lambda: GEMM().gemm_fp8(data, scales, data, scales),
+                 lambda: F.hip_blockwise_dropout_matmul_fp8_mask(x, torch.zeros(1, 2, dtype=torch.bool), 128, 0.5, x),
+                 lambda: F.hip_blockwise_dropout_matmul_fp8(x, x, 128, 0.5, seed=1),
+                 lambda: F.adamw_step([x], [x], [x.float()], [x.float()], torch.zeros((), dtype=torch.int64)),
+                 lambda: F.adamw_state_values([(torch.zeros(4, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8))] * 2,
+                                              [(torch.zeros(4, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8))] * 2)):
+        with pytest.raises(ValueError):
+            call()
+    for bs in (0, -128, 1.5, (128, 256)):
+        with pytest.raises(ValueError):
+            F.hip_blockwise_dropout_matmul_fp8(x, x, bs, 0.5)
+    p = torch.nn.Parameter(torch.zeros(3))
+    for kw in (dict(eps=1e-39), dict(eps=1e37), dict(eps=-1.0), dict(lr=-1e-3), dict(betas=(0.9, 1.0)), dict(weight_decay=-1.0), dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    p.grad = torch.zeros(3)
+    with pytest.raises(ValueError):
+        AdamW([p]).step()
+    with pytest.raises(ValueError, match="8 or in 32"):
+        AdamW([dict(params=[p], state_bits=4)]).step()
+    assert DropoutMM(4, 4, variant="blockwise[hip-fp8]", block_size=128).eval()(torch.zeros(2, 4)).shape == (2, 4)
+
+
+def test_the_states_random_bits_leave_averages_right_on_average():
+    """A value's two neighbours come up with the probabilities that its place says: over 4096 elements and 16 steps a share of 1/4 is
+    off by more than 6 sqrt(1/4 * 3/4 / 65536) = 0.0102 once in 10^8 draws."""
+    n, steps = 4096, range(1, 17)
+    for which, step_between in (("first", 2.0), ("second", 2.0)):
+        x = O.np.full(n, 16 + step_between / 4)  # a quarter of the way from 16 to 18
+        x[::128] = 448.0 if which == "first" else 61440.0  # scales of 1
+        got = O.np.stack([O.rounded_state(x, which, s) for s in steps])
+        got = O.np.delete(got, O.np.arange(0, n, 128), 1)
+        assert set(O.np.unique(got)) == {16.0, 18.0}
+        assert abs((got == 18.0).mean() - 0.25) <= 0.0104  # (a 128th of them are the large ones)
