@@ -124,32 +124,48 @@ __device__ inline bool dropped(const Fp8Gemm& g, int i, int j) {
   return g.mask[i * g.msr + j * g.msc] != 0;
 }
 
-// The patch of 64 rows (from m0) x 64 columns (from n0) of a wave: sums of row group i and column group j in acc[i][j], scaled and
-// rounded to C, or as they are to a part of a split reduction.  A whole patch is stored by straight code, four or eight elements
-// a lane at a time; one at C's edge element by element.
-template <typename T>
-__device__ inline void store_patch(const Fp8Gemm& g, int64_t m0, int64_t n0, const f32x4 (&acc)[4][4], float* part, int lane) {
+// N neighbouring elements of C, or of a part's sums, of which `left` are there.
+template <typename T, int N>
+__device__ inline void store_run(const Fp8Gemm& g, float* part, int64_t at, const float (&x)[N], int left) {
+  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
   typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+  if (left < N) {
+#pragma unroll
+    for (int e = 0; e < N - 1; ++e) {
+      if (e >= left) break;
+      if (part) part[at + e] = x[e];
+      else g.c[at + e] = T::from_float(x[e] * g.scale);
+    }
+  } else if (part) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4_any*>(part + at + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int e = 0; e < N; e += 2) w[e / 2] = T::pack2(x[e] * g.scale, x[e + 1] * g.scale);
+    if constexpr (N == 4) *reinterpret_cast<u32x2_any*>(g.c + at) = u32x2{w[0], w[1]};
+    else *reinterpret_cast<u32x4_any*>(g.c + at) = u32x4{w[0], w[1], w[2], w[3]};
+  }
+}
+// The patch of 64 rows (from m0) x 64 columns (from n0) of a wave: sums of row group i and column group j in acc[i][j], scaled and
+// rounded to C, or as they are to a part of a split reduction.  Four or eight elements a lane at a time, by straight code where the patch
+// is whole.  (Element by element at C's edge 200 rows take 3 us longer than 256 through 2048 to 8192.)
+template <typename T, bool WHOLE>
+__device__ inline void store_patch_rows(const Fp8Gemm& g, int64_t m0, int64_t n0, const f32x4 (&acc)[4][4], float* part, int lane) {
   const int r = lane & 15, q = lane >> 4;
   const bool along_n = g.c_sc == 1;
   const int64_t ld = part ? (along_n ? g.N : g.M) : (along_n ? g.c_sr : g.c_sc);
-  const bool whole = m0 + 64 <= g.M && n0 + 64 <= g.N && (!part || ld % 4 == 0);
-  if (whole && along_n) {
+  const int rows = WHOLE ? 64 : (int)(g.M - m0 < 64 ? g.M - m0 : 64) - 16 * q, cols = WHOLE ? 64 : (int)(g.N - n0 < 64 ? g.N - n0 : 64) - 4 * r;
+  if (along_n) {
     const int64_t at = (m0 + 16 * q) * ld + n0 + 4 * r;
-    if (part) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(part + at + (4 * v + i) * ld) = f32x4{acc[i][0][v], acc[i][1][v], acc[i][2][v], acc[i][3][v]};
-    } else {
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x2_any*>(g.c + at + (4 * v + i) * ld) =
-              u32x2{T::pack2(acc[i][0][v] * g.scale, acc[i][1][v] * g.scale), T::pack2(acc[i][2][v] * g.scale, acc[i][3][v] * g.scale)};
-    }
-  } else if (whole) {  // sixteen rows a lane and column
+      for (int i = 0; i < 4; ++i) {
+        const float x[4] = {acc[i][0][v], acc[i][1][v], acc[i][2][v], acc[i][3][v]};
+        if (WHOLE || 4 * v + i < rows) store_run<T>(g, part, at + (4 * v + i) * ld, x, WHOLE ? 4 : cols);
+      }
+  } else {  // sixteen rows a lane and column
     const int64_t at = (n0 + 4 * r) * ld + m0 + 16 * q;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -157,28 +173,16 @@ __device__ inline void store_patch(const Fp8Gemm& g, int64_t m0, int64_t n0, con
       for (int h = 0; h < 2; ++h) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = acc[e & 3][j][2 * h + e / 4] * (part ? 1.f : g.scale);
-        if (part) {
-          float* dst = part + at + j * ld + 8 * h;
-          *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
-          *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
-        } else {
-          *reinterpret_cast<u32x4_any*>(g.c + at + j * ld + 8 * h) = u32x4{T::pack2(x[0], x[1]), T::pack2(x[2], x[3]), T::pack2(x[4], x[5]), T::pack2(x[6], x[7])};
-        }
+        for (int e = 0; e < 8; ++e) x[e] = acc[e & 3][j][2 * h + e / 4];
+        if (WHOLE || j < cols) store_run<T>(g, part, at + j * ld + 8 * h, x, WHOLE ? 8 : rows - 8 * h);
       }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t m = m0 + 16 * q + 4 * v + i, n = n0 + 4 * r + j, at = along_n ? m * ld + n : n * ld + m;
-          if (m >= g.M || n >= g.N) continue;
-          if (part) part[at] = acc[i][j][v];
-          else g.c[at] = T::from_float(acc[i][j][v] * g.scale);
-        }
   }
+}
+template <typename T>
+__device__ inline void store_patch(const Fp8Gemm& g, int64_t m0, int64_t n0, const f32x4 (&acc)[4][4], float* part, int lane) {
+  if (m0 >= g.M || n0 >= g.N) return;
+  if (m0 + 64 <= g.M && n0 + 64 <= g.N) store_patch_rows<T, true>(g, m0, n0, acc, part, lane);
+  else store_patch_rows<T, false>(g, m0, n0, acc, part, lane);
 }
 
 // Entries 128-block | flags << 16 of blocks [lo, hi): in front, in their order, those with any flag set, whose number is
@@ -209,16 +213,20 @@ __device__ inline int make_list(int lo, int hi, uint32_t* list, uint8_t* scratch
 }
 
 // ---- 128 x 128 tiles ------------------------------------------------------------------------------------------------------
-// Four waves of 64 x 64.  Two stages and two workgroups to a CU: while one waits at its barrier the other's matrix instructions run; bound
-// by the LDS, 32 KB in and 64 KB out a step for 512 clocks of matrix instructions.  Four stages, a workgroup to a CU, where
-// there are no more of them than CUs: then a step costs what is left of a load's latency, of which three steps are on their way.
+// Waves of 64 x 64.  One group of four, two stages and two workgroups to a CU: while one waits at its barrier the other's matrix instructions
+// run; bound by the LDS, 32 KB in and 64 KB out a step for 512 clocks of matrix instructions.  Where there are no more of them than CUs, two
+// groups of four that take the steps in turn: a phase is a step, in which one group reads its step's fragments into registers and the
+// other's matrix instructions run from theirs; each has two of four stages, and loads the step after its next into the one that it has just
+// read.  At the end either group gives the other two of its four patches' sums through LDS and stores the other two.
 constexpr int kMidStage = 2 * kBlockBytes + 2 * 512;  // A block, B block, words of scales of either
-constexpr int mid_lds(int stages, int list) { return stages * kMidStage + list * 5 + 16; }
+constexpr int mid_lds(int groups, int list) { return 2 * groups * kMidStage + list * 5 + 16; }
+static_assert(mid_lds(2, kMaxList) <= kLdsLimit, "LDS");
 
-template <typename T, int MODE, bool SQUARE, int STAGES>
+template <typename T, int MODE, bool SQUARE, int GROUPS>
 __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
+  constexpr int STAGES = 2 * GROUPS;
   const Fp8Gemm& g = p.g;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = GROUPS == 1 ? 0 : wave >> 2, c = wave & 3;
   int tm, tn, part;
   tile_of_split_block<DSD_GROUP_M>(block, p.tiles_m, p.tiles_n, p.splits, tm, tn, part);
   const int64_t m0 = (int64_t)tm * kB, n0 = (int64_t)tn * kB;
@@ -229,73 +237,116 @@ __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
   if constexpr (MODE == kFp8Dsd) {
     uint8_t* const scratch = reinterpret_cast<uint8_t*>(list + p.per_split);
     int* const count = reinterpret_cast<int*>(smem);
-    steps = make_list<256, false>(lo, hi, list, scratch, count, [&](int k) { return dropped(g, tm, k) ? 0 : 1; });
+    steps = make_list<GROUPS * 256, false>(lo, hi, list, scratch, count, [&](int k) { return dropped(g, tm, k) ? 0 : 1; });
     __syncthreads();  // (count lies where the first stage goes)
   }
   if constexpr (MODE == kFp8Sdd) {
     if (dropped(g, tm, tn)) steps = 0;
   }
   steps = __builtin_amdgcn_readfirstlane(steps);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = c >> 1, wn = c & 1;
   const BlockRows rows_a(g.lda, lane), rows_b(g.ldb, lane);
   const u32x4 of_a = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_b = block_buffer(g.b + n0 * g.ldb, g.ldb, g.N - n0);
   const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
   const u32x4 bb = SQUARE ? buffer_over(g.sb + tn * g.sb_r, (int64_t)(p.nk - 1) * g.sb_k + 1) : buffer_over(g.sb + n0, (int64_t)p.nk * g.sb_k - n0);
   const uint32_t lds = lds_address(smem);
-  const int per_step = wave < 2 ? 9 : 8;  // loads of this wave
+  const int per_step = c < 2 ? 9 : 8;  // loads of this wave
   auto step_block = [&](int s) { return MODE == kFp8Dsd ? __builtin_amdgcn_readfirstlane((int)(list[s] & 0xffffu)) : lo + s; };
   auto load = [&](int s) {
     const int k = step_block(s);
     const uint32_t at = lds + (uint32_t)(s % STAGES) * kMidStage;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      rows_a.load(of_a, wave * 4 + q, k, at);
-      rows_b.load(of_b, wave * 4 + q, k, at + kBlockBytes);
+      rows_a.load(of_a, c * 4 + q, k, at);
+      rows_b.load(of_b, c * 4 + q, k, at + kBlockBytes);
     }
-    if (wave == 0) buffer4_to_lds(ba, (uint32_t)((int64_t)k * g.sa_ld) + (lane & 31) * 4, at + 2 * kBlockBytes);
-    if (wave == 1) {
+    if (c == 0) buffer4_to_lds(ba, (uint32_t)((int64_t)k * g.sa_ld) + (lane & 31) * 4, at + 2 * kBlockBytes);
+    if (c == 1) {
       if (SQUARE) buffer1_to_lds(bb, (uint32_t)((int64_t)k * g.sb_k), at + 2 * kBlockBytes + 512);
       else buffer4_to_lds(bb, (uint32_t)((int64_t)k * g.sb_k) + (lane & 31) * 4, at + 2 * kBlockBytes + 512);
     }
   };
   f32x4 acc[4][4] = {};
-  for (int s = 0; s < STAGES - 1 && s < steps; ++s) load(s);
-  for (int s = 0; s < steps; ++s) {
-    wait_loads_all_but(per_step * min(STAGES - 2, steps - 1 - s));
-    barrier();
-    if (s + STAGES - 1 < steps) load(s + STAGES - 1);  // (into the stage of step s - 1, which every wave is done with)
+  i32x8 fa[4], fb[4];
+  int sa, sb;
+  auto read = [&](int s) {
     const char* st = smem + (s % STAGES) * kMidStage;
     const char* scales = st + 2 * kBlockBytes;
-    const int sa = *reinterpret_cast<const int*>(scales + 64 * wm + 4 * (lane & 15));
-    int sb = *reinterpret_cast<const int*>(scales + 512 + (SQUARE ? 0 : 64 * wn + 4 * (lane & 15)));
+    sa = *reinterpret_cast<const int*>(scales + 64 * wm + 4 * (lane & 15));
+    sb = *reinterpret_cast<const int*>(scales + 512 + (SQUARE ? 0 : 64 * wn + 4 * (lane & 15)));
     if (SQUARE) sb *= 0x01010101;
-    i32x8 fa[4], fb[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       fa[i] = read_fragment(st + wm * 64 * kB, i, lane);
       fb[i] = read_fragment(st + kBlockBytes + wn * 64 * kB, i, lane);
     }
+  };
+  auto multiply = [&] {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j], sa, i, sb, j);
-    wait_reads();  // (before the stage that was read is loaded over, behind the next barrier)
+  };
+  if constexpr (GROUPS == 1) {
+    if (steps > 0) load(0);
+    for (int s = 0; s < steps; ++s) {
+      wait_loads();
+      barrier();
+      if (s + 1 < steps) load(s + 1);  // (into the stage of step s - 1, which every wave is done with)
+      read(s);
+      multiply();
+      wait_reads();  // (before the stage that was read is loaded over, behind the next barrier)
+    }
+  } else if (steps > 0) {
+    if (grp < steps) load(grp);
+    if (grp + 2 < steps) load(grp + 2);
+    wait_loads_all_but(grp + 2 < steps ? per_step : 0);
+    barrier();
+    if (grp == 1) barrier();
+    for (int s = grp; s < steps; s += 2) {
+      read(s);
+      wait_reads();
+      barrier();  // (the group is done with the stage)
+      if (s + 4 < steps) load(s + 4);
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      wait_loads_all_but(s + 4 < steps ? per_step : 0);  // (step s + 2 is there)
+      if (s + 1 < steps) barrier();
+    }
+    barrier();
+    f32x4* const sums = reinterpret_cast<f32x4*>(smem) + c * 16 * 64;
+    const bool stores = (c < 2) == (grp == 0);
+    if (!stores) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[(4 * i + j) * 64 + lane] = acc[i][j];
+    }
+    __syncthreads();
+    if (!stores) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] += sums[(4 * i + j) * 64 + lane];
+  } else if ((c < 2) != (grp == 0)) {
+    return;
   }
   store_patch<T>(g, m0 + 64 * wm, n0 + 64 * wn, acc, out_part, lane);
 }
 
-template <typename T, int MODE, bool SQUARE, int STAGES>
-__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void fp8_mid_kernel(Args p) {
+template <typename T, int MODE, bool SQUARE, int GROUPS>
+__global__ __launch_bounds__(GROUPS * 256, 2) void fp8_mid_kernel(Args p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  mid_tile<T, MODE, SQUARE, STAGES>(p, (int)blockIdx.x, smem);
+  mid_tile<T, MODE, SQUARE, GROUPS>(p, (int)blockIdx.x, smem);
 }
 
 // Both gradients of a layer in one launch, the weight gradient's workgroups behind the input gradient's.
-template <typename T, int STAGES>
-__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void fp8_pair_kernel(Args x, Args w, int first_w) {
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(GROUPS * 256, 2) void fp8_pair_kernel(Args x, Args w, int first_w) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  if ((int)blockIdx.x < first_w) mid_tile<T, kFp8Sdd, true, STAGES>(x, (int)blockIdx.x, smem);
-  else mid_tile<T, kFp8Dsd, false, STAGES>(w, (int)blockIdx.x - first_w, smem);
+  if ((int)blockIdx.x < first_w) mid_tile<T, kFp8Sdd, true, GROUPS>(x, (int)blockIdx.x, smem);
+  else mid_tile<T, kFp8Dsd, false, GROUPS>(w, (int)blockIdx.x - first_w, smem);
 }
 
 // ---- 256 x 256 tiles ------------------------------------------------------------------------------------------------------
@@ -595,8 +646,7 @@ int configure(const void* kernel, std::atomic<bool>* done) {
 
 // How a product is cut up.  256 x 256 tiles where they fill the chip; else 128 x 128 ones, and where there are few of them and the
 // reduction is long, that is cut into parts.  A part costs its fp32 sums, written and read once, and one more launch; what it saves are
-// steps, a microsecond each with two workgroups on a CU and 0.7 with one (128 x 32768 at 256 .. 2048: 6.5, 9.1, 11.9, 17.6 us).
-// 200 x 8192 over 2048 in two parts 19.4 us, in one 15.
+// steps, a microsecond each with two workgroups on a CU and 0.55 with one (128 x 32768 at 512, 1024, 2048: 8, 11, 16 us).
 struct Plan {
   bool big;
   int splits, per_split;
@@ -609,7 +659,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, int mode) {
     double least = 1e30;
     for (int64_t s = 1; s <= 16 && (s == 1 || nk / s >= 2); ++s) {
       const int64_t steps = ceil_div(nk, s), wgs = tiles * ceil_div(nk, steps);
-      const double us = wgs <= kCus ? 0.7 * steps : (double)ceil_div(wgs, 2 * kCus) * (1.0 * steps + 3.0);
+      const double us = wgs <= kCus ? 0.55 * steps : (double)ceil_div(wgs, 2 * kCus) * (1.0 * steps + 3.0);
       const double sum = s == 1 ? 0.0 : 4.0 + 8e-6 / 4.0 * (double)(ceil_div(nk, steps) * M * N);
       if (us + sum < least) {
         least = us + sum;
@@ -631,18 +681,20 @@ int launch_sum(const Args& p, hipStream_t stream) {
   return check_launch("fp8_sum");
 }
 
-template <typename T, int MODE, int STAGES>
+template <typename T, int MODE, int GROUPS>
 int launch_mid(const Args& p, hipStream_t stream) {
-  auto* kernel = p.g.sb_square ? &fp8_mid_kernel<T, MODE, true, STAGES> : &fp8_mid_kernel<T, MODE, false, STAGES>;
+  auto* kernel = p.g.sb_square ? &fp8_mid_kernel<T, MODE, true, GROUPS> : &fp8_mid_kernel<T, MODE, false, GROUPS>;
   static std::atomic<bool> configured[2][16] = {};
   if (int rc = configure(reinterpret_cast<const void*>(kernel), configured[p.g.sb_square])) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks_of(p)), dim3(256), mid_lds(STAGES, MODE == kFp8Dsd ? p.per_split : 0), stream, p);
-  note_kernel("fp8:mid stages=%d splits=%d", STAGES, p.splits);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks_of(p)), dim3(GROUPS * 256), mid_lds(GROUPS, MODE == kFp8Dsd ? p.per_split : 0), stream, p);
+  note_kernel("fp8:mid groups=%d splits=%d", GROUPS, p.splits);
   return check_launch("fp8_gemm");
 }
 
-// Four stages where every workgroup has a CU to itself and more than two steps
-bool deep(int64_t blocks, const Args& p) { return blocks <= kCus && p.per_split > 2; }
+// Two groups of waves where every workgroup has a CU to itself and more than eight steps (300 x 300 over 4096 in 11 parts 10.7 us with either,
+// 1024^3, eight steps, 9.0 with one and 9.8 with two, 512 x 4096 over 4096, 32 steps, 26.1 and 22.4; with few steps the exchange of sums at
+// the end, about 1 us, counts)
+bool deep(int64_t blocks, const Args& p) { return blocks <= kCus && p.per_split > 8; }
 
 template <typename T, int MODE>
 int launch_big(const Args& p, hipStream_t stream) {
@@ -673,17 +725,17 @@ int launch(const Args& p, hipStream_t stream) {
     return launch_sum<T>(p, stream);
   }
   if (blocks_of(p) >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8 product: %lld tiles are too many for one launch", (long long)blocks_of(p));
-  if (int rc = deep(blocks_of(p), p) ? launch_mid<T, MODE, 4>(p, stream) : launch_mid<T, MODE, 2>(p, stream)) return rc;
+  if (int rc = deep(blocks_of(p), p) ? launch_mid<T, MODE, 2>(p, stream) : launch_mid<T, MODE, 1>(p, stream)) return rc;
   return launch_sum<T>(p, stream);
 }
 
-template <typename T, int STAGES>
+template <typename T, int GROUPS>
 int launch_pair(const Args& x, const Args& w, hipStream_t stream) {
-  auto* kernel = &fp8_pair_kernel<T, STAGES>;
+  auto* kernel = &fp8_pair_kernel<T, GROUPS>;
   static std::atomic<bool> configured[16] = {};
   if (int rc = configure(reinterpret_cast<const void*>(kernel), configured)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_of(x) + blocks_of(w))), dim3(256), mid_lds(STAGES, w.per_split), stream, x, w, (int)blocks_of(x));
-  note_kernel("fp8:pair stages=%d splits=%d", STAGES, w.splits);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks_of(x) + blocks_of(w))), dim3(GROUPS * 256), mid_lds(GROUPS, w.per_split), stream, x, w, (int)blocks_of(x));
+  note_kernel("fp8:pair groups=%d splits=%d", GROUPS, w.splits);
   if (int rc = check_launch("fp8_pair")) return rc;
   return launch_sum<T>(w, stream);
 }
@@ -737,9 +789,9 @@ int launch_fp8_backward(const Fp8Gemm& gx, const Fp8Gemm& gw, int dtype, hipStre
     if (int rc = launch_fp8_gemm(gx, kFp8Sdd, dtype, stream)) return rc;
     return launch_fp8_gemm(gw, kFp8Dsd, dtype, stream);
   }
-  const bool four = deep(blocks, x) || deep(blocks, w);
-  if (dtype == SD_BF16) return four ? launch_pair<BF16, 4>(x, w, stream) : launch_pair<BF16, 2>(x, w, stream);
-  return four ? launch_pair<F16, 4>(x, w, stream) : launch_pair<F16, 2>(x, w, stream);
+  const bool two = deep(blocks, x) || deep(blocks, w);
+  if (dtype == SD_BF16) return two ? launch_pair<BF16, 2>(x, w, stream) : launch_pair<BF16, 1>(x, w, stream);
+  return two ? launch_pair<F16, 2>(x, w, stream) : launch_pair<F16, 1>(x, w, stream);
 }
 
 }  // namespace sd
