@@ -102,6 +102,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     OUT_DIR.mkdir(parents=True, exist_ok=True)
     headers = sorted(CSRC.glob("*.h")) + sorted((ROOT / "include").glob("*.h"))
     hash_inc = write_source_hash()  # included by api.hip (and the bridge) only
+    began_with = source_hash()
     jobs = []
     objs = []
     for src in sources():
@@ -120,6 +121,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     # (the bridge carries the hash of all sources too, so it follows every change of the library)
     if force or _stale(BRIDGE, [BRIDGE_SRC, LIB, hash_inc]):
         _run(bridge_command())
+    # A source is compiled twice, for the GPU and for the host: edited in between, a launch names a kernel that is not there, which
+    # aborts the process.
+    if source_hash() != began_with:
+        LIB.unlink()
+        raise RuntimeError("the sources changed while they were compiled: build again")
     return LIB
 
 
