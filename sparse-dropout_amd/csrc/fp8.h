@@ -93,8 +93,11 @@ __device__ inline uint32_t fp8_scale_of(uint32_t most) {
 }
 // 2^(127 - byte), for bytes that fp8_scale_of gives (up to 247)
 __device__ inline float fp8_inverse(uint32_t byte) { return __builtin_bit_cast(float, (254u - byte) << 23); }
-// 2^(byte - 127)
-__device__ inline float fp8_power(uint32_t byte) { return __builtin_bit_cast(float, byte ? byte << 23 : 0x400000u); }
+// 2^(byte - 127); of 255 NaN, as the matrix instruction has it
+__device__ inline float fp8_power(uint32_t byte) {
+  const uint32_t bits = byte << 23;
+  return __builtin_bit_cast(float, byte == 0u ? 0x400000u : byte == 255u ? 0x7fc00000u : bits);
+}
 __device__ inline uint32_t finite_magnitude(float x) {
   const uint32_t a = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
   return a < 0x7f800000u ? a : 0u;

@@ -2,9 +2,10 @@
 //
 // Bound by reading the weights, a byte each, as long as there are few rows.  So they go from memory straight into the matrix
 // instruction's registers, every byte once, and x, which a launch before would have to bring into 8 bits, is quantized by each workgroup as
-// it reads it out of the L2.  A workgroup owns 16 outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block
+// it reads it out of the L2.  A workgroup owns 16 or 32 outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block
 // w + waves * n, a few of them on their way at a time, and meet once in LDS.  Rows come in groups of 16, up to four; what a row behind the
-// last or an output behind the last holds is never stored, so their lanes read another's.
+// last or an output behind the last holds is never stored, so their lanes read another's.  One token through 4096 to 1024 6.3 us, most of it a
+// memory latency and the launch; through 8192 to 8192 FIGURE.
 #include "fp8.h"
 
 namespace sd {
@@ -12,13 +13,13 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// This lane's 32 elements of a row in one 128-block, two to a word: 16 q .. + 15 and 64 + 16 q .. + 15.
+// This lane's 32 elements of a row in one 128-block, two to a word: 32 q .. + 31.  (Each load of a wave touches whole lines then.)
 struct RowPart {
   uint32_t v[16];
-  __device__ inline void load(const uint16_t* at) {  // the block's first element plus 16 q
+  __device__ inline void load(const uint16_t* at) {  // the block's first element plus 32 q
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const u32x4 e = *reinterpret_cast<const u32x4_any*>(at + (h >> 1) * 64 + (h & 1) * 8);
+      const u32x4 e = *reinterpret_cast<const u32x4_any*>(at + 8 * h);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[4 * h + i] = e[i];
     }
@@ -28,7 +29,7 @@ struct RowPart {
     for (int h = 0; h < 4; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = (h >> 1) * 64 + (h & 1) * 8 + 2 * i;
+        const int c = 8 * h + 2 * i;
         v[4 * h + i] = (c < left ? at[c] : 0u) | (c + 1 < left ? (uint32_t)at[c + 1] << 16 : 0u);
       }
   }
@@ -58,8 +59,8 @@ struct RowPart {
   }
 };
 
-__device__ inline i32x8 load_weights(const uint8_t* at) {  // the block's first code plus 16 q
-  const u32x4 lo = *reinterpret_cast<const u32x4*>(at), hi = *reinterpret_cast<const u32x4*>(at + 64);
+__device__ inline i32x8 load_weights(const uint8_t* at) {  // the block's first code plus 32 q
+  const u32x4 lo = *reinterpret_cast<const u32x4*>(at), hi = *reinterpret_cast<const u32x4*>(at + 16);
   i32x8 b;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -69,35 +70,39 @@ __device__ inline i32x8 load_weights(const uint8_t* at) {  // the block's first 
   return b;
 }
 
-// AHEAD: 128-blocks of a wave on their way together
-template <typename T, int WAVES, int GROUPS, int AHEAD>
-__global__ __launch_bounds__(WAVES * 64, AHEAD == 2 && GROUPS == 1 ? 8 : WAVES / 4) void fp8_few_kernel(Fp8Few g) {
+// COLS: of 16 outputs; AHEAD: 128-blocks of a wave on their way together
+template <typename T, int WAVES, int GROUPS, int COLS, int AHEAD>
+__global__ __launch_bounds__(WAVES * 64, WAVES / 4) void fp8_few_kernel(Fp8Few g) {
   __shared__ float sums[WAVES][16][17];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15, q = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16, whole = g.K / kFp8Block, left = g.K - whole * kFp8Block;
-  const uint8_t* const w = g.w + (int64_t)min(n0 + r, g.N - 1) * g.ldw + 16 * q;
+  const int n0 = (int)blockIdx.x * 16 * COLS, whole = g.K / kFp8Block, left = g.K - whole * kFp8Block;
+  const uint8_t* w[COLS];
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) w[j] = g.w + (int64_t)min(n0 + 16 * j + r, g.N - 1) * g.ldw + 32 * q;
   const uint8_t* const sw = g.sw + (int64_t)(n0 / kFp8Block) * g.sw_r;
   const uint16_t* x[GROUPS];
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) x[i] = g.x + (int64_t)min(16 * i + r, g.M - 1) * g.ldx + 16 * q;
-  f32x4 acc[GROUPS] = {};
-  auto multiply = [&](const RowPart (&p)[GROUPS], const i32x8& b, int ws) {
+  for (int i = 0; i < GROUPS; ++i) x[i] = g.x + (int64_t)min(16 * i + r, g.M - 1) * g.ldx + 32 * q;
+  f32x4 acc[GROUPS][COLS] = {};
+  auto multiply = [&](const RowPart (&p)[GROUPS], const i32x8 (&b)[COLS], int ws) {
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) {
       int xs;
       const i32x8 a = p[i].template codes<T>(xs);
-      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i], 0, 0, 0, xs, 0, ws);
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b[j], acc[i][j], 0, 0, 0, xs, 0, ws);
     }
   };
   for (int k0 = wave; k0 < whole; k0 += WAVES * AHEAD) {
     RowPart p[AHEAD][GROUPS];
-    i32x8 b[AHEAD];
+    i32x8 b[AHEAD][COLS];
     int ws[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int64_t k = k0 + u * WAVES;
       if (k < whole) {
-        b[u] = load_weights(w + k * kFp8Block);
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) b[u][j] = load_weights(w[j] + k * kFp8Block);
         ws[u] = sw[k * g.sw_k];
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) p[u][i].load(x[i] + k * kFp8Block);
@@ -110,31 +115,36 @@ __global__ __launch_bounds__(WAVES * 64, AHEAD == 2 && GROUPS == 1 ? 8 : WAVES /
   if (left && wave == whole % WAVES) {
     RowPart p[GROUPS];
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) p[i].load_some(x[i] + (int64_t)whole * kFp8Block, left - 16 * q);
-    multiply(p, load_weights(w + (int64_t)whole * kFp8Block), sw[(int64_t)whole * g.sw_k]);
+    for (int i = 0; i < GROUPS; ++i) p[i].load_some(x[i] + (int64_t)whole * kFp8Block, left - 32 * q);
+    i32x8 b[COLS];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) b[j] = load_weights(w[j] + (int64_t)whole * kFp8Block);
+    multiply(p, b, sw[(int64_t)whole * g.sw_k]);
   }
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    if (i) __syncthreads();
+  for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sums[wave][4 * q + e][r] = acc[i][e];
-    __syncthreads();
-    if (t < 256) {
-      const int row = t >> 4, n = t & 15, m = 16 * i + row;
-      if (m < g.M && n0 + n < g.N) {
-        float sum = 0.f;
+    for (int j = 0; j < COLS; ++j) {
+      if (i || j) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < WAVES; ++j) sum += sums[j][row][n];
-        g.y[(int64_t)m * g.ldy + n0 + n] = T::from_float(sum);
+      for (int e = 0; e < 4; ++e) sums[wave][4 * q + e][r] = acc[i][j][e];
+      __syncthreads();
+      if (t < 256) {
+        const int row = t >> 4, n = n0 + 16 * j + (t & 15), m = 16 * i + row;
+        if (m < g.M && n < g.N) {
+          float sum = 0.f;
+#pragma unroll
+          for (int o = 0; o < WAVES; ++o) sum += sums[o][row][t & 15];
+          g.y[(int64_t)m * g.ldy + n] = T::from_float(sum);
+        }
       }
     }
-  }
 }
 
 struct FewPlan {
   int groups;  // of 16 rows
   bool wide;   // sixteen waves instead of four
-  bool many;   // more workgroups than CUs: two to a CU, with half of the registers
+  bool many;   // more workgroups than CUs: one row group then takes 32 outputs at a time, which quantizes x half as often
   double us;
 };
 // Sixteen waves a workgroup where the reduction is long.  The time, from 7 layers between 512^2 and 8192^2 at 1 to 64 rows: 5 us, and for
@@ -154,14 +164,15 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
 
 template <typename T>
 void launch_few(const Fp8Few& g, const FewPlan& p, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(g.N, 16)), block(p.wide ? 1024 : 256);
+  const bool two = p.groups == 1 && p.wide && p.many;
+  const dim3 grid((unsigned)ceil_div(g.N, two ? 32 : 16)), block(p.wide ? 1024 : 256);
   if (p.groups == 1) {
-    auto* kernel = !p.wide ? &fp8_few_kernel<T, 4, 1, 4> : p.many ? &fp8_few_kernel<T, 16, 1, 2> : &fp8_few_kernel<T, 16, 1, 4>;
+    auto* kernel = !p.wide ? &fp8_few_kernel<T, 4, 1, 1, 4> : p.many ? &fp8_few_kernel<T, 16, 1, 2, 2> : &fp8_few_kernel<T, 16, 1, 1, 2>;
     hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);
   } else if (p.groups == 2) {
-    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 2, 2> : &fp8_few_kernel<T, 4, 2, 2>), grid, block, 0, stream, g);
-  } else {
-    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 4, 1> : &fp8_few_kernel<T, 4, 4, 1>), grid, block, 0, stream, g);
+    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 2, 1, 2> : &fp8_few_kernel<T, 4, 2, 1, 2>), grid, block, 0, stream, g);
+  } else {  // (a long reduction of that many rows goes through the tiles)
+    hipLaunchKernelGGL((&fp8_few_kernel<T, 4, 4, 1, 1>), grid, dim3(256), 0, stream, g);
   }
 }
 

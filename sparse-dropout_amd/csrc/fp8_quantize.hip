@@ -7,6 +7,7 @@
 // Bound by its reads and writes, 2 bytes in and 1 or 2 out per element, as long as the arithmetic stays out of the way: magnitudes of
 // 16-bit elements are compared two at a time as whole numbers, and the conversion takes two of them and the scale in one
 // instruction (its results are those of multiplying in fp32 and converting, for every 16-bit number within the range).
+// 8192^2 in 128 x 128 blocks 38 us, 5.3 TB/s; an output gradient of that size both ways 60 us, X with half of its blocks dropped and W both ways 74.
 #include "fp8.h"
 
 #include <type_traits>

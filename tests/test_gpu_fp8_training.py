@@ -334,3 +334,48 @@ def test_the_model_harness_runs_layers_in_8_bits_and_the_optimizer(name, optimiz
         assert len(bm.time_model(net, x, warmup=0.0, rep=0.0, graph=graph, optimizer=opt)) >= 5
         assert all(not torch.equal(a, b) for a, b in zip(before, net.parameters()))
         assert {opt.state[q]["step"].item() for q in net.parameters()} != {0}
+
+
+def test_captured_serving_replays():
+    """Quantizing, both routes of the product with kept weights, and the product of two quantized matrices in one graph, on new inputs."""
+    w = spread(1030, 2000, torch.bfloat16, 1).div_(64)
+    few, many = torch.empty(5, 2000, device="cuda").bfloat16(), torch.empty(300, 2000, device="cuda").bfloat16()
+    kept = F.fp8_quantize(w, (128, 128))
+
+    def run():
+        q = F.fp8_quantize(many)
+        return (*(t.view(torch.uint8) for t in q), F.fp8_dequantize(*q, 2000), F.fp8_linear(few, *kept), F.fp8_linear(many, *kept), GEMM().gemm_fp8(*q, *kept))
+
+    def batch(i):
+        few.copy_(spread(5, 2000, torch.bfloat16, 10 + i).div_(64))
+        many.copy_(spread(300, 2000, torch.bfloat16, 20 + i).div_(64))
+
+    batch(0)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i in range(1, 4):
+        batch(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_scales_that_are_no_number():
+    """A scale's byte 255 stands for NaN: all of its block is."""
+    x, w = spread(140, 256, torch.float16).div_(64), spread(300, 256, torch.float16, 1).div_(64)
+    data, scales = F.fp8_quantize(w, (128, 128))
+    want = [F.fp8_linear(x[:rows], data, scales) for rows in (4, 140)]
+    values = F.fp8_dequantize(data, scales)
+    scales.view(torch.uint8)[1, 1] = 255
+    again = F.fp8_dequantize(data, scales)
+    assert again[128:256, 128:].isnan().all()
+    again[128:256, 128:] = values[128:256, 128:]
+    assert torch.equal(again, values)
+    for rows, y in zip((4, 140), want):
+        got = F.fp8_linear(x[:rows], data, scales)
+        assert got[:, 128:256].isnan().all() and torch.equal(got[:, :128], y[:, :128]) and torch.equal(got[:, 256:], y[:, 256:])
