@@ -5,7 +5,7 @@
 // it reads it out of the L2.  A workgroup owns 16 or 32 outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block
 // w + waves * n, a few of them on their way at a time, and meet once in LDS.  Rows come in groups of 16, up to four; what a row behind the
 // last or an output behind the last holds is never stored, so their lanes read another's.  One token through 4096 to 1024 6.3 us, most of it a
-// memory latency and the launch; through 8192 to 8192 FIGURE.
+// memory latency and the launch; through 8192 to 8192 18.7, 3.6 TB/s.
 #include "fp8.h"
 
 namespace sd {
@@ -144,12 +144,13 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void fp8_few_kernel(Fp8Few g
 struct FewPlan {
   int groups;  // of 16 rows
   bool wide;   // sixteen waves instead of four
-  bool many;   // more workgroups than CUs: one row group then takes 32 outputs at a time, which quantizes x half as often
+  bool many;   // more workgroups than CUs: of 32 outputs each, x is read and quantized half as often
   double us;
 };
 // Sixteen waves a workgroup where the reduction is long.  The time, from 7 layers between 512^2 and 8192^2 at 1 to 64 rows: 5 us, and for
-// each 128-block of a wave and group of rows 2.1 with sixteen waves (32 rows through 4096^2 12.8 us, 64 22.5), 1 with four (64
-// through 8192 x 2048 20).
+// each 128-block of a wave and group of rows 2.1 with sixteen waves (32 rows through 4096^2 12.5 us, 64 22.5), 1 with four (64
+// through 8192 x 2048 20).  More workgroups than CUs: 32 outputs each instead of 16 (8192 x 2048: 16 rows 6.7 us instead of 8.5, 32 rows 9.2
+// instead of 12.2; 16 rows through 8192^2 20 instead of 35); with a workgroup or less a CU they would leave CUs idle.
 FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
   FewPlan p;
   const int64_t nk = ceil_div(K, kFp8Block), wgs = ceil_div(N, 16);
@@ -164,13 +165,14 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
 
 template <typename T>
 void launch_few(const Fp8Few& g, const FewPlan& p, hipStream_t stream) {
-  const bool two = p.groups == 1 && p.wide && p.many;
+  const bool two = p.many && (p.groups == 1 || (p.groups == 2 && !p.wide));
   const dim3 grid((unsigned)ceil_div(g.N, two ? 32 : 16)), block(p.wide ? 1024 : 256);
   if (p.groups == 1) {
-    auto* kernel = !p.wide ? &fp8_few_kernel<T, 4, 1, 1, 4> : p.many ? &fp8_few_kernel<T, 16, 1, 2, 2> : &fp8_few_kernel<T, 16, 1, 1, 2>;
+    auto* kernel = !p.wide ? p.many ? &fp8_few_kernel<T, 4, 1, 2, 2> : &fp8_few_kernel<T, 4, 1, 1, 4> : p.many ? &fp8_few_kernel<T, 16, 1, 2, 2> : &fp8_few_kernel<T, 16, 1, 1, 2>;
     hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);
   } else if (p.groups == 2) {
-    hipLaunchKernelGGL((p.wide ? &fp8_few_kernel<T, 16, 2, 1, 2> : &fp8_few_kernel<T, 4, 2, 1, 2>), grid, block, 0, stream, g);
+    auto* kernel = p.wide ? &fp8_few_kernel<T, 16, 2, 1, 2> : p.many ? &fp8_few_kernel<T, 4, 2, 2, 2> : &fp8_few_kernel<T, 4, 2, 1, 2>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, g);
   } else {  // (a long reduction of that many rows goes through the tiles)
     hipLaunchKernelGGL((&fp8_few_kernel<T, 4, 4, 1, 1>), grid, dim3(256), 0, stream, g);
   }
