@@ -623,8 +623,9 @@ int sd_conv2d_taps_dw(const void* x_rows, int64_t x_ld, const void* dy_rows, int
  *   Few rows (16, and up to 64 where N K is not large) run in one launch that reads each weight once and needs no workspace.
  * sd_fp8_dropout_matmul_forward: Y = s (keep (.) X) W^T with X in 1 x 128 and W in 128 x 128 blocks; mask given, or drawn as
  *   sd_random_lists draws it and stored to mask_out [ceil(M/bs), ceil(K/bs)].  Dropped blocks are neither quantized nor multiplied.
- *   XT (a [K, M] matrix) and WT (a square [K, N] one), each NULL where its gradient is not wanted, receive what the backward reads: X in blocks along the tokens,
- *   for dW sums over them, and W turned.  block_size: multiples of 128 (SD_ERR_UNSUPPORTED otherwise).
+ *   XT (a [K, M] matrix) and WT (a square [K, N] one), each NULL where its gradient is not wanted, receive what the backward
+ *   reads: X in blocks along the tokens, for dW sums over them, and W turned.  block_size: multiples of 128
+ *   (SD_ERR_UNSUPPORTED otherwise).
  * sd_fp8_dropout_matmul_backward: dX = s (dY W) (.) keep (zeros in dropped blocks) from WT and / or dW = s dY^T (keep (.) X) from XT, dY
  *   quantized in blocks along the features for the one and along the tokens for the other.
  * Workspaces: as many bytes as the .._workspace_bytes functions say, on 16 bytes, and of one call at a time.
