@@ -379,3 +379,15 @@ def test_scales_that_are_no_number():
     for rows, y in zip((4, 140), want):
         got = F.fp8_linear(x[:rows], data, scales)
         assert got[:, 128:256].isnan().all() and torch.equal(got[:, :128], y[:, :128]) and torch.equal(got[:, 256:], y[:, 256:])
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("n,k", [(4110, 2200), (4097, 130), (8200, 2048), (500, 2200), (4112, 4100)])
+def test_few_rows_of_wide_and_narrow_layers(n, k, rows):
+    """Whole numbers up to 8, exact in 8 bits and in fp32 sums: 16 and 32 outputs a workgroup, four and sixteen waves, each with a ragged end."""
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    make = lambda *size: torch.randint(-8, 9, size, generator=gen, device="cuda").bfloat16()  # noqa: E731
+    w, buf = make(n, k), make(rows, k + 3)
+    kept = F.fp8_quantize(w, (128, 128))
+    for x in (buf[:, :k].contiguous(), buf[:, 3:]):
+        assert torch.equal(F.fp8_linear(x, *kept), (x.double() @ w.double().t()).bfloat16())
