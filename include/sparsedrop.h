@@ -612,7 +612,8 @@ int sd_conv2d_taps_dw(const void* x_rows, int64_t x_ld, const void* dy_rows, int
  * whole 128-blocks (columns behind the last are zeros), and a power of two for each block of 1 x 128 or 128 x 128, as
  * the byte exponent + 127 (e8m0).  The scale is the least one with which the block's largest finite magnitude stays within 448;
  * 127 for a block of zeros, 0 at least.  Values are rounded to nearest, halves to the even code; what is not finite becomes NaN.
- * Scales of 1 x 128 blocks that a product reads lie 128-block by 128-block: scale of (row, block k) at [k * ld + row].
+ * Scales of 1 x 128 blocks that a product reads lie 128-block by 128-block: scale of (row, block k) at [k * ld + row].  Nothing is read behind
+ * the 4 bytes that hold the last one, so they may be those of some rows of a larger matrix.
  *
  * The calls that make matrices for themselves hold them in one buffer each, of sd_fp8_matrix_bytes bytes on 16 bytes: pass it on as
  * it was filled.  square: blocks of 128 x 128.

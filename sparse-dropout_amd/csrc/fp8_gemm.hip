@@ -13,6 +13,7 @@
 // are then one word of the row order, in the lane that needs them, and the instruction picks its byte of it.  The sums come out in
 // patches of four rows by four columns a lane, so C is stored from registers in whole 128-byte lines along either index.
 #include "fp8.h"
+#include "fp8_scales.h"
 #include "gemm_device.h"
 #include "tile_map.h"
 
@@ -247,8 +248,8 @@ __device__ __forceinline__ void mid_tile(const Args& p, int block, char* smem) {
   const int wm = c >> 1, wn = c & 1;
   const BlockRows rows_a(g.lda, lane), rows_b(g.ldb, lane);
   const u32x4 of_a = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_b = block_buffer(g.b + n0 * g.ldb, g.ldb, g.N - n0);
-  const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
-  const u32x4 bb = SQUARE ? buffer_over(g.sb + tn * g.sb_r, (int64_t)(p.nk - 1) * g.sb_k + 1) : buffer_over(g.sb + n0, (int64_t)p.nk * g.sb_k - n0);
+  const u32x4 ba = buffer_over(g.sa + m0, row_scales_left(p.nk, g.sa_ld, g.M, m0));
+  const u32x4 bb = SQUARE ? buffer_over(g.sb + tn * g.sb_r, (int64_t)(p.nk - 1) * g.sb_k + 1) : buffer_over(g.sb + n0, row_scales_left(p.nk, g.sb_k, g.N, n0));
   const uint32_t lds = lds_address(smem);
   const int per_step = c < 2 ? 9 : 8;  // loads of this wave
   auto step_block = [&](int s) { return MODE == kFp8Dsd ? __builtin_amdgcn_readfirstlane((int)(list[s] & 0xffffu)) : lo + s; };
@@ -404,9 +405,9 @@ __global__ __launch_bounds__(512, 2) void fp8_big_kernel(Args p) {
   const BlockRows rows(grp == 0 ? g.ldb : g.lda, lane);
   const u32x4 of_b = block_buffer(g.b + n_mine * g.ldb, g.ldb, g.N - n_mine);
   const u32x4 of_a0 = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_a1 = block_buffer(g.a + (m0 + kB) * g.lda, g.lda, g.M - m0 - kB);
-  const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
+  const u32x4 ba = buffer_over(g.sa + m0, row_scales_left(p.nk, g.sa_ld, g.M, m0));
   const u32x4 bb = SQUARE ? buffer_over(g.sb, (int64_t)(col_blocks - 1) * g.sb_r + (int64_t)(p.nk - 1) * g.sb_k + 1)
-                          : buffer_over(g.sb + c0, (int64_t)p.nk * g.sb_k - c0);
+                          : buffer_over(g.sb + c0, row_scales_left(p.nk, g.sb_k, g.N, c0));
   const uint32_t square_at = SQUARE ? (uint32_t)((lane < 32 ? c0 : c1) / kB * g.sb_r) : 0u;
   const uint32_t lds = lds_address(smem);
   auto load_b = [&](int s, int k) {
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(512, 2) void fp8_duo_kernel(Args p) {
   // a wave loads a quarter of A's block and half of its column block
   const BlockRows rows_a(g.lda, lane), rows_b(g.ldb, lane);
   const u32x4 of_a = block_buffer(g.a + m0 * g.lda, g.lda, g.M - m0), of_b = block_buffer(g.b + n_mine * g.ldb, g.ldb, g.N - n_mine);
-  const u32x4 ba = buffer_over(g.sa + m0, (int64_t)p.nk * g.sa_ld - m0);
+  const u32x4 ba = buffer_over(g.sa + m0, row_scales_left(p.nk, g.sa_ld, g.M, m0));
   const u32x4 bb = buffer_over(g.sb, (int64_t)(col_blocks - 1) * g.sb_r + (int64_t)(p.nk - 1) * g.sb_k + 1);
   const uint32_t square_at = (uint32_t)((lane < 32 ? c0 : c1) / kB * g.sb_r);
   const uint32_t lds = lds_address(smem);

@@ -1,10 +1,14 @@
 """What the products in 8 bits and AdamW refuse before anything runs on a GPU, and the sizes that they ask for."""
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
 
 from oracle import fp8_oracle as O
+
+ROOT = Path(__file__).resolve().parent.parent
 
 
 @pytest.fixture(scope="module")
@@ -232,3 +236,51 @@ def test_the_states_random_bits_leave_averages_right_on_average():
         got = O.np.delete(got, O.np.arange(0, n, 128), 1)
         assert set(O.np.unique(got)) == {16.0, 18.0}
         assert abs((got == 18.0).mean() - 0.25) <= 0.0104  # (a 128th of them are the large ones)
+
+
+_SCALE_READS = r"""
+#include <stdio.h>
+#include <initializer_list>
+#include "fp8_scales.h"
+
+static long n_words = 0, n_cut = 0;
+
+// What the lanes of a tile of `tile` rows from `first` on ask for, a word each in every 128-block, of scales that are not followed by
+// anything: a word is read if it ends within the bound, whole words only.
+static bool holds(int64_t nk, int64_t ld, int64_t rows, int64_t first, int64_t tile) {
+  const int64_t left = sd::row_scales_left(nk, ld, rows, first), end = (nk - 1) * ld + rows;
+  for (int64_t k = 0; k < nk; ++k)
+    for (int64_t lane = 0; lane < tile / 4; ++lane) {
+      const int64_t off = k * ld + 4 * lane, row = first + 4 * lane;
+      const bool read = off + 4 <= left;
+      ++n_words;
+      n_cut += !read;
+      if (read && first + off >= end) return false;  // the word holds nothing that is there
+      if (!read && row < rows) return false;         // a row of the matrix is missing
+    }
+  return true;
+}
+
+int main() {
+  for (int64_t nk : {1, 2, 3, 9})
+    for (int64_t rows = 1; rows <= 600; rows += rows < 270 ? 1 : 37)
+      for (int64_t more : {0, 4, 12, 16, 128, 7916})
+        for (int64_t tile : {128, 256})
+          for (int64_t first = 0; first < rows; first += tile) {
+            const int64_t ld = (rows + 3) / 4 * 4 + more;
+            if (holds(nk, ld, rows, first, tile)) continue;
+            printf("%ld blocks of %ld rows, %ld apart, tile of %ld from %ld\n", (long)nk, (long)rows, (long)ld, (long)tile, (long)first);
+            return 1;
+          }
+  return n_words < 1000000 || n_cut < 10000;
+}
+"""
+
+
+def test_row_scales_are_not_read_behind_their_end(tmp_path):
+    """Scales of some rows of a larger matrix (csrc/fp8_scales.h): the last 128-block's row of them may be the end of the memory."""
+    (tmp_path / "sweep.cpp").write_text(_SCALE_READS)
+    subprocess.run(["g++", "-O2", "-std=c++17", f"-I{ROOT / 'sparse-dropout_amd' / 'csrc'}", str(tmp_path / "sweep.cpp"), "-o",
+                    str(tmp_path / "sweep")], check=True)
+    proc = subprocess.run([str(tmp_path / "sweep")], capture_output=True, text=True, timeout=100)
+    assert proc.returncode == 0, proc.stdout

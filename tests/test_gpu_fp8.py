@@ -200,6 +200,29 @@ def test_product_of_two_quantized_matrices(m, k, n, b_block):
     assert torch.equal(GEMM().gemm_fp8(data, scales.view(torch.uint8).contiguous().view(torch.float8_e8m0fnu), *F.fp8_quantize(b, b_block), torch.float16), c)
 
 
+@pytest.mark.parametrize("k", [100, 128, 1000])
+@pytest.mark.parametrize("m,n,a_rows,b_rows", [(700, 640, slice(500, 700), slice(512, 640)), (513, 300, slice(4, 513), slice(0, 127)),
+                                               # 128 x 128 and 256 x 256 tiles that end inside; one that starts off a word
+                                               (300, 500, slice(8, 263), slice(128, 387)), (8200, 8192, slice(4097, 8200), slice(4096, 8192)),
+                                               (8192, 8300, slice(4000, 8192), slice(128, 8300))])
+def test_products_of_some_rows_of_quantized_matrices(m, n, k, a_rows, b_rows):
+    """Codes and scales are sliced where they lie; the results are those rows and columns of the product of matrices of their own."""
+    a, b = spread(m, k, torch.float32, 1) / 256, spread(n, k, torch.float32, 2)
+    for b_block in ((1, 128), (128, 128)):
+        if b_block[0] == 128:
+            b_rows = slice(b_rows.start // 128 * 128, b_rows.stop)
+        qa, qb = F.fp8_quantize(a), F.fp8_quantize(b, b_block)
+        sb = slice(b_rows.start // b_block[0], -(-b_rows.stop // b_block[0]))
+        c = GEMM().gemm_fp8(qa[0][a_rows], qa[1][a_rows], qb[0][b_rows], qb[1][sb], torch.float16)
+        own_a, own_b = (qa[0][a_rows].clone(), qa[1][a_rows].contiguous()), (qb[0][b_rows].clone(), qb[1][sb].contiguous())
+        assert torch.equal(c, GEMM().gemm_fp8(*own_a, *own_b, torch.float16))
+        rows, cols = torch.arange(m)[a_rows][::61], torch.arange(n)[b_rows][::53]
+        va, vb = F.fp8_dequantize(*qa, k)[rows.cuda()], F.fp8_dequantize(*qb, k)[cols.cuda()]
+        sums = O.magnitudes(np64(a), 1)[rows] @ O.magnitudes(np64(b), b_block[0])[cols].T
+        picked = c[(rows - a_rows.start).cuda()][:, (cols - b_rows.start).cuda()]
+        check_product(picked, np64(va) @ np64(vb).T, sums, k, torch.float16)
+
+
 # ---- training ---------------------------------------------------------------------------------------------------------------
 def train(m, k, n, dtype, bs, p, seed=0, mask=None):
     gen = torch.Generator().manual_seed(seed)
