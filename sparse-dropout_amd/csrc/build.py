@@ -46,11 +46,15 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.hip"))
 
 
+def _compiled_files() -> list[Path]:
+    return [*sources(), *sorted(CSRC.glob("*.cpp")), *sorted(CSRC.glob("*.h")), *sorted((ROOT / "include").glob("*.h"))]
+
+
 def source_hash() -> str:
     """Hash of everything the library is compiled from; the library reports the one it was built with
     (sd_source_hash) and the loader refuses a library whose sources have changed since."""
     h = hashlib.sha256()
-    for f in [*sources(), *sorted(CSRC.glob("*.cpp")), *sorted(CSRC.glob("*.h")), *sorted((ROOT / "include").glob("*.h"))]:
+    for f in _compiled_files():
         h.update(f.name.encode())
         h.update(f.read_bytes())
     return h.hexdigest()[:16]
@@ -71,11 +75,11 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"command failed: {' '.join(cmd)}\n{proc.stdout}\n{err}")
 
 
-def write_source_hash() -> Path:
+def write_source_hash(value: str) -> Path:
     """(Re)writes the generated header api.hip includes; touched only when the hash changes."""
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     inc = OBJ_DIR / "source_hash.inc"
-    line = f'#define SD_SOURCE_HASH "{source_hash()}"\n'
+    line = f'#define SD_SOURCE_HASH "{value}"\n'
     if not inc.exists() or inc.read_text() != line:
         inc.write_text(line)  # newer than api.o: api.hip, which includes it, is recompiled by build()
     return inc
@@ -101,31 +105,44 @@ def bridge_command() -> list[str]:
 def build(force: bool = False, verbose: bool = False) -> Path:
     OUT_DIR.mkdir(parents=True, exist_ok=True)
     headers = sorted(CSRC.glob("*.h")) + sorted((ROOT / "include").glob("*.h"))
-    hash_inc = write_source_hash()  # included by api.hip (and the bridge) only
-    began_with = source_hash()
-    jobs = []
+    def state():
+        return source_hash(), [f.stat().st_mtime_ns for f in _compiled_files()]
+
+    began_with = state()
+    hash_inc = write_source_hash(began_with[0])  # included by api.hip (and the bridge) only
+    jobs = {}  # object -> (its name while it is made, command)
     objs = []
     for src in sources():
         obj = OBJ_DIR / (src.stem + ".o")
         objs.append(obj)
         if force or _stale(obj, [src, *headers, *([hash_inc] if src.stem == "api" else [])]):
-            jobs.append([HIPCC, *FLAGS, "-c", str(src), "-o", str(obj)])
+            made = OBJ_DIR / f"{src.stem}.{os.getpid()}.o"
+            jobs[obj] = made, [HIPCC, *FLAGS, "-c", str(src), "-o", str(made)]
     if verbose:
-        for j in jobs:
+        for _, j in jobs.values():
             print(" ".join(j), flush=True)
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(_run, jobs))
+        done = {obj: ex.submit(_run, j) for obj, (_, j) in jobs.items()}
+    # A source is compiled twice, for the GPU and for the host: edited in between, a launch names a kernel that is not there, which
+    # aborts the process.  Such an object is newer than its source and would pass for up to date ever after: objects get their names only
+    # once the sources are seen to be what they were.
+    changed = state() != began_with
+    for obj, job in done.items():
+        made = jobs[obj][0]
+        if changed or job.exception():
+            made.unlink(missing_ok=True)
+        else:
+            made.replace(obj)
+    if changed:
+        raise RuntimeError("the sources changed while they were compiled: build again")
+    for job in done.values():
+        job.result()
     if force or jobs or _stale(LIB, objs):
         _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-soname,libsparsedrop.so", "-o", str(LIB),
               *map(str, objs)])
     # (the bridge carries the hash of all sources too, so it follows every change of the library)
     if force or _stale(BRIDGE, [BRIDGE_SRC, LIB, hash_inc]):
         _run(bridge_command())
-    # A source is compiled twice, for the GPU and for the host: edited in between, a launch names a kernel that is not there, which
-    # aborts the process.
-    if source_hash() != began_with:
-        LIB.unlink()
-        raise RuntimeError("the sources changed while they were compiled: build again")
     return LIB
 
 

@@ -493,6 +493,74 @@ def test_loader_refuses_a_library_built_from_other_sources(monkeypatch):
         _loader.load.__wrapped__()
 
 
+_COMPILER = r"""#!/bin/sh
+# stands in for hipcc: an object is its source as the GPU's pass and as the host's pass read it, a library its objects; "$EDIT" is run in between
+# once, and sources that say so do not compile
+while [ $# -gt 0 ]; do
+  case "$1" in
+    -c) src="$2"; shift ;;
+    -o) out="$2"; shift ;;
+    *.o) objs="$objs $1" ;;
+  esac
+  shift
+done
+if [ -z "$src" ]; then exec cat $objs > "$out"; fi
+export out
+echo "$src" >> "$LOG"
+cp "$src" "$out"
+case "$src" in */kernel.hip) if [ -e "$EDIT" ]; then sh "$EDIT"; rm -f "$EDIT"; fi ;; esac
+cat "$src" >> "$out"
+! grep -q error "$src"
+"""
+
+
+@pytest.mark.parametrize("edit", ["source", "source and back", "header", "source and another does not compile"])
+def test_a_source_edited_while_it_was_compiled_is_compiled_again(edit, tmp_path, monkeypatch):
+    import importlib.util
+    import os
+
+    spec = importlib.util.spec_from_file_location("build_under_test", ROOT / "sparse-dropout_amd" / "csrc" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    csrc, objs, out = tmp_path / "csrc", tmp_path / "csrc" / "build", tmp_path / "_lib"
+    for d in (csrc, tmp_path / "include"):
+        d.mkdir()
+    (tmp_path / "cc").write_text(_COMPILER)
+    (tmp_path / "cc").chmod(0o755)
+    for name, value in dict(CSRC=csrc, ROOT=tmp_path, OBJ_DIR=objs, OUT_DIR=out, LIB=out / "lib.so", BRIDGE=out / "bridge.so",
+                            BRIDGE_SRC=csrc / "bridge.cpp", HIPCC=str(tmp_path / "cc"), bridge_command=lambda: ["touch", str(out / "bridge.so")]).items():
+        monkeypatch.setattr(build, name, value)
+    monkeypatch.setenv("EDIT", str(tmp_path / "edit"))
+    monkeypatch.setenv("LOG", str(tmp_path / "log"))
+    for name, text in {"kernel.hip": "old\n", "api.hip": "api\n", "other.hip": "error\n" if "another" in edit else "other\n", "k.h": "h\n",
+                       "bridge.cpp": "b\n"}.items():
+        (csrc / name).write_text(text)
+    commands = {"source": f"echo new > {csrc}/kernel.hip", "header": f"echo new > {csrc}/k.h",
+                "source and back": f"echo new > {csrc}/kernel.hip; cat {csrc}/kernel.hip >> $out; echo old > {csrc}/kernel.hip"}
+    (tmp_path / "edit").write_text(commands.get(edit, commands["source"]))
+    with pytest.raises(RuntimeError, match="changed while they were compiled"):
+        build.build()
+    (csrc / "other.hip").write_text("other\n")
+    now = (csrc / "kernel.hip").read_text()
+    (tmp_path / "log").write_text("")
+    assert build.build() == out / "lib.so"
+    assert f"{csrc}/kernel.hip" in (tmp_path / "log").read_text()
+    assert (objs / "kernel.o").read_text() == 2 * now
+    assert 2 * now in (out / "lib.so").read_text()
+    assert sorted(os.listdir(objs)) == ["api.o", "kernel.o", "other.o", "source_hash.inc"]
+    # what is up to date is kept, and so is what did compile beside what did not
+    (tmp_path / "log").write_text("")
+    build.build()
+    assert (tmp_path / "log").read_text() == ""
+    (csrc / "kernel.hip").write_text("newer\n")
+    (csrc / "other.hip").write_text("error\n")
+    for f in ("kernel", "other"):  # (a file system's clock may tick once for both)
+        os.utime(csrc / f"{f}.hip", ns=(2 * 10 ** 18,) * 2)
+    with pytest.raises(RuntimeError, match="command failed"):
+        build.build()
+    assert (objs / "kernel.o").read_text() == 2 * "newer\n"
+
+
 def test_as_matrix_lays_out_expanded_and_strided_views():
     from flash_dropout.hip.binding_gemm import _mat, as_matrix
 
