@@ -18,6 +18,7 @@ from collections.abc import Sequence
 import torch
 
 from ..hip import _loader
+from .tracing import refused_under_trace
 
 STATE_BLOCK = 128  # elements of a state in 8 bits that share a scale
 
@@ -33,13 +34,14 @@ def _split(averages, name):
     return [a[0] for a in averages], [a[1] for a in averages]
 
 
+@refused_under_trace
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence,
                step: torch.Tensor, *, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2) -> None:
     """Updates ``params`` (float16, bfloat16 or float32, also mixed), both averages and ``step`` in place.  The averages are float32
     tensors laid out like their parameters or ``(codes, scales)`` pairs of uint8 tensors.  ``step``: one int64 on the GPU, the
     number of steps so far, moved on by the call itself: a captured graph counts its replays.  ``lr`` may be a float32 tensor on the
-    GPU, which a captured graph reads at every replay.  One launch for each 56 tensors of a dtype."""
+    GPU, which a captured graph reads at every replay.  One launch for each 56 tensors of a dtype.  ``torch.jit.trace`` is refused."""
     beta1, beta2 = (float(b) for b in betas)
     firsts, first_scales = _split(exp_avgs, "exp_avgs")
     seconds, second_scales = _split(exp_avg_sqs, "exp_avg_sqs")
@@ -50,6 +52,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                                 0.0 if at is not None else float(lr), beta1, beta2, float(eps), float(weight_decay))
 
 
+@refused_under_trace
 def adamw_state_values(exp_avgs: Sequence, exp_avg_sqs: Sequence) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
     """Averages in 8 bits, ``(codes, scales)`` pairs, as float32 tensors of the codes' shapes, in one launch for each 56 of them."""
     firsts, first_scales = _split(exp_avgs, "exp_avgs")

@@ -23,22 +23,25 @@ import torch
 from ..hip import _loader
 from ..hip.binding_gemm import _block_size
 from .blockwise_dropout_matmul_hip import draw_source
-from .tracing import _RecordedPlainCall, traceable
+from .tracing import _RecordedConstantCall, _RecordedPlainCall, traceable
 
 
+@traceable(recorded=_RecordedConstantCall, cast=False)
 def fp8_quantize(x: torch.Tensor, block=(1, 128)) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of a float16, bfloat16 or float32 matrix, in blocks of (1, 128) or (128, 128).  The scales of (1, 128)
-    blocks lie one 128-block's after the other in memory (strides (1, n)), as the products read them."""
+    blocks lie one 128-block's after the other in memory (strides (1, n)), as the products read them.  They carry no gradient."""
     block = tuple(block)
     if block not in ((1, 128), (128, 128)):
         raise ValueError(f"block must be (1, 128) or (128, 128), got {block}")
     return _loader.bridge().fp8_quantize(x, block[0])
 
 
+@traceable(recorded=_RecordedConstantCall, cast=False)
 def fp8_dequantize(data: torch.Tensor, scales: torch.Tensor, cols: int | None = None,
                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of codes and scales as ``dtype``: the first ``cols`` columns (default: all, the zeros behind the last too)."""
-    return _loader.bridge().fp8_dequantize(data, scales, cols, dtype)
+    # (an extent that a trace takes off a tensor is a tensor itself)
+    return _loader.bridge().fp8_dequantize(data, scales, int(cols) if isinstance(cols, torch.Tensor) else cols, dtype)
 
 
 @traceable(recorded=_RecordedPlainCall)

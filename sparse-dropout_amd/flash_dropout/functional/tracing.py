@@ -66,11 +66,26 @@ class _RecordedPlainCall(torch.autograd.Function):
         raise NotImplementedError("the traced function has no gradient: call it under torch.no_grad()")
 
 
-def traceable(function=None, *, recorded=_RecordedCall):
-    """Makes a function of tensors that calls native code one recorded operation under ``torch.jit.trace``."""
+class _RecordedConstantCall(torch.autograd.Function):
+    """Of a function whose results carry no gradient."""
+
+    @staticmethod
+    def forward(ctx, call, *tensors):
+        results = call([t.detach() for t in tensors])
+        ctx.mark_non_differentiable(*(results if isinstance(results, tuple) else (results,)))
+        return results
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return (None,) * len(ctx.needs_input_grad)
+
+
+def traceable(function=None, *, recorded=_RecordedCall, cast=True):
+    """Makes a function of tensors that calls native code one recorded operation under ``torch.jit.trace``.  cast: under autocast it takes
+    its operands in autocast's dtype."""
 
     if function is None:
-        return functools.partial(traceable, recorded=recorded)
+        return functools.partial(traceable, recorded=recorded, cast=cast)
 
     @functools.wraps(function)
     def run(*args, **kwargs):
@@ -78,7 +93,7 @@ def traceable(function=None, *, recorded=_RecordedCall):
             return function(*args, **kwargs)
         tensors: list[torch.Tensor] = []
         names, values = list(kwargs), _take([*args, *kwargs.values()], tensors)
-        if torch.is_autocast_enabled("cuda"):  # the casts are the trace's own
+        if cast and torch.is_autocast_enabled("cuda"):  # the casts are the trace's own
             dtype = torch.get_autocast_dtype("cuda")
             tensors = [t.to(dtype) if t.is_floating_point() and t.element_size() > 1 else t for t in tensors]  # (8-bit codes stay)
 
@@ -87,5 +102,17 @@ def traceable(function=None, *, recorded=_RecordedCall):
             return function(*filled[:len(args)], **dict(zip(names, filled[len(args):])))
 
         return recorded.apply(call, *tensors)
+
+    return run
+
+
+def refused_under_trace(function):
+    """Of a function that a trace would record none of: it writes its arguments, or lists of any length are what it takes and gives."""
+
+    @functools.wraps(function)
+    def run(*args, **kwargs):
+        if _is_tracing():
+            raise NotImplementedError(f"{function.__name__} cannot be traced")
+        return function(*args, **kwargs)
 
     return run

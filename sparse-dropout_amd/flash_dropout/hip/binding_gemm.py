@@ -558,7 +558,9 @@ class GEMM:
     def gemm_fp8(self, A: torch.Tensor, A_scales: torch.Tensor, B: torch.Tensor, B_scales: torch.Tensor,
                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """Dense ``A @ B.T`` of matrices in 8 bits (codes and scales as ``flash_dropout.functional.fp8_quantize`` gives them): A in
-        (1, 128) blocks, B in (1, 128) or (128, 128) blocks, fp32 sums, the result in ``dtype``."""
+        (1, 128) blocks, B in (1, 128) or (128, 128) blocks, fp32 sums, the result in ``dtype``.  ``torch.jit.trace`` is refused."""
+        if torch._C._is_tracing():  # (it would record the allocation of the result and nothing that fills it)
+            raise NotImplementedError("gemm_fp8 cannot be traced")
         return _loader.bridge().fp8_gemm(A, A_scales, B, B_scales, dtype)
 
     # ------------------------------------------------------------------ the autograd function's two calls

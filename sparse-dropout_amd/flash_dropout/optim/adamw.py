@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from ..functional.adamw import adamw_empty_state, adamw_state_values, adamw_step
+from ..functional.tracing import refused_under_trace
 
 
 class AdamW(torch.optim.Optimizer):
@@ -51,6 +52,7 @@ class AdamW(torch.optim.Optimizer):
     def _averages(states, key):
         return [(s[key], s[key + "_scale"]) if key + "_scale" in s else s[key] for s in states]
 
+    @refused_under_trace
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

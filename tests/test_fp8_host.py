@@ -284,3 +284,48 @@ def test_row_scales_are_not_read_behind_their_end(tmp_path):
                     str(tmp_path / "sweep")], check=True)
     proc = subprocess.run([str(tmp_path / "sweep")], capture_output=True, text=True, timeout=100)
     assert proc.returncode == 0, proc.stdout
+
+
+def test_traces_record_the_quantizer_and_refuse_the_optimizer(monkeypatch):
+    """Around stand-ins for the native calls, whose results are filled behind torch's back."""
+    import flash_dropout.functional as F
+    from flash_dropout.functional import adamw, fp8_blocks
+    from flash_dropout.hip import GEMM
+    from flash_dropout.optim import AdamW
+
+    class Bridge:
+        @staticmethod
+        def fp8_quantize(x, rows):
+            data, scales = torch.empty(x.shape), torch.empty(x.shape[0], 1)
+            data.numpy()[:], scales.numpy()[:] = x.detach().numpy(), rows
+            return data.to(torch.float8_e4m3fn), scales.to(torch.float8_e8m0fnu)
+
+        @staticmethod
+        def fp8_dequantize(data, scales, cols, dtype):
+            out = torch.empty(data.shape[0], cols)
+            out.numpy()[:] = data.float().numpy()[:, :cols] * scales.float().numpy()
+            return out.to(dtype)
+
+        adamw_step = adamw_state_values = staticmethod(lambda *args: [])
+
+    for module in (fp8_blocks, adamw):
+        monkeypatch.setattr(module._loader, "bridge", lambda: Bridge)
+
+    def f(x):
+        data, scales = F.fp8_quantize(x, block=(128, 128))
+        return data.float(), scales.float(), F.fp8_dequantize(data, scales, x.shape[1], torch.float64) * 2
+
+    make = lambda start: torch.arange(start, start + 8.0).view(2, 4)  # noqa: E731
+    for wanted in (False, True):  # (the results carry no gradient, traced or not)
+        traced = torch.jit.trace(f, (make(0).requires_grad_(wanted),), check_trace=False)
+        got, want = traced(make(4).requires_grad_(wanted)), f(make(4).requires_grad_(wanted))
+        assert all(torch.equal(a, b) and not a.requires_grad and not b.requires_grad for a, b in zip(got, want))
+        assert want[2].dtype == torch.float64 and want[2][1, 3] == 2 * 128 * 11
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.zeros(3)
+    step = torch.zeros((), dtype=torch.int64)
+    for call in (lambda x: F.adamw_step([x], [x], [x], [x], step) or x, lambda x: F.adamw_state_values([(x, x)], [(x, x)]) and x,
+                 lambda x: AdamW([p]).step() or x, lambda x: GEMM().gemm_fp8(x, x, x, x)):
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            torch.jit.trace(call, (torch.zeros(3),), check_trace=False)
+    F.adamw_step([p], [p], [p], [p], step)

@@ -225,6 +225,39 @@ def test_forward_gradients_and_transforms_are_refused_and_traces_run():
         traced(other[0]).float().sum().backward()
 
 
+def test_traces_quantize_what_they_are_given():
+    """Codes, scales and values of the traced program's own inputs, whichever of its parts were traced; autocast changes none."""
+    x, other = spread(70, 300, torch.float32).div_(64), spread(70, 300, torch.float32, 5).div_(64)
+    w = torch.nn.Parameter(spread(140, 300, torch.float16, 2).div_(64))
+
+    def values(a):
+        data, scales = F.fp8_quantize(a)
+        return data.float(), scales.float(), F.fp8_dequantize(data, scales, a.shape[1], torch.bfloat16)
+
+    def served(a, b):  # (a weight that wants a gradient does not pass it on to its codes)
+        return F.fp8_linear(a, *F.fp8_quantize(b, (128, 128)))
+
+    traced = torch.jit.trace(values, (x,), check_trace=False)
+    for a in (other, other[:31]):
+        assert all(torch.equal(s, t) for s, t in zip(traced(a), values(a)))
+    with torch.autocast("cuda", torch.bfloat16):
+        cast = torch.jit.trace(values, (x,), check_trace=False)
+        assert all(torch.equal(s, t) for s, t in zip(cast(other), values(other)))
+    assert all(torch.equal(s, t) for s, t in zip(cast(other), values(other)))
+    traced = torch.jit.trace(served, (x.half(), w), check_trace=False)
+    for _ in range(2):
+        assert torch.equal(traced(other.half(), w), served(other.half(), w))
+        with torch.no_grad():
+            w.mul_(3)
+    p = torch.nn.Parameter(torch.zeros(3, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], state_bits=8)
+    opt.step()
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        torch.jit.trace(lambda a: opt.step() or a, (x,), check_trace=False)
+    assert opt.state[p]["step"].item() == 1
+
+
 def test_under_autocast_kept_weights_take_inputs_in_32_bits():
     x = spread(40, 256, torch.float32).div_(64)
     kept = F.fp8_quantize(spread(140, 256, torch.float16, 2), (128, 128))
