@@ -1260,6 +1260,7 @@ std::tuple<Tensor, Tensor> fp8_quantize(const Tensor& x_, int64_t block_rows) {
   TORCH_CHECK_VALUE(x_.is_cuda(), "x must be on the GPU (got ", x_.device(), ")");
   TORCH_CHECK_VALUE(x_.dim() == 2, "x must be 2D (got ", x_.dim(), "D)");
   const int dtype = dtype_with_f32("x", x_);
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(x_), "the quantizer has no jvp: forward mode AD is not supported");
   at::NoGradGuard no_grad;
   const Tensor x = as_matrix(x_);
   const int64_t rows = x.size(0), cols = x.size(1), nk = ceil_div(cols, kFp8), ld = ceil_div(rows, 16) * 16;

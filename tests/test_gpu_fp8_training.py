@@ -225,6 +225,22 @@ def test_forward_gradients_and_transforms_are_refused_and_traces_run():
         traced(other[0]).float().sum().backward()
 
 
+def test_the_quantizer_refuses_forward_gradients_and_transforms():
+    import torch.autograd.forward_ad as fwd
+
+    x = spread(70, 300, torch.float32)
+    for block in ((1, 128), (128, 128)):
+        with fwd.dual_level():
+            with pytest.raises(NotImplementedError, match="jvp"):
+                F.fp8_quantize(fwd.make_dual(x, torch.ones_like(x)), block)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.func.jvp(lambda a: F.fp8_dequantize(*F.fp8_quantize(a, block)), (x,), (x,))
+        with pytest.raises((RuntimeError, NotImplementedError, ValueError)):
+            torch.func.vmap(lambda a: F.fp8_dequantize(*F.fp8_quantize(a, block)))(torch.stack([x, x]))
+    data, scales = F.fp8_quantize(x.requires_grad_())
+    assert not data.requires_grad and not scales.requires_grad
+
+
 def test_traces_quantize_what_they_are_given():
     """Codes, scales and values of the traced program's own inputs, whichever of its parts were traced; autocast changes none."""
     x, other = spread(70, 300, torch.float32).div_(64), spread(70, 300, torch.float32, 5).div_(64)
