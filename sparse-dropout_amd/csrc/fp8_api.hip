@@ -296,6 +296,7 @@ int sd_fp8_dropout_matmul_forward(const void* X, int64_t xsr, int64_t xsc, const
   if (mask) {
     SD_REQUIRE(msr >= 1 && msc >= 1 && (msr == 1 || msc == 1), "%s: mask must be row or column major", fn);
   } else {
+    SD_REQUIRE((float)p < 1.f, "%s: p must be in [0, 1) in 32 bits to draw a mask (got %.17g)", fn, p);
     SD_REQUIRE(mask_out != nullptr, "%s: null mask_out", fn);
     SD_REQUIRE(rng_state == nullptr || reinterpret_cast<uintptr_t>(rng_state) % 8 == 0, "%s: state must be an aligned device pointer", fn);
   }

@@ -238,6 +238,18 @@ def test_the_states_random_bits_leave_averages_right_on_average():
         assert abs((got == 18.0).mean() - 0.25) <= 0.0104  # (a 128th of them are the large ones)
 
 
+def test_drop_rates_that_round_to_one_draw_no_mask(lib):
+    """The draw compares in 32 bits and would drop everything; a mask that is given has no rate to be drawn by."""
+    def fwd(p, mask, out, ws):
+        return lib.sd_fp8_dropout_matmul_forward(FAKE, 256, 1, FAKE, 256, 1, FAKE, 20, 1, mask, 2, 1, None, 0, 0, p, out, None, None, 10, 20, 256, 128, 0,
+                                                 ws, 1 << 40, None)
+
+    for p in (1 - 2.0 ** -26, 1 - 2.0 ** -53):
+        refused(lib, fwd(p, None, FAKE, FAKE), INVALID, b"in 32 bits")
+        refused(lib, fwd(p, FAKE, None, None), INVALID, b"workspace")
+    refused(lib, fwd(1 - 2.0 ** -24, None, FAKE, None), INVALID, b"workspace")
+
+
 _SCALE_READS = r"""
 #include <stdio.h>
 #include <initializer_list>
