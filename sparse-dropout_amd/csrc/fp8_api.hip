@@ -51,6 +51,12 @@ int check_reach(const char* fn, int64_t rows, int64_t K) {
   if (ceil_div(K, kFp8Block) * up(rows, 16) >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "%s: a %lld x %lld operand has too many scales", fn, (long long)rows, (long long)K);
   return SD_OK;
 }
+// the last of 128 x 128 blocks' scales within the tiles' 32-bit offsets
+int check_square_scales(const char* fn, int64_t rows, int64_t nk, int64_t sr, int64_t sk) {
+  const int64_t r = ceil_div(rows, kFp8Block) - 1, k = nk - 1, most = (1LL << 31) - 2;
+  const bool far = (r > 0 && sr > most) || (k > 0 && sk > most) || (r > 0 ? r * sr : 0) + (k > 0 ? k * sk : 0) > most;
+  return far ? fail(SD_ERR_UNSUPPORTED, "%s: scales %lld and %lld apart reach too far", fn, (long long)sr, (long long)sk) : SD_OK;
+}
 int check_matrix(const char* fn, const char* name, const void* p, int64_t sr, int64_t sc, int64_t rows, int64_t cols) {
   SD_REQUIRE(p != nullptr || rows == 0 || cols == 0, "%s: %s: null pointer", fn, name);
   SD_REQUIRE(sr == 1 || sc == 1, "%s: %s must be row or column major (strides %lld, %lld)", fn, name, (long long)sr, (long long)sc);
@@ -196,6 +202,8 @@ int sd_fp8_gemm(const void* A, int64_t lda, const uint8_t* SA, int64_t sa_ld, co
     SD_REQUIRE(sbr >= 1 && sbk >= 1, "fp8_gemm: B's scales: strides must be positive");
   const int64_t nk = ceil_div(K, kFp8Block);
   if (nk * sa_ld >= (1LL << 31) || nk * sbk >= (1LL << 31)) return fail(SD_ERR_UNSUPPORTED, "fp8_gemm: too many scales");
+  if (b_block_rows != 1)
+    if (int rc = check_square_scales("fp8_gemm", N, nk, sbr, sbk)) return rc;
   const bool ws_ok = workspace != nullptr && workspace_bytes > 0 && aligned16(workspace);
   Fp8Gemm g = {};
   g.a = static_cast<const uint8_t*>(A);
@@ -247,6 +255,7 @@ int sd_fp8_linear(const void* X, int64_t ldx, const void* W, int64_t ldw, const 
                       (int32_t)M, (int32_t)N, (int32_t)K};
     return launch_fp8_few(f, dtype, (hipStream_t)stream);
   }
+  if (int rc = check_square_scales("fp8_linear", N, ceil_div(K, kFp8Block), swr, swk)) return rc;
   if (int rc = check_workspace("fp8_linear", workspace, workspace_bytes, sd_fp8_linear_workspace_bytes(M, N, K))) return rc;
   const Packed x(M, K, false);
   QuantJobs js = {};

@@ -238,6 +238,22 @@ def test_the_states_random_bits_leave_averages_right_on_average():
         assert abs((got == 18.0).mean() - 0.25) <= 0.0104  # (a 128th of them are the large ones)
 
 
+def test_scales_that_lie_far_apart_are_refused(lib):
+    """The tiles read them by 32-bit offsets; strides over one block are nobody's business."""
+    def g(N, K, sbr, sbk):
+        return lib.sd_fp8_gemm(FAKE, 1 << 20, FAKE, 16, FAKE, 1 << 20, FAKE, sbr, sbk, 128, FAKE, N, 1, 10, N, K, 0, None, 0, None)
+
+    def f(N, K, swr, swk, ws=FAKE):
+        return lib.sd_fp8_linear(FAKE, K, FAKE, 1 << 20, FAKE, swr, swk, FAKE, N, 100, N, K, 0, ws, 1 << 40, None)
+
+    for call in (g, f):
+        for N, K, sr, sk in ((300, 256, 1 << 30, 1), (256, 128, 1 << 31, 1), (1000, 256, 1 << 40, 1), (1 << 20, 1 << 20, 1 << 62, 1),
+                             (300, 300, 1 << 29, (1 << 29) + 1), (128 << 10, 128, (1 << 21) + 4096, 1)):
+            refused(lib, call(N, K, sr, sk), UNSUPPORTED, b"too far")
+    refused(lib, f(128, 256, 1 << 40, 1, None), INVALID, b"workspace")
+    refused(lib, f(256, 256, (1 << 31) - 3, 1, None), INVALID, b"workspace")
+
+
 def test_drop_rates_that_round_to_one_draw_no_mask(lib):
     """The draw compares in 32 bits and would drop everything; a mask that is given has no rate to be drawn by."""
     def fwd(p, mask, out, ws):
