@@ -18,12 +18,12 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <mutex>
 #include <string>
 #include <tuple>
-#include <unordered_set>
 #include <vector>
 
 #include "sparsedrop.h"
@@ -1435,6 +1435,22 @@ Tensor linear_fp8(const Tensor& input, const Tensor& weight, const OptTensor& ma
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------------
 // (see functional/adamw.py for what is computed)
+// Memory of one of the step's tensors.  Workgroups take them in any order, so what is written must not be anybody else's.
+struct Span {
+  uintptr_t begin, end;
+  size_t parameter;
+  bool written;
+};
+void check_apart(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t any = 0, write = 0;  // ends of all spans so far and of the written ones
+  for (const Span& s : spans) {
+    TORCH_CHECK_VALUE(s.begin >= (s.written ? any : write), "parameter ", s.parameter,
+                      ": it, its averages or its gradient share memory with each other or with another parameter's, or were given twice");
+    any = std::max(any, s.end);
+    if (s.written) write = std::max(write, s.end);
+  }
+}
 // Launches write parameters and averages behind autograd's back: their versions say so.
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -1459,7 +1475,8 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     std::vector<uint8_t*> ms, vs;
     std::vector<int64_t> n;
   } groups[3];
-  std::unordered_set<void*> seen;
+  std::vector<Span> spans;
+  spans.reserve((in8 ? 6 : 4) * n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &m = avgs[i], &v = sqs[i];
     Tensor g = grads[i];
@@ -1484,14 +1501,20 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                         "parameter ", i, ": averages in 32 bits must be float32 tensors laid out like it (", p.sizes(), ", strides ", p.strides(), ")");
     }
     if (size == 0) continue;
-    for (void* at : {p.data_ptr(), m.data_ptr(), v.data_ptr()})
-      TORCH_CHECK_VALUE(seen.insert(at).second, "parameter ", i, " or an average of it was given twice");
     if (g.strides() != p.strides() || g.is_neg() || g.is_conj()) {
       Tensor like = at::empty_like(p);
       like.copy_(g);
       keep.push_back(like);
       g = like;
     }
+    auto spans_of = [&](const Tensor& t, bool is_written) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+      spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i, is_written});
+    };
+    for (const Tensor* t : {&p, &m, &v}) spans_of(*t, true);
+    if (in8)
+      for (const Tensor* t : {&avg_scales[i], &sq_scales[i]}) spans_of(*t, true);
+    if (g.data_ptr() != p.data_ptr()) spans_of(g, false);  // (a parameter that is its own gradient is read where it is written)
     Group& to = groups[code];
     to.p.push_back(p.data_ptr());
     to.g.push_back(g.data_ptr());
@@ -1503,6 +1526,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     }
     to.n.push_back(size);
   }
+  check_apart(spans);
   int last = 0;
   for (int i = 0; i < 3; ++i)
     if (!groups[i].n.empty()) last = i;

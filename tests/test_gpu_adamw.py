@@ -347,3 +347,33 @@ def test_refusals():
     with pytest.raises(ValueError):
         AdamW([z(3)], state_bits=16)
     assert count.item() == 1
+
+
+def test_tensors_that_share_memory_are_refused():
+    """Each written tensor is nobody else's, scales and parts of a buffer included; gradients may be shared, and neighbours touch."""
+    z = lambda *s, **k: torch.zeros(*s, device="cuda", **k)
+    count = z((), dtype=torch.int64)
+    flat, grad, m, v = z(512), torch.ones(512, device="cuda"), z(512), z(512)
+    F.adamw_step([flat[:256], flat[256:]], [grad[:256], grad[:256]], [m[:256], m[256:]], [v[:256], v[256:]], count)
+    assert count.item() == 1 and flat.all()
+    codes = lambda n=256: (z(n, dtype=torch.uint8), torch.full((-(-n // 128),), 127, dtype=torch.uint8, device="cuda"))
+    a, b, c, d = codes(), codes(), codes(), codes()
+    shared = (c[0], a[1])
+    before = [t.clone() for t in (flat, m, v, *a, *b, *c, *d)]
+    for bad in (([flat[:256], flat[128:384]], [grad[:256]] * 2, [m[:256], m[256:]], [v[:256], v[256:]]),
+                ([flat[:256], flat[256:]], [grad[:256]] * 2, [m[:256], m[255:511]], [v[:256], v[256:]]),
+                ([flat[:256]], [grad[:256]], [m[:256]], [m[128:384]]),
+                ([flat[:256]], [grad[:256]], [flat[256:]], [flat[255:511]]),
+                ([flat[:256], flat[256:]], [grad[:256], flat[:256]], [m[:256], m[256:]], [v[:256], v[256:]]),
+                ([flat[:256]], [m[100:356]], [m[:256]], [v[:256]]),
+                ([flat[:256], flat[256:]], [grad[:256]] * 2, [a, shared], [b, d]),
+                ([flat[:256]], [grad[:256]], [a], [(b[0], a[1])])):
+        with pytest.raises(ValueError, match="share memory"):
+            F.adamw_step(*bad, count)
+    assert count.item() == 1
+    assert all(torch.equal(s, t) for s, t in zip(before, (flat, m, v, *a, *b, *c, *d)))
+    F.adamw_step([flat[:256], flat[256:]], [grad[:256]] * 2, [a, c], [b, d], count)
+    assert count.item() == 2 and all(t[0].any() for t in (a, b, c, d))
+    own = torch.full((300,), 2.0, device="cuda")  # a parameter that is its own gradient
+    F.adamw_step([own], [own], [z(300)], [z(300)], z((), dtype=torch.int64), lr=0.5, eps=0.0, weight_decay=0.0)
+    assert ((own - 1.5).abs() <= 24 * 2.0 ** -24).all()
