@@ -1456,6 +1456,13 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// whether the elements of tensors of one shape lie in one order (strides over an extent of one say nothing)
+bool same_order(const Tensor& a, const Tensor& b) {
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
 void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& avgs,
                 const std::vector<Tensor>& sqs, const std::vector<Tensor>& avg_scales, const std::vector<Tensor>& sq_scales,
                 const Tensor& step, const OptTensor& lr_at, double lr, double beta1, double beta2, double eps, double decay) {
@@ -1491,10 +1498,13 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     if (in8) {
       const Tensor &a = avg_scales[i], &b = sq_scales[i];
       const bool fit = m.scalar_type() == at::kByte && v.scalar_type() == at::kByte && a.scalar_type() == at::kByte && b.scalar_type() == at::kByte &&
-                       m.numel() == size && v.numel() == size && a.numel() == ceil_div(size, kFp8) && b.numel() == a.numel() && m.is_contiguous() &&
-                       v.is_contiguous() && a.is_contiguous() && b.is_contiguous() && a.device() == step.device() && b.device() == step.device();
-      TORCH_CHECK_VALUE(fit, "parameter ", i, ": averages in 8 bits are ", size, " contiguous uint8 codes and ", ceil_div(size, kFp8),
-                        " uint8 scales on ", step.device());
+                       m.numel() == size && v.numel() == size && a.numel() == ceil_div(size, kFp8) && b.numel() == a.numel() &&
+                       a.is_contiguous() && b.is_contiguous() && a.device() == step.device() && b.device() == step.device();
+      TORCH_CHECK_VALUE(fit, "parameter ", i, ": averages in 8 bits are ", size, " uint8 codes and ", ceil_div(size, kFp8),
+                        " contiguous uint8 scales on ", step.device());
+      for (const Tensor* t : {&m, &v})
+        TORCH_CHECK_VALUE(t->sizes() == p.sizes() ? same_order(*t, p) : t->is_contiguous(), "parameter ", i, ": its averages' codes (", t->sizes(),
+                          ", strides ", t->strides(), ") are laid out neither like it (", p.sizes(), ", strides ", p.strides(), ") nor in one run");
     } else {
       TORCH_CHECK_VALUE(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat && m.sizes() == p.sizes() && v.sizes() == p.sizes() &&
                             m.strides() == p.strides() && v.strides() == p.strides(),
@@ -1555,10 +1565,10 @@ std::vector<Tensor> adamw_state_values(const std::vector<Tensor>& codes, const s
   for (size_t i = 0; i < codes.size(); ++i) {
     const Tensor &q = codes[i], &b = scales[i];
     TORCH_CHECK_VALUE(q.is_cuda() && q.device() == codes[0].device() && b.device() == q.device(), "averages must be on one GPU");
-    TORCH_CHECK_VALUE(q.scalar_type() == at::kByte && b.scalar_type() == at::kByte && q.is_contiguous() && b.is_contiguous() &&
+    TORCH_CHECK_VALUE(q.scalar_type() == at::kByte && b.scalar_type() == at::kByte && q.is_non_overlapping_and_dense() && b.is_contiguous() &&
                           b.numel() == ceil_div(q.numel(), kFp8),
-                      "averages in 8 bits are contiguous uint8 codes and a uint8 scale for each 128 of them");
-    out.push_back(at::empty(q.sizes(), q.options().dtype(at::kFloat)));
+                      "averages in 8 bits are uint8 codes without gaps and a contiguous uint8 scale for each 128 of them");
+    out.push_back(at::empty_strided(q.sizes(), q.strides(), q.options().dtype(at::kFloat)));
     if (q.numel() == 0) continue;
     c.push_back(static_cast<const uint8_t*>(q.data_ptr()));
     s.push_back(static_cast<const uint8_t*>(b.data_ptr()));

@@ -39,9 +39,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                step: torch.Tensor, *, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2) -> None:
     """Updates ``params`` (float16, bfloat16 or float32, also mixed), both averages and ``step`` in place.  The averages are float32
-    tensors laid out like their parameters or ``(codes, scales)`` pairs of uint8 tensors.  ``step``: one int64 on the GPU, the
-    number of steps so far, moved on by the call itself: a captured graph counts its replays.  ``lr`` may be a float32 tensor on the
-    GPU, which a captured graph reads at every replay.  One launch for each 56 tensors of a dtype.  ``torch.jit.trace`` is refused."""
+    tensors laid out like their parameters or ``(codes, scales)`` pairs of uint8 tensors, the codes laid out like their parameters too or in one
+    run.  ``step``: one int64 on the GPU, the number of steps so far, moved on by the call itself: a captured graph counts its replays.
+    ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  One launch for each 56 tensors of a dtype.
+    ``torch.jit.trace`` is refused."""
     beta1, beta2 = (float(b) for b in betas)
     firsts, first_scales = _split(exp_avgs, "exp_avgs")
     seconds, second_scales = _split(exp_avg_sqs, "exp_avg_sqs")
@@ -54,7 +55,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
 @refused_under_trace
 def adamw_state_values(exp_avgs: Sequence, exp_avg_sqs: Sequence) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
-    """Averages in 8 bits, ``(codes, scales)`` pairs, as float32 tensors of the codes' shapes, in one launch for each 56 of them."""
+    """Averages in 8 bits, ``(codes, scales)`` pairs, as float32 tensors laid out like the codes, in one launch for each 56 of them."""
     firsts, first_scales = _split(exp_avgs, "exp_avgs")
     seconds, second_scales = _split(exp_avg_sqs, "exp_avg_sqs")
     if len(first_scales) != len(firsts) or len(second_scales) != len(seconds):
@@ -65,6 +66,6 @@ def adamw_state_values(exp_avgs: Sequence, exp_avg_sqs: Sequence) -> tuple[list[
 
 
 def adamw_empty_state(param: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """A ``(codes, scales)`` pair of zeros for one average of ``param``."""
-    return (torch.zeros(param.numel(), dtype=torch.uint8, device=param.device),
+    """A ``(codes, scales)`` pair of zeros for one average of ``param``, the codes laid out like it."""
+    return (torch.zeros_like(param, dtype=torch.uint8, memory_format=torch.preserve_format),
             torch.full((-(-param.numel() // STATE_BLOCK),), 127, dtype=torch.uint8, device=param.device))

@@ -12,7 +12,7 @@ from ..functional.tracing import refused_under_trace
 
 class AdamW(torch.optim.Optimizer):
     """``state_bits``: 32, or 8 (a quarter of the memory and less than that to read and write; a state of a parameter is then
-    ``exp_avg`` and ``exp_avg_sq`` codes with ``exp_avg_scale`` and ``exp_avg_sq_scale``).
+    ``exp_avg`` and ``exp_avg_sq`` codes, laid out like it, with ``exp_avg_scale`` and ``exp_avg_sq_scale``).
 
     ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  ``step`` of a parameter's state is an int64
     on the GPU, shared by the parameters that have been updated the same number of times; parameters without a gradient are left out
@@ -95,28 +95,45 @@ class AdamW(torch.optim.Optimizer):
         if "exp_avg_scale" not in s:
             return s["exp_avg"], s["exp_avg_sq"]
         (m,), (v,) = adamw_state_values(self._averages([s], "exp_avg"), self._averages([s], "exp_avg_sq"))
-        if p.is_contiguous():
-            return m.view(p.shape), v.view(p.shape)
-        return tuple(torch.as_strided(t, p.shape, p.stride()) for t in (m, v))
+        return m, v
+
+    @staticmethod
+    def _codes_like(p: torch.Tensor, codes: torch.Tensor) -> torch.Tensor:
+        """Saved codes of an average of ``p`` with its strides.  They and their scales go by the order of the parameter's memory, so they fit
+        no other layout (codes without a shape are of a contiguous parameter)."""
+        kept = codes.view(p.shape) if codes.dim() == 1 and codes.numel() == p.numel() else codes
+        if kept.shape != p.shape or any(n > 1 and a != b for n, a, b in zip(p.shape, kept.stride(), p.stride())):
+            raise ValueError(f"averages in 8 bits of a parameter laid out as {tuple(codes.shape)}, strides {codes.stride()}, "
+                             f"fit none of {tuple(p.shape)}, strides {p.stride()}")
+        return torch.as_strided(kept, p.shape, p.stride())
+
+    def _saved(self, state_dict):
+        """(parameter, its saved state) pairs of a state dict with this optimizer's groups."""
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            for number, p in zip(saved["params"], group["params"]):
+                if state_dict["state"].get(number):
+                    yield group, p, state_dict["state"][number]
 
     def load_state_dict(self, state_dict) -> None:
-        """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved."""
+        """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved.  Averages in
+        32 bits are laid out like their parameters; those in 8 are refused where the layouts differ."""
+        for _, p, saved in self._saved(state_dict):
+            for key in ("exp_avg", "exp_avg_sq"):
+                if key + "_scale" in saved:
+                    self._codes_like(p, saved[key])
         super().load_state_dict(state_dict)
-        numbers = iter([i for g in state_dict["param_groups"] for i in g["params"]])
         shared: dict[tuple, torch.Tensor] = {}
-        for group in self.param_groups:
-            for p in group["params"]:
-                s = state_dict["state"].get(next(numbers))
-                if not s:
+        for group, p, saved in self._saved(state_dict):
+            state = self.state[p]
+            for key, value in saved.items():
+                if not isinstance(value, torch.Tensor):
+                    state[key] = value
                     continue
-                state = self.state[p]
-                for key, value in s.items():
-                    if not isinstance(value, torch.Tensor):
-                        state[key] = value
-                        continue
-                    kept = value.detach().to(p.device, copy=True)
-                    if key in ("exp_avg", "exp_avg_sq") and kept.dtype == torch.float32 and kept.stride() != p.stride():
-                        kept = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(kept)
-                    state[key] = kept
-                count = int(state["step"])
-                state["step"] = shared.setdefault((id(group), p.device, count), torch.full((), count, dtype=torch.int64, device=p.device))
+                kept = value.detach().to(p.device, copy=True)
+                if key + "_scale" in saved:
+                    kept = self._codes_like(p, kept)
+                elif key in ("exp_avg", "exp_avg_sq") and kept.dtype == torch.float32 and kept.shape == p.shape and kept.stride() != p.stride():
+                    kept = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(kept)
+                state[key] = kept
+            count = int(state["step"])
+            state["step"] = shared.setdefault((id(group), p.device, count), torch.full((), count, dtype=torch.int64, device=p.device))

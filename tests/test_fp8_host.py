@@ -357,3 +357,74 @@ def test_traces_record_the_quantizer_and_refuse_the_optimizer(monkeypatch):
         with pytest.raises(NotImplementedError, match="cannot be traced"):
             torch.jit.trace(call, (torch.zeros(3),), check_trace=False)
     F.adamw_step([p], [p], [p], [p], step)
+
+
+def _steps_taken(params, bits):
+    """An optimizer as it is after seven steps, its averages numbered by their place in memory."""
+    from flash_dropout.optim import AdamW
+
+    opt = AdamW(params, state_bits=bits)
+    for p in params:
+        opt._init_state(p, bits, torch.full((), 7, dtype=torch.int64))
+        state = opt.state[p]
+        for key in ("exp_avg", "exp_avg_sq"):
+            flat = torch.as_strided(state[key], (p.numel(),), (1,))
+            flat.copy_(torch.arange(p.numel()) % 100 + (key == "exp_avg_sq"))
+    return opt
+
+
+def _layouts():
+    w = torch.zeros(2, 3, 2, 2)
+    return {"rows": w, "channels last": w.contiguous(memory_format=torch.channels_last), "turned": torch.zeros(2, 2, 3, 2).permute(3, 2, 0, 1)}
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("saved", ["rows", "channels last", "turned"])
+@pytest.mark.parametrize("loaded", ["rows", "channels last", "turned"])
+def test_saved_averages_stay_with_their_elements(saved, loaded, bits, tmp_path):
+    """Averages in 32 bits take their parameter's layout; those in 8, whose codes share scales along the memory, are refused in another one."""
+    from flash_dropout.optim import AdamW
+
+    make = lambda kind: [torch.nn.Parameter(_layouts()[kind]), torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(4, 1, 3))]  # noqa: E731
+    old, new = make(saved), make(loaded)
+    opt, again = _steps_taken(old, bits), AdamW(new, state_bits=bits, lr=5.0)
+    torch.save(opt.state_dict(), tmp_path / "s.pt")
+    state_dict = torch.load(tmp_path / "s.pt", weights_only=True)
+    if bits == 8 and saved != loaded:
+        with pytest.raises(ValueError, match="fit none of"):
+            again.load_state_dict(state_dict)
+        assert not again.state and again.param_groups[0]["lr"] == 5.0
+        return
+    again.load_state_dict(state_dict)
+    for p, q in zip(old, new):
+        for key in ("exp_avg", "exp_avg_sq"):
+            a, b = opt.state[p][key], again.state[q][key]
+            assert torch.equal(a, b) and a.shape == b.shape and b.dtype == a.dtype and b.stride() == q.stride()
+        assert again.state[q]["step"].item() == 7 and again.state[q]["step"].dtype == torch.int64
+
+
+def test_strides_of_extents_of_one_are_no_layout():
+    from flash_dropout.optim import AdamW
+
+    p, q = (torch.nn.Parameter(torch.as_strided(torch.zeros(12), (4, 1, 3), strides)) for strides in ((3, 3, 1), (3, 100, 1)))
+    opt, again = _steps_taken([p], 8), AdamW([q], state_bits=8)
+    again.load_state_dict(opt.state_dict())
+    assert torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"]) and again.state[q]["exp_avg"].stride() == q.stride()
+
+
+def test_codes_saved_without_a_shape_are_of_contiguous_parameters():
+    from flash_dropout.optim import AdamW
+
+    opt = _steps_taken([torch.nn.Parameter(_layouts()["rows"])], 8)
+    state_dict = opt.state_dict()
+    for key in ("exp_avg", "exp_avg_sq"):
+        state_dict["state"][0][key] = state_dict["state"][0][key].view(-1)
+    for kind in ("rows", "channels last"):
+        p = torch.nn.Parameter(_layouts()[kind])
+        again = AdamW([p], state_bits=8)
+        if kind == "rows":
+            again.load_state_dict(state_dict)
+            assert torch.equal(again.state[p]["exp_avg"].view(-1), state_dict["state"][0]["exp_avg"])
+        else:
+            with pytest.raises(ValueError, match="fit none of"):
+                again.load_state_dict(state_dict)

@@ -377,3 +377,32 @@ def test_tensors_that_share_memory_are_refused():
     own = torch.full((300,), 2.0, device="cuda")  # a parameter that is its own gradient
     F.adamw_step([own], [own], [z(300)], [z(300)], z((), dtype=torch.int64), lr=0.5, eps=0.0, weight_decay=0.0)
     assert ((own - 1.5).abs() <= 24 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_averages_are_laid_out_like_their_parameters(bits):
+    """Steps, values, a save and a load of a channels-last and a turned parameter equal those of contiguous ones with each element's own
+    gradient; a parameter that is laid out anew keeps none of its averages' codes."""
+    shape = (24, 5, 3, 3)
+    w, g = spread(24 * 45, 1).view(shape).cuda(), spread(24 * 45, 2, 0.1).view(shape).cuda()
+    p = torch.nn.Parameter(w.clone().contiguous(memory_format=torch.channels_last))
+    flat = torch.nn.Parameter(w.permute(0, 2, 3, 1).contiguous().view(-1))  # the same memory
+    opts = [AdamW([t], lr=1e-2, state_bits=bits) for t in (p, flat)]
+    for i in range(3):
+        p.grad = (g * (i + 1)).contiguous()
+        flat.grad = (g * (i + 1)).permute(0, 2, 3, 1).contiguous().view(-1)
+        for o in opts:
+            o.step()
+        if i == 1:
+            state = opts[0].state_dict()
+            opts[0] = AdamW([p], lr=5.0, state_bits=bits)
+            opts[0].load_state_dict(state)
+    assert torch.equal(p.detach().permute(0, 2, 3, 1).reshape(-1), flat.detach())
+    for a, b in zip(opts[0].state_values(p), opts[1].state_values(flat)):
+        assert a.shape == p.shape and a.stride() == p.stride() and torch.equal(a.permute(0, 2, 3, 1).reshape(-1), b)
+    before = [t.clone() for t in opts[0].state_values(p)]
+    p.data = p.data.contiguous()
+    kept = p.detach().clone()
+    with pytest.raises(ValueError, match="laid out"):
+        opts[0].step()
+    assert torch.equal(p, kept) and all(torch.equal(a, b) for a, b in zip(before, opts[0].state_values(p)))
