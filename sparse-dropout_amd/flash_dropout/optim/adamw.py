@@ -115,13 +115,28 @@ class AdamW(torch.optim.Optimizer):
                     yield group, p, state_dict["state"][number]
 
     def load_state_dict(self, state_dict) -> None:
-        """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved.  Averages in
-        32 bits are laid out like their parameters; those in 8 are refused where the layouts differ."""
-        for _, p, saved in self._saved(state_dict):
-            for key in ("exp_avg", "exp_avg_sq"):
-                if key + "_scale" in saved:
-                    self._codes_like(p, saved[key])
-        super().load_state_dict(state_dict)
+        """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved, before hooks
+        behind it run.  Averages in 32 bits are laid out like their parameters; those in 8 are refused where the layouts differ."""
+        taken = []
+
+        def before(_, given):  # (behind other hooks, which may have replaced what is loaded)
+            for _, p, saved in self._saved(given):
+                for key in ("exp_avg", "exp_avg_sq"):
+                    if key + "_scale" in saved:
+                        self._codes_like(p, saved[key])
+            taken.append(given)
+
+        def after(_):
+            self._put_back(taken[0])
+
+        hooks = self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _put_back(self, state_dict) -> None:
         shared: dict[tuple, torch.Tensor] = {}
         for group, p, saved in self._saved(state_dict):
             state = self.state[p]

@@ -428,3 +428,31 @@ def test_codes_saved_without_a_shape_are_of_contiguous_parameters():
         else:
             with pytest.raises(ValueError, match="fit none of"):
                 again.load_state_dict(state_dict)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_hooks_around_a_load_see_what_is_loaded(bits):
+    """One in front may replace the state, one behind finds the averages as they were saved."""
+    import copy
+
+    from flash_dropout.optim import AdamW
+
+    make = lambda: [torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(2, dtype=torch.bfloat16))]  # noqa: E731
+    opt, ours = _steps_taken(make(), bits), make()
+    again, seen = AdamW(ours, state_bits=bits), []
+
+    def replace(_, given):
+        given = copy.deepcopy(given)
+        for state in given["state"].values():
+            state["exp_avg"] += 3
+            state["step"] += 1
+        return given
+
+    again.register_load_state_dict_pre_hook(replace)
+    again.register_load_state_dict_post_hook(lambda o: seen.append([(o.state[p]["exp_avg"].clone(), o.state[p]["step"].item()) for p in ours]))
+    saved = opt.state_dict()
+    for _ in range(2):
+        again.load_state_dict(saved)
+    for p, (average, step), state in zip(ours * 2, seen[0] + seen[1], [*saved["state"].values()] * 2):
+        assert torch.equal(average, state["exp_avg"] + 3) and average.dtype == state["exp_avg"].dtype and step == 8
+    assert again.state[ours[0]]["step"] is again.state[ours[1]]["step"]
