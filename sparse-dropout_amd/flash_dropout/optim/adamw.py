@@ -116,10 +116,15 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """torch's, which casts states to their parameters' dtypes; the averages and counts are then put back as they were saved, before hooks
-        behind it run.  Averages in 32 bits are laid out like their parameters; those in 8 are refused where the layouts differ."""
+        behind it run.  Averages in 32 bits are laid out like their parameters; those in 8 are refused where the layouts differ.  A state of
+        torch's own AdamW is taken too, but for its ``amsgrad`` and ``maximize``, which are refused."""
         taken = []
 
         def before(_, given):  # (behind other hooks, which may have replaced what is loaded)
+            for group in given["param_groups"]:
+                for key in ("amsgrad", "maximize"):
+                    if group.get(key):
+                        raise ValueError(f"{key} is not built")
             for _, p, saved in self._saved(given):
                 for key in ("exp_avg", "exp_avg_sq"):
                     if key + "_scale" in saved:
@@ -127,6 +132,9 @@ class AdamW(torch.optim.Optimizer):
             taken.append(given)
 
         def after(_):
+            for group in self.param_groups:
+                for key, value in self.defaults.items():
+                    group.setdefault(key, value)
             self._put_back(taken[0])
 
         hooks = self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True)
@@ -147,7 +155,7 @@ class AdamW(torch.optim.Optimizer):
                 kept = value.detach().to(p.device, copy=True)
                 if key + "_scale" in saved:
                     kept = self._codes_like(p, kept)
-                elif key in ("exp_avg", "exp_avg_sq") and kept.dtype == torch.float32 and kept.shape == p.shape and kept.stride() != p.stride():
+                elif key in ("exp_avg", "exp_avg_sq") and kept.shape == p.shape:
                     kept = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(kept)
                 state[key] = kept
             count = int(state["step"])

@@ -430,6 +430,38 @@ def test_codes_saved_without_a_shape_are_of_contiguous_parameters():
                 again.load_state_dict(state_dict)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_of_torchs_optimizer_is_loaded(bits, dtype):
+    """Averages in 32 bits whatever the parameters' type, the settings that torch's has no name for as they were, parameters without a state too."""
+    from flash_dropout.optim import AdamW
+
+    make = lambda: [torch.nn.Parameter(torch.ones(3, 5, dtype=dtype)), torch.nn.Parameter(torch.ones(4, dtype=dtype))]  # noqa: E731
+    theirs, ours = make(), make()
+    other = torch.optim.AdamW(theirs, lr=0.25, betas=(0.5, 0.75), eps=1e-6, weight_decay=0.125)
+    theirs[0].grad = torch.full((3, 5), 0.5, dtype=dtype)
+    for _ in range(2):
+        other.step()
+    opt = AdamW(ours, state_bits=bits)
+    opt.load_state_dict(other.state_dict())
+    group = opt.param_groups[0]
+    assert {k: group[k] for k in ("lr", "betas", "eps", "weight_decay", "state_bits")} == dict(lr=0.25, betas=(0.5, 0.75), eps=1e-6, weight_decay=0.125, state_bits=bits)
+    state = opt.state[ours[0]]
+    for key in ("exp_avg", "exp_avg_sq"):
+        assert state[key].dtype == torch.float32 and torch.equal(state[key], other.state[theirs[0]][key].float())
+    assert state["step"].item() == 2 and state["step"].dtype == torch.int64 and not opt.state.get(ours[1])
+    ours[1].grad = torch.ones(4, dtype=dtype)
+    with pytest.raises(ValueError, match="on the GPU"):  # (a step as far as it goes here)
+        opt.step()
+    assert ("exp_avg_scale" in opt.state[ours[1]]) == (bits == 8)
+    for key in ("amsgrad", "maximize"):
+        other = torch.optim.AdamW(theirs, **{key: True})
+        opt = AdamW(ours, state_bits=bits)
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(other.state_dict())
+        assert key not in opt.param_groups[0]
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_hooks_around_a_load_see_what_is_loaded(bits):
     """One in front may replace the state, one behind finds the averages as they were saved."""
