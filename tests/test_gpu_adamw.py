@@ -406,3 +406,44 @@ def test_averages_are_laid_out_like_their_parameters(bits):
     with pytest.raises(ValueError, match="laid out"):
         opts[0].step()
     assert torch.equal(p, kept) and all(torch.equal(a, b) for a, b in zip(before, opts[0].state_values(p)))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype,sizes,chunks", [
+    # workgroups of 1024 threads that take four runs of 2048 elements at a time, from a few hundred runs to the most
+    ("fp32", (700_001, 300, 12_345, 128, 390_625), 542), ("bf16", (5, 1_049_600, 2047), 515), ("fp16", (16_000_001, 771_000, 999), 8191),
+    # workgroups of 256 through several runs each
+    ("fp32", (129, 17_000_003, 5_000), 8305)])
+def test_many_elements_over_several_tensors(dtype, sizes, chunks, bits):
+    """A second step from averages that a first one left, every element of every tensor checked.  Averages in 8 bits are those of the
+    definition, but where their place between two codes and the random bits make a whole number within 2^-40: there either neighbour is right."""
+    assert sum(-(-n // 2048) for n in sizes) == chunks
+    dt, (b1, b2) = DT[dtype], HYPER["betas"]
+    p = [spread(n, 10 + i).to(dt).cuda() for i, n in enumerate(sizes)]
+    m, v = ([torch.zeros(n, device="cuda") if bits == 32 else codes_of(torch.zeros(n), k) for n in sizes] for k in ("first", "second"))
+    count = torch.zeros((), dtype=torch.int64, device="cuda")
+    values = lambda: (m, v) if bits == 32 else F.adamw_state_values(m, v)  # noqa: E731
+    for step in (1, 2):
+        g = [spread(n, 40 + 10 * step + i, 0.1).to(dt).cuda() for i, n in enumerate(sizes)]
+        before, (m0, v0) = [t.clone() for t in p], ([t.clone() for t in ts] for ts in values())
+        F.adamw_step(p, g, m, v, count, **HYPER)
+        assert count.item() == step
+    for i, (m1, v1) in enumerate(zip(*values())):
+        check_param(p[i], before[i], g[i], np64(m0[i]), np64(v0[i]), 2, dt)
+        gd = np64(g[i])
+        for which, got, old, new, b in (("first", m1, m0[i], gd, b1), ("second", v1, v0[i], gd * gd, b2)):
+            x, got = b * np64(old) + (1 - b) * new, np64(got)
+            if bits == 32:
+                assert (np.abs(got - x) <= 4 * 2.0 ** -24 * (b * np.abs(np64(old)) + (1 - b) * np.abs(new)) + 2.0 ** -149).all()
+                continue
+            want = O.rounded_state(x, which, 2)
+            at = np.flatnonzero(got != want)
+            if at.size:
+                limit, least, _ = O.FORMATS[which]
+                wide = np.zeros(-(-x.size // 128) * 128)
+                wide[: x.size] = np.abs(x)
+                y = np.abs(x[at]) / O.least_power(wide.reshape(-1, 128).max(1), limit)[at // 128]
+                grid = np.exp2(np.floor(np.log2(np.maximum(y, least))) - 3)
+                z = y / grid + O.dither(x.size, 2, which)[at]
+                assert (np.abs(z - np.rint(z)) < 2.0 ** -40).all()
+                assert (np.abs(got[at] - want[at]) <= grid * (np.abs(x[at]) / y)).all()
