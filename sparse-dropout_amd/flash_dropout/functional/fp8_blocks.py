@@ -39,7 +39,8 @@ def fp8_quantize(x: torch.Tensor, block=(1, 128)) -> tuple[torch.Tensor, torch.T
 @traceable(recorded=_RecordedConstantCall, cast=False)
 def fp8_dequantize(data: torch.Tensor, scales: torch.Tensor, cols: int | None = None,
                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values of codes and scales as ``dtype``: the first ``cols`` columns (default: all, the zeros behind the last too)."""
+    """The values of codes and scales as ``dtype``: the first ``cols`` columns (default: all, the zeros behind the last too),
+    without a gradient."""
     # (an extent that a trace takes off a tensor is a tensor itself)
     return _loader.bridge().fp8_dequantize(data, scales, int(cols) if isinstance(cols, torch.Tensor) else cols, dtype)
 
