@@ -18,6 +18,7 @@
 #include "tile_map.h"
 
 #include <atomic>
+#include <cmath>
 
 namespace sd {
 namespace {
@@ -26,7 +27,6 @@ constexpr int kB = kFp8Block;
 constexpr int kBlockBytes = kB * kB;  // of one 128 x 128 block of codes
 constexpr int kLdsLimit = 160 * 1024;
 constexpr int kCus = 256;
-constexpr float kDuoKeep = 0.55f;  // SDD: fraction of blocks kept up to which 128 x 256 tiles of kept blocks are faster than 256 x 256 ones
 constexpr int64_t kPairBlocks = 1024;  // workgroups of both gradients up to which they share a launch
 constexpr int kMaxList = 4096;        // 128-blocks that a workgroup's list can hold
 
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(512, 2) void fp8_big_kernel(Args p) {
 // and w + 4, one of either group, share a SIMD.  A phase is a step: while one group reads the step's fragments into registers (and
 // puts the blocks of the step after next on their way into the third stage), the other's matrix instructions run from theirs.  At the end the
 // groups swap halves of their sums through LDS, add and store a half each.
-// dX of 8192^3 at p = 0.5: 321 us, 371 on 256 x 256 tiles; it loads 48 KB for two blocks of C a step, those 64 for up to four.
+// dX of 8192^3 at p = 0.5: 321 us, 371 on 256 x 256 tiles (duo_pays has both at other sizes); it loads 48 KB for two blocks of C a step, those 64 for up to four.
 // (DSD in this shape, whose row blocks walk the reduction apart from each other and meet in the L2 less: 431 us, 310 on 256 x 256.)
 constexpr int kDuoStage = 3 * kBlockBytes;        // A's block, B's two
 constexpr int kDuoScales = 3 * kDuoStage;         // then 256 bytes of A's scales and 256 of B's for each stage
@@ -743,6 +743,32 @@ int launch_pair(const Args& x, const Args& w, hipStream_t stream) {
   return launch_sum<T>(w, stream);
 }
 
+// Rounds of the busiest XCD's 32 CUs through the workgroups that have work, of `rows` x `cols` of them of which each row's first `full` do: an
+// XCD gets one run of an order that walks DSD_GROUP_M rows column by column, and half of the XCDs may get the empty ends of rows.
+int64_t busiest_rounds(int64_t rows, int64_t cols, double full) {
+  const int64_t run = ceil_div(rows * cols, 8), group = DSD_GROUP_M * cols;
+  const double in_group = DSD_GROUP_M * (full < (double)cols ? full : (double)cols), rest = (double)(run % group);
+  const int64_t work = (int64_t)ceil((double)(run / group) * in_group + (rest < in_group ? rest : in_group));
+  return work > 32 ? ceil_div(work, 32) : 1;
+}
+// SDD on tiles of 128 x 256 of a row block's kept blocks instead of 256 x 256 of those that either row block of a pair keeps: where their
+// rounds are expected to take less.  Microseconds, with nk = N / 128 steps, a round 0.9 nk + 10 and 1.25 nk + 5.  Input gradients with their quantizing,
+// 128 x 256 and 256 x 256: 8192^3, p = 0.4 381 and 367 us, 0.5 327 and 364, 0.75 220 and 346; 4096^3, 0.5 74 and 58, 0.75 72 and 56;
+// 4096 x 8192 over 8192, 0.5 248 and 185 (the full ends of 32 row blocks go to four XCDs), 8192 x 8192 over 4096, 0.75 123 and 173.
+// Over 152 products of 4096 to 18000 rows, p from 0.2 to 0.9 and blocks of 128 to 384 the choice takes 0.7 % longer than the faster of both (17 % at
+// most), by the drop rate alone (from 0.45 on) 8 % (50 %), 256 x 256 tiles always 3.3 % (76 %).
+bool duo_pays(const Fp8Gemm& g) {
+  const double cols = (double)ceil_div(g.N, kB), keep = g.keep;
+  // a pair of row blocks shares its mask where the mask's blocks are a multiple of 256, else one of two keeps more; an odd number of kept
+  // blocks, every other row, leaves half a workgroup
+  const bool even = g.split % 2 == 0;
+  const double either = even ? keep : 1.0 - (1.0 - keep) * (1.0 - keep), odd = even ? 0.0 : 0.25;
+  const int64_t pairs = ceil_div(g.N, 2 * kB), nk = ceil_div(g.K, kB);
+  const double duo = (double)busiest_rounds(ceil_div(g.M, kB), pairs, cols * keep / 2 + odd) * (0.9 * nk + 10.0);
+  const double big = (double)busiest_rounds(ceil_div(g.M, 2 * kB), pairs, cols * either / 2 + odd) * (1.25 * nk + 5.0) + 5.0;
+  return duo < big;
+}
+
 int make_args(const Fp8Gemm& g, int mode, Args& p) {
   p.g = g;
   const Plan q = plan(g.M, g.N, g.K, mode);
@@ -756,7 +782,7 @@ int make_args(const Fp8Gemm& g, int mode, Args& p) {
   }
   // (SDD on large tiles lists a row pair's column blocks)
   p.big = q.big && !(mode == kFp8Sdd && (!g.sb_square || ceil_div(g.N, kB) > kMaxList));
-  p.duo = p.big && mode == kFp8Sdd && g.keep <= kDuoKeep && ceil_div(g.N, kB) <= kDuoMaxList;
+  p.duo = p.big && mode == kFp8Sdd && ceil_div(g.N, kB) <= kDuoMaxList && duo_pays(g);
   if (p.duo) p.big = false;
   p.tiles_m = (int)ceil_div(g.M, p.big ? 2 * kB : kB);
   p.tiles_n = (int)ceil_div(g.N, p.big || p.duo ? 2 * kB : kB);

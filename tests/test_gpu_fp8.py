@@ -283,6 +283,29 @@ def test_whole_numbers_come_out_exactly(m, k, n, bs, p, dtype):
         assert torch.equal(F.fp8_linear(x.detach()[:rows], data, scales), (xd[:rows] @ wd.t()).to(dt))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("m,k,n,bs,p,kernel", [
+    # kept blocks of a row two at a time, with rows of none and of odd numbers
+    (4777, 6601, 131, 128, 0.875, "fp8:duo"), (4777, 6601, 131, 256, 0.875, "fp8:duo"), (4800, 6656, 300, 384, 0.875, "fp8:duo"),
+    (8192, 8192, 260, 128, 0.75, "fp8:duo"),
+    # pairs of row blocks: hardly anything to leave out, few rounds, rows whose full ends share XCDs
+    (4777, 6601, 131, 128, 0.25, "fp8:big"), (4096, 4096, 256, 128, 0.75, "fp8:big"), (4096, 8192, 256, 128, 0.5, "fp8:big"),
+    (4200, 4099, 140, 256, 0.5, "fp8:big")])
+def test_input_gradients_of_large_layers_on_the_tiles_that_pay(m, k, n, bs, p, kernel, dtype):
+    dt = DT[dtype]
+    x, w, dy = whole(m, k, 1, dt).requires_grad_(), whole(n, k, 2, dt), whole(m, n, 3, dt)
+    mask = torch.rand(-(-m // bs), -(-k // bs), generator=torch.Generator().manual_seed(m + k)) < p
+    mask[1] = True
+    y = F.hip_blockwise_dropout_matmul_fp8_mask(x, mask.cuda(), bs, p, w)
+    with torch.autograd.set_multithreading_enabled(False):  # (the last kernel is known by thread)
+        dx, = torch.autograd.grad(y, x, dy)
+    assert GEMM().last_kernel_detail().startswith(kernel)
+    keep = torch.from_numpy(O.keep_matrix(mask.numpy(), bs, m, k)).cuda()
+    # (exact sums, scaled in 32 bits)
+    want = (dy.double() @ w.double()).float().mul_(1 / (1 - p)).double() * keep
+    assert torch.equal(dx, want.to(dt))
+
+
 @pytest.mark.parametrize("kind", ["all", "rows", "columns", "one kept"])
 def test_masks_that_leave_rows_and_columns_empty(kind):
     m, k, n, bs = 520, 600, 300, 128
