@@ -344,8 +344,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamTable a) {
       }
     }
   }
-  // The step moves on when every workgroup is done with it: the last to report writes it.  Its upper half counts the reports meanwhile, 10 ns
-  // each, one at a time.  (Made at the start they hold up the others' reads of the step: 58 us for 1.9 M parameters, at the end 19.
+  // The step moves on when every workgroup is done with it: the last to report writes it.  Its upper half counts the reports meanwhile, one
+  // at a time, 10 ns each where they are few; 2048 take 126 us more than 512 (launch_table).  (Made at the start they hold up the others' reads of the step: 58 us for 1.9 M parameters, at the end 19.
   // A launch that moves the step on takes 4 us.)
   if (a.last) {
     __syncthreads();
@@ -407,10 +407,15 @@ __global__ __launch_bounds__(kThreads) void state_values_kernel(ValueTable a) {
 unsigned grid_of(uint32_t chunks) { return chunks < 2048 ? chunks : 2048; }
 
 // Workgroups of 1024 threads where their number matters, for they report one after the other, and not where everything is done at once (too few
-// of them for all CUs) or goes on for long (5 % slower at 168 M parameters).
+// of them for all CUs).  With averages in 8 bits, whose arithmetic is what takes the time in the end, not for long tables either.  us with 256 threads
+// and with 1024, by runs of 2048 elements:
+//   32 bits, fp32   100: 5.6, 6.6   200: 7.3, 7.1   300: 9.0, 7.7   2048: 170, 44   8192: 207, 101   32768: 406, 375   81920: 925, 927
+//   32 bits, bf16   100: 6.3, 7.0   200: 7.7, 7.6   300: 9.0, 8.0   2048: 148, 26   8192: 138, 77    32768: 309, 300   81920: 733, 728
+//   8 bits, fp32    256: 10.4, 12.3   512: 13.8, 13.8   700: 16.7, 15.2   8192: 130, 77   16384: 158, 139   24576: 199, 199   65536: 477, 490
+//   8 bits, bf16    256: 10.0, 12.3   512: 13.7, 13.5   700: 15.8, 13.9   8192: 93, 68    16384: 125, 124   24576: 178, 193   65536: 458, 489
 template <typename T>
 void launch_table(const AdamTable& a, int bits, uint32_t chunks, hipStream_t stream) {
-  const bool wide = chunks > 512 && chunks <= 8192;
+  const bool wide = bits == 8 ? chunks > 512 && chunks <= 16384 : chunks >= 256;
   const dim3 grid(wide ? (chunks + 3) / 4 < 512 ? (chunks + 3) / 4 : 512 : chunks ? grid_of(chunks) : 1), block(wide ? kWide : kThreads);
   if (bits == 8) hipLaunchKernelGGL((wide ? &adamw_kernel<T, 8, kWide> : &adamw_kernel<T, 8, kThreads>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((wide ? &adamw_kernel<T, 32, kWide> : &adamw_kernel<T, 32, kThreads>), grid, block, 0, stream, a);

@@ -412,8 +412,8 @@ def test_averages_are_laid_out_like_their_parameters(bits):
 @pytest.mark.parametrize("dtype,sizes,chunks", [
     # workgroups of 1024 threads that take four runs of 2048 elements at a time, from a few hundred runs to the most
     ("fp32", (700_001, 300, 12_345, 128, 390_625), 542), ("bf16", (5, 1_049_600, 2047), 515), ("fp16", (16_000_001, 771_000, 999), 8191),
-    # workgroups of 256 through several runs each
-    ("fp32", (129, 17_000_003, 5_000), 8305)])
+    # 8 bits: workgroups of 256 through several runs each
+    ("fp32", (129, 33_600_003, 5_000), 16411)])
 def test_many_elements_over_several_tensors(dtype, sizes, chunks, bits):
     """A second step from averages that a first one left, every element of every tensor checked.  Averages in 8 bits are those of the
     definition, but where their place between two codes and the random bits make a whole number within 2^-40: there either neighbour is right."""
