@@ -4,8 +4,8 @@
 // instruction's registers, every byte once, and x, which a launch before would have to bring into 8 bits, is quantized by each workgroup as
 // it reads it out of the L2.  A workgroup owns 16 or 32 outputs and its waves share out the 128-blocks of the reduction, wave w every 128-block
 // w + waves * n, a few of them on their way at a time, and meet once in LDS.  Rows come in groups of 16, up to four; what a row behind the
-// last or an output behind the last holds is never stored, so their lanes read another's.  One token through 4096 to 1024 6.3 us, most of it a
-// memory latency and the launch; through 8192 to 8192 18.7, 3.6 TB/s.
+// last or an output behind the last holds is never stored, so their lanes read another's.  One token through 4096 to 1024 5.7 us, most of it a
+// memory latency and the launch; through 8192 to 8192 18.3, 3.7 TB/s.
 #include "fp8.h"
 
 namespace sd {
@@ -147,10 +147,12 @@ struct FewPlan {
   bool many;   // more workgroups than CUs: of 32 outputs each, x is read and quantized half as often
   double us;
 };
-// Sixteen waves a workgroup where the reduction is long.  The time, from 7 layers between 512^2 and 8192^2 at 1 to 64 rows: 5 us, and for
-// each 128-block of a wave and group of rows 2.1 with sixteen waves (32 rows through 4096^2 12.5 us, 64 22.5), 1 with four (64
-// through 8192 x 2048 20).  More workgroups than CUs: 32 outputs each instead of 16 (8192 x 2048: 16 rows 6.7 us instead of 8.5, 32 rows 9.2
-// instead of 12.2; 16 rows through 8192^2 20 instead of 35); with a workgroup or less a CU they would leave CUs idle.
+// Sixteen waves a workgroup where the reduction is long (one row, sixteen and four: 4096 to 4096 6.0 and 8.4 us, 4096 to 1024 5.6 and 6.8; 1500 to 10000
+// 10.3 and 7.5).  The time, from 7 layers between 512^2 and 8192^2 at 1 to 64 rows: 5 us, and for each 128-block of a wave and group of rows 2.1
+// with sixteen waves (32 rows through 4096^2 12.1 us, 64 19.9), 1 with four (64 rows of 2048 to 8192 19.8).  It leaves out what 32 outputs a
+// workgroup save (2048 to 8192: 32 rows 9.1 us).  More workgroups than CUs: 32 outputs each instead of 16 (16 rows of 2048 to 8192 6.8 us and 8.5, of
+// 8192 to 8192 19.9 and 26.0, of 1000 to 5000 5.5 and 6.1; one row of 8192 to 8192 18.3 and 17.1); with a workgroup or less a CU they would
+// leave CUs idle (16 rows of 4096 to 4096 10.1 and 8.3).
 FewPlan few_plan(int64_t M, int64_t N, int64_t K) {
   FewPlan p;
   const int64_t nk = ceil_div(K, kFp8Block), wgs = ceil_div(N, 16);
@@ -181,7 +183,10 @@ void launch_few(const Fp8Few& g, const FewPlan& p, hipStream_t stream) {
 }  // namespace
 
 // Whether the kernel takes the product: up to 16 rows always; up to 64 where it is expected to take less than quantizing x and 128 x 128
-// tiles do, 15 to 20 us at such sizes.
+// tiles do, 10 to 18 us at such sizes.  us here and on the tiles, features to outputs at 17, 32, 33 and 64 rows:
+//   1024 to 4096  5.5, 12.6   5.8, 12.6    7.4, 12.6   8.2, 11.8     2048 to 8192  8.3, 15.1   9.1, 15.8   15.5, 15.7   19.8, 16.4
+//   4096 to 1024  9.5, 15.2  12.0, 16.1   18.2, 15.9  19.7, 14.8     8192 to 2048  17.0, 17.2  22.1, 18.4  32.7, 18.0   35.2, 18.4
+//   1000 to 5000  7.5, 12.8   8.2, 12.8   13.5, 12.8  14.8, 12.4 (the one here that the rule gets wrong, from 33 rows on)
 bool fp8_few_takes(int64_t M, int64_t N, int64_t K) { return M <= 16 || (M <= kFp8FewRows && few_plan(M, N, K).us <= 15.0); }
 
 int launch_fp8_few(const Fp8Few& g, int dtype, hipStream_t stream) {

@@ -27,7 +27,9 @@ constexpr int kB = kFp8Block;
 constexpr int kBlockBytes = kB * kB;  // of one 128 x 128 block of codes
 constexpr int kLdsLimit = 160 * 1024;
 constexpr int kCus = 256;
-constexpr int64_t kPairBlocks = 1024;  // workgroups of both gradients up to which they share a launch
+// Workgroups of both gradients up to which they share a launch (layer steps, together and apart: 1024^3 34 and 41 us, 2048^3 50 and 60, 16384 x 512 over 512
+// 58 and 62; behind it 3000^3 106 and 116, 3840^3 144 and 163, 7000 x 2000 over 1500 undropped 136 and 133).
+constexpr int64_t kPairBlocks = 1024;
 constexpr int kMaxList = 4096;        // 128-blocks that a workgroup's list can hold
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -361,8 +363,9 @@ __global__ __launch_bounds__(GROUPS * 256, 2) void fp8_pair_kernel(Args x, Args 
 // DSD walks the 128-blocks that either row block keeps; a group whose row block drops one skips its phases' work, and the block is not
 // loaded.  SDD takes two of the column blocks that either row of the pair keeps, in their order (behind them those that neither
 // keeps, whose blocks of C come out as zeros); a wave whose block of C is dropped skips its work.
-// 8192^3: 404 us, 2720 TFLOP/s, at the clock that the power limit leaves.  Half of the blocks dropped: 285 us (DSD; the loads alone 192, reads and
-// products alone 242, phases of a row block that drops its 128-block idle).
+// 8192^3: 377 us, 2920 TFLOP/s, at the clock that the power limit leaves (the library's, with one scale for all, 337; the first 150 launches after
+// a pause, while the clock settles, take 400 to 545).  Half of the blocks dropped: 255 us (DSD; in a run of 20, 285, the loads alone took 192 and reads
+// and products alone 242: phases of a row block that drops its 128-block idle).
 constexpr int kBigStage = 4 * kBlockBytes;        // A's two blocks, B's two
 constexpr int kBigScales = 2 * kBigStage;         // then 256 bytes of A's scales and 256 of B's for each stage
 constexpr int kBigList = kBigScales + 2 * 512;
@@ -508,8 +511,8 @@ __global__ __launch_bounds__(512, 2) void fp8_big_kernel(Args p) {
 // and w + 4, one of either group, share a SIMD.  A phase is a step: while one group reads the step's fragments into registers (and
 // puts the blocks of the step after next on their way into the third stage), the other's matrix instructions run from theirs.  At the end the
 // groups swap halves of their sums through LDS, add and store a half each.
-// dX of 8192^3 at p = 0.5: 321 us, 371 on 256 x 256 tiles (duo_pays has both at other sizes); it loads 48 KB for two blocks of C a step, those 64 for up to four.
-// (DSD in this shape, whose row blocks walk the reduction apart from each other and meet in the L2 less: 431 us, 310 on 256 x 256.)
+// dX of 8192^3 at p = 0.5: 293 us, 307 on 256 x 256 tiles (duo_pays has both at other sizes); it loads 48 KB for two blocks of C a step, those 64 for up to four.
+// (DSD in this shape, whose row blocks walk the reduction apart from each other and meet in the L2 less: 431 us when 256 x 256 took 310.)
 constexpr int kDuoStage = 3 * kBlockBytes;        // A's block, B's two
 constexpr int kDuoScales = 3 * kDuoStage;         // then 256 bytes of A's scales and 256 of B's for each stage
 constexpr int kDuoList = kDuoScales + 3 * 512;
@@ -694,9 +697,9 @@ int launch_mid(const Args& p, hipStream_t stream) {
   return check_launch("fp8_gemm");
 }
 
-// Two groups of waves where every workgroup has a CU to itself and more than eight steps (300 x 300 over 4096 in 11 parts 10.7 us with either,
-// 1024^3, eight steps, 9.0 with one and 9.8 with two, 512 x 4096 over 4096, 32 steps, 26.1 and 22.4; with few steps the exchange of sums at
-// the end, about 1 us, counts)
+// Two groups of waves where every workgroup has a CU to itself and more than eight steps.  One group and two: 1024^2 over 512 6.0 and 7.4 us, 1024 8.4 and
+// 9.2, 1152 9.2 and 9.9, 1536 11.5 and 11.5, 2048 13.1 and 13.1; 2048^2 over 2048 15.0 and 14.5, over 4096 23.9 and 22.3, 512 x 4096 over 4096 22.6 and 20.8
+// (with few steps the exchange of sums at the end, about 1 us, counts); more tiles than CUs: 2176 x 2048 over 2048 16.0 and 25.2.
 bool deep(int64_t blocks, const Args& p) { return blocks <= kCus && p.per_split > 8; }
 
 template <typename T, int MODE>
@@ -753,7 +756,7 @@ int64_t busiest_rounds(int64_t rows, int64_t cols, double full) {
 }
 // SDD on tiles of 128 x 256 of a row block's kept blocks instead of 256 x 256 of those that either row block of a pair keeps: where their
 // rounds are expected to take less.  Microseconds, with nk = N / 128 steps, a round 0.9 nk + 10 and 1.25 nk + 5.  Input gradients with their quantizing,
-// 128 x 256 and 256 x 256: 8192^3, p = 0.4 381 and 367 us, 0.5 327 and 364, 0.75 220 and 346; 4096^3, 0.5 74 and 58, 0.75 72 and 56;
+// 128 x 256 and 256 x 256: 8192^3, p = 0.4 378 and 362 us, 0.5 329 and 343, 0.75 218 and 345; 4096^3, 0.5 74 and 58, 0.75 72 and 56;
 // 4096 x 8192 over 8192, 0.5 248 and 185 (the full ends of 32 row blocks go to four XCDs), 8192 x 8192 over 4096, 0.75 123 and 173.
 // Over 152 products of 4096 to 18000 rows, p from 0.2 to 0.9 and blocks of 128 to 384 the choice takes 0.7 % longer than the faster of both (17 % at
 // most), by the drop rate alone (from 0.45 on) 8 % (50 %), 256 x 256 tiles always 3.3 % (76 %).

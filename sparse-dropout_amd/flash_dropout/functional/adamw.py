@@ -8,8 +8,11 @@ Averages in 8 bits are codes, a byte an element in the order of the parameter's 
 (bias 15) and three of mantissa, the largest 61440.  The scale is the least with which the block stays within the largest
 number.  Both are rounded at random, up with the probability that the value's place between two codes says: an average moves by a
 thousandth of its distance in a step, and rounded to nearest it would stay where it is.  The random bits are a function of t
-and the element's index (M. O'Neill's permuted congruential generator), so equal runs have equal states.  Zeros are codes 0 with
-scales 127.
+and the element's index (M. O'Neill's permuted congruential generator), so equal runs have equal states: elements of one index in
+different tensors, and both averages of an element, are rounded by parts of one word.  Zeros are codes 0 with scales 127.
+
+The update is computed in 32 bits.  With averages in 8 bits, which are computed in 64, its root and reciprocal are the hardware's, one unit of
+the last place off, not the exact ones that it has with averages in 32 bits.
 """
 from __future__ import annotations
 
