@@ -623,7 +623,7 @@ int sd_conv2d_taps_dw(const void* x_rows, int64_t x_ld, const void* dy_rows, int
  * sd_fp8_linear: Y = X . W^T for X in 16 bits, which is quantized in 1 x 128 blocks, and weights in 128 x 128 blocks.
  *   Few rows (16, and up to 64 where N K is not large) run in one launch that reads each weight once and needs no workspace.
  * sd_fp8_dropout_matmul_forward: Y = s (keep (.) X) W^T with X in 1 x 128 and W in 128 x 128 blocks; mask given, or drawn as
- *   sd_random_lists draws it and stored to mask_out [ceil(M/bs), ceil(K/bs)].  Dropped blocks are neither quantized nor multiplied.
+ *   sd_random_lists draws it (p below one in 32 bits) and stored to mask_out [ceil(M/bs), ceil(K/bs)].  Dropped blocks are neither quantized nor multiplied.
  *   XT (a [K, M] matrix) and WT (a square [K, N] one), each NULL where its gradient is not wanted, receive what the backward
  *   reads: X in blocks along the tokens, for dW sums over them, and W turned.  block_size: multiples of 128
  *   (SD_ERR_UNSUPPORTED otherwise).
@@ -665,7 +665,8 @@ int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dy_stride_r, int64_t 
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
  *
  * count tensors of one dtype (f16, bf16 or f32, gradients alike), each of numels[i] elements without gaps; the arrays of pointers and sizes
- * are HOST arrays, read before the call returns.  state_bits 32: exp_avgs and exp_avg_sqs are floats.  8: codes, a byte an element, and
+ * are HOST arrays, read before the call returns.  Nothing that is written may share memory with another of the tensors; a
+ * parameter may be its own gradient.  state_bits 32: exp_avgs and exp_avg_sqs are floats.  8: codes, a byte an element, and
  * a power of two (exponent + 127) for each 128 elements in the scales: the first average e4m3, the second without a sign, five bits of exponent
  * (bias 15) and three of mantissa.  Both are rounded at random, up with the probability that the value's place between two codes says; the
  * random bits are a function of t and the element's index.  Zeros are codes 0 with scales 127.
