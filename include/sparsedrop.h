@@ -59,7 +59,7 @@ enum sd_status {
 enum sd_dtype { SD_F16 = 0, SD_BF16 = 1, SD_F32 = 2 };
 
 /* activations the GEMM epilogues can apply; GELU is the exact (erf) form, torch.nn.GELU's default */
-enum sd_act { SD_ACT_NONE = 0, SD_ACT_RELU = 1, SD_ACT_GELU = 2 };
+enum sd_act { SD_ACT_NONE = 0, SD_ACT_RELU = 1, SD_ACT_GELU = 2, SD_ACT_SILU = 3 /* x / (1 + exp(-x)); only in the gated calls */ };
 
 /* Library version (major*10000 + minor*100 + patch). No reference counterpart. */
 int sd_version(void);
@@ -681,6 +681,43 @@ int sd_adamw_step(int count, void* const* params, const void* const* grads, void
                   int state_bits, int advance, void* stream);
 int sd_adamw_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* values,
                           const int64_t* numels, const int32_t* second, void* stream);
+/* sd_adamw_step with every gradient taken times *grad_scale, a float in device memory (NULL: as it is), rounded to 32 bits: clipping
+ * without a pass over the gradients (sd_grad_norm gives the factor). */
+int sd_adamw_step_scaled(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                         uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales, const int64_t* numels, int64_t* step,
+                         const float* lr_at, double lr, double beta1, double beta2, double eps, double weight_decay, int dtype,
+                         int state_bits, int advance, const float* grad_scale, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (h) the norm of many gradients together, and clipping
+ *
+ *   norm = sqrt(sum of all squares) (SD_NORM_2) or the largest magnitude (SD_NORM_MAX);  c = min(1, max_norm / (norm + 1e-6))
+ *
+ * count tensors of dtypes[i] (f16, bf16 or f32), each of numels[i] elements without gaps, at any element's address; the arrays are HOST
+ * arrays, read before the call returns.  Squares are summed in 64 bits in an order that the sizes fix.  norm, scale: floats in device
+ * memory.  A norm that is not finite gives a factor of 0 or NaN, as the formula has it.
+ * sd_grad_norm: the norm, and c to scale where that is not NULL (max_norm is not looked at otherwise).
+ * sd_clip_grads: the norm, and every gradient times c, in place (they must not share memory); a factor of one writes nothing.
+ * workspace: sd_grad_norm_workspace_bytes bytes on 8 bytes, of one call at a time.
+ * ------------------------------------------------------------------------------------------- */
+enum sd_norm { SD_NORM_MAX = 0, SD_NORM_2 = 2 };
+int64_t sd_grad_norm_workspace_bytes(int count, const int64_t* numels);
+int sd_grad_norm(int count, const void* const* grads, const int64_t* numels, const int32_t* dtypes, int norm_type, double max_norm,
+                 float* norm, float* scale, void* workspace, int64_t workspace_bytes, void* stream);
+int sd_clip_grads(int count, void* const* grads, const int64_t* numels, const int32_t* dtypes, int norm_type, double max_norm,
+                  float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (i) a gated feed-forward block's hidden activations
+ *
+ * A[M, 2F] = [G | U] (pitch lda), both products' results beside one another; act: relu, gelu or silu.
+ * sd_gated_forward:  H = act(G) U                        (H [M, F], pitch ldh)
+ * sd_gated_backward: dA = [dH U act'(G) | dH act(G)]     (dH [M, F], pitch ldd; dA [M, 2F], pitch ldda; dA may be A)
+ * Computed in fp32, rounded once.
+ * ------------------------------------------------------------------------------------------- */
+int sd_gated_forward(const void* A, int64_t lda, void* H, int64_t ldh, int64_t M, int64_t F, int act, int dtype, void* stream);
+int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, void* dA, int64_t ldda, int64_t M, int64_t F, int act,
+                      int dtype, void* stream);
 
 #ifdef __cplusplus
 }

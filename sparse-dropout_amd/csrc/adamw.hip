@@ -38,7 +38,7 @@ struct AdamTable {
   int32_t n;
   int64_t* step;
   int32_t last;  // of the call's launches: moves the step on
-  const float* lr_at;
+  const float *lr_at, *grad_scale;
   double lr, beta1, beta2, eps, decay;
 };
 static_assert(sizeof(AdamTable) <= 4096, "a launch's arguments");
@@ -250,6 +250,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamTable a) {
   bool known = false;
   uint32_t t = 0u, key = 0u;
   const uint32_t chunks = a.first[a.n];
+  const float clip = a.grad_scale ? *a.grad_scale : 1.f;  // (times one nothing changes)
   int which = 0;
   // (with no elements at all one workgroup runs, to move the step on: through an empty piece of an empty tensor)
   for (uint32_t chunk = blockIdx.x * PART + part; chunk < chunks || !known; chunk += gridDim.x * PART) {
@@ -261,6 +262,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamTable a) {
     float p[kPer], g[kPer];
     load_typed<T>(x.p, at, left, p);
     load_typed<T>(x.g, at, left, g);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) g[i] *= clip;
     // the step's factors, worked out while the first loads are on their way
     auto factors = [&] {
       if (known) return;
@@ -425,10 +428,11 @@ void launch_table(const AdamTable& a, int bits, uint32_t chunks, hipStream_t str
 
 int launch_adamw(int count, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* ms, uint8_t* const* vs,
                  const int64_t* n, int64_t* step, const float* lr_at, double lr, double beta1, double beta2, double eps, double decay,
-                 int dtype, int bits, bool moves_on, hipStream_t stream) {
+                 int dtype, int bits, bool moves_on, const float* grad_scale, hipStream_t stream) {
   AdamTable a = {};
   a.step = step;
   a.lr_at = lr_at;
+  a.grad_scale = grad_scale;
   a.lr = lr;
   a.beta1 = beta1;
   a.beta2 = beta2;

@@ -9,7 +9,7 @@ int launch_dequantize(const uint8_t* data, int64_t ld, const uint8_t* scales, in
                       int64_t cols, void* out, int64_t out_ld, int dtype, hipStream_t stream);
 int launch_adamw(int count, void* const* p, const void* const* g, void* const* m, void* const* v, uint8_t* const* ms, uint8_t* const* vs,
                  const int64_t* n, int64_t* step, const float* lr_at, double lr, double beta1, double beta2, double eps, double decay,
-                 int dtype, int bits, bool moves_on, hipStream_t stream);
+                 int dtype, int bits, bool moves_on, const float* grad_scale, hipStream_t stream);
 int launch_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* out, const int64_t* n,
                         const int32_t* second, hipStream_t stream);
 
@@ -372,10 +372,10 @@ int sd_fp8_dropout_matmul_backward(const void* dY, int64_t dysr, int64_t dysc, c
   return dX ? launch_fp8_gemm(gx, kFp8Sdd, dtype, (hipStream_t)stream) : launch_fp8_gemm(gw, kFp8Dsd, dtype, (hipStream_t)stream);
 }
 
-int sd_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
-                  uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales, const int64_t* numels, int64_t* step,
-                  const float* lr_at, double lr, double beta1, double beta2, double eps, double weight_decay, int dtype, int state_bits,
-                  int advance, void* stream) {
+int sd_adamw_step_scaled(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                         uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales, const int64_t* numels, int64_t* step,
+                         const float* lr_at, double lr, double beta1, double beta2, double eps, double weight_decay, int dtype, int state_bits,
+                         int advance, const float* grad_scale, void* stream) {
   SD_REQUIRE(count >= 0, "adamw_step: negative count");
   SD_REQUIRE(dtype == SD_F16 || dtype == SD_BF16 || dtype == SD_F32, "adamw_step: dtype must be SD_F16, SD_BF16 or SD_F32 (got %d)", dtype);
   SD_REQUIRE(state_bits == 8 || state_bits == 32, "adamw_step: averages are held in 8 or in 32 bits (got %d)", state_bits);
@@ -392,7 +392,15 @@ int sd_adamw_step(int count, void* const* params, const void* const* grads, void
     SD_REQUIRE(state_bits == 32 || (exp_avg_scales && exp_avg_sq_scales && exp_avg_scales[i] && exp_avg_sq_scales[i]), "adamw_step: tensor %d: averages in 8 bits need their scales", i);
   }
   return launch_adamw(count, params, grads, exp_avgs, exp_avg_sqs, state_bits == 8 ? exp_avg_scales : nullptr, state_bits == 8 ? exp_avg_sq_scales : nullptr,
-                      numels, step, lr_at, lr, beta1, beta2, eps, weight_decay, dtype, state_bits, advance != 0, (hipStream_t)stream);
+                      numels, step, lr_at, lr, beta1, beta2, eps, weight_decay, dtype, state_bits, advance != 0, grad_scale, (hipStream_t)stream);
+}
+
+int sd_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                  uint8_t* const* exp_avg_scales, uint8_t* const* exp_avg_sq_scales, const int64_t* numels, int64_t* step,
+                  const float* lr_at, double lr, double beta1, double beta2, double eps, double weight_decay, int dtype, int state_bits,
+                  int advance, void* stream) {
+  return sd_adamw_step_scaled(count, params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, numels, step, lr_at, lr, beta1, beta2,
+                              eps, weight_decay, dtype, state_bits, advance, nullptr, stream);
 }
 
 int sd_adamw_state_values(int count, const uint8_t* const* codes, const uint8_t* const* scales, float* const* values, const int64_t* numels,

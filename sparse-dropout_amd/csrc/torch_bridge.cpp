@@ -335,7 +335,7 @@ Tensor layer_forward(Tensor x, Tensor w, int64_t bs, double p, const Draw& draw,
   return y;
 }
 
-// dX and / or dW of one layer in one library call; act_at: what dX's fused activation derivative is evaluated at.
+// dX and / or dW of one layer in one library call (without lists, of a dense product, in one each); act_at: what dX's fused activation derivative is evaluated at.
 // kept_only (without an activation): dropped blocks of dX are left as they are.
 std::pair<Tensor, Tensor> layer_products(const Tensor& dy, const Tensor& w, const Tensor& x, const Lists& lists, double p,
                                          bool need_dx, bool need_dw, int act, const Tensor& act_at, bool kept_only = false) {
@@ -343,6 +343,20 @@ std::pair<Tensor, Tensor> layer_products(const Tensor& dy, const Tensor& w, cons
   Tensor dx = need_dx ? new_matrix(x, M, K) : Tensor(), dw = need_dw ? new_matrix(x, N, K) : Tensor();
   if (!(need_dx || need_dw) || M == 0 || K == 0) return {dx, dw};
   if (N == 0) return {need_dx ? dx.zero_() : dx, dw};
+  if (!lists.buf.defined()) {  // nothing dropped
+    Scratch ws(x, need_dw ? sd_splitk_workspace_bytes(K, N, M, 0, 0) : 0);
+    const Mat gm(dy), wm(w), xm(x);
+    c10::DeviceGuard guard(x.device());
+    if (need_dx) {
+      const Mat d(dx);
+      check(sd_gemm(MAT(gm), wm.ptr, wm.sc, wm.sr, MAT(d), M, K, N, dtype_of(x), nullptr, 0, stream_of(x)), "sd_gemm");
+    }
+    if (need_dw) {
+      const Mat d(dw);
+      check(sd_gemm(xm.ptr, xm.sc, xm.sr, gm.ptr, gm.sc, gm.sr, d.ptr, d.sc, d.sr, K, N, M, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)), "sd_gemm");
+    }
+    return {dx, dw};
+  }
   const int64_t g = lists.kernel_bs == 32 ? 64 : lists.kernel_bs;
   Scratch ws(x, need_dw ? sd_splitk_workspace_bytes(K, N, M, g, 1) : 0);
   if (!need_dx) act = SD_ACT_NONE;
@@ -622,6 +636,105 @@ Tensor mlp(const Tensor& input, const std::vector<Tensor>& weights, int64_t bs, 
     torch::autograd::set_history(h, node);
   }
   return h;
+}
+
+// ---- a gated feed-forward block ------------------------------------------------------------------------------------------
+// (see functional/gated_mlp.py for what is computed)
+struct GatedMlpBackward : Node {
+  Saved x, w_in, w_out, pre, h;  // pre: [G | U], h = act(G) U
+  SavedLists lists[2];           // nothing kept: nothing is dropped
+  double p[2] = {0.0, 0.0};
+  int act = SD_ACT_NONE;
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    at::NoGradGuard no_grad;
+    variable_list out(3);
+    const Tensor xs = x.matrix(), wi = w_in.matrix(), wo = w_out.matrix();
+    TORCH_CHECK(xs.defined(), "Trying to backward through the graph a second time, or after its saved tensors were freed");
+    const bool need_x = task_should_compute_output(0), need_in = task_should_compute_output(1), need_out = task_should_compute_output(2);
+    if (xs.size(0) == 0 || !grads[0].defined()) {
+      if (need_x) out[0] = at::zeros(xs.sizes(), xs.options());
+      if (need_in) out[1] = at::zeros(wi.sizes(), wi.options());
+      if (need_out) out[2] = at::zeros(wo.sizes(), wo.options());
+      return out;
+    }
+    const Tensor dy = grad_matrix(grads[0], xs), hs = h.matrix(), a = pre.matrix();
+    const int64_t M = xs.size(0), F = wo.size(1);
+    Tensor dh;
+    std::tie(dh, out[2]) = layer_backward(dy, wo, hs, lists[1].get(), p[1], need_x || need_in, need_out, SD_ACT_NONE, Tensor());
+    if (!need_x && !need_in) return out;
+    const Tensor as = row_major(a) ? a : a.contiguous();
+    Tensor da = new_matrix(xs, M, 2 * F);
+    {
+      const Mat dm(dh), am(as), om(da);
+      c10::DeviceGuard guard(xs.device());
+      check(sd_gated_backward(dm.ptr, dm.sr, am.ptr, am.sr, om.ptr, om.sr, M, F, act, dtype_of(xs), stream_of(xs)), "sd_gated_backward");
+    }
+    std::tie(out[0], out[1]) = layer_backward(da, wi, xs, lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
+    return out;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (Saved* s : {&x, &w_in, &w_out, &pre, &h}) s->drop();
+    for (SavedLists& l : lists) l.drop();
+  }
+  std::string name() const override { return "GatedMLPHIPBackward"; }
+};
+
+// bs 0: nothing is dropped; else layers without a given mask and with ps[i] == 0 drop nothing and draw nothing
+Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& weight_out, int64_t bs, const std::vector<double>& ps, int act,
+                 const std::optional<std::vector<OptTensor>>& masks, std::optional<uint64_t> seed, const OptTensor& state) {
+  TORCH_CHECK_VALUE(input.dim() == 2 && weight_in.dim() == 2 && weight_out.dim() == 2,
+                    "input must be [M, K], weight_in [2 F, K] and weight_out [N, F]");
+  const Tensor x = as_matrix(autocast(input)), wi = as_matrix(autocast(weight_in)), wo = as_matrix(autocast(weight_out));
+  const variable_list inputs{x, wi, wo};
+  refuse_forward_mode(inputs);
+  check_pair(x, wi);
+  check_operand("weight_out", wo);
+  TORCH_CHECK_TYPE(wo.scalar_type() == x.scalar_type(), "input and weight_out must have the same dtype (", x.dtype(), " vs ", wo.dtype(), ")");
+  TORCH_CHECK_VALUE(wo.device() == x.device(), "input and weight_out must be on the same device");
+  const int64_t M = x.size(0), F = wo.size(1), N = wo.size(0);
+  TORCH_CHECK_VALUE(wi.size(0) == 2 * F, "weight_in must have the rows of both projections, 2 x ", F, " (got ", wi.size(0), ")");
+  TORCH_CHECK_VALUE(F > 0 && N > 0 && x.size(1) > 0, "the block's features, hidden width and outputs must not be empty");
+  const bool rec = records(inputs);
+  Lists lists[2];
+  Tensor pre, h, y;
+  {
+    NoRecord guard;
+    auto product = [&](int i, const Tensor& a, const Tensor& w) {
+      const OptTensor mask = masks ? (*masks)[i] : OptTensor();
+      if (bs == 0 || (ps[i] == 0.0 && !mask)) return dense(a, w, SD_ACT_NONE, false, nullptr);
+      const Draw draw{mask, seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
+      return layer_forward(a, w, bs, ps[i], draw, SD_ACT_NONE, false, lists[i], nullptr);
+    };
+    if (M == 0) {
+      y = new_matrix(x, 0, N);
+    } else {
+      pre = product(0, x, wi);
+      h = new_matrix(x, M, F);
+      {
+        const Mat am(pre), hm(h);
+        c10::DeviceGuard device(x.device());
+        check(sd_gated_forward(am.ptr, am.sr, hm.ptr, hm.sr, M, F, act, dtype_of(x), stream_of(x)), "sd_gated_forward");
+      }
+      y = product(1, h, wo);
+    }
+  }
+  if (rec) {
+    auto node = make_node<GatedMlpBackward>(inputs);
+    node->x.keep(x);
+    node->w_in.keep(wi);
+    node->w_out.keep(wo);
+    node->pre.keep(pre);
+    node->h.keep(h);
+    for (int i = 0; i < 2; ++i) {
+      if (lists[i].buf.defined()) node->lists[i].keep(std::move(lists[i]));
+      node->p[i] = bs ? ps[i] : 0.0;
+    }
+    node->act = act;
+    torch::autograd::set_history(y, node);
+  }
+  return y;
 }
 
 // ---- convolution --------------------------------------------------------------------------------------------------------
@@ -1465,7 +1578,8 @@ bool same_order(const Tensor& a, const Tensor& b) {
 
 void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& avgs,
                 const std::vector<Tensor>& sqs, const std::vector<Tensor>& avg_scales, const std::vector<Tensor>& sq_scales,
-                const Tensor& step, const OptTensor& lr_at, double lr, double beta1, double beta2, double eps, double decay) {
+                const Tensor& step, const OptTensor& lr_at, double lr, double beta1, double beta2, double eps, double decay,
+                const OptTensor& grad_scale) {
   at::NoGradGuard no_grad;
   const size_t n = params.size();
   const bool in8 = !avg_scales.empty() || !sq_scales.empty();
@@ -1475,6 +1589,8 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
                     step.sizes(), " ", step.dtype(), " on ", step.device(), ")");
   TORCH_CHECK_VALUE(!lr_at || (lr_at->device() == step.device() && lr_at->scalar_type() == at::kFloat && lr_at->numel() == 1),
                     "a learning rate in a tensor must be one float32 on ", step.device());
+  TORCH_CHECK_VALUE(!grad_scale || (grad_scale->device() == step.device() && grad_scale->scalar_type() == at::kFloat && grad_scale->numel() == 1),
+                    "a factor of the gradients must be one float32 on ", step.device());
   std::vector<Tensor> keep;  // gradients laid out here
   struct Group {
     std::vector<void*> p, m, v;
@@ -1544,10 +1660,11 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   for (int i = 0; i < 3; ++i) {
     Group& to = groups[i];
     if (to.n.empty() && i != last) continue;
-    check(sd_adamw_step((int)to.n.size(), to.p.data(), to.g.data(), to.m.data(), to.v.data(), to.ms.data(), to.vs.data(), to.n.data(),
+    check(sd_adamw_step_scaled((int)to.n.size(), to.p.data(), to.g.data(), to.m.data(), to.v.data(), to.ms.data(), to.vs.data(), to.n.data(),
                         static_cast<int64_t*>(step.data_ptr()), lr_at ? static_cast<const float*>(lr_at->data_ptr()) : nullptr, lr, beta1,
-                        beta2, eps, decay, i, in8 ? 8 : 32, i == last ? 1 : 0, stream_of(step)),
-          "sd_adamw_step");
+                        beta2, eps, decay, i, in8 ? 8 : 32, i == last ? 1 : 0,
+                        grad_scale ? static_cast<const float*>(grad_scale->data_ptr()) : nullptr, stream_of(step)),
+          "sd_adamw_step_scaled");
   }
   for (const auto* list : {&params, &avgs, &sqs, &avg_scales, &sq_scales})
     for (const Tensor& t : *list) written(t);
@@ -1582,6 +1699,80 @@ std::vector<Tensor> adamw_state_values(const std::vector<Tensor>& codes, const s
   return out;
 }
 
+// ---- the norm of gradients, and clipping ------------------------------------------------------------------------------------------
+// (see functional/clip.py for what is computed)
+struct GradList {
+  std::vector<void*> p;
+  std::vector<int64_t> n;
+  std::vector<int32_t> dtype;
+  std::vector<Tensor> keep;  // gradients laid out here
+  c10::Device device = c10::Device(at::kCPU);
+  // in_place: they are written, so they fill their memory and share none of it
+  GradList(const std::vector<Tensor>& grads, bool in_place) {
+    TORCH_CHECK_VALUE(!grads.empty(), "at least one gradient is needed");
+    device = grads[0].device();
+    std::vector<Span> spans;
+    for (size_t i = 0; i < grads.size(); ++i) {
+      const Tensor& g = grads[i];
+      TORCH_CHECK_VALUE(g.is_cuda() && g.device() == device, "gradient ", i, " is on ", g.device(), ", the first on ", device,
+                        ": all must be on one GPU");
+      TORCH_CHECK_VALUE(g.layout() == at::kStrided, "gradient ", i, ": sparse gradients are not taken");
+      const int code = dtype_with_f32("a gradient", g);
+      if (g.numel() == 0) continue;
+      Tensor t = g;
+      if (!g.is_non_overlapping_and_dense() || g.is_neg()) {
+        TORCH_CHECK_VALUE(!in_place, "gradient ", i, " must fill its memory to be scaled in place (strides ", g.strides(), ")");
+        t = at::empty(g.sizes(), g.options()).copy_(g);
+        keep.push_back(t);
+      }
+      if (in_place) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+        spans.push_back({at, at + static_cast<uintptr_t>(t.numel()) * t.element_size(), i, true});
+      }
+      p.push_back(t.data_ptr());
+      n.push_back(t.numel());
+      dtype.push_back(code);
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < spans.size(); ++i)
+      TORCH_CHECK_VALUE(spans[i].begin >= spans[i - 1].end, "gradients ", std::min(spans[i].parameter, spans[i - 1].parameter), " and ",
+                        std::max(spans[i].parameter, spans[i - 1].parameter), " share memory: they cannot be scaled in place");
+  }
+  at::TensorOptions floats() const { return at::TensorOptions().device(device).dtype(at::kFloat); }
+};
+
+void check_max_norm(double max_norm) { TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative (got ", max_norm, ")"); }
+
+// (norm, factor); the factor only with a limit
+std::tuple<Tensor, OptTensor> grad_norm(const std::vector<Tensor>& grads, int norm_type, std::optional<double> max_norm) {
+  at::NoGradGuard no_grad;
+  if (max_norm) check_max_norm(*max_norm);
+  const GradList g(grads, false);
+  c10::DeviceGuard guard(g.device);
+  Tensor norm = at::empty({}, g.floats());
+  OptTensor scale;
+  if (max_norm) scale = at::empty({}, g.floats());
+  const Scratch ws(norm, sd_grad_norm_workspace_bytes((int)g.n.size(), g.n.data()));
+  check(sd_grad_norm((int)g.n.size(), g.p.data(), g.n.data(), g.dtype.data(), norm_type, max_norm.value_or(0.0), static_cast<float*>(norm.data_ptr()),
+                     scale ? static_cast<float*>(scale->data_ptr()) : nullptr, ws.ptr, ws.bytes, stream_of(norm)),
+        "sd_grad_norm");
+  return {norm, scale};
+}
+
+Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, int norm_type) {
+  at::NoGradGuard no_grad;
+  check_max_norm(max_norm);
+  const GradList g(grads, true);
+  c10::DeviceGuard guard(g.device);
+  Tensor norm = at::empty({}, g.floats());
+  const Scratch ws(norm, sd_grad_norm_workspace_bytes((int)g.n.size(), g.n.data()));
+  check(sd_clip_grads((int)g.n.size(), g.p.data(), g.n.data(), g.dtype.data(), norm_type, max_norm, static_cast<float*>(norm.data_ptr()), ws.ptr,
+                      ws.bytes, stream_of(norm)),
+        "sd_clip_grads");
+  for (const Tensor& t : grads) written(t);
+  return norm;
+}
+
 std::array<int, 3> conv_routes() { return {last_routes[0].load(), last_routes[1].load(), last_routes[2].load()}; }
 
 }  // namespace
@@ -1601,4 +1792,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_fp8", torch::wrap_pybind_function(linear_fp8));
   m.def("adamw_step", torch::wrap_pybind_function(adamw_step));
   m.def("adamw_state_values", torch::wrap_pybind_function(adamw_state_values));
+  m.def("grad_norm", torch::wrap_pybind_function(grad_norm));
+  m.def("clip_grads", torch::wrap_pybind_function(clip_grads));
+  m.def("gated_mlp", torch::wrap_pybind_function(gated_mlp));
 }

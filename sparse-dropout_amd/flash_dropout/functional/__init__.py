@@ -5,9 +5,12 @@ from .adamw import adamw_state_values, adamw_step
 from .blockwise_dropout_matmul_hip import blockwise_dropout_matmul as hip_blockwise_dropout_matmul
 from .blockwise_dropout_matmul_hip import blockwise_dropout_matmul_mask as hip_blockwise_dropout_matmul_mask
 from .blockwise_dropout_mlp_hip import blockwise_dropout_mlp as hip_blockwise_dropout_mlp
+from .clip import clip_grad_norm_, grad_norm
 from .fp8_blocks import blockwise_dropout_matmul_fp8 as hip_blockwise_dropout_matmul_fp8
 from .fp8_blocks import blockwise_dropout_matmul_fp8_mask as hip_blockwise_dropout_matmul_fp8_mask
 from .fp8_blocks import fp8_dequantize, fp8_linear, fp8_quantize
+from .gated_mlp import blockwise_dropout_gated_mlp as hip_blockwise_dropout_gated_mlp
+from .gated_mlp import gated_mlp
 from .im2col_conv2d import (
     blockwise_dropout_conv2d,
     blockwise_dropout_conv2d_mask,

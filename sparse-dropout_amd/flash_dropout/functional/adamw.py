@@ -40,11 +40,12 @@ def _split(averages, name):
 @refused_under_trace
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence, exp_avg_sqs: Sequence,
                step: torch.Tensor, *, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
-               weight_decay: float = 1e-2) -> None:
+               weight_decay: float = 1e-2, grad_scale: torch.Tensor | None = None) -> None:
     """Updates ``params`` (float16, bfloat16 or float32, also mixed), both averages and ``step`` in place.  The averages are float32
     tensors laid out like their parameters or ``(codes, scales)`` pairs of uint8 tensors, the codes laid out like their parameters too or in one
     run.  ``step``: one int64 on the GPU, the number of steps so far, moved on by the call itself: a captured graph counts its replays.
-    ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  One launch for each 56 tensors of a dtype.
+    ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay, and so may ``grad_scale``, which gradients are
+    multiplied by as they are read (:func:`grad_norm` gives the one that clips).  One launch for each 56 tensors of a dtype.
     ``torch.jit.trace`` is refused."""
     beta1, beta2 = (float(b) for b in betas)
     firsts, first_scales = _split(exp_avgs, "exp_avgs")
@@ -53,7 +54,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("both averages are held in 32 bits, or both in 8")
     at = lr if isinstance(lr, torch.Tensor) else None
     _loader.bridge().adamw_step(list(params), list(grads), firsts, seconds, first_scales, second_scales, step, at,
-                                0.0 if at is not None else float(lr), beta1, beta2, float(eps), float(weight_decay))
+                                0.0 if at is not None else float(lr), beta1, beta2, float(eps), float(weight_decay), grad_scale)
 
 
 @refused_under_trace

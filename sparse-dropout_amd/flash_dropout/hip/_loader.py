@@ -136,7 +136,14 @@ SIGNATURES = {
     "sd_fp8_dropout_matmul_backward": (c_int, [*_mat, *_mat, c_void_p, c_void_p, *_mat, *_mat, c_int64, c_int64, c_int64, c_int64,
                                                c_double, c_int, c_void_p, c_int64, c_void_p]),
     "sd_adamw_step": (c_int, [c_int, *([c_void_p] * 9), c_double, c_double, c_double, c_double, c_double, c_int, c_int, c_int, c_void_p]),
+    "sd_adamw_step_scaled": (c_int, [c_int, *([c_void_p] * 9), c_double, c_double, c_double, c_double, c_double, c_int, c_int, c_int, c_void_p,
+                                     c_void_p]),
     "sd_adamw_state_values": (c_int, [c_int, *([c_void_p] * 5), c_void_p]),
+    "sd_grad_norm_workspace_bytes": (c_int64, [c_int, c_void_p]),
+    "sd_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "sd_clip_grads": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_int64, c_void_p]),
+    "sd_gated_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "sd_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
 }
 
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from ..functional.adamw import adamw_empty_state, adamw_state_values, adamw_step
+from ..functional.clip import grad_norm
 from ..functional.tracing import refused_under_trace
 
 
@@ -17,9 +18,17 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay.  ``step`` of a parameter's state is an int64
     on the GPU, shared by the parameters that have been updated the same number of times; parameters without a gradient are left out
     of a step, as torch's optimizers leave them out.  A step can be captured into a graph once one with the same gradients has been
-    taken.  Parameters must be on the GPU, float16, bfloat16 or float32, and fill their memory."""
+    taken.  Parameters must be on the GPU, float16, bfloat16 or float32, and fill their memory.
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32) -> None:
+    ``max_norm``: gradients are clipped to that joint norm (of all groups) as the step reads them; ``p.grad`` stays as it is, and ``grad_norm`` is
+    the norm that the last step found, a float32 on the GPU (of a captured step: of its last replay).  It belongs to the optimizer, not to its
+    state, and may be changed between steps."""
+
+    max_norm: float | None = None
+    grad_norm: torch.Tensor | None = None
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits: int = 32,
+                 max_norm: float | None = None) -> None:
         if not isinstance(lr, torch.Tensor) and not lr >= 0:
             raise ValueError(f"lr must not be negative (got {lr})")
         if not all(0 <= b < 1 for b in betas):
@@ -28,7 +37,13 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"eps must be 0 or from 2^-126 to 2^120 and weight_decay not negative (got {eps}, {weight_decay})")
         if state_bits not in (8, 32):
             raise ValueError(f"averages are held in 8 or in 32 bits (got {state_bits})")
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"max_norm must not be negative (got {max_norm})")
+        self.max_norm = max_norm
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "grad_norm": self.grad_norm}
 
     def _init_state(self, p: torch.Tensor, bits: int, step: torch.Tensor) -> None:
         if bits not in (8, 32):
@@ -59,6 +74,11 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        factor = None
+        if self.max_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if grads:
+                self.grad_norm, factor = grad_norm(grads, max_norm=self.max_norm)
         for group in self.param_groups:
             fresh: dict[torch.device, torch.Tensor] = {}
             together: dict[int, list[torch.Tensor]] = {}  # by the step tensor that the parameters share
@@ -86,7 +106,8 @@ class AdamW(torch.optim.Optimizer):
                     for s in states:
                         s["step"] = step
                 adamw_step(params, [p.grad for p in params], self._averages(states, "exp_avg"), self._averages(states, "exp_avg_sq"), step,
-                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
+                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           grad_scale=factor)
         return loss
 
     def state_values(self, p: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

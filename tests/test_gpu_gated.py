@@ -1,0 +1,289 @@
+"""The gated feed-forward block on the GPU against its formulas in 64 bits: element by element within the bounds that oracle/gated_oracle.py
+derives from the roundings, and within the package's bar of 1e-2 in the relative Frobenius norm."""
+import pytest
+import torch
+
+from _util import REL_FRO_TOL, rel_fro
+from oracle import gated_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import flash_dropout.functional as F
+    from flash_dropout.layers import GatedMLP
+
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+NAMES = ("y", "dx", "dw_in", "dw_out")
+
+
+def operands(m, k, f, n, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    make = lambda r, c, std: (torch.randn(r, c, generator=gen) * std).to(DT[dtype]).cuda()
+    return make(m, k, 1.0), make(2 * f, k, k ** -0.5), make(n, f, f ** -0.5), make(m, n, 0.1)
+
+
+def masks_of(m, k, f, bs, p, seed=5):
+    gen = torch.Generator().manual_seed(seed)
+    return [(torch.rand(-(-m // bs), -(-c // bs), generator=gen) < p).cuda() for c in (k, f)]
+
+
+def run(x, w_in, w_out, dy, act, bs=None, p=0.0, masks=None):
+    leaves = [t.detach().requires_grad_() for t in (x, w_in, w_out)]
+    y = F.gated_mlp(*leaves, act) if bs is None else F.hip_blockwise_dropout_gated_mlp(*leaves, bs, p, act, masks=masks)
+    return dict(zip(NAMES, (y, *torch.autograd.grad(y, leaves, dy))))
+
+
+def check(got, ref):
+    for name in got:
+        value, bound = ref[name]
+        g = got[name].detach().double()
+        assert g.shape == value.shape, name
+        over = ((g - value).abs() > bound) | ~torch.isfinite(g)
+        assert not over.any(), (name, int(over.sum()), over.nonzero()[0].tolist(), float((g - value).abs().max()))
+        if value.numel() > 200 and float(value.abs().max()) > 1e-3:
+            assert rel_fro(g, value) < REL_FRO_TOL, name
+
+
+SIZES = [(1, 64, 64, 64), (1, 1024, 4096, 1024), (2, 8, 8, 8), (3, 1, 1, 1), (1, 130, 1, 5), (5, 77, 33, 19), (16, 512, 1024, 512), (17, 512, 1000, 200),
+         (33, 264, 136, 72), (64, 256, 512, 256), (65, 256, 512, 256), (128, 128, 64, 128), (130, 200, 96, 72), (257, 320, 704, 320), (301, 1025, 777, 640),
+         (512, 1024, 2048, 1024), (1100, 392, 1304, 264)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_block(size, act):
+    for dtype in ("fp16", "bf16"):
+        ops = operands(*size, dtype)
+        check(run(*ops, act), O.reference(*ops, act, DT[dtype]))
+        with torch.no_grad():
+            y = F.gated_mlp(*ops[:3], act)
+        check({"y": y}, O.reference(*ops, act, DT[dtype]))
+
+
+@pytest.mark.parametrize("bs,p", [(64, 0.5), (64, 0.1), (128, 0.3), (32, 0.5), (96, 0.25), (64, 0.9)])
+@pytest.mark.parametrize("size", [(64, 64, 64, 64), (130, 200, 96, 72), (301, 1025, 777, 640), (1024, 512, 1024, 512), (70, 640, 1300, 130)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_dropped_blocks(size, bs, p):
+    for dtype, act in (("fp16", "gelu"), ("bf16", "silu"), ("bf16", "relu")):
+        ops = operands(*size, dtype, seed=1)
+        masks = masks_of(*size[:3], bs, p)
+        got = run(*ops, act, bs, p, masks)
+        check(got, O.reference(*ops, act, DT[dtype], masks, bs, (p, p)))
+
+
+def test_large_products():
+    ops = operands(2048, 1024, 4096, 1024, "bf16", seed=2)
+    check(run(*ops, "silu"), O.reference(*ops, "silu", torch.bfloat16))
+    masks = masks_of(2048, 1024, 4096, 64, 0.5)
+    check(run(*ops, "gelu", 64, 0.5, masks), O.reference(*ops, "gelu", torch.bfloat16, masks, 64, (0.5, 0.5)))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("size", [(128, 256, 320, 64), (300, 136, 200, 88), (1024, 1024, 1024, 256)])
+def test_rows_and_operands_with_nothing_kept(size, which):
+    m, k, f, n = size
+    ops = operands(*size, "bf16", seed=3)
+    none = [torch.zeros(-(-m // 64), -(-c // 64), dtype=torch.bool, device="cuda") for c in (k, f)]
+    for rows in (slice(0, 1), slice(None)):
+        masks = [t.clone() for t in none]
+        masks[which][rows] = True
+        got = run(*ops, "silu", 64, (0.5, 0.0), masks)
+        check(got, O.reference(*ops, "silu", torch.bfloat16, masks, 64, (0.5, 0.0)))
+        assert not got["y"][:64].any() and not got["dx"][:64].any()
+        if rows == slice(None):
+            assert not got["dw_in"].any() and not got["dw_out"].any()
+
+
+def test_what_stands_in_dropped_blocks_reaches_nothing():
+    size = (192, 256, 320, 128)
+    ops = operands(*size, "fp16", seed=4)
+    masks = masks_of(192, 256, 320, 64, 0.4)
+    ref = run(*ops, "gelu", 64, 0.4, masks)
+    x = ops[0].clone()
+    drop = masks[0].repeat_interleave(64, 0).repeat_interleave(64, 1)
+    x[drop] = float("nan")
+    got = run(x, *ops[1:], "gelu", 64, 0.4, masks)
+    for name in NAMES:
+        assert torch.equal(got[name], ref[name]), name
+    # hidden activations that overflow in a dropped block
+    w_in = ops[1].clone()
+    w_in[64:128] *= 30000  # the gate's columns 64 .. 127
+    masks[1][:, 1] = True
+    got, ref = (run(ops[0], w, *ops[2:], "gelu", 64, 0.4, masks) for w in (w_in, ops[1]))
+    for name in ("y", "dw_out"):
+        assert torch.equal(got[name], ref[name]), name
+    assert not got["dw_in"][64:128].any() and torch.equal(got["dx"], ref["dx"])
+
+
+def test_layouts_of_operands():
+    ops = operands(72, 136, 200, 56, "bf16", seed=6)
+    ref = O.reference(*ops, "silu", torch.bfloat16)
+    turned = [t.t().contiguous().t() for t in ops]
+    check(run(*turned, "silu"), ref)
+    wide = [torch.cat((t, t), 1)[:, : t.shape[1]] for t in ops]
+    check(run(*wide, "silu"), ref)
+    off = [torch.cat((t[:, :3], t), 1)[:, 3:] for t in ops]
+    check(run(*off, "silu"), ref)
+    got = run(ops[0][:1].expand(72, 136), *ops[1:], "silu")
+    check(got, O.reference(ops[0][:1].expand(72, 136), *ops[1:], "silu", torch.bfloat16))
+    for few in (1, 7):  # the few rows of serving, strided
+        part = [ops[0][:few], *ops[1:3], ops[3][:few]]
+        with torch.no_grad():
+            for xs in (part[0], wide[0][:few], off[0][:few], turned[0][:few]):
+                for ws in (ops, wide, off, turned):
+                    check({"y": F.gated_mlp(xs, ws[1], ws[2])}, O.reference(*part, "silu", torch.bfloat16))
+
+
+def test_only_the_wanted_gradients():
+    ops = operands(96, 128, 192, 64, "fp16", seed=7)
+    full = run(*ops, "silu")
+    for wanted in range(1, 8):
+        leaves = [t.detach().requires_grad_(bool(wanted >> i & 1)) for i, t in enumerate(ops[:3])]
+        y = F.gated_mlp(*leaves)
+        y.backward(ops[3])
+        for t, name in zip(leaves, NAMES[1:]):
+            assert (t.grad is None) if not t.requires_grad else torch.equal(t.grad, full[name]), name
+
+
+def test_no_rows():
+    _, w_in, w_out, _ = operands(1, 64, 96, 32, "bf16")
+    leaves = [torch.empty(0, 64, dtype=torch.bfloat16, device="cuda").requires_grad_(), w_in.requires_grad_(), w_out.requires_grad_()]
+    y = F.gated_mlp(*leaves)
+    assert y.shape == (0, 32)
+    y.sum().backward()
+    assert leaves[0].grad.shape == (0, 64) and not leaves[1].grad.any() and not leaves[2].grad.any()
+
+
+def test_draws():
+    ops = operands(256, 256, 512, 128, "bf16", seed=8)
+    draw = lambda **kw: F.hip_blockwise_dropout_gated_mlp(*ops[:3], 64, 0.5, "silu", **kw)
+    assert torch.equal(draw(seed=3), draw(seed=3)) and not torch.equal(draw(seed=3), draw(seed=4))
+    assert not torch.equal(draw(), draw())
+    # the input's mask is drawn from the seed, the hidden activations' from the next: blocks of either with one row of inputs tell which they are
+    both = masks_of(256, 256, 512, 64, 0.5)
+    a, b = (draw(masks=[both[0], None], seed=s) for s in (11, 11))
+    assert torch.equal(a, b) and not torch.equal(a, draw(masks=[both[0], None], seed=12))
+    # nothing dropped where p is 0
+    y = F.hip_blockwise_dropout_gated_mlp(*ops[:3], 64, 0.0)
+    assert torch.equal(y, F.gated_mlp(*ops[:3]))
+    half = F.hip_blockwise_dropout_gated_mlp(*ops[:3], 64, (0.0, 0.5), masks=[None, both[1]])
+    check({"y": half}, O.reference(*ops, "silu", torch.bfloat16, (None, both[1]), 64, (0.0, 0.5)))
+
+
+@pytest.mark.parametrize("p", [0.0, 0.4])
+@pytest.mark.parametrize("size", [(1, 256, 512, 256), (24, 200, 333, 120), (512, 256, 768, 256)], ids=lambda s: "x".join(map(str, s)))
+def test_captured_and_replayed(size, p):
+    ops = operands(*size, "bf16", seed=9)
+    masks = masks_of(*size[:3], 64, p) if p else None
+    static = [t.clone() for t in ops]
+    leaves = [t.requires_grad_() for t in static[:3]]
+
+    def step():
+        y = F.hip_blockwise_dropout_gated_mlp(*leaves, 64, p, "silu", masks=masks)
+        return (y, *torch.autograd.grad(y, leaves, static[3]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (20, 21, 22):
+        fresh = operands(*size, "bf16", seed=seed)
+        with torch.no_grad():
+            for t, v in zip(static, fresh):
+                t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = run(*fresh, "silu", 64, p, masks)
+        for name, t in zip(NAMES, out):
+            assert torch.equal(t, eager[name]), name
+
+
+def test_other_streams_and_calls_beside_each_other():
+    cases = [operands(16, 512, 1024, 512, "bf16", seed=30), operands(300, 256, 512, 128, "bf16", seed=31)]
+    refs = [run(*c, "silu") for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(4):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(run(*c, "silu"))
+    torch.cuda.synchronize()
+    for i, ref in enumerate(refs):
+        for g in got[i]:
+            assert all(torch.equal(g[name], ref[name]) for name in NAMES)
+
+
+def test_autocast_and_leading_dimensions():
+    layer = GatedMLP(128, 320, p=0.0, variant="blockwise[hip]", block_size=64).cuda()
+    x = torch.randn(4, 33, 128, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = layer(x)
+    assert y.shape == (4, 33, 128) and y.dtype == torch.bfloat16
+    y.float().square().mean().backward()
+    assert layer.weight_in.grad.shape == (640, 128) and layer.weight_out.grad.dtype == torch.float32
+
+
+@pytest.mark.parametrize("variant", ["none", "vanilla", "blockwise[naive]", "blockwise[hip]"])
+def test_layer_variants_agree_without_dropout(variant):
+    torch.manual_seed(0)
+    layer = GatedMLP(192, 256, 64, p=0.3, variant=variant, activation="gelu", block_size=64).cuda().bfloat16()
+    x = torch.randn(100, 192, device="cuda").bfloat16()
+    ref, bound = O.reference(x, layer.weight_in, layer.weight_out, torch.zeros(100, 64, device="cuda"), "gelu", torch.bfloat16)["y"]
+    y = layer.eval()(x)
+    # (torch's products, activation and multiplication round once more each)
+    assert ((y.double() - ref).abs() <= (bound if variant == "blockwise[hip]" else 3 * bound)).all()
+    layer.train()(x.requires_grad_()).float().square().sum().backward()
+    assert x.grad.isfinite().all() and layer.weight_in.grad.any() and layer.weight_out.grad.any()
+
+
+def test_backward_twice_and_changed_tensors():
+    ops = operands(64, 64, 64, 64, "bf16", seed=12)
+    leaves = [t.requires_grad_() for t in ops[:3]]
+    y = F.gated_mlp(*leaves)
+    y.backward(ops[3], retain_graph=True)
+    first = [t.grad.clone() for t in leaves]
+    for t in leaves:
+        t.grad = None
+    y.backward(ops[3])
+    assert all(torch.equal(t.grad, g) for t, g in zip(leaves, first))
+    with pytest.raises(RuntimeError):
+        y.backward(ops[3])
+    y = F.gated_mlp(*leaves)
+    with torch.no_grad():
+        leaves[1].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(ops[3])
+
+
+def test_traced():
+    x, w_in, w_out, _ = operands(64, 64, 96, 64, "bf16", seed=13)
+    traced = torch.jit.trace(lambda a, b, c: F.gated_mlp(a, b, c, "gelu"), (x, w_in, w_out), check_trace=False)
+    other = operands(64, 64, 96, 64, "bf16", seed=14)[:3]
+    assert torch.equal(traced(*other), F.gated_mlp(*other, "gelu"))
+
+
+def test_refusals():
+    x, w_in, w_out, _ = operands(8, 64, 96, 32, "bf16")
+    with pytest.raises(ValueError, match="both projections"):
+        F.gated_mlp(x, w_in[:-1], w_out)
+    with pytest.raises(ValueError, match="reduction dims"):
+        F.gated_mlp(x[:, :-1], w_in, w_out)
+    with pytest.raises(TypeError, match="same dtype"):
+        F.gated_mlp(x, w_in, w_out.half())
+    with pytest.raises(TypeError, match="float16 or bfloat16"):
+        F.gated_mlp(x.float(), w_in.float(), w_out.float())
+    with pytest.raises(ValueError, match="must not be empty"):
+        F.gated_mlp(x, w_in[:0], w_out[:, :0])
+    with pytest.raises(ValueError, match="on the GPU|same device"):
+        F.gated_mlp(x, w_in, w_out.cpu())
+    with pytest.raises(ValueError, match="mask shape"):
+        F.hip_blockwise_dropout_gated_mlp(x, w_in, w_out, 64, 0.5, masks=[torch.zeros(2, 1, dtype=torch.bool, device="cuda"), None], seed=1)
+    with pytest.raises(NotImplementedError, match="forward mode"):
+        with torch.autograd.forward_ad.dual_level():
+            F.gated_mlp(torch.autograd.forward_ad.make_dual(x, x), w_in, w_out)
