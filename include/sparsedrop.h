@@ -710,11 +710,26 @@ int sd_clip_grads(int count, void* const* grads, const int64_t* numels, const in
 /* ---------------------------------------------------------------------------------------------
  * (i) a gated feed-forward block's hidden activations
  *
- * A[M, 2F] = [G | U] (pitch lda), both products' results beside one another; act: relu, gelu or silu.
+ * A[M, 2F] = [G | U] (pitch lda), both projections' results beside one another; act: relu, gelu or silu.
  * sd_gated_forward:  H = act(G) U                        (H [M, F], pitch ldh)
  * sd_gated_backward: dA = [dH U act'(G) | dH act(G)]     (dH [M, F], pitch ldd; dA [M, 2F], pitch ldda; dA may be A)
+ *   where dH is 0 both gradients are 0, whatever stands in A: what was dropped has none.
  * Computed in fp32, rounded once.
+ *
+ * The products with the gate in their store; SD_ERR_UNSUPPORTED with nothing launched where none of the specialised kernels takes the
+ * operands (the caller then takes the product and the gate apart):
+ * sd_gated_matmul: [G | U] = scale * sum over kept blocks of X (W_in)^T, H = act(G) U; W_in [2F, K], the gate's rows first.  A (NULL:
+ *   not wanted) receives [G | U] rounded, H is computed from the fp32 sums.  row_ptr / col_idx: kept blocks of X, NULL for all.
+ * sd_gated_matmul_gradient: dH = scale * (dY W_out) where kept, which is rounded nowhere, and dA as above; dropped blocks of both halves are
+ *   zeros.  dY [M, N], W_out [N, F]; lists over dH's blocks, NULL for all; keep_hint as in sd_gemm_sdd_lists_ex.
  * ------------------------------------------------------------------------------------------- */
+int sd_gated_matmul(const void* X, int64_t x_stride_r, int64_t x_stride_c, const void* W_in, int64_t w_stride_r, int64_t w_stride_c,
+                    void* H, int64_t ldh, void* A, int64_t lda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F,
+                    int64_t K, int64_t block_size, float scale, int act, int dtype, void* stream);
+int sd_gated_matmul_gradient(const void* dY, int64_t dy_stride_r, int64_t dy_stride_c, const void* W_out, int64_t w_stride_r,
+                             int64_t w_stride_c, const void* A, int64_t lda, void* dA, int64_t ldda, const int32_t* row_ptr,
+                             const int32_t* col_idx, int64_t M, int64_t F, int64_t N, int64_t block_size, float scale, float keep_hint,
+                             int act, int dtype, void* stream);
 int sd_gated_forward(const void* A, int64_t lda, void* H, int64_t ldh, int64_t M, int64_t F, int act, int dtype, void* stream);
 int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, void* dA, int64_t ldda, int64_t M, int64_t F, int act,
                       int dtype, void* stream);

@@ -136,6 +136,7 @@ GemmArgs make_args(const void* A, int64_t asr, int64_t asc, const void* B, int64
   g.act = SD_ACT_NONE;
   g.aux = nullptr;
   g.aux_sr = g.aux_sc = 0;
+  g.gate = 0;
   return g;
 }
 
@@ -864,6 +865,57 @@ int sd_conv2d_dw_lists(const void* x, int64_t sn, int64_t sc, int64_t sh, int64_
   GemmArgs g = make_args(nullptr, 1, c * r * s, dy, 1, dyld, dw, 1, dwld, c * r * s, k_out, n * P * Q, bs, scale,
                          col_ptr, row_idx, workspace, workspace_bytes);
   const int rc = launch_conv_implicit_dw(g, cg, P, stride_h, stride_w, dil_h, dil_w, r, sw, dtype, (hipStream_t)stream);
+  if (rc == SD_OK) last_kernel = "specialised";
+  return rc;
+}
+
+static int check_gated(const char* name, int64_t F, int act, const void* A, int64_t lda, int64_t M, const int32_t* row_ptr, const int32_t* col_idx,
+                       int64_t bs, float scale) {
+  SD_REQUIRE(F >= 0 && F < kMaxDim / 2, "%s: hidden width out of range", name);
+  SD_REQUIRE(act == SD_ACT_RELU || act == SD_ACT_GELU || act == SD_ACT_SILU, "%s: act must be SD_ACT_RELU, SD_ACT_GELU or SD_ACT_SILU (got %d)", name, act);
+  SD_REQUIRE(!A || M <= 1 || lda >= 2 * F, "%s: pitch %lld of 2 x %lld columns", name, (long long)lda, (long long)F);
+  SD_REQUIRE((row_ptr == nullptr) == (col_idx == nullptr), "%s: row_ptr and col_idx must both be given or both be null", name);
+  SD_REQUIRE(scale == scale, "%s: scale is NaN", name);
+  return row_ptr ? check_sparse(bs, scale) : SD_OK;
+}
+
+int sd_gated_matmul(const void* X, int64_t xsr, int64_t xsc, const void* W_in, int64_t wsr, int64_t wsc, void* H, int64_t ldh, void* A,
+                    int64_t lda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t K, int64_t bs, float scale,
+                    int act, int dtype, void* stream) {
+  if (int rc = check_gated("gated_matmul", F, act, A, lda, M, row_ptr, col_idx, bs, scale)) return rc;
+  if (int rc = check_common(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, dtype)) return rc;
+  if (int rc = check_mat("W_in", W_in, wsr, wsc, 2 * F, K)) return rc;
+  if (M == 0 || F == 0) return SD_OK;
+  if (generic_forced() || K == 0) return SD_ERR_UNSUPPORTED;
+  GemmArgs g = make_args(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, row_ptr ? bs : 0, scale, row_ptr, col_idx);
+  g.act = act;
+  g.aux = static_cast<uint16_t*>(A);
+  g.aux_sr = lda;
+  g.aux_sc = 1;
+  g.gate = F;
+  const int rc = launch_gated(g, dtype, (hipStream_t)stream);
+  if (rc == SD_OK) last_kernel = "specialised";
+  return rc;
+}
+
+int sd_gated_matmul_gradient(const void* dY, int64_t gsr, int64_t gsc, const void* W_out, int64_t wsr, int64_t wsc, const void* A, int64_t lda,
+                             void* dA, int64_t ldda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t N,
+                             int64_t bs, float scale, float keep_hint, int act, int dtype, void* stream) {
+  if (int rc = check_gated("gated_matmul_gradient", F, act, A, lda, M, row_ptr, col_idx, bs, scale)) return rc;
+  if (int rc = check_common(dY, gsr, gsc, W_out, wsc, wsr, dA, ldda, 1, M, F, N, dtype)) return rc;
+  SD_REQUIRE(M <= 1 || ldda >= 2 * F, "gated_matmul_gradient: pitch %lld of 2 x %lld columns", (long long)ldda, (long long)F);
+  SD_REQUIRE(!(keep_hint > 1.f), "gated_matmul_gradient: keep_hint must be a fraction in [0, 1], or negative for unknown");
+  if (M == 0 || F == 0) return SD_OK;
+  SD_REQUIRE(A != nullptr, "gated_matmul_gradient: null [G | U]");
+  if (generic_forced() || N == 0) return SD_ERR_UNSUPPORTED;
+  GemmArgs g = make_args(dY, gsr, gsc, W_out, wsc, wsr, dA, ldda, 1, M, F, N, row_ptr ? bs : 0, scale, row_ptr, col_idx);
+  g.keep_hint = keep_hint == keep_hint ? keep_hint : -1.f;
+  g.act = act;
+  g.aux = const_cast<uint16_t*>(static_cast<const uint16_t*>(A));
+  g.aux_sr = lda;
+  g.aux_sc = 1;
+  g.gate = F;
+  const int rc = launch_gated_gradient(g, dtype, (hipStream_t)stream);
   if (rc == SD_OK) last_kernel = "specialised";
   return rc;
 }

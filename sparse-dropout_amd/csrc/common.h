@@ -131,6 +131,8 @@ struct GemmArgs {
   int act;
   uint16_t* aux;
   int64_t aux_sr, aux_sc;
+  // F, a gated block's hidden width (gated.h), in the instances that are built for it; nobody else looks at it
+  int64_t gate;
 };
 
 // SDD: the fraction of blocks expected to be kept (unknown counts as everything), and of the 64-blocks: one of a mask of
@@ -420,6 +422,11 @@ int launch_conv_dx(const void* dy, int64_t dy_ld, const void* w, int64_t w_ld, v
 // whether it does: a question to the host alone
 bool conv_dx_taken(const void* dy, int64_t dy_ld, const void* w, int64_t w_ld, int64_t n, int64_t c, int64_t h, int64_t wd, int64_t k_out,
                    int64_t r, int64_t s, int64_t pad_h, int64_t pad_w, int64_t stride_h, int64_t stride_w, int64_t dil_h, int64_t dil_w);
+// Products with a gate in their store (gated.h); SD_ERR_UNSUPPORTED (without a message) where no specialised kernel takes them.
+// g.b: [2 F, K], g.c: H, g.aux: [G | U] or null, g.gate: F; g.N is not looked at
+int launch_gated(const GemmArgs& g, int dtype, hipStream_t stream);
+// an SDD (or dense) product dH that leaves [dG | dU] in g.c, g.aux: [G | U], g.N == g.gate
+int launch_gated_gradient(const GemmArgs& g, int dtype, hipStream_t stream);
 // which workgroup shape the DSD kernel runs in: chosen from the shape, or forced (tuning and tests);
 // returns the previous policy, -1 for an unknown one
 enum { kTileAuto = 0, kTileBig = 1, kTileMid = 2 };

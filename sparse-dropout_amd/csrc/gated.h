@@ -1,4 +1,11 @@
-// A gate's arithmetic: h = act(g) u and its gradients.
+// A gate's arithmetic, h = act(g) u and its gradients, and the stores of the products that carry it.
+//
+// Forward.  Both projections are one product with W_in [2 F, K], whose columns a workgroup takes 16 of the gate and the same 16 of the other
+// projection at a time: 16-column tile 2 q of its output is g, tile 2 q + 1 is u of the hidden columns 16 q .. + 15.  Either tile of a pair is
+// in the same registers of the same lanes, so H needs nothing from another wave, and where nothing will be differentiated G and U never leave the
+// registers: 3 of the 4 bytes a passing gate would move.  gated_row: the row of W_in, from the first of a workgroup's, that column n of its tile is.
+//
+// Backward.  dH = (dY W_out) . keep is a product whose store reads g and u of its place and writes dg and du instead of dh.
 #pragma once
 #include "common.h"
 
@@ -23,6 +30,157 @@ __device__ inline void gate_slope(int act, float g, float& value, float& slope) 
   } else {
     value = act_apply(act, g);
     slope = act_derivative(act, g);
+  }
+}
+
+// columns of the product's output as its tiles see them
+__host__ __device__ inline int64_t gated_columns(int64_t F) { return (F + 15) / 16 * 32; }
+// hidden column of column n, from the first of a tile, and whether it is the other projection's
+__device__ inline int gated_hidden(int n) { return n / 32 * 16 + n % 16; }
+__device__ inline bool gated_up(int n) { return (n & 16) != 0; }
+
+template <typename T>
+__device__ inline u32x4 pack_eight(const float (&v)[8]) {
+  return u32x4{T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7])};
+}
+template <typename T>
+__device__ inline void unpack_eight(u32x4 w, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = T::to_float((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+}
+
+// N hidden columns from column c of row m on, unscaled fp32 accumulators of both projections
+template <typename T, int N>
+__device__ inline void store_gate(const GemmArgs& g, int64_t m, int64_t c, float (&gate)[N], float (&up)[N]) {
+  if (m >= g.M || c >= g.gate) return;
+  const int valid = g.gate - c < N ? (int)(g.gate - c) : N;
+  uint16_t* h = g.c + m * g.c_sr + c;
+  float out[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    gate[i] *= g.scale;
+    up[i] *= g.scale;
+  }
+  auto apply = [&](int act) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = gate_value(act, gate[i]) * up[i];
+  };
+  if (g.act == SD_ACT_SILU) apply(SD_ACT_SILU);
+  else if (g.act == SD_ACT_GELU) apply(SD_ACT_GELU);
+  else apply(SD_ACT_RELU);
+  auto put = [&](uint16_t* at, const float (&v)[N]) {
+    if (valid < N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < valid) at[i] = T::from_float(v[i]);
+    } else if constexpr (N == 8) {
+      *reinterpret_cast<u32x4_any*>(at) = pack_eight<T>(v);
+    } else {
+      static_assert(N == 4, "8 or 16 bytes");
+      typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+      *reinterpret_cast<u32x2_any*>(at) = u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+    }
+  };
+  if (g.aux) {
+    uint16_t* a = g.aux + m * g.aux_sr + c;
+    put(a, gate);
+    put(a + g.gate, up);
+  }
+  put(h, out);
+}
+
+// A wave's tile [64 rows][32 gate and 32 other columns, 16 by 16] of accumulators staged in LDS with a pitch of 68 floats; c0: its first
+// hidden column.
+template <typename T>
+__device__ inline void store_staged_gate(const GemmArgs& g, const float* stg, int lane, int64_t m0, int64_t c0) {
+  constexpr int PITCH = 68;
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int row = pass * 16 + lane / 4, ch = lane % 4;
+    const float* at = stg + row * PITCH + ch / 2 * 32 + ch % 2 * 8;
+    float gate[8], up[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(at + 4 * i), b = *reinterpret_cast<const f32x4*>(at + 16 + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        gate[4 * i + e] = a[e];
+        up[4 * i + e] = b[e];
+      }
+    }
+    store_gate<T, 8>(g, m0 + row, c0 + ch * 8, gate, up);
+  }
+}
+
+// What the gradient's store reads of a position, on its way ahead of the stores in front (see aux_eight); nothing where it does not take eight.
+struct GateAt {
+  u32x4 gate, up;
+  __device__ inline void load(const GemmArgs& g, int64_t m, int64_t c) {
+    gate = up = u32x4{0u, 0u, 0u, 0u};
+    if (m >= g.M || c + 8 > g.gate) return;
+    const uint16_t* at = g.aux + m * g.aux_sr + c;
+    gate = *reinterpret_cast<const u32x4_any*>(at);
+    up = *reinterpret_cast<const u32x4_any*>(at + g.gate);
+  }
+};
+// eight of dh, unscaled fp32 accumulators.  What was dropped has no gradient, whatever stands in g and u.
+template <typename T>
+__device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t c, float (&dh)[8], const GateAt& pre) {
+  if (m >= g.M || c >= g.gate) return;
+  const int valid = g.gate - c < 8 ? (int)(g.gate - c) : 8;
+  uint16_t* out = g.c + m * g.c_sr + c;
+  float gate[8], up[8];
+  if (valid == 8) {
+    unpack_eight<T>(pre.gate, gate);
+    unpack_eight<T>(pre.up, up);
+  } else {
+    const uint16_t* at = g.aux + m * g.aux_sr + c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      gate[i] = i < valid ? T::to_float(at[i]) : 0.f;
+      up[i] = i < valid ? T::to_float(at[g.gate + i]) : 0.f;
+    }
+  }
+  auto apply = [&](int act) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float value, slope;
+      gate_slope(act, gate[i], value, slope);
+      const float d = dh[i] * g.scale;
+      gate[i] = dh[i] != 0.f ? d * up[i] * slope : 0.f;
+      up[i] = dh[i] != 0.f ? d * value : 0.f;
+    }
+  };
+  if (g.act == SD_ACT_SILU) apply(SD_ACT_SILU);
+  else if (g.act == SD_ACT_GELU) apply(SD_ACT_GELU);
+  else apply(SD_ACT_RELU);
+  if (valid == 8) {
+    *reinterpret_cast<u32x4_any*>(out) = pack_eight<T>(gate);
+    *reinterpret_cast<u32x4_any*>(out + g.gate) = pack_eight<T>(up);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) {
+        out[i] = T::from_float(gate[i]);
+        out[g.gate + i] = T::from_float(up[i]);
+      }
+  }
+}
+// a wave's 64 x 64 tile of dh staged in LDS with a pitch of 68 floats
+template <typename T>
+__device__ inline void store_staged_gate_gradient(const GemmArgs& g, const float* stg, int lane, int64_t m0, int64_t c0) {
+  constexpr int PITCH = 68, AHEAD = 4;
+  GateAt pre[AHEAD];
+#pragma unroll
+  for (int pass = 0; pass < 8; ++pass) {
+    const int row = pass * 8 + lane / 8, ch = lane % 8;
+    if (pass % AHEAD == 0) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) pre[i].load(g, m0 + row + 8 * i, c0 + ch * 8);
+    }
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(stg + row * PITCH + ch * 8), hi = *reinterpret_cast<const f32x4*>(stg + row * PITCH + ch * 8 + 4);
+    float dh[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    store_gate_gradient<T>(g, m0 + row, c0 + ch * 8, dh, pre[pass % AHEAD]);
   }
 }
 

@@ -50,6 +50,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gated.h"
 #include "gemm_device.h"
 #include "gemm_tile_api.h"
 #include "mask_source.h"
@@ -109,11 +110,13 @@ constexpr int CONV_T_PATCH_MAX = 24 * 1024;  // weight gradient: bytes of one st
 // workgroup takes part `split` (the kernels below pass their block indices; the fused backward launch its own)
 // ms: where the mask comes from when the kept lists do not exist yet (the forward launch that also builds them);
 // the keep bits of the workgroup's row blocks are then evaluated from it directly, g.row_ptr is not read
-template <typename T, bool TRANS, bool CM, bool RAGGED, typename S, int IMPLICIT = 0>
+// GATED: B is W_in, its columns taken 16 by 16 of either projection, and the store gates (gated.h)
+template <typename T, bool TRANS, bool CM, bool RAGGED, typename S, int IMPLICIT = 0, bool GATED = false>
 __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int tiles_n, int Mb, int Kb_all,
                                          const ImplicitConv& cg, const int bid, const int nsplit, const int split,
                                          const MaskSrc* ms = nullptr) {
   static_assert(!IMPLICIT || (S::R == 4 && S::THREADS == 512), "the gather assumes 512 threads x 4 row blocks");
+  static_assert(!GATED || (!TRANS && !CM && !IMPLICIT && S::NT == 2), "the gate's store");
   static_assert(S::R <= 4, "a step's keep bits are four per row block in 16 bits");
   constexpr int R = S::R, BN = S::BN, THREADS = S::THREADS, NT = S::NT, STAGE = S::STAGE, A_OFF = S::A_OFF;
   constexpr int BL = S::BL, AL = S::AL, RW = S::RW;
@@ -134,7 +137,8 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
   const int rh = wave / S::NS;  // row-block pair
   const int rb0 = tm * R;   // first row block
   const int64_t n0 = (int64_t)tn * BN;
-  const int nvalid = (int)((g.N - n0) < BN ? (g.N - n0) : BN);  // columns of this tile inside C
+  const int64_t n_all = GATED ? gated_columns(g.gate) : g.N;
+  const int nvalid = (int)((n_all - n0) < BN ? (n_all - n0) : BN);  // columns of this tile inside C
   // split reduction: part `split` takes the reduction blocks [kb_lo, kb_lo + Kb) and leaves an fp32 partial
   const int kb_lo = (int)((int64_t)Kb_all * split / nsplit);
   const int Kb = (int)((int64_t)Kb_all * (split + 1) / nsplit) - kb_lo;
@@ -445,6 +449,10 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
       b_lane[jj] = chunk_at(row, g.b.sr, 0, false, false);
       b_delta_k[jj] = chunk_at(row, g.b.sr, 0, false, kb_tail >= 0) - b_lane[jj];
       b_valid[jj] = row < nvalid;
+      if constexpr (GATED) {
+        b_lane[jj] += (uint32_t)((gated_hidden(row) - row + (gated_up(row) ? g.gate : 0)) * g.b.sr) * 2u;
+        b_valid[jj] = n0 / 2 + gated_hidden(row) < g.gate;
+      }
     }
 #pragma unroll
     for (int i = 0; i < AL; ++i) {
@@ -454,7 +462,7 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
       a_delta_k[i] = chunk_at(row, g.a.sr, 0, false, kb_tail >= 0) - a_lane[i];
     }
     a_tile0 = reinterpret_cast<const char*>(g.a.ptr + (int64_t)rb0 * BS * g.a.sr);
-    b_tile0 = reinterpret_cast<const char*>(g.b.ptr + n0 * g.b.sr);
+    b_tile0 = reinterpret_cast<const char*>(g.b.ptr + (GATED ? n0 / 2 : n0) * g.b.sr);
     red_stride = BS * 2;
     a_rstride = (uint32_t)(BS * g.a.sr) * 2u;
   } else {
@@ -680,7 +688,8 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
     }
     const int64_t w_step = (TRANS ? 2 * g.b.sc : 8 * g.b.sr) * 2;  // bytes between the rows of consecutive W loads
     const int64_t x_step = (TRANS ? 8 * g.a.sc : 8 * g.a.sr) * 2;  // ... X loads
-    const char* b_wave0 = b_tile0 + wg * 8 * w_step;
+    const char* b_wave0 = b_tile0 + wg * (GATED ? 4 : 8) * w_step;
+    [[maybe_unused]] const int64_t up_step = GATED ? g.gate * g.b.sr * 2 : 0;  // from the gate's rows to the other projection's
     const char* a_wave0 = a_tile0 + wg * 2 * x_step;
     auto load_w = [&](uint32_t entry, int stage) {  // the W tile of a step: 32 loads, 8 per wave of group 0
       const char* bp = b_wave0 + step_block(entry) * b_red_stride;
@@ -688,6 +697,13 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
       // tile rows are columns of C: a wave's 64 are all inside the matrix or all past N (N is a multiple of 64).  One test
       // for all eight loads: a test per load puts every load behind two taken branches (3 % of the kernel).
       if (!TRANS && wg * 64 >= nvalid) return;
+      if constexpr (GATED) {  // (two loads to 16 columns)
+        const char* up = bp + up_step;
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj)
+          load16_to_lds((jj & 2 ? up : bp) + (jj / 4 * 2 + (jj & 1)) * w_step, ld_off[jj & 1], dst + (uint32_t)(jj * 1024));
+        return;
+      }
 #pragma unroll
       for (int jj = 0; jj < 8; ++jj)
         load16_to_lds(bp + jj * w_step, ld_off[TRANS ? ((jj & 1) | (((jj >> 2) & 1) << 1)) : (jj & 1)], dst + (uint32_t)(jj * 1024));
@@ -939,16 +955,20 @@ __device__ __forceinline__ void dsd_body(const GemmArgs& g, int tiles_m, int til
           }
         }
       const int64_t m_first = (int64_t)rb * BS, n_first = n0 + ns * WN + h * WC;
+      if constexpr (GATED) {
+        store_staged_gate<T>(g, stg, lane, m_first, n_first / 2);
+        continue;
+      }
       store_staged_tile<T, false, S_ROWS, S_COLS>(g, stg, lane, !CM, CM ? n_first : m_first, CM ? m_first : n_first,
                                                   part);
     }
   }
 }
 
-template <typename T, bool TRANS, bool CM, bool RAGGED, typename S, int IMPLICIT = 0>
+template <typename T, bool TRANS, bool CM, bool RAGGED, typename S, int IMPLICIT = 0, bool GATED = false>
 __global__ __launch_bounds__(S::THREADS) void dsd_kernel(GemmArgs g, int tiles_m, int tiles_n,
                                                          int Mb, int Kb_all, ImplicitConv cg) {
-  dsd_body<T, TRANS, CM, RAGGED, S, IMPLICIT>(g, tiles_m, tiles_n, Mb, Kb_all, cg, (int)blockIdx.x, (int)gridDim.y,
+  dsd_body<T, TRANS, CM, RAGGED, S, IMPLICIT, GATED>(g, tiles_m, tiles_n, Mb, Kb_all, cg, (int)blockIdx.x, (int)gridDim.y,
                                               (int)blockIdx.y);
 }
 
@@ -1173,7 +1193,7 @@ __device__ inline GroupAt find_group(const GemmArgs& g, char* smem, int tiles_m,
 }
 
 // Zeros for the tiles of a group that are not kept: those of its column blocks that the flags leave out and all of the empty ones.
-template <int R, bool EDGE>
+template <int R, bool EDGE, bool GATED>
 __device__ inline void zero_dropped(const GemmArgs& g, const uint32_t* flags, const int* cols, int ncols, const int* empty, int nempty,
                                     int rb0, int Mb, int tid) {
   const int row = tid / 8, ch = tid % 8;
@@ -1183,8 +1203,11 @@ __device__ inline void zero_dropped(const GemmArgs& g, const uint32_t* flags, co
     const uint32_t f = (uint32_t)__builtin_amdgcn_readfirstlane((int)flags[c]);
     for (int r = 0; r < R; ++r) {
       if (rb0 + r >= Mb) break;
-      if (!((f >> r) & 1u) && (int64_t)(rb0 + r) * BS + row < g.M && (!EDGE || (int64_t)c * BS + ch * 8 < g.N))
-        *reinterpret_cast<u32x4*>(g.c + ((int64_t)(rb0 + r) * BS + row) * g.c_sr + (int64_t)c * BS + ch * 8) = z;
+      if (!((f >> r) & 1u) && (int64_t)(rb0 + r) * BS + row < g.M && (!EDGE || (int64_t)c * BS + ch * 8 < g.N)) {
+        u32x4* at = reinterpret_cast<u32x4*>(g.c + ((int64_t)(rb0 + r) * BS + row) * g.c_sr + (int64_t)c * BS + ch * 8);
+        *at = z;
+        if (GATED) at[g.gate / 8] = z;
+      }
     }
   }
 }
@@ -1193,7 +1216,8 @@ __device__ inline void zero_dropped(const GemmArgs& g, const uint32_t* flags, co
 // overhanging 16-byte chunks / rows of the last column block / reduction block are fetched from inside the
 // matrix instead, as in the DSD kernel, the fragments of the last reduction block are zeroed past the end,
 // and nothing is stored past the last column.  (A ragged M costs nothing worth a separate instance.)
-template <typename T, bool EDGE, typename G>
+// GATED: the store leaves both gradients of a gate (gated.h)
+template <typename T, bool EDGE, typename G, bool GATED = false>
 __device__ __forceinline__ void sdd_body(const GemmArgs& g, int tiles_m, int gsure, int Mb, int Cb, const int bid) {
   constexpr int R = G::R, GW = G::GW, SLOTS = G::SLOTS, G_BOFF = G::BOFF, G_STAGE = G::STAGE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1243,7 +1267,7 @@ __device__ __forceinline__ void sdd_body(const GemmArgs& g, int tiles_m, int gsu
 #pragma unroll
   for (int j = 0; j < GW; ++j) rowmask |= (kept >> (4 * j)) & 0xfu;
 
-  if (!g.kept_only) zero_dropped<R, EDGE>(g, flags, at.cols, ncols, at.empty, at.nempty, rb0, Mb, tid);
+  if (!g.kept_only) zero_dropped<R, EDGE, GATED>(g, flags, at.cols, ncols, at.empty, at.nempty, rb0, Mb, tid);
   if (kept == 0) return;
   __syncthreads();  // flags and rec are dead: the stages may be written
 
@@ -1440,8 +1464,8 @@ __device__ __forceinline__ void sdd_body(const GemmArgs& g, int tiles_m, int gsu
           const bool keep = !EDGE || ((my_q[k] >> (2 * (mt / 2) + nt / 2)) & 1u);
           stg[(mt * 16 + 4 * (lane / 16) + v) * S_PITCH + nt * 16 + lane % 16] = keep ? acc[k][mt][nt][v] : 0.f;
         }
-    store_staged_tile<T, true, BS, BS>(g, stg, lane, true, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c[k] * BS,
-                                       nullptr);
+    if constexpr (GATED) store_staged_gate_gradient<T>(g, stg, lane, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c[k] * BS);
+    else store_staged_tile<T, true, BS, BS>(g, stg, lane, true, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c[k] * BS, nullptr);
   }
 }
 
@@ -1460,7 +1484,7 @@ __device__ __forceinline__ void sdd_body(const GemmArgs& g, int tiles_m, int gsu
 // 1 %): letting a column block's two waves sit in different groups (13 instead of 10.5 tiles per group at p = 0.5)
 // with the W loads shared out evenly between the groups - what a step costs is the instructions of its memory
 // phase, and the fuller groups need more of them per wave.
-template <typename T>
+template <typename T, bool GATED = false>
 __device__ __forceinline__ void sdd_pp_body(const GemmArgs& g, int tiles_m, int gsure, int Mb, int Cb, const int bid) {
   using G = SddBig;
   constexpr int R = G::R, GW = G::GW, G_BOFF = G::BOFF, G_STAGE = G::STAGE;
@@ -1511,7 +1535,7 @@ __device__ __forceinline__ void sdd_pp_body(const GemmArgs& g, int tiles_m, int 
     }
   }
 
-  if (!g.kept_only) zero_dropped<R, false>(g, flags, at.cols, ncols, at.empty, at.nempty, rb0, Mb, tid);
+  if (!g.kept_only) zero_dropped<R, false, GATED>(g, flags, at.cols, ncols, at.empty, at.nempty, rb0, Mb, tid);
   if (ncols == 0) return;
   __syncthreads();  // flags and rec are dead: the stages may be written
 
@@ -1681,20 +1705,21 @@ __device__ __forceinline__ void sdd_pp_body(const GemmArgs& g, int tiles_m, int 
 #pragma unroll
         for (int v = 0; v < 4; ++v)  // register v of lane l is element (4*(l/16) + v, l%16) of the 16 x 16 tile
           stg[(mt * 16 + 4 * (lane / 16) + v) * S_PITCH + nt * 16 + lane % 16] = acc[k][mt][nt][v];
-    store_staged_tile<T, true, BS, BS>(g, stg, lane, true, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c * BS, nullptr);
+    if constexpr (GATED) store_staged_gate_gradient<T>(g, stg, lane, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c * BS);
+    else store_staged_tile<T, true, BS, BS>(g, stg, lane, true, (int64_t)(rb0 + my_r[k]) * BS, (int64_t)my_c * BS, nullptr);
   }
 }
 
-template <typename T, bool EDGE, typename G>
+template <typename T, bool EDGE, typename G, bool GATED = false>
 __device__ __forceinline__ void sdd_any_body(const GemmArgs& g, int tiles_m, int gsure, int Mb, int Cb, const int bid) {
   // aligned operands on the 4-row-block shape: the kernel whose waves alternate between memory and compute phases
-  if constexpr (!EDGE && G::R == 4) sdd_pp_body<T>(g, tiles_m, gsure, Mb, Cb, bid);
-  else sdd_body<T, EDGE, G>(g, tiles_m, gsure, Mb, Cb, bid);
+  if constexpr (!EDGE && G::R == 4) sdd_pp_body<T, GATED>(g, tiles_m, gsure, Mb, Cb, bid);
+  else sdd_body<T, EDGE, G, GATED>(g, tiles_m, gsure, Mb, Cb, bid);
 }
 
-template <typename T, bool EDGE, typename G>
+template <typename T, bool EDGE, typename G, bool GATED = false>
 __global__ __launch_bounds__(THREADS) void sdd_group_kernel(GemmArgs g, int tiles_m, int gsure, int Mb, int Cb) {
-  sdd_any_body<T, EDGE, G>(g, tiles_m, gsure, Mb, Cb, (int)blockIdx.x);
+  sdd_any_body<T, EDGE, G, GATED>(g, tiles_m, gsure, Mb, Cb, (int)blockIdx.x);
 }
 
 // Both gradients of one layer in one launch: workgroups [0, n_first) are one product's (those past its own grid exit:
@@ -1749,16 +1774,16 @@ std::atomic<int> tile_policy{0};
 
 bool is_bf16(int dtype) { return dtype == SD_BF16; }
 
-template <typename T, bool TRANS, bool CM, bool RAGGED>
+template <typename T, bool TRANS, bool CM, bool RAGGED, bool GATED = false>
 int launch_big_t(const GemmArgs& g, int splits, hipStream_t stream) {
   using S = DsdBig;
   static std::atomic<bool> configured[kMaxDevices] = {};
-  if (int rc = allow_big_lds(reinterpret_cast<const void*>(&dsd_kernel<T, TRANS, CM, RAGGED, S>), S::SMEM_BYTES,
+  if (int rc = allow_big_lds(reinterpret_cast<const void*>(&dsd_kernel<T, TRANS, CM, RAGGED, S, 0, GATED>), S::SMEM_BYTES,
                              configured))
     return rc;
   const int Mb = (int)((g.M + BS - 1) / BS), Kb = (int)((g.K + BS - 1) / BS);
-  const int tiles_m = (Mb + S::R - 1) / S::R, tiles_n = (int)((g.N + S::BN - 1) / S::BN);
-  hipLaunchKernelGGL((dsd_kernel<T, TRANS, CM, RAGGED, S>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)splits),
+  const int tiles_m = (Mb + S::R - 1) / S::R, tiles_n = (int)(((GATED ? gated_columns(g.gate) : g.N) + S::BN - 1) / S::BN);
+  hipLaunchKernelGGL((dsd_kernel<T, TRANS, CM, RAGGED, S, 0, GATED>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)splits),
                      dim3(S::THREADS), S::SMEM_BYTES, stream, g, tiles_m, tiles_n, Mb, Kb, ImplicitConv{});
   return check_launch("dsd_kernel");
 }
@@ -1934,14 +1959,14 @@ bool sdd_counts_all(const GemmArgs& g) {
 }
 // The groups that nearly every row quad has (those above come last in the launch order).
 int sdd_sure_groups(const GemmArgs& g) { return std::min(sdd_most_groups(g), (int)(sdd_row_groups(g) + 1.0)); }
-template <typename T, bool EDGE>
+template <typename T, bool EDGE, bool GATED = false>
 int launch_sdd_big(const GemmArgs& g, hipStream_t stream) {
   using G = SddBig;
   static std::atomic<bool> configured[kMaxDevices] = {};
-  if (int rc = allow_big_lds(reinterpret_cast<const void*>(&sdd_group_kernel<T, EDGE, G>), G::SMEM, configured)) return rc;
+  if (int rc = allow_big_lds(reinterpret_cast<const void*>(&sdd_group_kernel<T, EDGE, G, GATED>), G::SMEM, configured)) return rc;
   const int Mb = (int)((g.M + BS - 1) / BS), Cb = (int)((g.N + BS - 1) / BS);
   const int tiles_m = (Mb + G::R - 1) / G::R;
-  hipLaunchKernelGGL((sdd_group_kernel<T, EDGE, G>), dim3((unsigned)(tiles_m * sdd_most_groups(g))), dim3(THREADS), G::SMEM,
+  hipLaunchKernelGGL((sdd_group_kernel<T, EDGE, G, GATED>), dim3((unsigned)(tiles_m * sdd_most_groups(g))), dim3(THREADS), G::SMEM,
                      stream, g, tiles_m, sdd_counts_all(g) ? 0 : sdd_sure_groups(g), Mb, Cb);
   return check_launch("sdd_group_kernel");
 }
@@ -2223,6 +2248,58 @@ int launch_fast(const GemmArgs& g, int mode, int dtype, hipStream_t stream) {
   note_kernel("dsd:%s%s%s splits=%d", dsd_name(plan.shape), f.kc ? "" : ":strided",
               f.ragged && plan.shape == kShapeBig ? ":ragged" : "", plan.splits);
   return plan.splits > 1 ? launch_splitk_reduce(g, plan.splits, f.cm, dtype, stream) : SD_OK;
+}
+
+// ---- products with a gate in their store ---------------------------------------------------------------------------------------
+// The shape with the smallest expected time of the ungated product, its reduction uncut: a gate needs whole sums.
+int launch_gated(const GemmArgs& g_, int dtype, hipStream_t stream) {
+  GemmArgs g = g_;
+  g.N = gated_columns(g.gate);
+  if (g.row_ptr && g.bs != BS) return SD_ERR_UNSUPPORTED;
+  DsdForm f = dsd_form(g);
+  if (!f.ok || !f.kc || f.cm || (g.aux && g.aux_sc != 1)) return SD_ERR_UNSUPPORTED;
+  // rows of either projection are reached by one 32-bit offset
+  if ((g.gate + 256) * g.b.sr * 2 >= (1LL << 31)) return SD_ERR_UNSUPPORTED;
+  f.ragged = g.M % BS != 0 || g.gate % 32 != 0 || g.K % BS != 0;
+  const int policy = tile_policy.load(std::memory_order_relaxed);
+  const double kept = planned_kept(g);
+  int shape = -1;
+  double t_best = 1e30;
+  for (int s = kShapeOne; s <= kShapeBig; ++s) {
+    if ((policy == kTileBig && s != kShapeBig) || (policy == kTileMid && s != kShapeQuad && s != kShapeWide)) continue;
+    if (blocks_of(g.K) > (s == kShapeBig ? MAX_STEPS : kTileMaxSteps)) continue;
+    const double t = dsd_work(true, s, g.M, g.N, g.K, 1, kept, g.act == SD_ACT_RELU ? SD_ACT_RELU : SD_ACT_GELU).time();
+    if (t < t_best) {
+      t_best = t;
+      shape = s;
+    }
+  }
+  if (shape < 0) return SD_ERR_UNSUPPORTED;
+  int rc;
+  if (shape != kShapeBig)
+    rc = is_bf16(dtype) ? tile_gated<BF16>(g, shape, stream) : tile_gated<F16>(g, shape, stream);
+  else if (is_bf16(dtype))
+    rc = f.ragged ? launch_big_t<BF16, false, false, true, true>(g, 1, stream) : launch_big_t<BF16, false, false, false, true>(g, 1, stream);
+  else
+    rc = f.ragged ? launch_big_t<F16, false, false, true, true>(g, 1, stream) : launch_big_t<F16, false, false, false, true>(g, 1, stream);
+  if (rc == SD_OK) note_kernel("dsd:%s:gated%s", dsd_name(shape), f.ragged && shape == kShapeBig ? ":ragged" : "");
+  return rc;
+}
+
+int launch_gated_gradient(const GemmArgs& g, int dtype, hipStream_t stream) {
+  if (g.row_ptr && g.bs != BS) return SD_ERR_UNSUPPORTED;
+  if (!sdd_operands_ok(g) || blocks_of(g.M) * blocks_of(g.N) > 0x7fffffffLL || g.aux_sc != 1) return SD_ERR_UNSUPPORTED;
+  const int shape = plan_sdd(g);
+  const bool ragged = g.N % BS != 0 || g.K % BS != 0;
+  int rc;
+  if (shape != kShapeBig)
+    rc = is_bf16(dtype) ? tile_gated_gradient<BF16>(g, shape, stream) : tile_gated_gradient<F16>(g, shape, stream);
+  else if (is_bf16(dtype))
+    rc = ragged ? launch_sdd_big<BF16, true, true>(g, stream) : launch_sdd_big<BF16, false, true>(g, stream);
+  else
+    rc = ragged ? launch_sdd_big<F16, true, true>(g, stream) : launch_sdd_big<F16, false, true>(g, stream);
+  if (rc == SD_OK) note_kernel("sdd:%s:gated%s", shape == kShapeBig ? "big" : (shape == kShapeWide ? "mid" : "small"), ragged && shape == kShapeBig ? ":ragged" : "");
+  return rc;
 }
 
 // ---- the forward product and the kept lists of its mask in one launch -------------------------------------------

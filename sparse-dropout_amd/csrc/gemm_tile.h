@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gated.h"
 #include "gemm_device.h"
 #include "mask_source.h"
 #include "tile_map.h"
@@ -80,6 +81,11 @@ struct TileLoads {
     }
     const int64_t c = outer0 + ch[i] * 8;
     return c < ext ? (uint32_t)((row[i] * ld + (c - origin)) * 2) : kNoData;
+  }
+  // of W_in's rows for a gate (gated.h): block c of the workgroup, whose hidden columns begin at h0; bytes from that row
+  __device__ inline uint32_t gated_offset(int i, int c, int64_t h0, int64_t F) const {
+    const int n = c * BS + row[i], h = gated_hidden(n);
+    return h0 + h < F ? (uint32_t)(((h + (gated_up(n) ? F : 0)) * ld + ch[i] * 8) * 2) : kNoData;
   }
 };
 
@@ -173,6 +179,63 @@ __device__ inline void store_piece(const GemmArgs& g, f32x4 (&v)[MT][NT16], int 
   }
 }
 
+// Stores what a gate makes of a wave's piece; c0: its first hidden column.  Four 16-column tiles hold 32 hidden columns, eight of them a lane
+// after the exchange, two tiles 16, of which a lane has four.
+template <typename T, int MT, int NT16>
+__device__ inline void store_gate_piece(const GemmArgs& g, f32x4 (&v)[MT][NT16], int lane, int64_t m0, int64_t c0) {
+  static_assert(NT16 == 2 || NT16 == 4, "one or two pairs");
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int64_t m = m0 + mt * 16 + lane % 16;
+    if constexpr (NT16 == 4) {
+      float gate[8], up[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gate[i] = v[mt][0][i];
+        gate[4 + i] = v[mt][2][i];
+        swap_rows16(gate[i], gate[4 + i]);
+        up[i] = v[mt][1][i];
+        up[4 + i] = v[mt][3][i];
+        swap_rows16(up[i], up[4 + i]);
+      }
+      store_gate<T, 8>(g, m, c0 + piece_at(lane), gate, up);
+    } else {
+      float gate[4], up[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gate[i] = v[mt][0][i];
+        up[i] = v[mt][1][i];
+      }
+      store_gate<T, 4>(g, m, c0 + 4 * (lane / 16), gate, up);
+    }
+  }
+}
+// Stores both gradients of a gate for a piece of dh; pre: what stands at its places, in the order of the stores.
+template <typename T, int MT, int NT16>
+__device__ inline void load_gate_piece(const GemmArgs& g, int lane, int64_t m0, int64_t n0, GateAt (&pre)[MT * NT16 / 2]) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT16; nt += 2) pre[mt * (NT16 / 2) + nt / 2].load(g, m0 + mt * 16 + lane % 16, n0 + nt * 16 + piece_at(lane));
+}
+template <typename T, int MT, int NT16>
+__device__ inline void store_gate_gradient_piece(const GemmArgs& g, f32x4 (&v)[MT][NT16], int lane, int64_t m0, int64_t n0,
+                                                 const GateAt (&pre)[MT * NT16 / 2]) {
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT16; nt += 2) {
+      float dh[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dh[i] = v[mt][nt][i];
+        dh[4 + i] = v[mt][nt + 1][i];
+        swap_rows16(dh[i], dh[4 + i]);
+      }
+      store_gate_gradient<T>(g, m0 + mt * 16 + lane % 16, n0 + nt * 16 + piece_at(lane), dh, pre[mt * (NT16 / 2) + nt / 2]);
+    }
+}
+
 // The pre-activations of a row-major piece, in the order in which store_piece takes them
 template <int MT, int NT16>
 __device__ inline void load_aux(const GemmArgs& g, int lane, int64_t m0, int64_t n0, u32x4 (&pre)[MT * NT16 / 2]) {
@@ -231,10 +294,12 @@ __device__ inline void union_steps(const GemmArgs& g, const MaskSrc* ms, int rb0
 // ---- DSD and dense: C = s (keep . A) B^T ------------------------------------------------------------------------------
 // KC: both operands reduction-contiguous (forward) or both reduction-strided (weight gradient).  Arguments as for the
 // large shapes' dsd_body.
-template <typename T, bool KC, bool CM, typename S, bool TABLED = false>
+// GATED: B is W_in and the store gates (gated.h)
+template <typename T, bool KC, bool CM, typename S, bool TABLED = false, bool GATED = false>
 __device__ __forceinline__ void tile_dsd_body(const GemmArgs& g, int tiles_m, int tiles_n, int Mb, int Kb_all, int bid,
                                               int nsplit, const MaskSrc* ms = nullptr) {
   constexpr int R = S::R, C = S::C, NST = S::NST, LPW = S::LPW, MT = S::MT, NT16 = S::NT16, KG = S::HALVES ? 2 : 1;
+  static_assert(!GATED || (KC && !CM && !S::HALVES), "the gate's store");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const uint32_t smem_a = lds_address(smem);
   uint32_t* scratch = reinterpret_cast<uint32_t*>(smem);  // uint32 per K block while merging; the stages come later
@@ -270,10 +335,10 @@ __device__ __forceinline__ void tile_dsd_body(const GemmArgs& g, int tiles_m, in
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) b_off[c][i] = lb.offset(i, n0 + c * BS, n0, g.N);
+    for (int i = 0; i < LPW; ++i) b_off[c][i] = GATED ? lb.gated_offset(i, c, n0 / 2, g.gate) : lb.offset(i, n0 + c * BS, n0, g.N);
   const int ncb = (int)((g.N - n0 + BS - 1) / BS) < C ? (int)((g.N - n0 + BS - 1) / BS) : C;  // column blocks inside C
   const char* a0 = reinterpret_cast<const char*>(g.a.ptr + (int64_t)rb0 * BS * (KC ? lda : 1));
-  const char* b0 = reinterpret_cast<const char*>(g.b.ptr + n0 * (KC ? ldb : 1));
+  const char* b0 = reinterpret_cast<const char*>(g.b.ptr + (GATED ? n0 / 2 : n0) * (KC ? ldb : 1));
   const int64_t a_step = KC ? BS * 2 : BS * 2 * lda, b_step = KC ? BS * 2 : BS * 2 * ldb;
   auto issue = [&](uint32_t e, int stage) {
     const int kb = step_block(e);
@@ -475,7 +540,8 @@ __device__ __forceinline__ void tile_dsd_body(const GemmArgs& g, int tiles_m, in
     store_piece<T, false, CM, 2, NT16>(g, half, lane, (int64_t)rb * BS + 32 * kk, nw, part);
   } else {
     if (rb >= Mb || nw >= g.N) return;
-    store_piece<T, false, CM, MT, NT16>(g, acc, lane, (int64_t)rb * BS + 16 * a_t0, nw, part);
+    if constexpr (GATED) store_gate_piece<T, MT, NT16>(g, acc, lane, (int64_t)rb * BS + 16 * a_t0, nw / 2);
+    else store_piece<T, false, CM, MT, NT16>(g, acc, lane, (int64_t)rb * BS + 16 * a_t0, nw, part);
   }
 }
 
@@ -483,7 +549,8 @@ __device__ __forceinline__ void tile_dsd_body(const GemmArgs& g, int tiles_m, in
 // A reduction-contiguous, B reduction-strided, C row-major.  A workgroup owns one row block and C consecutive KEPT
 // column blocks of it, straight from the row's list, and stores the zeros of column blocks [C * j, C * j + C) that the
 // list leaves out: every product it computes is wanted, and dropped tiles cost the zeros alone.
-template <typename T, typename S>
+// GATED: the store leaves both gradients of a gate (gated.h)
+template <typename T, typename S, bool GATED = false>
 __device__ __forceinline__ void tile_sdd_body(const GemmArgs& g, int sure, int Mb, int Cb, int bid) {
   static_assert(S::R == 1 && S::HALVES, "one row block");
   constexpr int C = S::C, NST = S::NST, LPW = S::LPW, NT16 = S::NT16;
@@ -523,7 +590,14 @@ __device__ __forceinline__ void tile_sdd_body(const GemmArgs& g, int sure, int M
       const uint32_t f = *found;
 #pragma unroll
       for (int c = 0; c < C; ++c)
-        if (!((f >> c) & 1u) && tn * C + c < Cb) zero_tile<S::THREADS>(g, m0, (int64_t)(tn * C + c) * BS);
+        if (!((f >> c) & 1u) && tn * C + c < Cb) {
+          zero_tile<S::THREADS>(g, m0, (int64_t)(tn * C + c) * BS);
+          if constexpr (GATED) {
+            GemmArgs up = g;
+            up.c += g.gate;
+            zero_tile<S::THREADS>(up, m0, (int64_t)(tn * C + c) * BS);
+          }
+        }
       __syncthreads();
     }
   } else {
@@ -667,10 +741,19 @@ __device__ __forceinline__ void tile_sdd_body(const GemmArgs& g, int sure, int M
   // at p = 0.3 58.2 -> 54.4 us, 16384 x 1536 from 384 at p = 0.1 53.1 -> 51.1
   const int64_t m_out = m0 + 32 * kk, n_out = (int64_t)my_col * BS + b_t0 * 16;
   u32x4 pre[NT16] = {};
-  if (active && g.act != SD_ACT_NONE) load_aux<2, NT16>(g, lane, m_out, n_out, pre);
+  GateAt gate[NT16];
+  if constexpr (GATED) {
+    if (active) load_gate_piece<T, 2, NT16>(g, lane, m_out, n_out, gate);
+  } else {
+    if (active && g.act != SD_ACT_NONE) load_aux<2, NT16>(g, lane, m_out, n_out, pre);
+  }
   f32x4 half[2][NT16];
   meet_halves<NT16>(acc, half, smem, wave, kk, lane);
   if (!active) return;
+  if constexpr (GATED) {
+    store_gate_gradient_piece<T, 2, NT16>(g, half, lane, m_out, n_out, gate);
+    return;
+  }
   store_piece<T, true, false, 2, NT16>(g, half, lane, m_out, n_out, nullptr, pre);
 }
 

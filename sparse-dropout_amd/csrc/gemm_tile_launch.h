@@ -36,16 +36,16 @@ using SddOne = TileShape<1, 1, 4, 2, true, 4, 2>;
 using SddStrip = TileShape<1, 4, 3, 2, true>;
 using SddWide = TileShape<1, 2, 2, 0, true>;
 
-template <typename T, bool KC, bool CM, typename S>
+template <typename T, bool KC, bool CM, typename S, bool GATED = false>
 __global__ __launch_bounds__(S::THREADS) void tile_dsd_kernel(GemmArgs g, int tiles_m, int tiles_n, int Mb, int Kb) {
-  tile_dsd_body<T, KC, CM, S>(g, tiles_m, tiles_n, Mb, Kb, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)gridDim.y);
+  tile_dsd_body<T, KC, CM, S, false, GATED>(g, tiles_m, tiles_n, Mb, Kb, (int)(blockIdx.y * gridDim.x + blockIdx.x), (int)gridDim.y);
 }
 
 // Without loading waves three workgroups share a CU, three waves a SIMD: 168 registers.  Not asked for the third, the compiler
 // took 169, and 4096 x 4096 from 1024 with GELU's derivative was 5 % slower than without the loads ahead of its store.
-template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS, S::LW ? 1 : 3) void tile_sdd_kernel(GemmArgs g, int sure, int Mb, int Cb) {
-  tile_sdd_body<T, S>(g, sure, Mb, Cb, (int)blockIdx.x);
+template <typename T, typename S, bool GATED = false>
+__global__ __launch_bounds__(S::THREADS, S::LW ? 1 : (GATED ? 2 : 3)) void tile_sdd_kernel(GemmArgs g, int sure, int Mb, int Cb) {
+  tile_sdd_body<T, S, GATED>(g, sure, Mb, Cb, (int)blockIdx.x);
 }
 
 // The forward product and the kept lists of its mask in one launch (see forward_lists_kernel of the large shapes).
@@ -101,10 +101,10 @@ bool more_than_resident(const GemmArgs& g, int splits) {  // of the 64 x 64 shap
   return (int64_t)blocks_of(g.M) * blocks_of(g.N) * splits > 512;
 }
 
-template <typename T, bool KC, bool CM, typename S>
+template <typename T, bool KC, bool CM, typename S, bool GATED = false>
 int dsd_launch(const GemmArgs& g, int splits, hipStream_t stream) {
   static std::atomic<bool> done[64] = {};
-  auto* kernel = &tile_dsd_kernel<T, KC, CM, S>;
+  auto* kernel = &tile_dsd_kernel<T, KC, CM, S, GATED>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), S::SMEM, done)) return rc;
   const int Mb = blocks_of(g.M), Kb = blocks_of(g.K), tm = (Mb + S::R - 1) / S::R, tn = (blocks_of(g.N) + S::C - 1) / S::C;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn), (unsigned)splits), dim3(S::THREADS), S::smem_for(Kb), stream, g, tm, tn, Mb, Kb);
@@ -137,10 +137,10 @@ int sure_strips(const GemmArgs& g, int C, int most) {
   return keep > 0.999 ? most : std::min(most, std::max(1, (int)((Cb * keep + spread) / C + (C - 1) / (2.0 * C) + 0.5)));
 }
 
-template <typename T, typename S>
+template <typename T, typename S, bool GATED = false>
 int sdd_launch(const GemmArgs& g, hipStream_t stream) {
   static std::atomic<bool> done[64] = {};
-  auto* kernel = &tile_sdd_kernel<T, S>;
+  auto* kernel = &tile_sdd_kernel<T, S, GATED>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), S::SMEM_STEPS, done)) return rc;
   const int Mb = blocks_of(g.M), Cb = blocks_of(g.N), tn = (Cb + S::C - 1) / S::C;
   // No step table, and no more stages than there are steps, down to what the halves meet in.  With the table's 8 KB behind
@@ -188,6 +188,24 @@ int tile_dsd(const GemmArgs& g, bool kc, bool cm, int shape, int splits, hipStre
 }
 
 template <typename T>
+int tile_gated(const GemmArgs& g, int shape, hipStream_t stream) {
+  switch (shape) {
+    case kShapeOne: return more_than_resident(g, 1) ? dsd_launch<T, true, false, FwdOneMany, true>(g, 1, stream) : dsd_launch<T, true, false, FwdOne, true>(g, 1, stream);
+    case kShapeQuad: return dsd_launch<T, true, false, FwdQuad, true>(g, 1, stream);
+    default: return dsd_launch<T, true, false, FwdWide, true>(g, 1, stream);
+  }
+}
+
+template <typename T>
+int tile_gated_gradient(const GemmArgs& g, int shape, hipStream_t stream) {
+  switch (shape) {
+    case kShapeOne: return sdd_launch<T, SddOne, true>(g, stream);
+    case kShapeQuad: return sdd_launch<T, SddStrip, true>(g, stream);
+    default: return sdd_launch<T, SddWide, true>(g, stream);
+  }
+}
+
+template <typename T>
 int tile_forward(const GemmArgs& g, int shape, int splits, const FlatJobs& f, hipStream_t stream) {
   switch (shape) {
     case kShapeOne:
@@ -215,6 +233,8 @@ int tile_pair(const GemmArgs& gx, const GemmArgs& gw, int shape, int splits, hip
 
 #define SD_TILE_INSTANCES(T)                                                                    \
   template int tile_dsd<T>(const GemmArgs&, bool, bool, int, int, hipStream_t);                 \
+  template int tile_gated<T>(const GemmArgs&, int, hipStream_t);                                \
+  template int tile_gated_gradient<T>(const GemmArgs&, int, hipStream_t);                       \
   template int tile_forward<T>(const GemmArgs&, int, int, const FlatJobs&, hipStream_t);        \
   template int tile_sdd<T>(const GemmArgs&, int, hipStream_t);                                  \
   template int tile_pair<T>(const GemmArgs&, const GemmArgs&, int, int, hipStream_t);

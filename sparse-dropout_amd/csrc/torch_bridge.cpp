@@ -640,6 +640,91 @@ Tensor mlp(const Tensor& input, const std::vector<Tensor>& weights, int64_t bs, 
 
 // ---- a gated feed-forward block ------------------------------------------------------------------------------------------
 // (see functional/gated_mlp.py for what is computed)
+// Lists of a layer's mask, drawn here unless it is given, in a launch of their own.
+void layer_lists(const Tensor& x, int64_t rows, int64_t cols, int64_t bs, double p, const Draw& draw, Lists& l) {
+  check_p(p);
+  l.shape(rows, cols, bs);
+  TORCH_CHECK_NOT_IMPLEMENTED(bs % 32 == 0, "block_size ", bs, ": only multiples of 32 are supported");
+  l.allocate(x, draw.mask);
+  const int64_t split = bs % 64 == 32 ? -(bs / 32) : bs / 64;
+  c10::DeviceGuard guard(x.device());
+  if (draw.mask) {
+    const MaskArg m = l.mask();
+    check(sd_build_lists_split(m.ptr, l.mb, l.kb, m.sr, m.sc, split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(), l.row_idx(), stream_of(x)),
+          "sd_build_lists_split");
+  } else if (uint64_t* st = draw.state_ptr()) {
+    check(sd_random_lists_state(st, (float)p, l.mb, l.kb, l.drawn(), split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(), l.row_idx(),
+                                stream_of(x)),
+          "sd_random_lists_state");
+  } else {
+    check(sd_random_lists(draw.seed.value_or(0), 0, (float)p, l.mb, l.kb, l.drawn(), split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(),
+                          l.row_idx(), stream_of(x)),
+          "sd_random_lists");
+  }
+}
+
+// H = act(G) U of [G | U] = s (keep . X) W_in^T, in one launch where a kernel takes it; pre: [G | U] if it is wanted.  lists: of X's mask, if any
+Tensor gated_forward(Tensor x, Tensor w, int64_t F, int act, double p, const Lists& lists, bool want_pre, Tensor& pre) {
+  pad_reduction(x, w);
+  const int64_t M = x.size(0), K = x.size(1);
+  Tensor h = new_matrix(x, M, F);
+  if (want_pre) pre = new_matrix(x, M, 2 * F);
+  const bool masked = lists.buf.defined();
+  const int32_t *rows = masked ? lists.row_ptr() : nullptr, *cols = masked ? lists.col_idx() : nullptr;
+  const float scale = masked ? (float)(1.0 / (1.0 - p)) : 1.f;
+  const Mat xm(x), wm(w), hm(h);
+  Mat pm;
+  if (want_pre) pm = Mat(pre);
+  c10::DeviceGuard guard(x.device());
+  const int rc = sd_gated_matmul(MAT(xm), MAT(wm), hm.ptr, hm.sr, pm.ptr, pm.sr, rows, cols, M, F, K, masked ? lists.kernel_bs : 0, scale, act, dtype_of(x),
+                                 stream_of(x));
+  if (rc == SD_OK) return h;
+  if (rc != SD_ERR_UNSUPPORTED) check(rc, "sd_gated_matmul");
+  if (!want_pre) pre = new_matrix(x, M, 2 * F);
+  pm = Mat(pre);
+  const int64_t g = masked && lists.kernel_bs != 32 ? lists.kernel_bs : 64;
+  Scratch ws(x, sd_splitk_workspace_bytes(M, 2 * F, K, masked ? g : 0, masked ? 1 : 0));
+  if (masked)
+    check(sd_gemm_dsd_lists(MAT(xm), MAT(wm), MAT(pm), rows, cols, M, 2 * F, K, lists.kernel_bs, scale, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
+          "sd_gemm_dsd_lists");
+  else
+    check(sd_gemm(MAT(xm), MAT(wm), MAT(pm), M, 2 * F, K, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)), "sd_gemm");
+  check(sd_gated_forward(pm.ptr, pm.sr, hm.ptr, hm.sr, M, F, act, dtype_of(x), stream_of(x)), "sd_gated_forward");
+  return h;
+}
+
+// [dG | dU] and / or dW_out from dY.
+std::pair<Tensor, Tensor> gated_backward(Tensor dy, Tensor w, Tensor h, const Tensor& a, int act, double p, const Lists& lists, bool need_da, bool need_dw) {
+  const int64_t M = dy.size(0), N = dy.size(1), F = h.size(1), n8 = ceil_div(N, 8) * 8;
+  TORCH_CHECK_VALUE(M == h.size(0) && N == w.size(0) && dy.device() == h.device(), "dy must be a [", h.size(0), ", ", w.size(0), "] tensor on ", h.device());
+  RowPadding pad;  // as in layer_backward
+  if (N % 8 || (row_major(dy) && !rows_on_16_bytes(dy))) dy = pad.add(dy, M);
+  if (need_da && (N % 8 || (row_major(w) && !rows_on_16_bytes(w)))) w = pad.add(w, n8).narrow(1, 0, F);
+  else if (N % 8) w = at::empty({n8, F}, w.options());  // dW alone: only its shape is looked at
+  if (need_dw && row_major(h) && !rows_on_16_bytes(h)) h = pad.add(h, M).narrow(1, 0, F);
+  pad.launch();
+  Tensor da, dw;
+  if (need_da) {
+    da = new_matrix(h, M, 2 * F);
+    const bool masked = lists.buf.defined();
+    const Mat gm(dy), wm(w), am(a), om(da);
+    c10::DeviceGuard guard(h.device());
+    const int rc = sd_gated_matmul_gradient(MAT(gm), MAT(wm), am.ptr, am.sr, om.ptr, om.sr, masked ? lists.row_ptr() : nullptr, masked ? lists.col_idx() : nullptr, M,
+                                            F, dy.size(1), masked ? lists.kernel_bs : 0, masked ? (float)(1.0 / (1.0 - p)) : 1.f, (float)(1.0 - p), act, dtype_of(h),
+                                            stream_of(h));
+    if (rc == SD_ERR_UNSUPPORTED) {
+      const auto [dh, dw_too] = layer_products(dy, w, h, lists, p, true, need_dw, SD_ACT_NONE, Tensor());
+      dw = dw_too;
+      const Mat dm(dh);
+      check(sd_gated_backward(dm.ptr, dm.sr, am.ptr, am.sr, om.ptr, om.sr, M, F, act, dtype_of(h), stream_of(h)), "sd_gated_backward");
+    } else {
+      check(rc, "sd_gated_matmul_gradient");
+    }
+  }
+  if (need_dw && !dw.defined()) dw = layer_products(dy, w, h, lists, p, false, true, SD_ACT_NONE, Tensor()).second;
+  return {da, dw.defined() && dw.size(0) != N ? dw.narrow(0, 0, N) : dw};
+}
+
 struct GatedMlpBackward : Node {
   Saved x, w_in, w_out, pre, h;  // pre: [G | U], h = act(G) U
   SavedLists lists[2];           // nothing kept: nothing is dropped
@@ -659,17 +744,9 @@ struct GatedMlpBackward : Node {
       return out;
     }
     const Tensor dy = grad_matrix(grads[0], xs), hs = h.matrix(), a = pre.matrix();
-    const int64_t M = xs.size(0), F = wo.size(1);
-    Tensor dh;
-    std::tie(dh, out[2]) = layer_backward(dy, wo, hs, lists[1].get(), p[1], need_x || need_in, need_out, SD_ACT_NONE, Tensor());
+    Tensor da;
+    std::tie(da, out[2]) = gated_backward(dy, wo, hs, row_major(a) ? a : a.contiguous(), act, p[1], lists[1].get(), need_x || need_in, need_out);
     if (!need_x && !need_in) return out;
-    const Tensor as = row_major(a) ? a : a.contiguous();
-    Tensor da = new_matrix(xs, M, 2 * F);
-    {
-      const Mat dm(dh), am(as), om(da);
-      c10::DeviceGuard guard(xs.device());
-      check(sd_gated_backward(dm.ptr, dm.sr, am.ptr, am.sr, om.ptr, om.sr, M, F, act, dtype_of(xs), stream_of(xs)), "sd_gated_backward");
-    }
     std::tie(out[0], out[1]) = layer_backward(da, wi, xs, lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
     return out;
   }
@@ -701,23 +778,16 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
   Tensor pre, h, y;
   {
     NoRecord guard;
-    auto product = [&](int i, const Tensor& a, const Tensor& w) {
-      const OptTensor mask = masks ? (*masks)[i] : OptTensor();
-      if (bs == 0 || (ps[i] == 0.0 && !mask)) return dense(a, w, SD_ACT_NONE, false, nullptr);
-      const Draw draw{mask, seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
-      return layer_forward(a, w, bs, ps[i], draw, SD_ACT_NONE, false, lists[i], nullptr);
+    const auto drops = [&](int i) { return bs != 0 && (ps[i] != 0.0 || (masks && (*masks)[i])); };
+    const auto draw = [&](int i) {
+      return Draw{masks ? (*masks)[i] : OptTensor(), seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
     };
     if (M == 0) {
       y = new_matrix(x, 0, N);
     } else {
-      pre = product(0, x, wi);
-      h = new_matrix(x, M, F);
-      {
-        const Mat am(pre), hm(h);
-        c10::DeviceGuard device(x.device());
-        check(sd_gated_forward(am.ptr, am.sr, hm.ptr, hm.sr, M, F, act, dtype_of(x), stream_of(x)), "sd_gated_forward");
-      }
-      y = product(1, h, wo);
+      if (drops(0)) layer_lists(x, M, x.size(1), bs, ps[0], draw(0), lists[0]);
+      h = gated_forward(x, wi, F, act, ps[0], lists[0], rec, pre);
+      y = drops(1) ? layer_forward(h, wo, bs, ps[1], draw(1), SD_ACT_NONE, false, lists[1], nullptr) : dense(h, wo, SD_ACT_NONE, false, nullptr);
     }
   }
   if (rec) {

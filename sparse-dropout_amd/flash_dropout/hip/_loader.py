@@ -143,6 +143,10 @@ SIGNATURES = {
     "sd_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "sd_clip_grads": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_int64, c_void_p]),
     "sd_gated_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "sd_gated_matmul": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float,
+                                c_int, c_int, c_void_p]),
+    "sd_gated_matmul_gradient": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                         c_float, c_float, c_int, c_int, c_void_p]),
     "sd_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
 }
 
