@@ -427,6 +427,9 @@ bool conv_dx_taken(const void* dy, int64_t dy_ld, const void* w, int64_t w_ld, i
 int launch_gated(const GemmArgs& g, int dtype, hipStream_t stream);
 // an SDD (or dense) product dH that leaves [dG | dU] in g.c, g.aux: [G | U], g.N == g.gate
 int launch_gated_gradient(const GemmArgs& g, int dtype, hipStream_t stream);
+// What a dense product, and one with a gate in its store (F hidden columns), is expected to take in tiles, us.
+double dense_expected_us(int64_t M, int64_t N, int64_t K);
+double gated_expected_us(int64_t M, int64_t F, int64_t K);
 // which workgroup shape the DSD kernel runs in: chosen from the shape, or forced (tuning and tests);
 // returns the previous policy, -1 for an unknown one
 enum { kTileAuto = 0, kTileBig = 1, kTileMid = 2 };

@@ -1,0 +1,266 @@
+// A gated feed-forward block for few rows, the tokens of a serving step: two launches that read each weight once.
+//
+//   h = act(x W_g^T) (x W_u^T)        y = h W_out^T
+//
+// Bound by the weights' bytes, 2 (2 F K + N F), and with few of them by a memory latency and a launch each.  So weights go from memory straight
+// into the matrix instruction's registers.  A workgroup owns 16 outputs (or 32, or 8 or 4 where there would be too few workgroups: the others' lanes load
+// nothing); its waves share out the 64-deep pieces of the reduction, which are whole 128-byte lines of its weight rows, wave w every piece
+// w + WAVES n, AHEAD of them on their way at a time, and meet once in LDS.  A lane takes 32 consecutive bytes of a line (two loads, four lanes to a
+// line); the order of the reduction within a piece is the same for both operands and shows in nothing but the last bits.  Rows come in groups of
+// 16.  What comes back to a CU, 64 bytes a clock, is what a full group of rows costs beside the weights, so lanes of rows that are not there load nothing.
+//
+// Up to 8 rows leave room for h twice in a group: h, which nothing but the second launch reads, is then held as the sum of two 16-bit numbers, the
+// low halves in rows 8 to 15, and its rounding, the largest of the path, is saved.
+#include "gated.h"
+
+namespace sd {
+namespace {
+
+constexpr int kDeep = 64;  // elements of a piece
+constexpr int kTwice = 8;  // rows up to which h is held in two halves
+
+struct Few {
+  const uint16_t *x, *w;  // x: rows of the input, or of h
+  uint16_t* h;            // [rows, or high halves and from row 8 on low ones][ldh]
+  uint16_t* y;
+  int64_t ldx, ldw, ldh, ldy;
+  int M, N, K, act;  // N: hidden columns or outputs
+  int cols;          // of a workgroup, where that owns 16 or fewer
+};
+
+// 16 consecutive elements of a row, 16 q .. + 15 of a piece; left: those behind `at` that are there
+__device__ inline void load_some16(const uint16_t* at, int left, u32x4 (&v)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = 8 * h + 2 * i;
+      v[h][i] = (c < left ? at[c] : 0u) | (c + 1 < left ? (uint32_t)at[c + 1] << 16 : 0u);
+    }
+}
+__device__ inline void load16(const uint16_t* at, u32x4 (&v)[2]) {
+  v[0] = *reinterpret_cast<const u32x4_any*>(at);
+  v[1] = *reinterpret_cast<const u32x4_any*>(at + 8);
+}
+
+// HIDDEN: the first launch (both projections), else the second
+template <typename T, bool HIDDEN, int WAVES, int GROUPS, int COLS, int AHEAD>
+__global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
+  constexpr int WP = HIDDEN ? 2 : 1;
+  __shared__ float sums[WAVES][WP][16][17];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15, q = lane >> 4;
+  const int per = COLS == 1 ? g.cols : 16 * COLS, n0 = (int)blockIdx.x * per, whole = g.K / kDeep, left = g.K - whole * kDeep;
+  const bool twice = g.M <= kTwice;
+  const uint16_t* w[COLS][WP];
+#pragma unroll
+  for (int j = 0; j < COLS; ++j)
+#pragma unroll
+    for (int p = 0; p < WP; ++p) w[j][p] = g.w + (int64_t)(min(n0 + 16 * j + r, g.N - 1) + p * g.N) * g.ldw + 16 * q;
+  const bool reads_w = COLS > 1 || r < per;
+  const uint16_t* x[GROUPS];
+  bool reads_x[GROUPS];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const int row = 16 * i + r;
+    reads_x[i] = HIDDEN || !twice ? row < g.M : (r & (kTwice - 1)) < g.M;
+    x[i] = g.x + (int64_t)(reads_x[i] ? row : 0) * g.ldx + 16 * q;
+  }
+  f32x4 acc[GROUPS][COLS][WP] = {};
+  auto multiply = [&](const u32x4 (&a)[GROUPS][2], const u32x4 (&b)[COLS][WP][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int p = 0; p < WP; ++p)
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+          for (int j = 0; j < COLS; ++j) acc[i][j][p] = T::mfma16(a[i][h], b[j][p][h], acc[i][j][p]);
+  };
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  for (int c0 = wave; c0 < whole; c0 += WAVES * AHEAD) {
+    u32x4 b[AHEAD][COLS][WP][2], a[AHEAD][GROUPS][2];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+#pragma unroll
+          for (int p = 0; p < WP; ++p) b[u][j][p][h] = none;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) a[u][i][h] = none;
+      }
+    }
+    if (reads_w) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (c0 + u * WAVES < whole) {
+#pragma unroll
+          for (int j = 0; j < COLS; ++j)
+#pragma unroll
+            for (int p = 0; p < WP; ++p) load16(w[j][p] + (int64_t)(c0 + u * WAVES) * kDeep, b[u][j][p]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i)
+      if (reads_x[i]) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+          if (c0 + u * WAVES < whole) load16(x[i] + (int64_t)(c0 + u * WAVES) * kDeep, a[u][i]);
+      }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (c0 + u * WAVES < whole) multiply(a[u], b[u]);
+  }
+  if (left && wave == whole % WAVES) {
+    const int64_t k = (int64_t)whole * kDeep;
+    u32x4 b[COLS][WP][2], a[GROUPS][2];
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+#pragma unroll
+      for (int p = 0; p < WP; ++p) load_some16(w[j][p] + k, reads_w ? left - 16 * q : 0, b[j][p]);
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) load_some16(x[i] + k, reads_x[i] ? left - 16 * q : 0, a[i]);
+    multiply(a, b);
+  }
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) {
+      if (i || j) __syncthreads();
+#pragma unroll
+      for (int p = 0; p < WP; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[wave][p][4 * q + e][r] = acc[i][j][p][e];
+      __syncthreads();
+      if (t < 256) {
+        const int at = t >> 4, col = t & 15, n = n0 + 16 * j + col, m = 16 * i + at;
+        if (m < g.M && (COLS > 1 || col < per)) {
+          float s[WP] = {};
+#pragma unroll
+          for (int o = 0; o < WAVES; ++o)
+#pragma unroll
+            for (int p = 0; p < WP; ++p) s[p] += sums[o][p][at][col];
+          if constexpr (HIDDEN) {
+            if (n < g.N) {
+              const float h = gate_value(g.act, s[0]) * s[WP - 1];
+              const uint16_t high = T::from_float(h);
+              g.h[m * g.ldh + n] = high;
+              if (twice) {
+                const float rounded = T::to_float(high);
+                g.h[(kTwice + m) * g.ldh + n] = __builtin_isinf(rounded) ? (uint16_t)0 : T::from_float(h - rounded);  // (what overflows stays infinite)
+              }
+            }
+          } else {
+            if (twice) {
+              float low = 0.f;
+#pragma unroll
+              for (int o = 0; o < WAVES; ++o) low += sums[o][0][kTwice + (at & (kTwice - 1))][col];
+              s[0] += low;
+            }
+            if (n < g.N) g.y[(int64_t)m * g.ldy + n] = T::from_float(s[0]);
+          }
+        }
+      }
+    }
+}
+
+int groups_of(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
+// Outputs of a workgroup.  At least 256 workgroups, down to 4 outputs each: one row of 4096 to 1024 takes 7.6 us with 16, 5.8 with 4, of 8192 to 2048
+// 12.0 with 16, 10.4 with 8.  32 for 33 and more rows where 16 would make more than 256 of them, for x is read half as often (64 rows, hidden of 2048
+// to 8192 28.6 us and 23.8; 1024 to 4096 9.6 and 13.1, with half of the CUs idle).
+int cols_of(int64_t M, int64_t N) {
+  if (groups_of(M) == 4 && ceil_div(N, 16) > 256) return 32;
+  for (int cols = 16; cols > 4; cols /= 2)
+    if (ceil_div(N, cols) >= 256) return cols;
+  return 4;
+}
+// What a launch is expected to take, us: 2.3, and for every CU the lines that come back to it at 33 GB/s, or the weights at 4.6 TB/s.
+// Measured and so expected, hidden of 2048 to 8192 at 16, 24 and 64 rows: 15.1, 14.2   17.2, 18.2   23.8, 18.2 (of x nobody's lanes share); outputs of 8192
+// to 2048: 14.2, 14.2   18.5, 22.2   35.7, 38.0.
+double few_us(int64_t M, int64_t N, int64_t K, int parts) {
+  const int cols = cols_of(M, N);
+  const double pieces = (double)ceil_div(K, kDeep), wgs = (double)ceil_div(N, cols), rounds = wgs > 256.0 ? wgs / 256.0 : 1.0;
+  const double rows = groups_of(M) == 1 ? (double)(parts == 1 && M <= kTwice ? 2 * M : M) : 16.0 * groups_of(M);
+  const double returned = rounds * pieces * 128.0 * (cols * parts + rows) / 33e3, weights = 2.0 * parts * (double)N * (double)K / 4.6e6;
+  return 2.3 + (returned > weights ? returned : weights);
+}
+
+template <typename T, bool HIDDEN>
+void launch_few(const Few& f, hipStream_t stream) {
+  Few g = f;
+  const int groups = groups_of(g.M), cols = cols_of(g.M, g.N);
+  g.cols = cols;
+  const dim3 grid((unsigned)ceil_div(g.N, cols)), block(512);
+  // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 15.0 us, with one 16.0), one for more (24 rows 17.2, with two 19.3)
+  if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2>), grid, block, 0, stream, g);
+  else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1>), grid, block, 0, stream, g);
+  else if (cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1>), grid, block, 0, stream, g);
+  else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1>), grid, block, 0, stream, g);
+}
+
+// Pitch of h: an odd number of whole pieces (rows a power of two apart lie in one channel of the L2).
+int64_t hidden_pitch(int64_t F) { return (ceil_div(F, kDeep) | 1) * kDeep; }
+int64_t hidden_rows(int64_t M) { return M <= kTwice ? 2 * kTwice : M; }
+
+}  // namespace
+}  // namespace sd
+
+using namespace sd;
+
+extern "C" {
+
+int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F) {
+  return M <= 0 || M > SD_GATED_FEW_ROWS || F <= 0 || F >= (1LL << 29) ? 0 : 2 * hidden_rows(M) * hidden_pitch(F);
+}
+
+int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N) {
+  if (M <= 0 || M > SD_GATED_FEW_ROWS || K <= 0 || F <= 0 || N <= 0 || K >= (1LL << 29) || F >= (1LL << 29) || N >= (1LL << 29)) return 0;
+  if (M <= 16) return 1;
+  // Rows that do not begin on 16 bytes are copied first on the other way: weights and activations at 3 TB/s, a launch each
+  const double copied = (K % 8 ? 4.0 + 8.0 * F * K / 3e6 : 0.0) + (F % 8 ? 4.0 + 4.0 * N * F / 3e6 : 0.0);
+  return few_us(M, F, K, 2) + few_us(M, N, F, 1) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
+}
+
+int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi, const void* W_out, int64_t ldwo, void* Y, int64_t ldy, int64_t M,
+                     int64_t K, int64_t F, int64_t N, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  SD_REQUIRE(M >= 0 && K > 0 && F > 0 && N > 0 && K < (1LL << 29) && F < (1LL << 29) && N < (1LL << 29), "gated_mlp_few: bad extents %lld, %lld, %lld, %lld",
+             (long long)M, (long long)K, (long long)F, (long long)N);
+  SD_REQUIRE(dtype == SD_F16 || dtype == SD_BF16, "gated_mlp_few: dtype must be SD_F16 or SD_BF16 (got %d)", dtype);
+  SD_REQUIRE(act == SD_ACT_RELU || act == SD_ACT_GELU || act == SD_ACT_SILU, "gated_mlp_few: act must be SD_ACT_RELU, SD_ACT_GELU or SD_ACT_SILU (got %d)", act);
+  if (M == 0) return SD_OK;
+  if (M > SD_GATED_FEW_ROWS) return fail(SD_ERR_UNSUPPORTED, "gated_mlp_few: %lld rows, at most %d", (long long)M, SD_GATED_FEW_ROWS);
+  SD_REQUIRE(X && W_in && W_out && Y, "gated_mlp_few: null pointer");
+  SD_REQUIRE((M == 1 || (ldx >= K && ldy >= N)) && ldwi >= K && (N == 1 || ldwo >= F), "gated_mlp_few: a pitch is shorter than its row");
+  const int64_t need = sd_gated_mlp_few_workspace_bytes(M, F);
+  SD_REQUIRE(workspace && workspace_bytes >= need, "gated_mlp_few: workspace too small: need %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
+  SD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "gated_mlp_few: workspace must be 16-byte aligned");
+  Few g = {};
+  g.x = static_cast<const uint16_t*>(X);
+  g.w = static_cast<const uint16_t*>(W_in);
+  g.h = static_cast<uint16_t*>(workspace);
+  g.ldx = ldx;
+  g.ldw = ldwi;
+  g.ldh = hidden_pitch(F);
+  g.M = (int)M;
+  g.N = (int)F;
+  g.K = (int)K;
+  g.act = act;
+  if (dtype == SD_BF16) launch_few<BF16, true>(g, (hipStream_t)stream);
+  else launch_few<F16, true>(g, (hipStream_t)stream);
+  if (int rc = check_launch("gated_mlp_few")) return rc;
+  g.x = g.h;
+  g.w = static_cast<const uint16_t*>(W_out);
+  g.y = static_cast<uint16_t*>(Y);
+  g.ldx = g.ldh;
+  g.ldw = ldwo;
+  g.ldy = ldy;
+  g.N = (int)N;
+  g.K = (int)F;
+  if (dtype == SD_BF16) launch_few<BF16, false>(g, (hipStream_t)stream);
+  else launch_few<F16, false>(g, (hipStream_t)stream);
+  note_kernel("gated:few groups=%d cols=%d,%d", groups_of(M), cols_of(M, F), cols_of(M, N));
+  return check_launch("gated_mlp_few");
+}
+
+}  // extern "C"

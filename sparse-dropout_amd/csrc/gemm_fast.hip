@@ -48,6 +48,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "gated.h"
@@ -2251,7 +2252,24 @@ int launch_fast(const GemmArgs& g, int mode, int dtype, hipStream_t stream) {
 }
 
 // ---- products with a gate in their store ---------------------------------------------------------------------------------------
-// The shape with the smallest expected time of the ungated product, its reduction uncut: a gate needs whole sums.
+// The shape with the smallest expected time of the ungated product, its reduction uncut, and that time: a gate needs whole sums.  N: columns of both
+// projections.  shape -1: none takes it.
+std::pair<int, double> plan_gated(int64_t M, int64_t N, int64_t K, double kept, int act) {
+  const int policy = tile_policy.load(std::memory_order_relaxed);
+  std::pair<int, double> best{-1, 1e30};
+  for (int s = kShapeOne; s <= kShapeBig; ++s) {
+    if ((policy == kTileBig && s != kShapeBig) || (policy == kTileMid && s != kShapeQuad && s != kShapeWide)) continue;
+    if (blocks_of(K) > (s == kShapeBig ? MAX_STEPS : kTileMaxSteps)) continue;
+    const double t = dsd_work(true, s, M, N, K, 1, kept, act == SD_ACT_RELU ? SD_ACT_RELU : SD_ACT_GELU).time();
+    if (t < best.second) best = {s, t};
+  }
+  return best;
+}
+double gated_expected_us(int64_t M, int64_t F, int64_t K) { return plan_gated(M, gated_columns(F), K, 1.0, SD_ACT_SILU).second; }
+double dense_expected_us(int64_t M, int64_t N, int64_t K) {
+  const DsdPlan plan = plan_dsd(M, N, K, true, 1.0, SD_ACT_NONE);
+  return dsd_work(true, plan.shape, M, N, K, plan.splits, 1.0, SD_ACT_NONE).time();
+}
 int launch_gated(const GemmArgs& g_, int dtype, hipStream_t stream) {
   GemmArgs g = g_;
   g.N = gated_columns(g.gate);
@@ -2261,19 +2279,7 @@ int launch_gated(const GemmArgs& g_, int dtype, hipStream_t stream) {
   // rows of either projection are reached by one 32-bit offset
   if ((g.gate + 256) * g.b.sr * 2 >= (1LL << 31)) return SD_ERR_UNSUPPORTED;
   f.ragged = g.M % BS != 0 || g.gate % 32 != 0 || g.K % BS != 0;
-  const int policy = tile_policy.load(std::memory_order_relaxed);
-  const double kept = planned_kept(g);
-  int shape = -1;
-  double t_best = 1e30;
-  for (int s = kShapeOne; s <= kShapeBig; ++s) {
-    if ((policy == kTileBig && s != kShapeBig) || (policy == kTileMid && s != kShapeQuad && s != kShapeWide)) continue;
-    if (blocks_of(g.K) > (s == kShapeBig ? MAX_STEPS : kTileMaxSteps)) continue;
-    const double t = dsd_work(true, s, g.M, g.N, g.K, 1, kept, g.act == SD_ACT_RELU ? SD_ACT_RELU : SD_ACT_GELU).time();
-    if (t < t_best) {
-      t_best = t;
-      shape = s;
-    }
-  }
+  const int shape = plan_gated(g.M, g.N, g.K, planned_kept(g), g.act).first;
   if (shape < 0) return SD_ERR_UNSUPPORTED;
   int rc;
   if (shape != kShapeBig)

@@ -784,6 +784,14 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
     };
     if (M == 0) {
       y = new_matrix(x, 0, N);
+    } else if (!rec && !drops(0) && !drops(1) && row_major(wi) && row_major(wo) && sd_gated_mlp_few_taken(M, x.size(1), F, N)) {
+      const Tensor rows = row_major(x) ? x : x.contiguous();
+      y = new_matrix(x, M, N);
+      const Scratch ws(x, sd_gated_mlp_few_workspace_bytes(M, F));
+      const Mat xm(rows), im(wi), om(wo);
+      c10::DeviceGuard device(x.device());
+      check(sd_gated_mlp_few(xm.ptr, xm.sr, im.ptr, im.sr, om.ptr, om.sr, y.data_ptr(), N, M, x.size(1), F, N, act, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
+            "sd_gated_mlp_few");
     } else {
       if (drops(0)) layer_lists(x, M, x.size(1), bs, ps[0], draw(0), lists[0]);
       h = gated_forward(x, wi, F, act, ps[0], lists[0], rec, pre);

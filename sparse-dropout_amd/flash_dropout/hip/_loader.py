@@ -145,6 +145,10 @@ SIGNATURES = {
     "sd_gated_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
     "sd_gated_matmul": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float,
                                 c_int, c_int, c_void_p]),
+    "sd_gated_mlp_few_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "sd_gated_mlp_few_taken": (c_int, [c_int64] * 4),
+    "sd_gated_mlp_few": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
+                                 c_void_p, c_int64, c_void_p]),
     "sd_gated_matmul_gradient": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                          c_float, c_float, c_int, c_int, c_void_p]),
     "sd_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
