@@ -710,22 +710,40 @@ int sd_clip_grads(int count, void* const* grads, const int64_t* numels, const in
 /* ---------------------------------------------------------------------------------------------
  * (i) a gated feed-forward block's hidden activations
  *
- * A[M, 2F] = [G | U] (pitch lda), both projections' results beside one another; act: relu, gelu or silu.
+ * A[M, ..] = [G | U] (pitch lda): both projections' results, F columns each, U's `up` columns behind G's; act: relu, gelu or silu.
  * sd_gated_forward:  H = act(G) U                        (H [M, F], pitch ldh)
- * sd_gated_backward: dA = [dH U act'(G) | dH act(G)]     (dH [M, F], pitch ldd; dA [M, 2F], pitch ldda; dA may be A)
+ * sd_gated_backward: dA = [dH U act'(G) | dH act(G)]     (dH [M, F], pitch ldd; dA [M, 2F], pitch ldda, side by side)
  *   where dH is 0 both gradients are 0, whatever stands in A: what was dropped has none.
- * Computed in fp32, rounded once.
+ * Computed in fp32, rounded once.  h_cols, da_cols (here and below): the columns behind the last, up to these, are filled with zeros, at most up to the
+ * next multiple of 8: H and dA are the next product's operands, whose reduction comes in 16 bytes.
  *
- * The products with the gate in their store; SD_ERR_UNSUPPORTED with nothing launched where none of the specialised kernels takes the
- * operands (the caller then takes the product and the gate apart):
+ * The products with the gate in their store; SD_ERR_UNSUPPORTED where none of the specialised kernels takes the operands, with nothing launched but
+ * the lists of sd_gated_dropout_matmul_forward (the caller then takes the product and the gate apart):
  * sd_gated_matmul: [G | U] = scale * sum over kept blocks of X (W_in)^T, H = act(G) U; W_in [2F, K], the gate's rows first.  A (NULL:
  *   not wanted) receives [G | U] rounded, H is computed from the fp32 sums.  row_ptr / col_idx: kept blocks of X, NULL for all.
+ * sd_gated_dropout_matmul_forward: the same with X's mask, given or drawn, and its lists as in sd_dropout_matmul_forward, in one launch for small
+ *   products.
  * sd_gated_matmul_gradient: dH = scale * (dY W_out) where kept, which is rounded nowhere, and dA as above; dropped blocks of both halves are
- *   zeros.  dY [M, N], W_out [N, F]; lists over dH's blocks, NULL for all; keep_hint as in sd_gemm_sdd_lists_ex.
+ *   zeros.  dY [M, N], W_out [N, F]; lists over dH's blocks, NULL for all, scale = 1 / (1 - p) with them.  dW (NULL: not wanted) receives scale * dY^T
+ *   (keep . H) [N, F], in the same launch for small products; workspace: sd_splitk_workspace_bytes(F, N, M, ..), optional.
  * ------------------------------------------------------------------------------------------- */
+int sd_gated_forward(const void* A, int64_t lda, int64_t up, void* H, int64_t ldh, int64_t h_cols, int64_t M, int64_t F, int act, int dtype,
+                     void* stream);
+int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, int64_t up, void* dA, int64_t ldda, int64_t da_cols, int64_t M,
+                      int64_t F, int act, int dtype, void* stream);
 int sd_gated_matmul(const void* X, int64_t x_stride_r, int64_t x_stride_c, const void* W_in, int64_t w_stride_r, int64_t w_stride_c,
-                    void* H, int64_t ldh, void* A, int64_t lda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F,
-                    int64_t K, int64_t block_size, float scale, int act, int dtype, void* stream);
+                    void* H, int64_t ldh, int64_t h_cols, void* A, int64_t lda, int64_t up, const int32_t* row_ptr, const int32_t* col_idx,
+                    int64_t M, int64_t F, int64_t K, int64_t block_size, float scale, int act, int dtype, void* stream);
+int sd_gated_dropout_matmul_forward(const void* X, int64_t x_stride_r, int64_t x_stride_c, const void* W_in, int64_t w_stride_r,
+                                    int64_t w_stride_c, void* H, int64_t ldh, int64_t h_cols, void* A, int64_t lda, int64_t up,
+                                    const uint8_t* mask, int64_t mask_stride_r, int64_t mask_stride_c, uint64_t* rng_state, uint64_t seed,
+                                    uint64_t offset, double p, uint8_t* mask_out, int32_t* row_ptr, int32_t* col_idx, int32_t* col_ptr,
+                                    int32_t* row_idx, int64_t M, int64_t F, int64_t K, int64_t block_size, int act, int dtype, void* stream);
+int sd_gated_matmul_gradient(const void* dY, int64_t dy_stride_r, int64_t dy_stride_c, const void* W_out, int64_t w_stride_r,
+                             int64_t w_stride_c, const void* A, int64_t lda, int64_t up, void* dA, int64_t ldda, int64_t da_cols, const void* H,
+                             int64_t h_stride_r, int64_t h_stride_c, void* dW, int64_t dw_stride_r, int64_t dw_stride_c, const int32_t* row_ptr,
+                             const int32_t* col_idx, const int32_t* col_ptr, const int32_t* row_idx, int64_t M, int64_t F, int64_t N,
+                             int64_t block_size, double p, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 /* sd_gated_mlp_few: Y = (act(X W_g^T) (X W_u^T)) W_out^T for up to SD_GATED_FEW_ROWS rows in two launches that read each weight once; everything
  * row-major, rows of any pitch at any address.  Up to 8 rows keep the hidden activations to twice 16 bits, more round them to the operands' type.
  * workspace: sd_gated_mlp_few_workspace_bytes bytes on 16 bytes, of one call at a time.  sd_gated_mlp_few_taken: whether that is expected to be faster
@@ -735,13 +753,6 @@ int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F);
 int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N);
 int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi, const void* W_out, int64_t ldwo, void* Y, int64_t ldy,
                      int64_t M, int64_t K, int64_t F, int64_t N, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
-int sd_gated_matmul_gradient(const void* dY, int64_t dy_stride_r, int64_t dy_stride_c, const void* W_out, int64_t w_stride_r,
-                             int64_t w_stride_c, const void* A, int64_t lda, void* dA, int64_t ldda, const int32_t* row_ptr,
-                             const int32_t* col_idx, int64_t M, int64_t F, int64_t N, int64_t block_size, float scale, float keep_hint,
-                             int act, int dtype, void* stream);
-int sd_gated_forward(const void* A, int64_t lda, void* H, int64_t ldh, int64_t M, int64_t F, int act, int dtype, void* stream);
-int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, void* dA, int64_t ldda, int64_t M, int64_t F, int act,
-                      int dtype, void* stream);
 
 #ifdef __cplusplus
 }

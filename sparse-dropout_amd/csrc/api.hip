@@ -136,7 +136,7 @@ GemmArgs make_args(const void* A, int64_t asr, int64_t asc, const void* B, int64
   g.act = SD_ACT_NONE;
   g.aux = nullptr;
   g.aux_sr = g.aux_sc = 0;
-  g.gate = 0;
+  g.gate = g.aux_up = g.c_up = g.c_cols = 0;
   return g;
 }
 
@@ -869,53 +869,131 @@ int sd_conv2d_dw_lists(const void* x, int64_t sn, int64_t sc, int64_t sh, int64_
   return rc;
 }
 
-static int check_gated(const char* name, int64_t F, int act, const void* A, int64_t lda, int64_t M, const int32_t* row_ptr, const int32_t* col_idx,
-                       int64_t bs, float scale) {
+static int check_gated(const char* name, int64_t F, int act, const void* A, int64_t lda, int64_t up, int64_t M, const int32_t* row_ptr,
+                       const int32_t* col_idx, int64_t bs, float scale) {
   SD_REQUIRE(F >= 0 && F < kMaxDim / 2, "%s: hidden width out of range", name);
   SD_REQUIRE(act == SD_ACT_RELU || act == SD_ACT_GELU || act == SD_ACT_SILU, "%s: act must be SD_ACT_RELU, SD_ACT_GELU or SD_ACT_SILU (got %d)", name, act);
-  SD_REQUIRE(!A || M <= 1 || lda >= 2 * F, "%s: pitch %lld of 2 x %lld columns", name, (long long)lda, (long long)F);
+  SD_REQUIRE(!A || up >= F, "%s: U begins %lld columns behind G's %lld", name, (long long)up, (long long)F);
+  SD_REQUIRE(!A || M <= 1 || lda >= up + F, "%s: pitch %lld of [G | U], %lld columns", name, (long long)lda, (long long)(up + F));
   SD_REQUIRE((row_ptr == nullptr) == (col_idx == nullptr), "%s: row_ptr and col_idx must both be given or both be null", name);
   SD_REQUIRE(scale == scale, "%s: scale is NaN", name);
   return row_ptr ? check_sparse(bs, scale) : SD_OK;
 }
-
-int sd_gated_matmul(const void* X, int64_t xsr, int64_t xsc, const void* W_in, int64_t wsr, int64_t wsc, void* H, int64_t ldh, void* A,
-                    int64_t lda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t K, int64_t bs, float scale,
-                    int act, int dtype, void* stream) {
-  if (int rc = check_gated("gated_matmul", F, act, A, lda, M, row_ptr, col_idx, bs, scale)) return rc;
-  if (int rc = check_common(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, dtype)) return rc;
-  if (int rc = check_mat("W_in", W_in, wsr, wsc, 2 * F, K)) return rc;
-  if (M == 0 || F == 0) return SD_OK;
-  if (generic_forced() || K == 0) return SD_ERR_UNSUPPORTED;
-  GemmArgs g = make_args(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, row_ptr ? bs : 0, scale, row_ptr, col_idx);
+static int check_filled(const char* name, int64_t cols, int64_t filled, int64_t ld, int64_t M) {
+  SD_REQUIRE(filled >= cols && filled <= (cols + 7) / 8 * 8, "%s: columns %lld to %lld are to be zeros; up to the next multiple of 8 can be", name, (long long)cols,
+             (long long)filled);
+  SD_REQUIRE(M <= 1 || ld >= filled, "%s: pitch %lld of %lld columns", name, (long long)ld, (long long)filled);
+  return SD_OK;
+}
+static GemmArgs gated_args(const void* X, int64_t xsr, int64_t xsc, const void* W_in, int64_t wsr, int64_t wsc, void* H, int64_t ldh, int64_t h_cols,
+                           void* A, int64_t lda, int64_t up, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t K, int64_t bs,
+                           float scale, int act) {
+  GemmArgs g = make_args(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, 2 * F, K, row_ptr ? bs : 0, scale, row_ptr, col_idx);
   g.act = act;
   g.aux = static_cast<uint16_t*>(A);
   g.aux_sr = lda;
   g.aux_sc = 1;
   g.gate = F;
-  const int rc = launch_gated(g, dtype, (hipStream_t)stream);
+  g.aux_up = up;
+  g.c_cols = h_cols;
+  return g;
+}
+
+int sd_gated_matmul(const void* X, int64_t xsr, int64_t xsc, const void* W_in, int64_t wsr, int64_t wsc, void* H, int64_t ldh, int64_t h_cols,
+                    void* A, int64_t lda, int64_t up, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t K, int64_t bs,
+                    float scale, int act, int dtype, void* stream) {
+  if (int rc = check_gated("gated_matmul", F, act, A, lda, up, M, row_ptr, col_idx, bs, scale)) return rc;
+  if (int rc = check_common(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, dtype)) return rc;
+  if (int rc = check_mat("W_in", W_in, wsr, wsc, 2 * F, K)) return rc;
+  if (int rc = check_filled("gated_matmul", F, h_cols, ldh, M)) return rc;
+  if (M == 0 || F == 0) return SD_OK;
+  if (generic_forced() || K == 0) return SD_ERR_UNSUPPORTED;
+  const int rc = launch_gated(gated_args(X, xsr, xsc, W_in, wsr, wsc, H, ldh, h_cols, A, lda, up, row_ptr, col_idx, M, F, K, bs, scale, act), dtype,
+                              (hipStream_t)stream);
+  if (rc == SD_OK) last_kernel = "specialised";
+  return rc;
+}
+
+int sd_gated_dropout_matmul_forward(const void* X, int64_t xsr, int64_t xsc, const void* W_in, int64_t wsr, int64_t wsc, void* H, int64_t ldh,
+                                    int64_t h_cols, void* A, int64_t lda, int64_t up, const uint8_t* mask, int64_t msr, int64_t msc,
+                                    uint64_t* rng_state, uint64_t seed, uint64_t offset, double p, uint8_t* mask_out, int32_t* row_ptr,
+                                    int32_t* col_idx, int32_t* col_ptr, int32_t* row_idx, int64_t M, int64_t F, int64_t K, int64_t bs, int act, int dtype,
+                                    void* stream) {
+  const char* name = "gated_dropout_matmul_forward";
+  SD_REQUIRE(p >= 0.f && p < 1.f, "%s: p must be in [0, 1) (got %g)", name, p);
+  if (int rc = check_sparse(bs, 1.f)) return rc;
+  SD_REQUIRE(row_ptr && col_idx, "%s: the CSR list arrays are required", name);
+  const float scale = (float)(1.0 / (1.0 - p));  // in double, as the reference's Python evaluates it
+  if (int rc = check_gated(name, F, act, A, lda, up, M, row_ptr, col_idx, bs, scale)) return rc;
+  if (int rc = check_common(X, xsr, xsc, W_in, wsr, wsc, H, ldh, 1, M, F, K, dtype)) return rc;
+  if (int rc = check_mat("W_in", W_in, wsr, wsc, 2 * F, K)) return rc;
+  if (int rc = check_filled(name, F, h_cols, ldh, M)) return rc;
+  SD_REQUIRE(M > 0 && K > 0, "%s: empty operand", name);
+  const int64_t g = list_granule(bs), split = list_split(bs);
+  const int64_t mb = ceil_div(M, bs), kb = ceil_div(K, bs), out_mb = ceil_div(M, g), out_kb = ceil_div(K, g);
+  if (int rc = check_list_grid(mb, kb, split, out_mb, out_kb, row_ptr, col_idx, col_ptr, row_idx)) return rc;
+  if (mask) {
+    SD_REQUIRE(msr >= 1 && msc >= 1 && (msr == 1 || msc == 1), "build_lists: mask must be row or column major");
+  } else {
+    SD_REQUIRE(mask_out != nullptr, "random_lists: null mask_out");
+    SD_REQUIRE(rng_state == nullptr || reinterpret_cast<uintptr_t>(rng_state) % 8 == 0, "random_lists: state must be an aligned device pointer");
+  }
+  const GemmArgs a = gated_args(X, xsr, xsc, W_in, wsr, wsc, H, ldh, h_cols, A, lda, up, row_ptr, col_idx, M, F, K, lists_block_size(bs), scale, act);
+  if (F > 0 && !generic_forced() && !separate_forward_forced()) {
+    const int rc = forward_with_lists(a, mask, msr, msc, seed, offset, rng_state, (float)p, mb, kb, mask_out, split, out_mb, out_kb, row_ptr, col_idx, col_ptr,
+                                      row_idx, dtype, (hipStream_t)stream);
+    if (rc != SD_ERR_UNSUPPORTED) {
+      last_kernel = "specialised";
+      return rc;
+    }
+  }
+  int rc;
+  if (mask) rc = sd_build_lists_split(mask, mb, kb, msr, msc, split, out_mb, out_kb, row_ptr, col_idx, col_ptr, row_idx, stream);
+  else if (rng_state) rc = sd_random_lists_state(rng_state, (float)p, mb, kb, mask_out, split, out_mb, out_kb, row_ptr, col_idx, col_ptr, row_idx, stream);
+  else rc = sd_random_lists(seed, offset, (float)p, mb, kb, mask_out, split, out_mb, out_kb, row_ptr, col_idx, col_ptr, row_idx, stream);
+  if (rc || F == 0) return rc;
+  if (generic_forced()) return SD_ERR_UNSUPPORTED;
+  rc = launch_gated(a, dtype, (hipStream_t)stream);
   if (rc == SD_OK) last_kernel = "specialised";
   return rc;
 }
 
 int sd_gated_matmul_gradient(const void* dY, int64_t gsr, int64_t gsc, const void* W_out, int64_t wsr, int64_t wsc, const void* A, int64_t lda,
-                             void* dA, int64_t ldda, const int32_t* row_ptr, const int32_t* col_idx, int64_t M, int64_t F, int64_t N,
-                             int64_t bs, float scale, float keep_hint, int act, int dtype, void* stream) {
-  if (int rc = check_gated("gated_matmul_gradient", F, act, A, lda, M, row_ptr, col_idx, bs, scale)) return rc;
+                             int64_t up, void* dA, int64_t ldda, int64_t da_cols, const void* H, int64_t hsr, int64_t hsc, void* dW, int64_t dwsr,
+                             int64_t dwsc, const int32_t* row_ptr, const int32_t* col_idx, const int32_t* col_ptr, const int32_t* row_idx, int64_t M, int64_t F,
+                             int64_t N, int64_t bs, double p, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "gated_matmul_gradient";
+  SD_REQUIRE(p >= 0.f && p < 1.f, "%s: p must be in [0, 1) (got %g)", name, p);
+  const float scale = row_ptr ? (float)(1.0 / (1.0 - p)) : 1.f;
+  if (int rc = check_gated(name, F, act, A, lda, up, M, row_ptr, col_idx, bs, scale)) return rc;
   if (int rc = check_common(dY, gsr, gsc, W_out, wsc, wsr, dA, ldda, 1, M, F, N, dtype)) return rc;
-  SD_REQUIRE(M <= 1 || ldda >= 2 * F, "gated_matmul_gradient: pitch %lld of 2 x %lld columns", (long long)ldda, (long long)F);
-  SD_REQUIRE(!(keep_hint > 1.f), "gated_matmul_gradient: keep_hint must be a fraction in [0, 1], or negative for unknown");
+  if (int rc = check_filled(name, 2 * F, da_cols, ldda, M)) return rc;
+  SD_REQUIRE((col_ptr == nullptr) == (row_idx == nullptr), "%s: col_ptr and row_idx must both be given or both be null", name);
+  SD_REQUIRE(!dW || (row_ptr == nullptr) == (col_ptr == nullptr), "%s: dW needs the CSC lists where there are CSR lists", name);
+  if (dW) {
+    if (int rc = check_common(H, hsc, hsr, dY, gsc, gsr, dW, dwsc, dwsr, F, N, M, dtype)) return rc;
+  }
   if (M == 0 || F == 0) return SD_OK;
-  SD_REQUIRE(A != nullptr, "gated_matmul_gradient: null [G | U]");
+  SD_REQUIRE(A != nullptr, "%s: null [G | U]", name);
   if (generic_forced() || N == 0) return SD_ERR_UNSUPPORTED;
-  GemmArgs g = make_args(dY, gsr, gsc, W_out, wsc, wsr, dA, ldda, 1, M, F, N, row_ptr ? bs : 0, scale, row_ptr, col_idx);
-  g.keep_hint = keep_hint == keep_hint ? keep_hint : -1.f;
+  GemmArgs g = make_args(dY, gsr, gsc, W_out, wsc, wsr, dA, ldda, 1, M, F, N, row_ptr ? lists_block_size(bs) : 0, scale, row_ptr, col_idx);
+  g.keep_hint = row_ptr ? (float)(1.0 - p) : -1.f;
   g.act = act;
   g.aux = const_cast<uint16_t*>(static_cast<const uint16_t*>(A));
   g.aux_sr = lda;
   g.aux_sc = 1;
-  g.gate = F;
-  const int rc = launch_gated_gradient(g, dtype, (hipStream_t)stream);
+  g.gate = g.c_up = F;
+  g.aux_up = up;
+  g.c_cols = da_cols;
+  GemmArgs gw = dW ? make_args(H, hsc, hsr, dY, gsc, gsr, dW, dwsc, dwsr, F, N, M, row_ptr ? lists_block_size(bs) : 0, scale, col_ptr, row_idx, workspace,
+                               workspace_bytes)
+                   : g;
+  int rc = SD_ERR_UNSUPPORTED;
+  if (dW && row_ptr && !separate_backward_forced()) rc = launch_backward_pair(g, gw, dtype, (hipStream_t)stream);
+  if (rc == SD_ERR_UNSUPPORTED) {
+    rc = launch_gated_gradient(g, dtype, (hipStream_t)stream);
+    if (rc == SD_OK && dW) rc = run(gw, row_ptr ? kDsd : kDense, dtype, (hipStream_t)stream);
+  }
   if (rc == SD_OK) last_kernel = "specialised";
   return rc;
 }

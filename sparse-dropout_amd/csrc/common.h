@@ -131,8 +131,9 @@ struct GemmArgs {
   int act;
   uint16_t* aux;
   int64_t aux_sr, aux_sc;
-  // F, a gated block's hidden width (gated.h), in the instances that are built for it; nobody else looks at it
-  int64_t gate;
+  // A gated block's (gated.h), in the instances that are built for it; nobody else looks at them: the hidden width F, how far behind the gate's
+  // columns the other projection's begin in aux and (gradients) in c, and up to which column behind the last c is filled with zeros
+  int64_t gate, aux_up, c_up, c_cols;
 };
 
 // SDD: the fraction of blocks expected to be kept (unknown counts as everything), and of the 64-blocks: one of a mask of
@@ -423,9 +424,9 @@ int launch_conv_dx(const void* dy, int64_t dy_ld, const void* w, int64_t w_ld, v
 bool conv_dx_taken(const void* dy, int64_t dy_ld, const void* w, int64_t w_ld, int64_t n, int64_t c, int64_t h, int64_t wd, int64_t k_out,
                    int64_t r, int64_t s, int64_t pad_h, int64_t pad_w, int64_t stride_h, int64_t stride_w, int64_t dil_h, int64_t dil_w);
 // Products with a gate in their store (gated.h); SD_ERR_UNSUPPORTED (without a message) where no specialised kernel takes them.
-// g.b: [2 F, K], g.c: H, g.aux: [G | U] or null, g.gate: F; g.N is not looked at
+// g.b: [2 F, K], g.c: H, g.aux: [G | U] or null; g.N is not looked at
 int launch_gated(const GemmArgs& g, int dtype, hipStream_t stream);
-// an SDD (or dense) product dH that leaves [dG | dU] in g.c, g.aux: [G | U], g.N == g.gate
+// an SDD (or dense) product dH that leaves [dG | dU] in g.c, g.aux: [G | U], g.N == g.gate; launch_backward_pair takes it as gx too
 int launch_gated_gradient(const GemmArgs& g, int dtype, hipStream_t stream);
 // What a dense product, and one with a gate in its store (F hidden columns), is expected to take in tiles, us.
 double dense_expected_us(int64_t M, int64_t N, int64_t K);

@@ -52,9 +52,12 @@ __device__ inline void unpack_eight(u32x4 w, float (&v)[8]) {
 // N hidden columns from column c of row m on, unscaled fp32 accumulators of both projections
 template <typename T, int N>
 __device__ inline void store_gate(const GemmArgs& g, int64_t m, int64_t c, float (&gate)[N], float (&up)[N]) {
-  if (m >= g.M || c >= g.gate) return;
+  if (m >= g.M || c >= g.c_cols) return;
   const int valid = g.gate - c < N ? (int)(g.gate - c) : N;
   uint16_t* h = g.c + m * g.c_sr + c;
+  if (valid < N)  // zeros behind the last column
+    for (int i = valid > 0 ? valid : 0; i < N && c + i < g.c_cols; ++i) h[i] = 0;
+  if (valid <= 0) return;
   float out[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -84,7 +87,7 @@ __device__ inline void store_gate(const GemmArgs& g, int64_t m, int64_t c, float
   if (g.aux) {
     uint16_t* a = g.aux + m * g.aux_sr + c;
     put(a, gate);
-    put(a + g.gate, up);
+    put(a + g.aux_up, up);
   }
   put(h, out);
 }
@@ -120,9 +123,13 @@ struct GateAt {
     if (m >= g.M || c + 8 > g.gate) return;
     const uint16_t* at = g.aux + m * g.aux_sr + c;
     gate = *reinterpret_cast<const u32x4_any*>(at);
-    up = *reinterpret_cast<const u32x4_any*>(at + g.gate);
+    up = *reinterpret_cast<const u32x4_any*>(at + g.aux_up);
   }
 };
+// zeros behind both gradients of row m (where F is no multiple of 8)
+__device__ inline void fill_gradient(const GemmArgs& g, int64_t m) {
+  for (int64_t i = 2 * g.gate; i < g.c_cols; ++i) g.c[m * g.c_sr + i] = 0;
+}
 // eight of dh, unscaled fp32 accumulators.  What was dropped has no gradient, whatever stands in g and u.
 template <typename T>
 __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t c, float (&dh)[8], const GateAt& pre) {
@@ -138,7 +145,7 @@ __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       gate[i] = i < valid ? T::to_float(at[i]) : 0.f;
-      up[i] = i < valid ? T::to_float(at[g.gate + i]) : 0.f;
+      up[i] = i < valid ? T::to_float(at[g.aux_up + i]) : 0.f;
     }
   }
   auto apply = [&](int act) {
@@ -156,14 +163,15 @@ __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t
   else apply(SD_ACT_RELU);
   if (valid == 8) {
     *reinterpret_cast<u32x4_any*>(out) = pack_eight<T>(gate);
-    *reinterpret_cast<u32x4_any*>(out + g.gate) = pack_eight<T>(up);
+    *reinterpret_cast<u32x4_any*>(out + g.c_up) = pack_eight<T>(up);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < valid) {
         out[i] = T::from_float(gate[i]);
-        out[g.gate + i] = T::from_float(up[i]);
+        out[g.c_up + i] = T::from_float(up[i]);
       }
+    fill_gradient(g, m);
   }
 }
 // a wave's 64 x 64 tile of dh staged in LDS with a pitch of 68 floats

@@ -14,8 +14,8 @@ constexpr int kThreads = 256;
 struct Gate {
   const uint16_t *dh, *a;
   uint16_t* out;
-  int64_t ldd, lda, ldo, M, F;
-  int64_t eights;  // of a row
+  int64_t ldd, lda, up, ldo, M, F, cols;  // cols: of out, zeros behind the last
+  int64_t eights;                         // of a row
 };
 
 struct Eight {
@@ -42,6 +42,10 @@ struct Eight {
     }
   }
 };
+// zeros from column `from` of a row up to the last that is to be filled
+__device__ inline void fill_row(uint16_t* row, int64_t from, int64_t cols) {
+  for (int64_t i = from; i < cols; ++i) row[i] = 0;
+}
 
 template <typename T, int ACT, bool BACKWARD>
 __global__ __launch_bounds__(kThreads) void gate_kernel(Gate g) {
@@ -51,11 +55,12 @@ __global__ __launch_bounds__(kThreads) void gate_kernel(Gate g) {
     const int left = g.F - c < 8 ? (int)(g.F - c) : 8;
     Eight gate, up;
     gate.load<T>(g.a + m * g.lda + c, left);
-    up.load<T>(g.a + m * g.lda + g.F + c, left);
+    up.load<T>(g.a + m * g.lda + g.up + c, left);
     if constexpr (!BACKWARD) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) gate.v[e] = gate_value(ACT, gate.v[e]) * up.v[e];
       gate.store<T>(g.out + m * g.ldo + c, left);
+      if (c + 8 >= g.F) fill_row(g.out + m * g.ldo, g.F, g.cols);
     } else {
       Eight d;
       d.load<T>(g.dh + m * g.ldd + c, left);
@@ -68,6 +73,7 @@ __global__ __launch_bounds__(kThreads) void gate_kernel(Gate g) {
       }
       gate.store<T>(g.out + m * g.ldo + c, left);
       up.store<T>(g.out + m * g.ldo + g.F + c, left);
+      if (c + 8 >= g.F) fill_row(g.out + m * g.ldo, 2 * g.F, g.cols);
     }
   }
 }
@@ -81,12 +87,15 @@ int launch_gate(const Gate& g, int act, hipStream_t stream) {
   return check_launch("gate_kernel");
 }
 
-int check_gate(const char* name, const void* a, int64_t lda, int64_t M, int64_t F, int act, int dtype) {
+int check_gate(const char* name, const void* a, int64_t lda, int64_t up, const void* out, int64_t ldo, int64_t wide, int64_t cols, int64_t M, int64_t F, int act,
+               int dtype) {
   SD_REQUIRE(M >= 0 && F >= 0 && M < (1LL << 31) && F < (1LL << 30), "%s: bad extents %lld x %lld", name, (long long)M, (long long)F);
   SD_REQUIRE(dtype == SD_F16 || dtype == SD_BF16, "%s: dtype must be SD_F16 or SD_BF16 (got %d)", name, dtype);
   SD_REQUIRE(act == SD_ACT_RELU || act == SD_ACT_GELU || act == SD_ACT_SILU, "%s: act must be SD_ACT_RELU, SD_ACT_GELU or SD_ACT_SILU (got %d)", name, act);
-  SD_REQUIRE(M == 0 || F == 0 || a, "%s: null pointer", name);
-  SD_REQUIRE(M <= 1 || lda >= 2 * F, "%s: pitch %lld of 2 x %lld columns", name, (long long)lda, (long long)F);
+  SD_REQUIRE(M == 0 || F == 0 || (a && out), "%s: null pointer", name);
+  SD_REQUIRE(up >= F && (M <= 1 || lda >= up + F), "%s: U begins %lld columns behind G's %lld, at a pitch of %lld", name, (long long)up, (long long)F, (long long)lda);
+  SD_REQUIRE(cols >= wide && cols <= (wide + 7) / 8 * 8 && (M <= 1 || ldo >= cols), "%s: a result of %lld columns, zeros up to %lld, at a pitch of %lld", name, (long long)wide,
+             (long long)cols, (long long)ldo);
   return SD_OK;
 }
 
@@ -97,21 +106,19 @@ using namespace sd;
 
 extern "C" {
 
-int sd_gated_forward(const void* A, int64_t lda, void* H, int64_t ldh, int64_t M, int64_t F, int act, int dtype, void* stream) {
-  if (int rc = check_gate("gated_forward", A, lda, M, F, act, dtype)) return rc;
+int sd_gated_forward(const void* A, int64_t lda, int64_t up, void* H, int64_t ldh, int64_t h_cols, int64_t M, int64_t F, int act, int dtype, void* stream) {
+  if (int rc = check_gate("gated_forward", A, lda, up, H, ldh, F, h_cols, M, F, act, dtype)) return rc;
   if (M == 0 || F == 0) return SD_OK;
-  SD_REQUIRE(H && (M == 1 || ldh >= F), "gated_forward: null result, or its pitch %lld of %lld columns", (long long)ldh, (long long)F);
-  Gate g = {nullptr, static_cast<const uint16_t*>(A), static_cast<uint16_t*>(H), 0, lda, ldh, M, F, ceil_div(F, 8)};
+  Gate g = {nullptr, static_cast<const uint16_t*>(A), static_cast<uint16_t*>(H), 0, lda, up, ldh, M, F, h_cols, ceil_div(F, 8)};
   return dtype == SD_BF16 ? launch_gate<BF16, false>(g, act, (hipStream_t)stream) : launch_gate<F16, false>(g, act, (hipStream_t)stream);
 }
 
-int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, void* dA, int64_t ldda, int64_t M, int64_t F, int act, int dtype,
-                      void* stream) {
-  if (int rc = check_gate("gated_backward", A, lda, M, F, act, dtype)) return rc;
+int sd_gated_backward(const void* dH, int64_t ldd, const void* A, int64_t lda, int64_t up, void* dA, int64_t ldda, int64_t da_cols, int64_t M, int64_t F,
+                      int act, int dtype, void* stream) {
+  if (int rc = check_gate("gated_backward", A, lda, up, dA, ldda, 2 * F, da_cols, M, F, act, dtype)) return rc;
   if (M == 0 || F == 0) return SD_OK;
   SD_REQUIRE(dH && (M == 1 || ldd >= F), "gated_backward: null gradient, or its pitch %lld of %lld columns", (long long)ldd, (long long)F);
-  SD_REQUIRE(dA && (M == 1 || ldda >= 2 * F), "gated_backward: null result, or its pitch %lld of 2 x %lld columns", (long long)ldda, (long long)F);
-  Gate g = {static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(A), static_cast<uint16_t*>(dA), ldd, lda, ldda, M, F, ceil_div(F, 8)};
+  Gate g = {static_cast<const uint16_t*>(dH), static_cast<const uint16_t*>(A), static_cast<uint16_t*>(dA), ldd, lda, up, ldda, M, F, da_cols, ceil_div(F, 8)};
   return dtype == SD_BF16 ? launch_gate<BF16, true>(g, act, (hipStream_t)stream) : launch_gate<F16, true>(g, act, (hipStream_t)stream);
 }
 

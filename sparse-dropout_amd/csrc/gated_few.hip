@@ -219,7 +219,7 @@ int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N) {
   if (M <= 16) return 1;
   // Rows that do not begin on 16 bytes are copied first on the other way: weights and activations at 3 TB/s, a launch each
   const double copied = (K % 8 ? 4.0 + 8.0 * F * K / 3e6 : 0.0) + (F % 8 ? 4.0 + 4.0 * N * F / 3e6 : 0.0);
-  return few_us(M, F, K, 2) + few_us(M, N, F, 1) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
+  return 1.1 * (few_us(M, F, K, 2) + few_us(M, N, F, 1)) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
 }
 
 int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi, const void* W_out, int64_t ldwo, void* Y, int64_t ldy, int64_t M,

@@ -1207,7 +1207,7 @@ __device__ inline void zero_dropped(const GemmArgs& g, const uint32_t* flags, co
       if (!((f >> r) & 1u) && (int64_t)(rb0 + r) * BS + row < g.M && (!EDGE || (int64_t)c * BS + ch * 8 < g.N)) {
         u32x4* at = reinterpret_cast<u32x4*>(g.c + ((int64_t)(rb0 + r) * BS + row) * g.c_sr + (int64_t)c * BS + ch * 8);
         *at = z;
-        if (GATED) at[g.gate / 8] = z;
+        if (GATED) at[g.c_up / 8] = z;
       }
     }
   }
@@ -2270,15 +2270,21 @@ double dense_expected_us(int64_t M, int64_t N, int64_t K) {
   const DsdPlan plan = plan_dsd(M, N, K, true, 1.0, SD_ACT_NONE);
   return dsd_work(true, plan.shape, M, N, K, plan.splits, 1.0, SD_ACT_NONE).time();
 }
+// What the specialised kernels ask of its operands; g.N: gated_columns.
+DsdForm gated_form(const GemmArgs& g) {
+  DsdForm f = dsd_form(g);
+  // (rows of either projection are reached by one 32-bit offset)
+  f.ok = f.ok && f.kc && !f.cm && (!g.aux || g.aux_sc == 1) && (g.gate + 256) * g.b.sr * 2 < (1LL << 31);
+  f.ragged = g.M % BS != 0 || g.gate % 32 != 0 || g.K % BS != 0;
+  return f;
+}
+
 int launch_gated(const GemmArgs& g_, int dtype, hipStream_t stream) {
   GemmArgs g = g_;
   g.N = gated_columns(g.gate);
   if (g.row_ptr && g.bs != BS) return SD_ERR_UNSUPPORTED;
-  DsdForm f = dsd_form(g);
-  if (!f.ok || !f.kc || f.cm || (g.aux && g.aux_sc != 1)) return SD_ERR_UNSUPPORTED;
-  // rows of either projection are reached by one 32-bit offset
-  if ((g.gate + 256) * g.b.sr * 2 >= (1LL << 31)) return SD_ERR_UNSUPPORTED;
-  f.ragged = g.M % BS != 0 || g.gate % 32 != 0 || g.K % BS != 0;
+  const DsdForm f = gated_form(g);
+  if (!f.ok) return SD_ERR_UNSUPPORTED;
   const int shape = plan_gated(g.M, g.N, g.K, planned_kept(g), g.act).first;
   if (shape < 0) return SD_ERR_UNSUPPORTED;
   int rc;
@@ -2358,6 +2364,17 @@ int launch_forward_with_lists(const GemmArgs& g, const MaskSrc& src, int64_t mb,
                               int64_t mask_rows, int dtype, hipStream_t stream) {
   if (g.bs != BS || mb * kb > kFlatMaxEntries) return SD_ERR_UNSUPPORTED;
   if (mb != (g.M + BS - 1) / BS || kb != (g.K + BS - 1) / BS) return SD_ERR_UNSUPPORTED;
+  if (g.gate) {  // (the big shape's lists are a launch of their own, of 5 to 8 us beside 70 and more)
+    GemmArgs a = g;
+    a.N = gated_columns(g.gate);
+    const int shape = gated_form(a).ok ? plan_gated(a.M, a.N, a.K, planned_kept(a), a.act).first : -1;
+    if (shape < 0 || shape == kShapeBig) return SD_ERR_UNSUPPORTED;
+    FlatJobs f = flat_jobs(src, mb, kb, row_ptr, col_idx, col_ptr, row_idx, mask_out, mask_rows, tile_threads(shape));
+    f.tabled = mask_table_pays(src, shape, shape_tiles(shape, a.M, a.N));
+    const int rc = is_bf16(dtype) ? tile_gated_forward<BF16>(a, shape, f, stream) : tile_gated_forward<F16>(a, shape, f, stream);
+    if (rc == SD_OK) note_kernel("dsd+lists:%s:gated", dsd_name(shape));
+    return rc;
+  }
   const DsdForm form = dsd_form(g);
   if (!form.ok || !form.kc || form.cm) return SD_ERR_UNSUPPORTED;
   const DsdPlan plan = plan_for(g, form);
@@ -2436,6 +2453,7 @@ int launch_backward_pair(const GemmArgs& gx, const GemmArgs& gw, int dtype, hipS
   };
   const double apart = w_work(plan.shape).time() + sdd_work(x_alone, gx).time();
   if (big) {
+    if (gx.gate) return SD_ERR_UNSUPPORTED;  // (built for the tile shapes)
     if (!sdd_big_ok(gx) || (x_alone != kShapeBig && (blocks_of(gx.K) < 4 || pair_time(kShapeBig) > apart)) ||
         sdd_plan_groups(gx) > limit || shape_tiles(kShapeBig, gw.M, gw.N) * plan.splits > limit)
       return SD_ERR_UNSUPPORTED;
@@ -2463,10 +2481,13 @@ int launch_backward_pair(const GemmArgs& gx, const GemmArgs& gw, int dtype, hipS
     }
   }
   if (shape < 0) return SD_ERR_UNSUPPORTED;
-  const int rc = is_bf16(dtype) ? tile_pair<BF16>(gx, gw, shape, plan.splits, stream)
-                                : tile_pair<F16>(gx, gw, shape, plan.splits, stream);
+  int rc;
+  if (gx.gate)
+    rc = is_bf16(dtype) ? tile_gated_pair<BF16>(gx, gw, shape, plan.splits, stream) : tile_gated_pair<F16>(gx, gw, shape, plan.splits, stream);
+  else
+    rc = is_bf16(dtype) ? tile_pair<BF16>(gx, gw, shape, plan.splits, stream) : tile_pair<F16>(gx, gw, shape, plan.splits, stream);
   if (rc) return rc;
-  note_kernel("pair:sdd+dsd:%s splits=%d", dsd_name(shape), plan.splits);
+  note_kernel("pair:sdd+dsd:%s%s splits=%d", dsd_name(shape), gx.gate ? ":gated" : "", plan.splits);
   return plan.splits > 1 ? launch_splitk_reduce(gw, plan.splits, true, dtype, stream) : SD_OK;
 }
 

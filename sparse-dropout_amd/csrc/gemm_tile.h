@@ -594,8 +594,9 @@ __device__ __forceinline__ void tile_sdd_body(const GemmArgs& g, int sure, int M
           zero_tile<S::THREADS>(g, m0, (int64_t)(tn * C + c) * BS);
           if constexpr (GATED) {
             GemmArgs up = g;
-            up.c += g.gate;
+            up.c += g.c_up;
             zero_tile<S::THREADS>(up, m0, (int64_t)(tn * C + c) * BS);
+            if (tn * C + c == Cb - 1 && tid < BS && m0 + tid < g.M) fill_gradient(g, m0 + tid);
           }
         }
       __syncthreads();

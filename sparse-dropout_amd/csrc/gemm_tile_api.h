@@ -25,11 +25,15 @@ int tile_sdd(const GemmArgs& g, int shape, hipStream_t stream);
 template <typename T>
 int tile_pair(const GemmArgs& gx, const GemmArgs& gw, int shape, int splits, hipStream_t stream);
 
-// the same two with a gate in their store (gated.h): tile_dsd's forward and tile_sdd
+// the same with a gate in their store (gated.h): tile_dsd's forward, tile_forward, tile_sdd, tile_pair
 template <typename T>
 int tile_gated(const GemmArgs& g, int shape, hipStream_t stream);
 template <typename T>
+int tile_gated_forward(const GemmArgs& g, int shape, const FlatJobs& f, hipStream_t stream);
+template <typename T>
 int tile_gated_gradient(const GemmArgs& g, int shape, hipStream_t stream);
+template <typename T>
+int tile_gated_pair(const GemmArgs& gx, const GemmArgs& gw, int shape, int splits, hipStream_t stream);
 
 int tile_threads(int shape);  // of tile_forward's workgroups (what flat_jobs must be laid out for)
 

@@ -1,5 +1,5 @@
 // Launchers of the 64 x 64 ... 128 x 128 tile kernels for one element type; gemm_tile_f16.hip and gemm_tile_bf16.hip
-// compile one each.
+// compile one each, gemm_tile_gated_f16.hip and gemm_tile_gated_bf16.hip those with a gate in their store.
 #pragma once
 #include <algorithm>
 #include <atomic>
@@ -49,14 +49,14 @@ __global__ __launch_bounds__(S::THREADS, S::LW ? 1 : (GATED ? 2 : 3)) void tile_
 }
 
 // The forward product and the kept lists of its mask in one launch (see forward_lists_kernel of the large shapes).
-template <typename T, typename S, bool TABLED>
+template <typename T, typename S, bool TABLED, bool GATED = false>
 __global__ __launch_bounds__(S::THREADS) void tile_forward_kernel(GemmArgs g, int tiles_m, int tiles_n, int Mb, int Kb,
                                                                   int nsplit, int n_gemm, FlatJobs f) {
   const int bid = (int)blockIdx.x;
   if (bid < n_gemm) {
     MaskSrc ms = f.job0.src;
     ms.resolve();
-    tile_dsd_body<T, true, false, S, TABLED>(g, tiles_m, tiles_n, Mb, Kb, bid, nsplit, &ms);
+    tile_dsd_body<T, true, false, S, TABLED, GATED>(g, tiles_m, tiles_n, Mb, Kb, bid, nsplit, &ms);
   } else {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     static_assert(flat_lds(kTableEntriesMost) <= S::SMEM_STEPS, "the table lies where the stages would");
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(S::THREADS) void tile_forward_kernel(GemmArgs g, in
 
 // Both gradients in one launch: workgroups [0, n_first) are one product's, the rest the other's.  n_first is a multiple of 8, so
 // that the second product's tile map keeps its XCD assignment.  Which comes first: dw_before_dx.
-template <typename T, typename X, typename W>
+template <typename T, typename X, typename W, bool GATED = false>
 __global__ __launch_bounds__(W::THREADS) void tile_pair_kernel(GemmArgs gx, int x_tiles_n, int x_sure, int x_Mb, int x_Cb,
                                                                int n_first, bool dw_first, GemmArgs gw, int w_tiles_m,
                                                                int w_tiles_n, int w_Mb, int w_Kb, int w_splits) {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(W::THREADS) void tile_pair_kernel(GemmArgs gx, int 
   const bool second = bid >= n_first;
   const int i = second ? bid - n_first : bid;
   if (second == dw_first) {
-    if (i < x_tiles_n * x_Mb) tile_sdd_body<T, X>(gx, x_sure, x_Mb, x_Cb, i);
+    if (i < x_tiles_n * x_Mb) tile_sdd_body<T, X, GATED>(gx, x_sure, x_Mb, x_Cb, i);
   } else {
     if (i < w_tiles_m * w_tiles_n * w_splits) tile_dsd_body<T, false, true, W>(gw, w_tiles_m, w_tiles_n, w_Mb, w_Kb, i, w_splits);
   }
@@ -111,10 +111,10 @@ int dsd_launch(const GemmArgs& g, int splits, hipStream_t stream) {
   return check_launch("tile_dsd_kernel");
 }
 
-template <typename T, typename S, bool TABLED>
+template <typename T, typename S, bool TABLED, bool GATED = false>
 int forward_launch_t(const GemmArgs& g, int splits, const FlatJobs& f, hipStream_t stream) {
   static std::atomic<bool> done[64] = {};
-  auto* kernel = &tile_forward_kernel<T, S, TABLED>;
+  auto* kernel = &tile_forward_kernel<T, S, TABLED, GATED>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), S::SMEM, done)) return rc;
   const int Mb = blocks_of(g.M), Kb = blocks_of(g.K), tm = (Mb + S::R - 1) / S::R, tn = (blocks_of(g.N) + S::C - 1) / S::C;
   const int n_gemm = tm * tn * splits;
@@ -123,9 +123,9 @@ int forward_launch_t(const GemmArgs& g, int splits, const FlatJobs& f, hipStream
   return check_launch("tile_forward_kernel");
 }
 
-template <typename T, typename S>
+template <typename T, typename S, bool GATED = false>
 int forward_launch(const GemmArgs& g, int splits, const FlatJobs& f, hipStream_t stream) {
-  return f.tabled ? forward_launch_t<T, S, true>(g, splits, f, stream) : forward_launch_t<T, S, false>(g, splits, f, stream);
+  return f.tabled ? forward_launch_t<T, S, true, GATED>(g, splits, f, stream) : forward_launch_t<T, S, false, GATED>(g, splits, f, stream);
 }
 
 // Of the strips of C kept column blocks that a row of the block grid can have, `most`, those that all but one row in six have: the
@@ -152,11 +152,11 @@ int sdd_launch(const GemmArgs& g, hipStream_t stream) {
   return check_launch("tile_sdd_kernel");
 }
 
-template <typename T, typename X, typename W>
+template <typename T, typename X, typename W, bool GATED = false>
 int pair_launch(const GemmArgs& gx, const GemmArgs& gw, int splits, hipStream_t stream) {
   static std::atomic<bool> done[64] = {};
   constexpr int SMEM = X::SMEM > W::SMEM ? X::SMEM : W::SMEM;
-  auto* kernel = &tile_pair_kernel<T, X, W>;
+  auto* kernel = &tile_pair_kernel<T, X, W, GATED>;
   if (int rc = allow_lds(reinterpret_cast<const void*>(kernel), SMEM, done)) return rc;
   const int x_Mb = blocks_of(gx.M), x_Cb = blocks_of(gx.N), x_tn = (x_Cb + X::C - 1) / X::C;
   const int w_Mb = blocks_of(gw.M), w_Kb = blocks_of(gw.K), w_tm = (w_Mb + W::R - 1) / W::R, w_tn = (blocks_of(gw.N) + W::C - 1) / W::C;
@@ -197,6 +197,20 @@ int tile_gated(const GemmArgs& g, int shape, hipStream_t stream) {
 }
 
 template <typename T>
+int tile_gated_forward(const GemmArgs& g, int shape, const FlatJobs& f, hipStream_t stream) {
+  switch (shape) {
+    case kShapeOne: return more_than_resident(g, 1) ? forward_launch<T, FwdOneMany, true>(g, 1, f, stream) : forward_launch<T, FwdOne, true>(g, 1, f, stream);
+    case kShapeQuad: return forward_launch<T, FwdQuad, true>(g, 1, f, stream);
+    default: return forward_launch<T, FwdWide, true>(g, 1, f, stream);
+  }
+}
+
+template <typename T>
+int tile_gated_pair(const GemmArgs& gx, const GemmArgs& gw, int shape, int splits, hipStream_t stream) {
+  return shape == kShapeOne ? pair_launch<T, SddOne, GradOne, true>(gx, gw, splits, stream) : pair_launch<T, SddStrip, GradQuad, true>(gx, gw, splits, stream);
+}
+
+template <typename T>
 int tile_gated_gradient(const GemmArgs& g, int shape, hipStream_t stream) {
   switch (shape) {
     case kShapeOne: return sdd_launch<T, SddOne, true>(g, stream);
@@ -233,10 +247,14 @@ int tile_pair(const GemmArgs& gx, const GemmArgs& gw, int shape, int splits, hip
 
 #define SD_TILE_INSTANCES(T)                                                                    \
   template int tile_dsd<T>(const GemmArgs&, bool, bool, int, int, hipStream_t);                 \
-  template int tile_gated<T>(const GemmArgs&, int, hipStream_t);                                \
-  template int tile_gated_gradient<T>(const GemmArgs&, int, hipStream_t);                       \
   template int tile_forward<T>(const GemmArgs&, int, int, const FlatJobs&, hipStream_t);        \
   template int tile_sdd<T>(const GemmArgs&, int, hipStream_t);                                  \
   template int tile_pair<T>(const GemmArgs&, const GemmArgs&, int, int, hipStream_t);
+
+#define SD_TILE_GATED_INSTANCES(T)                                                              \
+  template int tile_gated<T>(const GemmArgs&, int, hipStream_t);                                \
+  template int tile_gated_forward<T>(const GemmArgs&, int, const FlatJobs&, hipStream_t);       \
+  template int tile_gated_gradient<T>(const GemmArgs&, int, hipStream_t);                       \
+  template int tile_gated_pair<T>(const GemmArgs&, const GemmArgs&, int, int, hipStream_t);
 
 }  // namespace sd

@@ -640,94 +640,113 @@ Tensor mlp(const Tensor& input, const std::vector<Tensor>& weights, int64_t bs, 
 
 // ---- a gated feed-forward block ------------------------------------------------------------------------------------------
 // (see functional/gated_mlp.py for what is computed)
-// Lists of a layer's mask, drawn here unless it is given, in a launch of their own.
-void layer_lists(const Tensor& x, int64_t rows, int64_t cols, int64_t bs, double p, const Draw& draw, Lists& l) {
-  check_p(p);
-  l.shape(rows, cols, bs);
-  TORCH_CHECK_NOT_IMPLEMENTED(bs % 32 == 0, "block_size ", bs, ": only multiples of 32 are supported");
-  l.allocate(x, draw.mask);
-  const int64_t split = bs % 64 == 32 ? -(bs / 32) : bs / 64;
-  c10::DeviceGuard guard(x.device());
-  if (draw.mask) {
-    const MaskArg m = l.mask();
-    check(sd_build_lists_split(m.ptr, l.mb, l.kb, m.sr, m.sc, split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(), l.row_idx(), stream_of(x)),
-          "sd_build_lists_split");
-  } else if (uint64_t* st = draw.state_ptr()) {
-    check(sd_random_lists_state(st, (float)p, l.mb, l.kb, l.drawn(), split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(), l.row_idx(),
-                                stream_of(x)),
-          "sd_random_lists_state");
-  } else {
-    check(sd_random_lists(draw.seed.value_or(0), 0, (float)p, l.mb, l.kb, l.drawn(), split, l.out_mb, l.out_kb, l.row_ptr(), l.col_idx(), l.col_ptr(),
-                          l.row_idx(), stream_of(x)),
-          "sd_random_lists");
+int64_t up8(int64_t n) { return ceil_div(n, 8) * 8; }
+Tensor rows_of(const Tensor& t) { return row_major(t) ? t : t.contiguous(); }
+// (of a layer's lists: none where nothing is dropped)
+struct ListArgs {
+  const int32_t *row_ptr = nullptr, *col_idx = nullptr, *col_ptr = nullptr, *row_idx = nullptr;
+  explicit ListArgs(const Lists& l) {
+    if (!l.buf.defined()) return;
+    row_ptr = l.row_ptr();
+    col_idx = l.col_idx();
+    col_ptr = l.col_ptr();
+    row_idx = l.row_idx();
   }
-}
+};
 
-// H = act(G) U of [G | U] = s (keep . X) W_in^T, in one launch where a kernel takes it; pre: [G | U] if it is wanted.  lists: of X's mask, if any
-Tensor gated_forward(Tensor x, Tensor w, int64_t F, int act, double p, const Lists& lists, bool want_pre, Tensor& pre) {
-  pad_reduction(x, w);
-  const int64_t M = x.size(0), K = x.size(1);
-  Tensor h = new_matrix(x, M, F);
-  if (want_pre) pre = new_matrix(x, M, 2 * F);
-  const bool masked = lists.buf.defined();
-  const int32_t *rows = masked ? lists.row_ptr() : nullptr, *cols = masked ? lists.col_idx() : nullptr;
-  const float scale = masked ? (float)(1.0 / (1.0 - p)) : 1.f;
-  const Mat xm(x), wm(w), hm(h);
-  Mat pm;
-  if (want_pre) pm = Mat(pre);
-  c10::DeviceGuard guard(x.device());
-  const int rc = sd_gated_matmul(MAT(xm), MAT(wm), hm.ptr, hm.sr, pm.ptr, pm.sr, rows, cols, M, F, K, masked ? lists.kernel_bs : 0, scale, act, dtype_of(x),
-                                 stream_of(x));
+// The block's operands with rows on 16-byte boundaries and whole 16 bytes of a reduction: copies, filled up with zeros, where they have none, made in one
+// launch.  W_in and W_out get as many rows as make 16 bytes too, since in the backward these are the reductions.
+struct GatedOperands {
+  Tensor x, w_in, w_out;
+  int64_t M, K, F, N;
+  bool copied[3] = {false, false, false};
+  GatedOperands(const Tensor& x_, const Tensor& w_in_, const Tensor& w_out_)
+      : x(rows_of(x_)), w_in(rows_of(w_in_)), w_out(rows_of(w_out_)), M(x_.size(0)), K(x_.size(1)), F(w_out_.size(1)), N(w_out_.size(0)) {
+    RowPadding pad;
+    auto copy = [&](int i, Tensor& t, int64_t rows) {
+      copied[i] = true;
+      t = pad.add(t, rows);
+    };
+    if (K % 8 || !rows_on_16_bytes(x)) copy(0, x, M);
+    if (K % 8 || !rows_on_16_bytes(w_in)) copy(1, w_in, up8(2 * F));
+    if (F % 8 || !rows_on_16_bytes(w_out)) copy(2, w_out, up8(N));
+    pad.launch();
+  }
+};
+
+// H = act(G) U (as wide as 16 bytes make it, zeros behind F), [G | U] to pre if it is wanted.  draw: where lists are to come from, if blocks are dropped
+Tensor gated_forward(const GatedOperands& o, int act, int64_t bs, double p, const Draw* draw, Lists& lists, bool want_pre, Tensor& pre) {
+  const int64_t M = o.M, F = o.F, K8 = up8(o.K), F8 = up8(F);
+  Tensor h = new_matrix(o.x, M, F8);
+  if (want_pre) pre = new_matrix(o.x, M, 2 * F8);
+  const Mat xm(o.x), wm(o.w_in);
+  c10::DeviceGuard guard(o.x.device());
+  void* const stream = stream_of(o.x);
+  const int dtype = dtype_of(o.x);
+  auto pre_ptr = [&] { return pre.defined() ? pre.data_ptr() : nullptr; };
+  int rc;
+  if (draw) {
+    lists.shape(M, o.K, bs);
+    TORCH_CHECK_NOT_IMPLEMENTED(bs % 32 == 0, "block_size ", bs, ": only multiples of 32 are supported");
+    lists.allocate(o.x, draw->mask);
+    const MaskArg given = draw->mask ? lists.mask() : MaskArg();
+    rc = sd_gated_dropout_matmul_forward(MAT(xm), MAT(wm), h.data_ptr(), F8, F8, pre_ptr(), 2 * F8, F8, given.ptr, given.sr, given.sc, draw->state_ptr(),
+                                         draw->seed.value_or(0), 0, p, lists.drawn(), lists.row_ptr(), lists.col_idx(), lists.col_ptr(), lists.row_idx(), M, F,
+                                         K8, bs, act, dtype, stream);
+  } else {
+    rc = sd_gated_matmul(MAT(xm), MAT(wm), h.data_ptr(), F8, F8, pre_ptr(), 2 * F8, F8, nullptr, nullptr, M, F, K8, 0, 1.f, act, dtype, stream);
+  }
   if (rc == SD_OK) return h;
   if (rc != SD_ERR_UNSUPPORTED) check(rc, "sd_gated_matmul");
-  if (!want_pre) pre = new_matrix(x, M, 2 * F);
-  pm = Mat(pre);
-  const int64_t g = masked && lists.kernel_bs != 32 ? lists.kernel_bs : 64;
-  Scratch ws(x, sd_splitk_workspace_bytes(M, 2 * F, K, masked ? g : 0, masked ? 1 : 0));
-  if (masked)
-    check(sd_gemm_dsd_lists(MAT(xm), MAT(wm), MAT(pm), rows, cols, M, 2 * F, K, lists.kernel_bs, scale, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
+  // product and gate apart (the lists are there)
+  Tensor a = new_matrix(o.x, M, 2 * F);
+  Scratch ws(o.x, sd_splitk_workspace_bytes(M, 2 * F, K8, draw ? 64 : 0, draw ? 1 : 0));
+  const Mat am(a);
+  if (draw)
+    check(sd_gemm_dsd_lists(MAT(xm), MAT(wm), MAT(am), lists.row_ptr(), lists.col_idx(), M, 2 * F, K8, lists.kernel_bs, (float)(1.0 / (1.0 - p)), dtype, ws.ptr,
+                            ws.bytes, stream),
           "sd_gemm_dsd_lists");
   else
-    check(sd_gemm(MAT(xm), MAT(wm), MAT(pm), M, 2 * F, K, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)), "sd_gemm");
-  check(sd_gated_forward(pm.ptr, pm.sr, hm.ptr, hm.sr, M, F, act, dtype_of(x), stream_of(x)), "sd_gated_forward");
+    check(sd_gemm(MAT(xm), MAT(wm), MAT(am), M, 2 * F, K8, dtype, ws.ptr, ws.bytes, stream), "sd_gemm");
+  check(sd_gated_forward(a.data_ptr(), 2 * F, F, h.data_ptr(), F8, F8, M, F, act, dtype, stream), "sd_gated_forward");
+  if (want_pre) {
+    pre.narrow(1, 0, F).copy_(a.narrow(1, 0, F));
+    pre.narrow(1, F8, F).copy_(a.narrow(1, F, F));
+  }
   return h;
 }
 
-// [dG | dU] and / or dW_out from dY.
-std::pair<Tensor, Tensor> gated_backward(Tensor dy, Tensor w, Tensor h, const Tensor& a, int act, double p, const Lists& lists, bool need_da, bool need_dw) {
-  const int64_t M = dy.size(0), N = dy.size(1), F = h.size(1), n8 = ceil_div(N, 8) * 8;
-  TORCH_CHECK_VALUE(M == h.size(0) && N == w.size(0) && dy.device() == h.device(), "dy must be a [", h.size(0), ", ", w.size(0), "] tensor on ", h.device());
-  RowPadding pad;  // as in layer_backward
-  if (N % 8 || (row_major(dy) && !rows_on_16_bytes(dy))) dy = pad.add(dy, M);
-  if (need_da && (N % 8 || (row_major(w) && !rows_on_16_bytes(w)))) w = pad.add(w, n8).narrow(1, 0, F);
-  else if (N % 8) w = at::empty({n8, F}, w.options());  // dW alone: only its shape is looked at
-  if (need_dw && row_major(h) && !rows_on_16_bytes(h)) h = pad.add(h, M).narrow(1, 0, F);
-  pad.launch();
-  Tensor da, dw;
-  if (need_da) {
-    da = new_matrix(h, M, 2 * F);
-    const bool masked = lists.buf.defined();
-    const Mat gm(dy), wm(w), am(a), om(da);
-    c10::DeviceGuard guard(h.device());
-    const int rc = sd_gated_matmul_gradient(MAT(gm), MAT(wm), am.ptr, am.sr, om.ptr, om.sr, masked ? lists.row_ptr() : nullptr, masked ? lists.col_idx() : nullptr, M,
-                                            F, dy.size(1), masked ? lists.kernel_bs : 0, masked ? (float)(1.0 / (1.0 - p)) : 1.f, (float)(1.0 - p), act, dtype_of(h),
-                                            stream_of(h));
-    if (rc == SD_ERR_UNSUPPORTED) {
-      const auto [dh, dw_too] = layer_products(dy, w, h, lists, p, true, need_dw, SD_ACT_NONE, Tensor());
-      dw = dw_too;
-      const Mat dm(dh);
-      check(sd_gated_backward(dm.ptr, dm.sr, am.ptr, am.sr, om.ptr, om.sr, M, F, act, dtype_of(h), stream_of(h)), "sd_gated_backward");
-    } else {
-      check(rc, "sd_gated_matmul_gradient");
-    }
+// [dG | dU] (as wide as 16 bytes make it) and / or dW_out.  dy, w_out: N filled up to whole 16 bytes
+std::pair<Tensor, Tensor> gated_backward(const Tensor& dy, const Tensor& w_out, const Tensor& h, const Tensor& pre, int64_t F, int act, double p, const Lists& lists,
+                                         bool need_da, bool need_dw) {
+  const int64_t M = dy.size(0), N = dy.size(1), F8 = h.size(1), R8 = up8(2 * F);
+  const Tensor hf = h.narrow(1, 0, F), wf = w_out.narrow(1, 0, F);
+  if (!need_da) return {Tensor(), layer_products(dy, wf, hf, lists, p, false, need_dw, SD_ACT_NONE, Tensor()).second};
+  Tensor da = new_matrix(h, M, R8), dw;
+  const bool masked = lists.buf.defined();
+  const ListArgs l(lists);
+  const Mat gm(dy), wm(wf), hm(hf);
+  Mat dm;
+  if (need_dw) {
+    dw = new_matrix(h, N, F);
+    dm = Mat(dw);
   }
-  if (need_dw && !dw.defined()) dw = layer_products(dy, w, h, lists, p, false, true, SD_ACT_NONE, Tensor()).second;
-  return {da, dw.defined() && dw.size(0) != N ? dw.narrow(0, 0, N) : dw};
+  Scratch ws(h, need_dw ? sd_splitk_workspace_bytes(F, N, M, masked ? 64 : 0, masked ? 1 : 0) : 0);
+  c10::DeviceGuard guard(h.device());
+  void* const stream = stream_of(h);
+  const int rc = sd_gated_matmul_gradient(MAT(gm), MAT(wm), pre.data_ptr(), 2 * F8, F8, da.data_ptr(), R8, R8, MAT(hm), MAT(dm), l.row_ptr, l.col_idx, l.col_ptr, l.row_idx,
+                                          M, F, N, masked ? lists.bs : 0, p, act, dtype_of(h), ws.ptr, ws.bytes, stream);
+  if (rc == SD_OK) return {da, dw};
+  if (rc != SD_ERR_UNSUPPORTED) check(rc, "sd_gated_matmul_gradient");
+  const auto [dh, dw_apart] = layer_products(dy, wf, hf, lists, p, true, need_dw, SD_ACT_NONE, Tensor());
+  check(sd_gated_backward(dh.data_ptr(), F, pre.data_ptr(), 2 * F8, F8, da.data_ptr(), R8, R8, M, F, act, dtype_of(h), stream), "sd_gated_backward");
+  return {da, dw_apart};
 }
 
 struct GatedMlpBackward : Node {
-  Saved x, w_in, w_out, pre, h;  // pre: [G | U], h = act(G) U
+  Saved x, w_in, w_out, pre, h;  // pre: [G | U], h = act(G) U, both as gated_forward makes them
   SavedLists lists[2];           // nothing kept: nothing is dropped
+  Tensor copies[3];              // of the operands, where the forward took copies
   double p[2] = {0.0, 0.0};
   int act = SD_ACT_NONE;
   variable_list apply(variable_list&& grads) override {
@@ -735,7 +754,6 @@ struct GatedMlpBackward : Node {
     at::NoGradGuard no_grad;
     variable_list out(3);
     const Tensor xs = x.matrix(), wi = w_in.matrix(), wo = w_out.matrix();
-    TORCH_CHECK(xs.defined(), "Trying to backward through the graph a second time, or after its saved tensors were freed");
     const bool need_x = task_should_compute_output(0), need_in = task_should_compute_output(1), need_out = task_should_compute_output(2);
     if (xs.size(0) == 0 || !grads[0].defined()) {
       if (need_x) out[0] = at::zeros(xs.sizes(), xs.options());
@@ -743,17 +761,34 @@ struct GatedMlpBackward : Node {
       if (need_out) out[2] = at::zeros(wo.sizes(), wo.options());
       return out;
     }
-    const Tensor dy = grad_matrix(grads[0], xs), hs = h.matrix(), a = pre.matrix();
-    Tensor da;
-    std::tie(da, out[2]) = gated_backward(dy, wo, hs, row_major(a) ? a : a.contiguous(), act, p[1], lists[1].get(), need_x || need_in, need_out);
+    const int64_t M = xs.size(0), K = xs.size(1), N = wo.size(0), F = wo.size(1);
+    Tensor dy = rows_of(grad_matrix(grads[0], xs));
+    TORCH_CHECK_VALUE(dy.size(0) == M && dy.size(1) == N && dy.device() == xs.device(), "dy must be a [", M, ", ", N, "] tensor on ", xs.device());
+    Tensor xr = copies[0].defined() ? copies[0] : rows_of(xs), wir = copies[1].defined() ? copies[1] : rows_of(wi),
+           wor = copies[2].defined() ? copies[2] : rows_of(wo);
+    {
+      // (saved-tensor hooks may have moved what was on 16 bytes)
+      RowPadding pad;
+      if (N % 8 || !rows_on_16_bytes(dy)) dy = pad.add(dy, M);
+      if (wor.size(0) % 8 || !rows_on_16_bytes(wor)) wor = pad.add(wor, up8(N));
+      if (need_x && (wir.size(0) % 8 || !rows_on_16_bytes(wir))) wir = pad.add(wir, up8(2 * F));
+      if (need_in && !rows_on_16_bytes(xr)) xr = pad.add(xr, M);
+      pad.launch();
+    }
+    Tensor da, dw;
+    std::tie(da, dw) = gated_backward(dy, wor, h.matrix().contiguous(), pre.matrix().contiguous(), F, act, p[1], lists[1].get(), need_x || need_in, need_out);
+    if (need_out) out[2] = dw.size(0) != N ? dw.narrow(0, 0, N) : dw;
     if (!need_x && !need_in) return out;
-    std::tie(out[0], out[1]) = layer_backward(da, wi, xs, lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
+    if (wir.size(0) != da.size(1)) wir = at::empty({da.size(1), K}, wir.options());  // dW_in alone: only its shape is looked at
+    std::tie(out[0], dw) = layer_products(da, wir.narrow(1, 0, K), xr.narrow(1, 0, K), lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
+    if (need_in) out[1] = dw.size(0) != 2 * F ? dw.narrow(0, 0, 2 * F) : dw;
     return out;
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     for (Saved* s : {&x, &w_in, &w_out, &pre, &h}) s->drop();
     for (SavedLists& l : lists) l.drop();
+    for (Tensor& t : copies) t = Tensor();
   }
   std::string name() const override { return "GatedMLPHIPBackward"; }
 };
@@ -770,32 +805,42 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
   check_operand("weight_out", wo);
   TORCH_CHECK_TYPE(wo.scalar_type() == x.scalar_type(), "input and weight_out must have the same dtype (", x.dtype(), " vs ", wo.dtype(), ")");
   TORCH_CHECK_VALUE(wo.device() == x.device(), "input and weight_out must be on the same device");
-  const int64_t M = x.size(0), F = wo.size(1), N = wo.size(0);
+  const int64_t M = x.size(0), K = x.size(1), F = wo.size(1), N = wo.size(0);
   TORCH_CHECK_VALUE(wi.size(0) == 2 * F, "weight_in must have the rows of both projections, 2 x ", F, " (got ", wi.size(0), ")");
-  TORCH_CHECK_VALUE(F > 0 && N > 0 && x.size(1) > 0, "the block's features, hidden width and outputs must not be empty");
+  TORCH_CHECK_VALUE(F > 0 && N > 0 && K > 0, "the block's features, hidden width and outputs must not be empty");
   const bool rec = records(inputs);
+  const auto drops = [&](int i) { return bs != 0 && (ps[i] != 0.0 || (masks && (*masks)[i])); };
+  const auto draw = [&](int i) {
+    check_p(ps[i]);
+    return Draw{masks ? (*masks)[i] : OptTensor(), seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
+  };
   Lists lists[2];
-  Tensor pre, h, y;
+  Tensor pre, h, y, copies[3];
   {
     NoRecord guard;
-    const auto drops = [&](int i) { return bs != 0 && (ps[i] != 0.0 || (masks && (*masks)[i])); };
-    const auto draw = [&](int i) {
-      return Draw{masks ? (*masks)[i] : OptTensor(), seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
-    };
     if (M == 0) {
       y = new_matrix(x, 0, N);
-    } else if (!rec && !drops(0) && !drops(1) && row_major(wi) && row_major(wo) && sd_gated_mlp_few_taken(M, x.size(1), F, N)) {
-      const Tensor rows = row_major(x) ? x : x.contiguous();
+    } else if (!rec && !drops(0) && !drops(1) && row_major(wi) && row_major(wo) && sd_gated_mlp_few_taken(M, K, F, N)) {
+      const Tensor rows = rows_of(x);
       y = new_matrix(x, M, N);
       const Scratch ws(x, sd_gated_mlp_few_workspace_bytes(M, F));
       const Mat xm(rows), im(wi), om(wo);
       c10::DeviceGuard device(x.device());
-      check(sd_gated_mlp_few(xm.ptr, xm.sr, im.ptr, im.sr, om.ptr, om.sr, y.data_ptr(), N, M, x.size(1), F, N, act, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
+      check(sd_gated_mlp_few(xm.ptr, xm.sr, im.ptr, im.sr, om.ptr, om.sr, y.data_ptr(), N, M, K, F, N, act, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),
             "sd_gated_mlp_few");
     } else {
-      if (drops(0)) layer_lists(x, M, x.size(1), bs, ps[0], draw(0), lists[0]);
-      h = gated_forward(x, wi, F, act, ps[0], lists[0], rec, pre);
-      y = drops(1) ? layer_forward(h, wo, bs, ps[1], draw(1), SD_ACT_NONE, false, lists[1], nullptr) : dense(h, wo, SD_ACT_NONE, false, nullptr);
+      const GatedOperands o(x, wi, wo);
+      Draw d[2];
+      for (int i = 0; i < 2; ++i)
+        if (drops(i)) d[i] = draw(i);
+      h = gated_forward(o, act, bs, ps[0], drops(0) ? &d[0] : nullptr, lists[0], rec, pre);
+      const Tensor w = o.w_out.size(0) != N ? o.w_out.narrow(0, 0, N) : o.w_out;
+      y = drops(1) ? layer_forward(h, w, bs, ps[1], d[1], SD_ACT_NONE, false, lists[1], nullptr) : dense(h, w, SD_ACT_NONE, false, nullptr);
+      if (rec) {
+        const Tensor* from[3] = {&o.x, &o.w_in, &o.w_out};
+        for (int i = 0; i < 3; ++i)
+          if (o.copied[i]) copies[i] = *from[i];
+      }
     }
   }
   if (rec) {
@@ -805,6 +850,7 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
     node->w_out.keep(wo);
     node->pre.keep(pre);
     node->h.keep(h);
+    for (int i = 0; i < 3; ++i) node->copies[i] = copies[i];
     for (int i = 0; i < 2; ++i) {
       if (lists[i].buf.defined()) node->lists[i].keep(std::move(lists[i]));
       node->p[i] = bs ? ps[i] : 0.0;

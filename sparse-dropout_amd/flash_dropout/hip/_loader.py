@@ -142,16 +142,18 @@ SIGNATURES = {
     "sd_grad_norm_workspace_bytes": (c_int64, [c_int, c_void_p]),
     "sd_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "sd_clip_grads": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p, c_int64, c_void_p]),
-    "sd_gated_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
-    "sd_gated_matmul": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float,
-                                c_int, c_int, c_void_p]),
+    "sd_gated_forward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "sd_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "sd_gated_matmul": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                c_float, c_int, c_int, c_void_p]),
+    "sd_gated_dropout_matmul_forward": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, *_mat, c_void_p, c_uint64, c_uint64, c_double,
+                                                *([c_void_p] * 5), *([c_int64] * 4), c_int, c_int, c_void_p]),
+    "sd_gated_matmul_gradient": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, *_mat, *_mat, *([c_void_p] * 4), *([c_int64] * 4),
+                                         c_double, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "sd_gated_mlp_few_workspace_bytes": (c_int64, [c_int64, c_int64]),
     "sd_gated_mlp_few_taken": (c_int, [c_int64] * 4),
     "sd_gated_mlp_few": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
                                  c_void_p, c_int64, c_void_p]),
-    "sd_gated_matmul_gradient": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                         c_float, c_float, c_int, c_int, c_void_p]),
-    "sd_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
 }
 
 

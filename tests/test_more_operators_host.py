@@ -16,16 +16,60 @@ fake = 0x1000
 
 def test_gate_calls_refuse_bad_arguments():
     lib = _loader.load()
-    ok = dict(A=fake, lda=16, H=fake, ldh=8, M=4, F=8, act=3, dtype=1)
+    ok = dict(A=fake, lda=16, up=8, H=fake, ldh=8, h_cols=8, M=4, F=8, act=3, dtype=1)
     fwd = lambda **kw: lib.sd_gated_forward(*{**ok, **kw}.values(), None)
-    for bad, message in ((dict(A=None), b"null pointer"), (dict(lda=15), b"pitch"), (dict(ldh=7), b"pitch"), (dict(H=None), b"null result"), (dict(M=-1), b"extents"),
-                         (dict(F=1 << 30), b"extents"), (dict(act=0), b"act must be"), (dict(act=4), b"act must be"), (dict(dtype=2), b"dtype")):
+    for bad, message in ((dict(A=None), b"null pointer"), (dict(lda=15), b"pitch"), (dict(up=7), b"U begins"), (dict(ldh=7), b"pitch"), (dict(H=None), b"null pointer"),
+                         (dict(h_cols=9, ldh=16), b"zeros up to"), (dict(h_cols=7), b"zeros up to"), (dict(M=-1), b"extents"), (dict(F=1 << 30), b"extents"),
+                         (dict(act=0), b"act must be"), (dict(act=4), b"act must be"), (dict(dtype=2), b"dtype")):
         assert fwd(**bad) == 1 and message in lib.sd_last_error(), bad
-    assert fwd(M=0, A=None, H=None) == 0 and fwd(F=0, A=None, H=None) == 0
-    ok = dict(dH=fake, ldd=8, A=fake, lda=16, dA=fake, ldda=16, M=4, F=8, act=2, dtype=0)
-    bwd = lambda **kw: lib.sd_gated_backward(*{**ok, **kw}.values(), None)
-    for bad, message in ((dict(dH=None), b"null gradient"), (dict(ldd=7), b"pitch"), (dict(dA=None), b"null result"), (dict(ldda=15), b"pitch"), (dict(lda=8), b"pitch")):
+    assert fwd(M=0, A=None, H=None) == 0
+    ok_back = dict(dH=fake, ldd=8, A=fake, lda=16, up=8, dA=fake, ldda=16, da_cols=16, M=4, F=8, act=2, dtype=0)
+    bwd = lambda **kw: lib.sd_gated_backward(*{**ok_back, **kw}.values(), None)
+    for bad, message in ((dict(dH=None), b"null gradient"), (dict(ldd=7), b"pitch"), (dict(dA=None), b"null pointer"), (dict(ldda=15), b"pitch"), (dict(lda=8), b"pitch"),
+                         (dict(da_cols=17, ldda=24), b"zeros up to")):
         assert bwd(**bad) == 1 and message in lib.sd_last_error(), bad
+
+
+def test_gated_products_refuse_bad_arguments():
+    lib = _loader.load()
+    ok = dict(X=fake, xr=64, xc=1, W=fake, wr=64, wc=1, H=fake, ldh=32, h_cols=32, A=fake, lda=64, up=32, rows=None, cols=None, M=128, F=32, K=64, bs=64, scale=1.0, act=3,
+              dtype=1)
+    call = lambda **kw: lib.sd_gated_matmul(*{**ok, **kw}.values(), None)
+    for bad, message in ((dict(act=0), b"act must be"), (dict(up=31), b"U begins"), (dict(lda=63), b"pitch"), (dict(rows=fake), b"both be given"), (dict(scale=math.nan), b"NaN"),
+                         (dict(rows=fake, cols=fake, bs=0), b"positive"), (dict(xr=63), b"row stride"), (dict(wr=63), b"row stride"), (dict(W=None), b"null pointer"),
+                         (dict(ldh=31), b"row stride"), (dict(h_cols=33, ldh=40), b"next multiple of 8"), (dict(h_cols=31), b"next multiple of 8"), (dict(dtype=2), b"dtype")):
+        assert call(**bad) == 1 and message in lib.sd_last_error(), bad
+    assert call(rows=fake, cols=fake, bs=48) == 2 and call(K=0) == 2 and call(M=0) == 0 and call(F=0, h_cols=0) == 0
+    ok = dict(X=fake, xr=64, xc=1, W=fake, wr=64, wc=1, H=fake, ldh=32, h_cols=32, A=fake, lda=64, up=32, mask=fake, mr=1, mc=1, state=None, seed=0, offset=0, p=0.5, out=None,
+              rp=fake, ci=fake, cp=fake, ri=fake, M=128, F=32, K=64, bs=64, act=3, dtype=1)
+    call = lambda **kw: lib.sd_gated_dropout_matmul_forward(*{**ok, **kw}.values(), None)
+    for bad, message in ((dict(p=1.0), b"p must be"), (dict(p=-0.1), b"p must be"), (dict(rp=None), b"CSR list arrays"), (dict(mask=None), b"null mask_out"), (dict(M=0), b"empty"),
+                         (dict(mr=2, mc=2), b"row or column major"), (dict(mask=None, out=fake, state=fake + 4), b"aligned device pointer"), (dict(act=5), b"act must be")):
+        assert call(**bad) == 1 and message in lib.sd_last_error(), bad
+    assert call(bs=48) == 2
+    ok = dict(dY=fake, gr=16, gc=1, W=fake, wr=32, wc=1, A=fake, lda=64, up=32, dA=fake, ldda=64, cols=64, H=fake, hr=32, hc=1, dW=fake, dr=32, dc=1, rp=None, ci=None, cp=None,
+              ri=None, M=128, F=32, N=16, bs=64, p=0.0, act=3, dtype=1, ws=None, nbytes=0)
+    call = lambda **kw: lib.sd_gated_matmul_gradient(*{**ok, **kw}.values(), None)
+    for bad, message in ((dict(p=1.0), b"p must be"), (dict(A=None), b"null [G | U]"), (dict(dA=None), b"null pointer"), (dict(ldda=63), b"pitch"), (dict(cols=65, ldda=72), b"multiple of 8"),
+                         (dict(rp=fake, ci=fake), b"CSC lists"), (dict(cp=fake), b"both be given"), (dict(hr=31), b"stride"), (dict(gr=15), b"row stride"), (dict(act=0), b"act")):
+        assert call(**bad) == 1 and message in lib.sd_last_error(), bad
+    assert call(N=0) == 2 and call(M=0) == 0
+
+
+def test_few_rows_refuse_bad_arguments():
+    lib = _loader.load()
+    assert lib.sd_gated_mlp_few_workspace_bytes(1, 64) == 2 * 16 * 64 and lib.sd_gated_mlp_few_workspace_bytes(9, 65) == 2 * 9 * 192
+    assert [lib.sd_gated_mlp_few_workspace_bytes(*a) for a in ((0, 64), (65, 64), (4, 0), (4, 1 << 29))] == [0] * 4
+    assert lib.sd_gated_mlp_few_taken(1, 1024, 4096, 1024) == 1 and lib.sd_gated_mlp_few_taken(16, 8192, 8192, 8192) == 1
+    assert [lib.sd_gated_mlp_few_taken(*a) for a in ((0, 64, 64, 64), (65, 64, 64, 64), (4, 0, 64, 64), (4, 64, 1 << 29, 64), (64, 2048, 8192, 2048))] == [0] * 5
+    need = lib.sd_gated_mlp_few_workspace_bytes(4, 64)
+    ok = dict(X=fake, ldx=32, Wi=fake, ldwi=32, Wo=fake, ldwo=64, Y=fake, ldy=16, M=4, K=32, F=64, N=16, act=3, dtype=0, ws=fake, nbytes=need)
+    call = lambda **kw: lib.sd_gated_mlp_few(*{**ok, **kw}.values(), None)
+    for bad, message in ((dict(K=0), b"extents"), (dict(M=-1), b"extents"), (dict(F=1 << 29), b"extents"), (dict(dtype=2), b"dtype"), (dict(act=0), b"act"), (dict(X=None), b"null"),
+                         (dict(ldx=31), b"pitch"), (dict(ldwi=31), b"pitch"), (dict(ldwo=63), b"pitch"), (dict(ldy=15), b"pitch"), (dict(nbytes=need - 1), b"too small"),
+                         (dict(ws=fake + 8), b"aligned")):
+        assert call(**bad) == 1 and message in lib.sd_last_error(), bad
+    assert call(M=0) == 0 and call(M=65) == 2 and b"at most 64" in lib.sd_last_error()
 
 
 def test_norm_calls_refuse_bad_arguments():
