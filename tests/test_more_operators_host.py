@@ -76,13 +76,13 @@ def test_norm_calls_refuse_bad_arguments():
     lib = _loader.load()
     n = 3
 
-    def call(fn, sizes=(5, 0, 4097), types=(0, 1, 2), pointers=(fake, None, fake), kind=2, limit=1.0, norm=fake, ws=fake, nbytes=1 << 20, count=n):
+    def call(fn, sizes=(5, 0, 8193), types=(0, 1, 2), pointers=(fake, None, fake), kind=2, limit=1.0, norm=fake, ws=fake, nbytes=1 << 20, count=n):
         p, s, t = (ctypes.c_void_p * n)(*pointers), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*types)
         if fn == "clip":
             return lib.sd_clip_grads(count, p, s, t, kind, limit, norm, ws, nbytes, None)
         return lib.sd_grad_norm(count, p, s, t, kind, limit, norm, fake, ws, nbytes, None)
 
-    need = lib.sd_grad_norm_workspace_bytes(n, (ctypes.c_int64 * n)(5, 0, 4097))
+    need = lib.sd_grad_norm_workspace_bytes(n, (ctypes.c_int64 * n)(5, 0, 8193))
     assert need == 8 * 3 and lib.sd_grad_norm_workspace_bytes(0, None) == 0
     assert lib.sd_grad_norm_workspace_bytes(1, (ctypes.c_int64 * 1)(1 << 40)) == 8 * 1024
     for fn in ("norm", "clip"):
