@@ -1,6 +1,6 @@
 """Whole-model forward + backward time as the drop rate varies (reference: benchmark/model.py:119-229).
 
-    python -m benchmark.model --model mlp mlp-784 vit-ffn gpt-ffn --p 0 0.1 0.3 0.5 0.7
+    python -m benchmark.model --model mlp mlp-784 vit-ffn gpt-ffn gated-ffn --p 0 0.1 0.3 0.5 0.7
 
 Models are built from ``DropoutMM`` the way the reference's evaluation models are:
   mlp      flattened 32x32 images -> [hidden]*layers -> 10 classes padded to 128, ReLU between, dropout on
@@ -10,12 +10,14 @@ Models are built from ``DropoutMM`` the way the reference's evaluation models ar
            inputs of both linears
   gpt-ffn  the feed-forward block of the reference's GPT (benchmark/model.py:96-112: n_embed 1024, context 128,
            batch 32; eval/llm/model.py:58-66: 1024 -> 4096 -> GELU -> 1024) on its 32x128 = 4096 tokens
+  gated-ffn  a gated feed-forward block with about as many parameters, 1024 -> 2 x 2752 -> silu -> 1024, on the same tokens
 Each is timed with variant "none" (dense), "vanilla" (element dropout + dense), "blockwise[hip]" and
 "blockwise[hip-fused]": the same layers as one autograd function whose GEMM stores apply the activation and
 its derivative (no activation kernels in either direction), and "blockwise[hip-fp8]": products of operands in 8 bits, on
-blocks of 128 (or --block-size, where that is a multiple of it).
+blocks of 128 (or --block-size, where that is a multiple of it).  The gated block's products and gate are one autograd function in
+"blockwise[hip]"; it has no variant in 8 bits.
 
---optimizer adds an AdamW step with averages in 32 or 8 bits to what is timed."""
+--optimizer adds an AdamW step with averages in 32 or 8 bits to what is timed, --max-norm the clipping of its gradients."""
 from __future__ import annotations
 
 import argparse
@@ -26,7 +28,7 @@ import torch
 from torch import nn
 
 import flash_dropout.functional as F
-from flash_dropout.layers import DropoutMM
+from flash_dropout.layers import DropoutMM, GatedMLP
 from flash_dropout.optim import AdamW
 
 from .utils import FLUSH_BYTES
@@ -99,7 +101,15 @@ class GptFfn(VitFfn):
         super().__init__(variant, p, block_size, dim=1024, hidden=4096)
 
 
+class GatedFfn(GatedMLP):
+    """The gated block of as many parameters as ``GptFfn`` has, but for the rounding of its width."""
+
+    def __init__(self, variant, p, block_size):
+        super().__init__(1024, 2752, p=p, variant=variant, block_size=block_size)
+
+
 MODELS = {
+    "gated-ffn": (GatedFfn, lambda: torch.randn(32, 128, 1024)),
     "gpt-ffn": (GptFfn, lambda: torch.randn(32, 128, 1024)),
     "mlp": (Mlp, lambda: torch.rand(1024, 1, 32, 32)),
     "mlp-784": (Mlp784, lambda: torch.rand(4096, 1, 28, 28)),
@@ -167,20 +177,25 @@ def main() -> None:
     ap.add_argument("--rep", type=float, default=0.3, help="seconds of timed repetitions per point")
     ap.add_argument("--graph", action="store_true", help="capture the step in a HIP graph and time replays")
     ap.add_argument("--optimizer", choices=list(OPTIMIZERS), default="none", help="AdamW step after the backward pass, by its averages' bits")
+    ap.add_argument("--max-norm", type=float, help="clip the gradients to this joint norm in the optimizer's step")
     args = ap.parse_args()
     bits = OPTIMIZERS[args.optimizer]
+    if args.max_norm is not None and bits is None:
+        ap.error("--max-norm clips in the optimizer's step: choose one with --optimizer")
     torch.manual_seed(0)
     for name in args.model:
         cls, make_x = MODELS[name]
         x = make_x().cuda().half()
         print(f"=== {name}  input {tuple(x.shape)}  block_size {args.block_size}{'  (graph replay)' if args.graph else ''}"
-              f"{'' if bits is None else f'  with AdamW, averages in {bits} bits'}")
+              f"{'' if bits is None else f'  with AdamW, averages in {bits} bits'}{'' if args.max_norm is None else f', clipped to {args.max_norm}'}")
         for variant, ps in (("none", [0.0]), ("vanilla", [0.5]), ("blockwise[hip]", args.p),
                             ("blockwise[hip-fused]", args.p), ("blockwise[hip-fp8]", args.p)):
+            if name == "gated-ffn" and variant in ("blockwise[hip-fused]", "blockwise[hip-fp8]"):
+                continue
             for p in ps:
                 size = 128 if variant.endswith("fp8]") and args.block_size % 128 else args.block_size
                 model = (fused_variant(name, p, size) if variant.endswith("fused]") else cls(variant, p, size)).cuda().half().train()
-                optimizer = None if bits is None else AdamW(model.parameters(), lr=1e-4, state_bits=bits)
+                optimizer = None if bits is None else AdamW(model.parameters(), lr=1e-4, state_bits=bits, max_norm=args.max_norm)
                 ts = time_model(model, x, warmup=0.2, rep=args.rep, graph=args.graph, optimizer=optimizer)
                 sem = statistics.stdev(ts) / len(ts) ** 0.5 if len(ts) > 1 else 0.0
                 print(f"{variant:<21} p={p:<4} median {statistics.median(ts):8.4f} ms  "

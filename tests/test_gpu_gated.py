@@ -1,5 +1,9 @@
 """The gated feed-forward block on the GPU against its formulas in 64 bits: element by element within the bounds that oracle/gated_oracle.py
 derives from the roundings, and within the package's bar of 1e-2 in the relative Frobenius norm."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -10,6 +14,7 @@ pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
     import flash_dropout.functional as F
+    from flash_dropout.hip import _loader
     from flash_dropout.layers import GatedMLP
 
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
@@ -287,3 +292,120 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match="forward mode"):
         with torch.autograd.forward_ad.dual_level():
             F.gated_mlp(torch.autograd.forward_ad.make_dual(x, x), w_in, w_out)
+
+
+def few(x, w_in, w_out, act, pitches=(0, 0, 0, 0)):
+    """The two launches for few rows, whatever is expected to be faster, between rows and bytes that must stay as they are."""
+    (m, k), (n, f) = x.shape, w_out.shape
+    lib, guard = _loader.load(), 7777.0
+
+    def wide(t, more):
+        big = torch.full((t.shape[0], t.shape[1] + more), guard, dtype=x.dtype, device="cuda")
+        big[:, : t.shape[1]] = t
+        return big
+
+    xs, ws, os_ = (wide(t, p) for t, p in zip((x, w_in, w_out), pitches))
+    y = torch.full((m + 2, n + pitches[3]), guard, dtype=x.dtype, device="cuda")
+    need = lib.sd_gated_mlp_few_workspace_bytes(m, f)
+    scratch = torch.full((need + 64,), 0x5a, dtype=torch.uint8, device="cuda")
+    rc = lib.sd_gated_mlp_few(xs.data_ptr(), xs.stride(0), ws.data_ptr(), ws.stride(0), os_.data_ptr(), os_.stride(0), y[1:].data_ptr(), y.stride(0), m, k, f, n,
+                              {"relu": 1, "gelu": 2, "silu": 3}[act], 1 if x.dtype == torch.bfloat16 else 0, scratch.data_ptr(), need,
+                              torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.sd_last_error()
+    assert (y[0] == guard).all() and (y[-1] == guard).all() and (y[:, n:] == guard).all() and (scratch[need:] == 0x5a).all()
+    return y[1:-1, :n]
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 50, 64])
+def test_few_rows(m):
+    for i, (k, f, n) in enumerate(((64, 64, 64), (1, 1, 1), (63, 65, 3), (1024, 4096, 1024), (130, 5461, 300), (2048, 333, 2048), (200, 9000, 100))):
+        dtype, act = ("bf16", "fp16")[i % 2], ("silu", "gelu", "relu")[i % 3]
+        ops = operands(m, k, f, n, dtype, seed=40 + i)
+        ref = O.reference(*ops, act, DT[dtype])
+        check({"y": few(*ops[:3], act)}, ref)
+        check({"y": few(*ops[:3], act, (3, 1, 5, 2))}, ref)
+
+
+def test_few_rows_keep_the_hidden_activations_to_more_than_their_type():
+    """Up to 8 rows only the result is rounded to 16 bits: half a step of it, and the 32-bit sums' errors of the reference's bounds without u in them."""
+    ops = operands(8, 512, 1024, 512, "bf16", seed=50)
+    exact = O.reference(*ops, "silu", torch.bfloat16)["y"][0]
+    wide = O.reference(*(t.double() for t in ops), "silu", torch.float32)["y"]  # (h in two halves is off by 2^-16 of itself, u^2)
+    h = O.act((ops[0].double() @ ops[1].double().t())[:, :1024], "silu")[0] * (ops[0].double() @ ops[1].double().t())[:, 1024:]
+    bound = wide[1] + 2.0 ** -8 * exact.abs() * 1.01 + 2.0 ** -16 * (h.abs() @ ops[2].double().abs().t())
+    got = few(*ops[:3], "silu").double()
+    assert ((got - exact).abs() <= bound).all()
+    assert float(((got - exact).norm() / exact.norm())) < 2.0 ** -8 / 3 ** 0.5 * 1.05  # a uniform rounding error's, no more
+
+
+def test_rows_behind_two_to_the_31_elements():
+    m, k, f, n = 66000, 64, 16384 + 320, 64  # [G | U] has 2.2e9 elements
+    gen = torch.Generator("cuda").manual_seed(51)
+    make = lambda r, c, std: (torch.randn(r, c, generator=gen, device="cuda") * std).bfloat16()
+    x, w_in, w_out, dy = make(m, k, 1.0), make(2 * f, k, k ** -0.5), make(n, f, f ** -0.5), make(m, n, 0.1)
+    got = run(x, w_in, w_out, dy, "silu")
+    for rows in (slice(0, 100), slice(m - 130, m)):
+        ref = O.reference(x[rows], w_in, w_out, dy[rows], "silu", torch.bfloat16)
+        check({name: got[name][rows] for name in ("y", "dx")}, ref)
+    assert all(got[name].isfinite().all() for name in NAMES)
+
+
+def test_product_and_gate_apart():
+    """What is left to the kernel that takes any layout: the gate in passes of its own, in a process that is told to."""
+    code = """
+import sys
+sys.path[:0] = [%r, %r, %r]
+import torch
+import test_gpu_gated as T
+from oracle import gated_oracle as O
+for size, p in (((64, 128, 192, 64), 0.0), ((130, 77, 99, 50), 0.0), ((130, 200, 332, 72), 0.4), ((70, 65, 130, 33), 0.4)):
+    ops = T.operands(*size, "bf16", seed=60)
+    masks = T.masks_of(*size[:3], 64, p) if p else (None, None)
+    got = T.run(*ops, "gelu", 64, p, list(masks)) if p else T.run(*ops, "gelu")
+    T.check(got, O.reference(*ops, "gelu", torch.bfloat16, masks, 64, (p, p)))
+print("apart: right")
+""" % tuple(os.path.join(os.path.dirname(os.path.abspath(__file__)), d) for d in (".", "..", os.path.join("..", "sparse-dropout_amd")))
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "SPARSEDROP_FORCE_GENERIC": "1"}, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "apart: right" in done.stdout, done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("policy", [1, 2])
+def test_either_size_of_tile(policy):
+    """The large and the middle shapes on sizes that would not be given to them: ragged in every extent, dropped and not."""
+    lib = _loader.load()
+    was = lib.sd_set_tile_policy(policy)
+    try:
+        for i, size in enumerate(((257, 328, 712, 320), (64, 64, 64, 64), (300, 130, 1000, 136), (512, 512, 512, 512))):
+            ops = operands(*size, "bf16", seed=70 + i)
+            check(run(*ops, "silu"), O.reference(*ops, "silu", torch.bfloat16))
+            for bs in (64, 32):
+                masks = masks_of(*size[:3], bs, 0.4, seed=i)
+                check(run(*ops, "gelu", bs, 0.4, masks), O.reference(*ops, "gelu", torch.bfloat16, masks, bs, (0.4, 0.4)))
+    finally:
+        lib.sd_set_tile_policy(was)
+
+
+def test_saved_tensors_that_come_back_elsewhere():
+    """Hooks that hand back copies in another layout (offloading does)."""
+    ops = operands(65, 130, 99, 33, "bf16", seed=80)
+    masks = masks_of(65, 130, 99, 64, 0.3)
+    ref = run(*ops, "silu", 64, 0.3, masks)
+    back = lambda t: t.t().contiguous().t() if t.dim() == 2 and t.is_floating_point() else t.clone()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: back(t.cuda())):
+        got = run(*ops, "silu", 64, 0.3, masks)
+    for name in NAMES:
+        assert torch.equal(got[name], ref[name]), name
+
+
+def test_a_gradient_in_any_layout_or_type():
+    ops = operands(130, 64, 96, 40, "bf16", seed=81)
+    leaves = [t.detach().requires_grad_() for t in ops[:3]]
+    ref = run(*ops, "silu")
+    for dy in (ops[3].t().contiguous().t(), torch.cat((ops[3], ops[3]), 1)[:, :40], torch.cat((ops[3][:, :1], ops[3]), 1)[:, 1:]):
+        y = F.gated_mlp(*leaves)
+        for g, name in zip(torch.autograd.grad(y, leaves, dy), NAMES[1:]):
+            assert torch.equal(g, ref[name]), name
+    y = F.gated_mlp(*leaves)
+    y.float().sum().backward()  # an expanded gradient
+    ones = run(*ops[:3], torch.ones(130, 40, device="cuda").bfloat16(), "silu")
+    assert all(torch.equal(t.grad, ones[name]) for t, name in zip(leaves, NAMES[1:]))
