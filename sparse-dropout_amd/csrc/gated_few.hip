@@ -166,30 +166,38 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
 }
 
 int groups_of(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
-// Outputs of a workgroup.  At least 256 workgroups, down to 4 outputs each: one row of 4096 to 1024 takes 7.6 us with 16, 5.8 with 4, of 8192 to 2048
-// 12.0 with 16, 10.4 with 8.  32 for 33 and more rows where 16 would make more than 256 of them, for x is read half as often (64 rows, hidden of 2048
-// to 8192 28.6 us and 23.8; 1024 to 4096 9.6 and 13.1, with half of the CUs idle).
-int cols_of(int64_t M, int64_t N) {
-  if (groups_of(M) == 4 && ceil_div(N, 16) > 256) return 32;
-  for (int cols = 16; cols > 4; cols /= 2)
-    if (ceil_div(N, cols) >= 256) return cols;
-  return 4;
+// rows of x that a workgroup reads (in the second launch either half of h for few of them)
+int rows_read(int64_t M, int parts) { return (int)(parts == 1 && M <= kTwice ? 2 * M : M); }
+// Outputs of a workgroup: of 16, 8, 4, and 32 for 33 and more rows, those with which a CU, in as many rounds as it has workgroups, reads the fewest
+// rows of weights and x.  One row of 4096 to 1024 takes 7.6 us with 16, 5.8 with 4; of 8192 to 2048 12.0 with 16, 10.4 with 8; hidden of 2048 to 5461 13.3
+// with 16, 11.4 with 8.  64 rows, hidden of 2048 to 8192 28.6 us with 16 and 23.8 with 32; of 1024 to 4096 9.6 and 13.1.  (24 rows, 2048 to 8192 and to 5461:
+// 17.3 and 17.0 with 16, 18.3 and 15.3 with 32, which were not worth an instance.)
+int cols_of(int64_t M, int64_t N, int parts) {
+  int best = 0;
+  int64_t least = 0;
+  for (int cols = groups_of(M) == 4 ? 32 : 16; cols >= 4; cols /= 2) {
+    const int64_t cost = ceil_div(ceil_div(N, cols), 256) * (cols * parts + rows_read(M, parts));
+    if (best == 0 || cost < least) {
+      best = cols;
+      least = cost;
+    }
+  }
+  return best;
 }
-// What a launch is expected to take, us: 2.3, and for every CU the lines that come back to it at 33 GB/s, or the weights at 4.6 TB/s.
-// Measured and so expected, hidden of 2048 to 8192 at 16, 24 and 64 rows: 15.1, 14.2   17.2, 18.2   23.8, 18.2 (of x nobody's lanes share); outputs of 8192
-// to 2048: 14.2, 14.2   18.5, 22.2   35.7, 38.0.
+// What a launch is expected to take, us: 2, 0.35 for each 16 x 16 outputs whose parts its waves add up, and for every CU the lines that come back to it
+// at 33 GB/s, or the weights at 4.6 TB/s.  Measured and so expected, hidden of 2048 to 8192 at 16, 24 and 64 rows: 15.1, 16.9   17.2, 17.3   23.8, 20.7;
+// outputs of 8192 to 2048: 14.2, 14.3   18.5, 18.6   35.7, 39.1.
 double few_us(int64_t M, int64_t N, int64_t K, int parts) {
-  const int cols = cols_of(M, N);
+  const int cols = cols_of(M, N, parts);
   const double pieces = (double)ceil_div(K, kDeep), wgs = (double)ceil_div(N, cols), rounds = wgs > 256.0 ? wgs / 256.0 : 1.0;
-  const double rows = groups_of(M) == 1 ? (double)(parts == 1 && M <= kTwice ? 2 * M : M) : 16.0 * groups_of(M);
-  const double returned = rounds * pieces * 128.0 * (cols * parts + rows) / 33e3, weights = 2.0 * parts * (double)N * (double)K / 4.6e6;
-  return 2.3 + (returned > weights ? returned : weights);
+  const double returned = rounds * pieces * 128.0 * (cols * parts + rows_read(M, parts)) / 33e3, weights = 2.0 * parts * (double)N * (double)K / 4.6e6;
+  return 2.0 + 0.35 * groups_of(M) * (cols > 16 ? 2 : 1) + (returned > weights ? returned : weights);
 }
 
 template <typename T, bool HIDDEN>
 void launch_few(const Few& f, hipStream_t stream) {
   Few g = f;
-  const int groups = groups_of(g.M), cols = cols_of(g.M, g.N);
+  const int groups = groups_of(g.M), cols = cols_of(g.M, g.N, HIDDEN ? 2 : 1);
   g.cols = cols;
   const dim3 grid((unsigned)ceil_div(g.N, cols)), block(512);
   // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 15.0 us, with one 16.0), one for more (24 rows 17.2, with two 19.3)
@@ -259,7 +267,7 @@ int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi,
   g.K = (int)F;
   if (dtype == SD_BF16) launch_few<BF16, false>(g, (hipStream_t)stream);
   else launch_few<F16, false>(g, (hipStream_t)stream);
-  note_kernel("gated:few groups=%d cols=%d,%d", groups_of(M), cols_of(M, F), cols_of(M, N));
+  note_kernel("gated:few groups=%d cols=%d,%d", groups_of(M), cols_of(M, F, 2), cols_of(M, N, 1));
   return check_launch("gated_mlp_few");
 }
 
