@@ -28,34 +28,69 @@ struct Few {
   int cols;          // of a workgroup, where that owns 16 or fewer
 };
 
-// 16 consecutive elements of a row, 16 q .. + 15 of a piece; left: those behind `at` that are there
-__device__ inline void load_some16(const uint16_t* at, int left, u32x4 (&v)[2]) {
+// 16 consecutive elements of a row, 16 q .. + 15 of a piece, as whole dwords, with one more behind them where rows may begin inside a dword (ODD):
+// a load that begins there takes twice as long as one that is shifted afterwards (one row of 5461 to 2048 at a pitch of 5461: 13.6 us, at 5462 8.8).  No
+// dword is read of which no element is wanted.
+typedef u32x4 __attribute__((aligned(4))) u32x4_dwords;
+template <bool ODD>
+struct Sixteen {
+  u32x4 v[2];
+  uint32_t behind;
+  __device__ inline void none() {
+    v[0] = v[1] = u32x4{0u, 0u, 0u, 0u};
+    if constexpr (ODD) behind = 0u;
+  }
+  __device__ inline void load(const uint16_t* at) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+    const char* from = reinterpret_cast<const char*>(ODD ? a & ~uintptr_t(3) : a);
+    v[0] = *reinterpret_cast<const u32x4_dwords*>(from);
+    v[1] = *reinterpret_cast<const u32x4_dwords*>(from + 16);
+    if constexpr (ODD) behind = *reinterpret_cast<const uint32_t*>(from + 28 + (a & 2) * 2);
+  }
+  // those of `left` that are there, zeros behind them: the dwords in which one is wanted, the last one's upper half taken out where it is none
+  __device__ inline void load_some(const uint16_t* at, int left, uint32_t shift) {
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(3));
+    const int halves = left <= 0 ? 0 : left + (int)(shift >> 4);  // from the first dword on
+    auto dword = [&](int i) { return 2 * i >= halves ? 0u : 2 * i + 1 < halves ? from[i] : from[i] & 0xffffu; };
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = dword(i);
+    if constexpr (ODD) behind = dword(8);
+  }
+  // shift: 16 where the first element is a dword's upper half
+  __device__ inline void settle(uint32_t shift) {
+    if constexpr (!ODD) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = 8 * h + 2 * i;
-      v[h][i] = (c < left ? at[c] : 0u) | (c + 1 < left ? (uint32_t)at[c + 1] << 16 : 0u);
-    }
-}
-__device__ inline void load16(const uint16_t* at, u32x4 (&v)[2]) {
-  v[0] = *reinterpret_cast<const u32x4_any*>(at);
-  v[1] = *reinterpret_cast<const u32x4_any*>(at + 8);
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = __builtin_amdgcn_alignbit(i < 7 ? v[(i + 1) / 4][(i + 1) % 4] : behind, v[i / 4][i % 4], shift);
+  }
+  // zeros for the first n
+  __device__ inline void drop(int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = 2 * i >= n ? v[i / 4][i % 4] : 2 * i + 1 >= n ? v[i / 4][i % 4] & 0xffff0000u : 0u;
+  }
+};
+template <bool ODD>
+__device__ inline uint32_t shift_of(const uint16_t* at) {
+  return ODD ? (uint32_t)(reinterpret_cast<uintptr_t>(at) & 2u) << 3 : 0u;
 }
 
-// HIDDEN: the first launch (both projections), else the second
-template <typename T, bool HIDDEN, int WAVES, int GROUPS, int COLS, int AHEAD>
+// HIDDEN: the first launch (both projections), else the second.  ODD: rows of weights or x may begin inside a dword
+template <typename T, bool HIDDEN, int WAVES, int GROUPS, int COLS, int AHEAD, bool ODD>
 __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
   constexpr int WP = HIDDEN ? 2 : 1;
+  constexpr bool ODD_X = ODD && HIDDEN;  // (h has rows of whole lines)
   __shared__ float sums[WAVES][WP][16][17];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15, q = lane >> 4;
-  const int per = COLS == 1 ? g.cols : 16 * COLS, n0 = (int)blockIdx.x * per, whole = g.K / kDeep, left = g.K - whole * kDeep;
+  const int per = COLS == 1 ? g.cols : 16 * COLS, n0 = (int)blockIdx.x * per;
   const bool twice = g.M <= kTwice;
   const uint16_t* w[COLS][WP];
+  uint32_t w_shift[COLS][WP], x_shift[GROUPS];
 #pragma unroll
   for (int j = 0; j < COLS; ++j)
 #pragma unroll
-    for (int p = 0; p < WP; ++p) w[j][p] = g.w + (int64_t)(min(n0 + 16 * j + r, g.N - 1) + p * g.N) * g.ldw + 16 * q;
+    for (int p = 0; p < WP; ++p) {
+      w[j][p] = g.w + (int64_t)(min(n0 + 16 * j + r, g.N - 1) + p * g.N) * g.ldw + 16 * q;
+      w_shift[j][p] = shift_of<ODD>(w[j][p]);
+    }
   const bool reads_w = COLS > 1 || r < per;
   const uint16_t* x[GROUPS];
   bool reads_x[GROUPS];
@@ -64,9 +99,24 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
     const int row = 16 * i + r;
     reads_x[i] = HIDDEN || !twice ? row < g.M : (r & (kTwice - 1)) < g.M;
     x[i] = g.x + (int64_t)(reads_x[i] ? row : 0) * g.ldx + 16 * q;
+    x_shift[i] = shift_of<ODD_X>(x[i]);
   }
   f32x4 acc[GROUPS][COLS][WP] = {};
-  auto multiply = [&](const u32x4 (&a)[GROUPS][2], const u32x4 (&b)[COLS][WP][2]) {
+  // k: where the piece begins; over: how many of its elements pieces in front have
+  auto multiply = [&](Sixteen<ODD_X> (&a)[GROUPS], Sixteen<ODD> (&b)[COLS][WP], int k, int over) {
+    const uint32_t turned = (uint32_t)(k & 1) << 4;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      a[i].settle(x_shift[i] ^ turned);
+      if (over) a[i].drop(over - 16 * q);
+    }
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+#pragma unroll
+      for (int p = 0; p < WP; ++p) {
+        b[j][p].settle(w_shift[j][p] ^ turned);
+        if (over) b[j][p].drop(over - 16 * q);
+      }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -74,31 +124,30 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-          for (int j = 0; j < COLS; ++j) acc[i][j][p] = T::mfma16(a[i][h], b[j][p][h], acc[i][j][p]);
+          for (int j = 0; j < COLS; ++j) acc[i][j][p] = T::mfma16(a[i].v[h], b[j][p].v[h], acc[i][j][p]);
   };
-  const u32x4 none = {0u, 0u, 0u, 0u};
-  for (int c0 = wave; c0 < whole; c0 += WAVES * AHEAD) {
-    u32x4 b[AHEAD][COLS][WP][2], a[AHEAD][GROUPS][2];
+  // Workgroups begin at different pieces: rows a power of two apart lie in one channel of memory, which all of them would ask for the same pieces at a
+  // time (one row, hidden of 2048 to 8192: 15.0 us, so 13.3; 64 rows 23.5 and 21.3).
+  const int whole = g.K / kDeep, first = whole ? (int)((blockIdx.x / 8u) % (unsigned)whole) : 0;
+  auto place = [&](int c) { return (c + first < whole ? c + first : c + first - whole) * kDeep; };
+  auto load = [&](Sixteen<ODD_X> (&a)[AHEAD][GROUPS], Sixteen<ODD> (&b)[AHEAD][COLS][WP], auto&& there, auto&& at) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int j = 0; j < COLS; ++j)
 #pragma unroll
-        for (int j = 0; j < COLS; ++j)
+        for (int p = 0; p < WP; ++p) b[u][j][p].none();
 #pragma unroll
-          for (int p = 0; p < WP; ++p) b[u][j][p][h] = none;
-#pragma unroll
-        for (int i = 0; i < GROUPS; ++i) a[u][i][h] = none;
-      }
+      for (int i = 0; i < GROUPS; ++i) a[u][i].none();
     }
     if (reads_w) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
-        if (c0 + u * WAVES < whole) {
+        if (there(u)) {
 #pragma unroll
           for (int j = 0; j < COLS; ++j)
 #pragma unroll
-            for (int p = 0; p < WP; ++p) load16(w[j][p] + (int64_t)(c0 + u * WAVES) * kDeep, b[u][j][p]);
+            for (int p = 0; p < WP; ++p) b[u][j][p].load(w[j][p] + at(u));
         }
     }
 #pragma unroll
@@ -106,22 +155,30 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
       if (reads_x[i]) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-          if (c0 + u * WAVES < whole) load16(x[i] + (int64_t)(c0 + u * WAVES) * kDeep, a[u][i]);
+          if (there(u)) a[u][i].load(x[i] + at(u));
       }
+  };
+  Sixteen<ODD> b[AHEAD][COLS][WP];
+  Sixteen<ODD_X> a[AHEAD][GROUPS];
+  for (int c0 = wave; c0 < whole; c0 += WAVES * AHEAD) {
+    load(a, b, [&](int u) { return c0 + u * WAVES < whole; }, [&](int u) { return place(c0 + u * WAVES); });
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (c0 + u * WAVES < whole) multiply(a[u], b[u]);
+      if (c0 + u * WAVES < whole) multiply(a[u], b[u], 0, 0);
   }
-  if (left && wave == whole % WAVES) {
-    const int64_t k = (int64_t)whole * kDeep;
-    u32x4 b[COLS][WP][2], a[GROUPS][2];
+  if (g.K % kDeep && wave == whole % WAVES) {
+    if (whole) {  // what no whole piece has, as the end of one more
+      load(a, b, [](int u) { return u == 0; }, [&](int) { return g.K - kDeep; });
+      multiply(a[0], b[0], g.K, kDeep - g.K % kDeep);
+    } else {
 #pragma unroll
-    for (int j = 0; j < COLS; ++j)
+      for (int j = 0; j < COLS; ++j)
 #pragma unroll
-      for (int p = 0; p < WP; ++p) load_some16(w[j][p] + k, reads_w ? left - 16 * q : 0, b[j][p]);
+        for (int p = 0; p < WP; ++p) b[0][j][p].load_some(w[j][p], reads_w ? g.K - 16 * q : 0, w_shift[j][p]);
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) load_some16(x[i] + k, reads_x[i] ? left - 16 * q : 0, a[i]);
-    multiply(a, b);
+      for (int i = 0; i < GROUPS; ++i) a[0][i].load_some(x[i], reads_x[i] ? g.K - 16 * q : 0, x_shift[i]);
+      multiply(a[0], b[0], 0, 0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i)
@@ -194,17 +251,25 @@ double few_us(int64_t M, int64_t N, int64_t K, int parts) {
   return 2.0 + 0.35 * groups_of(M) * (cols > 16 ? 2 : 1) + (returned > weights ? returned : weights);
 }
 
-template <typename T, bool HIDDEN>
+template <typename T, bool HIDDEN, bool ODD>
 void launch_few(const Few& f, hipStream_t stream) {
   Few g = f;
   const int groups = groups_of(g.M), cols = cols_of(g.M, g.N, HIDDEN ? 2 : 1);
   g.cols = cols;
   const dim3 grid((unsigned)ceil_div(g.N, cols)), block(512);
   // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 15.0 us, with one 16.0), one for more (24 rows 17.2, with two 19.3)
-  if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2>), grid, block, 0, stream, g);
-  else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1>), grid, block, 0, stream, g);
-  else if (cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1>), grid, block, 0, stream, g);
-  else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1>), grid, block, 0, stream, g);
+  if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2, ODD>), grid, block, 0, stream, g);
+  else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1, ODD>), grid, block, 0, stream, g);
+  else if (cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1, ODD>), grid, block, 0, stream, g);
+  else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1, ODD>), grid, block, 0, stream, g);
+}
+
+template <bool HIDDEN>
+void launch_few_of(const Few& g, int dtype, hipStream_t stream) {
+  const auto inside_dwords = [](const uint16_t* at, int64_t ld) { return (reinterpret_cast<uintptr_t>(at) & 2) != 0 || ld % 2 != 0; };
+  const bool odd = inside_dwords(g.w, g.ldw) || (HIDDEN && inside_dwords(g.x, g.ldx));
+  if (dtype == SD_BF16) odd ? launch_few<BF16, HIDDEN, true>(g, stream) : launch_few<BF16, HIDDEN, false>(g, stream);
+  else odd ? launch_few<F16, HIDDEN, true>(g, stream) : launch_few<F16, HIDDEN, false>(g, stream);
 }
 
 // Pitch of h: an odd number of whole pieces (rows a power of two apart lie in one channel of the L2).
@@ -254,8 +319,7 @@ int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi,
   g.N = (int)F;
   g.K = (int)K;
   g.act = act;
-  if (dtype == SD_BF16) launch_few<BF16, true>(g, (hipStream_t)stream);
-  else launch_few<F16, true>(g, (hipStream_t)stream);
+  launch_few_of<true>(g, dtype, (hipStream_t)stream);
   if (int rc = check_launch("gated_mlp_few")) return rc;
   g.x = g.h;
   g.w = static_cast<const uint16_t*>(W_out);
@@ -265,8 +329,7 @@ int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi,
   g.ldy = ldy;
   g.N = (int)N;
   g.K = (int)F;
-  if (dtype == SD_BF16) launch_few<BF16, false>(g, (hipStream_t)stream);
-  else launch_few<F16, false>(g, (hipStream_t)stream);
+  launch_few_of<false>(g, dtype, (hipStream_t)stream);
   note_kernel("gated:few groups=%d cols=%d,%d", groups_of(M), cols_of(M, F, 2), cols_of(M, N, 1));
   return check_launch("gated_mlp_few");
 }

@@ -1,5 +1,6 @@
 """The gated feed-forward block on the GPU against its formulas in 64 bits: element by element within the bounds that oracle/gated_oracle.py
 derives from the roundings, and within the package's bar of 1e-2 in the relative Frobenius norm."""
+import math
 import os
 import subprocess
 import sys
@@ -409,3 +410,83 @@ def test_a_gradient_in_any_layout_or_type():
     y.float().sum().backward()  # an expanded gradient
     ones = run(*ops[:3], torch.ones(130, 40, device="cuda").bfloat16(), "silu")
     assert all(torch.equal(t.grad, ones[name]) for t, name in zip(leaves, NAMES[1:]))
+
+
+@pytest.mark.parametrize("m", [3, 24, 40, 200])
+@pytest.mark.parametrize("k,f,n", [(100, 77, 33), (65, 130, 64), (63, 62, 40), (136, 200, 72)])
+def test_what_is_not_finite_stays_in_its_row(m, k, f, n):
+    """An infinity or a NaN of a row reaches no other, wherever in the row it stands (the last elements are read with those in front of them)."""
+    ops = operands(m, k, f, n, "fp16", seed=90)
+    with torch.no_grad():
+        ref = F.gated_mlp(*ops[:3], "relu")
+        for bad in (math.inf, math.nan):
+            for at in {0, k // 2, k - 2, k - 1}:
+                x = ops[0].clone()
+                x[1, at] = bad
+                y = F.gated_mlp(x, *ops[1:3], "relu")
+                others = torch.arange(m, device="cuda") != 1
+                assert torch.equal(y[others], ref[others]), (bad, at)
+                assert not torch.isfinite(y[1]).any(), (bad, at)
+
+
+@pytest.mark.parametrize("m", [2, 20, 64])
+@pytest.mark.parametrize("k,f,n", [(63, 65, 3), (129, 100, 66), (70, 64, 33), (5, 7, 3)])
+def test_few_rows_read_nothing_beside_their_rows(m, k, f, n):
+    """NaN in front of, behind and between all rows, which begin at every place of 16 bytes."""
+    assert _loader.load().sd_gated_mlp_few_taken(m, k, f, n)
+    ops = operands(m, k, f, n, "bf16", seed=91)
+    ref = O.reference(*ops, "silu", torch.bfloat16)
+    for before in range(8):
+        views = []
+        for t in ops[:3]:
+            for behind in (1, 2):
+                wide = torch.full((t.shape[0] + 2, before + t.shape[1] + behind), math.nan, dtype=t.dtype, device="cuda")
+                inner = wide[1:-1, before:before + t.shape[1]]
+                inner.copy_(t)
+                views.append(inner)
+        for shift in (0, 1):
+            with torch.no_grad():
+                check({"y": F.gated_mlp(*views[shift::2], "silu")}, ref)
+
+
+@pytest.mark.parametrize("size", [(40, 140000, 64, 64), (8, 64, 140000, 40), (72, 64, 140000, 40)], ids=lambda s: "x".join(map(str, s)))
+def test_very_long_reductions(size):
+    """More blocks than a workgroup of the tile kernels walks: the gate in a pass of its own, or the reduction in parts."""
+    ops = operands(*size, "bf16", seed=92)
+    ref = O.reference(*ops, "silu", torch.bfloat16)
+    check(run(*ops, "silu"), ref)
+    with torch.no_grad():
+        check({"y": F.gated_mlp(*ops[:3], "silu")}, ref)
+    masks = masks_of(*size[:3], 64, 0.5)
+    check(run(*ops, "gelu", 64, 0.5, masks), O.reference(*ops, "gelu", torch.bfloat16, masks, 64, (0.5, 0.5)))
+
+
+def test_few_rows_captured_and_replayed():
+    """Two graphs of the few rows of serving beside each other: either has a workspace of its own."""
+    calls = []
+    for i, size in enumerate(((1, 1024, 4096, 1024), (24, 333, 777, 100))):
+        ops = operands(*size, "bf16", seed=93 + i)
+        static = [t.clone() for t in ops[:3]]
+        with torch.no_grad():
+            F.gated_mlp(*static)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = F.gated_mlp(*static)
+        calls.append((size, static, graph, y))
+    side = torch.cuda.Stream()
+    for seed in (95, 96, 97):
+        refs = []
+        for size, static, _, _ in calls:
+            fresh = operands(*size, "bf16", seed=seed)
+            with torch.no_grad():
+                for t, v in zip(static, fresh):
+                    t.copy_(v)
+                refs.append(F.gated_mlp(*fresh[:3]))
+        torch.cuda.synchronize()
+        calls[0][2].replay()
+        with torch.cuda.stream(side):
+            calls[1][2].replay()
+        torch.cuda.synchronize()
+        for (_, _, _, y), ref in zip(calls, refs):
+            assert torch.equal(y, ref)
