@@ -744,12 +744,12 @@ int sd_gated_matmul_gradient(const void* dY, int64_t dy_stride_r, int64_t dy_str
                              int64_t h_stride_r, int64_t h_stride_c, void* dW, int64_t dw_stride_r, int64_t dw_stride_c, const int32_t* row_ptr,
                              const int32_t* col_idx, const int32_t* col_ptr, const int32_t* row_idx, int64_t M, int64_t F, int64_t N,
                              int64_t block_size, double p, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
-/* sd_gated_mlp_few: Y = (act(X W_g^T) (X W_u^T)) W_out^T for up to SD_GATED_FEW_ROWS rows in two launches that read each weight once; everything
+/* sd_gated_mlp_few: Y = (act(X W_g^T) (X W_u^T)) W_out^T for up to SD_GATED_FEW_ROWS rows in two or three launches that read each weight once; everything
  * row-major, rows of any pitch at any address.  Up to 8 rows keep the hidden activations to twice 16 bits, more round them to the operands' type.
  * workspace: sd_gated_mlp_few_workspace_bytes bytes on 16 bytes, of one call at a time.  sd_gated_mlp_few_taken: whether that is expected to be faster
  * than sd_gated_matmul and sd_gemm (up to 16 rows always). */
 #define SD_GATED_FEW_ROWS 64
-int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F);
+int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F, int64_t N);
 int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N);
 int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi, const void* W_out, int64_t ldwo, void* Y, int64_t ldy,
                      int64_t M, int64_t K, int64_t F, int64_t N, int act, int dtype, void* workspace, int64_t workspace_bytes, void* stream);

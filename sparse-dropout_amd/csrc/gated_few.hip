@@ -1,13 +1,14 @@
-// A gated feed-forward block for few rows, the tokens of a serving step: two launches that read each weight once.
+// A gated feed-forward block for few rows, the tokens of a serving step: launches that read each weight once.
 //
 //   h = act(x W_g^T) (x W_u^T)        y = h W_out^T
 //
 // Bound by the weights' bytes, 2 (2 F K + N F), and with few of them by a memory latency and a launch each.  So weights go from memory straight
-// into the matrix instruction's registers.  A workgroup owns 16 outputs (or 32, or 8 or 4 where there would be too few workgroups: the others' lanes load
+// into the matrix instruction's registers.  A workgroup owns 16 outputs (or 32; or 8 or 4 where there would be too few workgroups: the others' lanes load
 // nothing); its waves share out the 64-deep pieces of the reduction, which are whole 128-byte lines of its weight rows, wave w every piece
 // w + WAVES n, AHEAD of them on their way at a time, and meet once in LDS.  A lane takes 32 consecutive bytes of a line (two loads, four lanes to a
 // line); the order of the reduction within a piece is the same for both operands and shows in nothing but the last bits.  Rows come in groups of
-// 16.  What comes back to a CU, 64 bytes a clock, is what a full group of rows costs beside the weights, so lanes of rows that are not there load nothing.
+// 16.  What comes back to a CU is what a group of rows costs beside the weights: lanes of rows that are not there load nothing, and where a workgroup
+// would read more of h than of weights, the second launch's reduction is shared out over workgroups of more outputs, whose sums a third adds up.
 //
 // Up to 8 rows leave room for h twice in a group: h, which nothing but the second launch reads, is then held as the sum of two 16-bit numbers, the
 // low halves in rows 8 to 15, and its rounding, the largest of the path, is saved.
@@ -26,6 +27,8 @@ struct Few {
   int64_t ldx, ldw, ldh, ldy;
   int M, N, K, act;  // N: hidden columns or outputs
   int cols;          // of a workgroup, where that owns 16 or fewer
+  float* parts;      // of the second launch's sums, [gridDim.y][M][N], where its reduction is shared out over more workgroups ...
+  int share;         // ... of so many pieces each
 };
 
 // 16 consecutive elements of a row, 16 q .. + 15 of a piece, as whole dwords, with one more behind them where rows may begin inside a dword (ODD):
@@ -73,8 +76,9 @@ __device__ inline uint32_t shift_of(const uint16_t* at) {
   return ODD ? (uint32_t)(reinterpret_cast<uintptr_t>(at) & 2u) << 3 : 0u;
 }
 
-// HIDDEN: the first launch (both projections), else the second.  ODD: rows of weights or x may begin inside a dword
-template <typename T, bool HIDDEN, int WAVES, int GROUPS, int COLS, int AHEAD, bool ODD>
+// HIDDEN: the first launch (both projections), else the second.  ODD: rows of weights or x may begin inside a dword.  SHARED: the reduction is shared
+// out (0.2 us of a row's 6 where it is not)
+template <typename T, bool HIDDEN, int WAVES, int GROUPS, int COLS, int AHEAD, bool ODD, bool SHARED>
 __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
   constexpr int WP = HIDDEN ? 2 : 1;
   constexpr bool ODD_X = ODD && HIDDEN;  // (h has rows of whole lines)
@@ -128,8 +132,9 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
   };
   // Workgroups begin at different pieces: rows a power of two apart lie in one channel of memory, which all of them would ask for the same pieces at a
   // time (one row, hidden of 2048 to 8192: 15.0 us, so 13.3; 64 rows 23.5 and 21.3).
-  const int whole = g.K / kDeep, first = whole ? (int)((blockIdx.x / 8u) % (unsigned)whole) : 0;
-  auto place = [&](int c) { return (c + first < whole ? c + first : c + first - whole) * kDeep; };
+  const int pieces = g.K / kDeep, from = SHARED ? (int)blockIdx.y * g.share : 0, whole = SHARED ? min(g.share, pieces - from) : pieces;
+  const int first = (int)(((blockIdx.x >> 3) & 31u) * (unsigned)whole >> 5);
+  auto place = [&](int c) { return (from + (c + first < whole ? c + first : c + first - whole)) * kDeep; };
   auto load = [&](Sixteen<ODD_X> (&a)[AHEAD][GROUPS], Sixteen<ODD> (&b)[AHEAD][COLS][WP], auto&& there, auto&& at) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
@@ -166,8 +171,8 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
     for (int u = 0; u < AHEAD; ++u)
       if (c0 + u * WAVES < whole) multiply(a[u], b[u], 0, 0);
   }
-  if (g.K % kDeep && wave == whole % WAVES) {
-    if (whole) {  // what no whole piece has, as the end of one more
+  if (g.K % kDeep && wave == whole % WAVES && from + whole == pieces) {
+    if (pieces) {  // what no whole piece has, as the end of one more
       load(a, b, [](int u) { return u == 0; }, [&](int) { return g.K - kDeep; });
       multiply(a[0], b[0], g.K, kDeep - g.K % kDeep);
     } else {
@@ -215,66 +220,88 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
               for (int o = 0; o < WAVES; ++o) low += sums[o][0][kTwice + (at & (kTwice - 1))][col];
               s[0] += low;
             }
-            if (n < g.N) g.y[(int64_t)m * g.ldy + n] = T::from_float(s[0]);
+            if (n < g.N) {
+              if constexpr (SHARED) g.parts[((int64_t)blockIdx.y * g.M + m) * g.N + n] = s[0];
+              else g.y[(int64_t)m * g.ldy + n] = T::from_float(s[0]);
+            }
           }
         }
       }
     }
 }
 
-int groups_of(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
-// rows of x that a workgroup reads (in the second launch either half of h for few of them)
-int rows_read(int64_t M, int parts) { return (int)(parts == 1 && M <= kTwice ? 2 * M : M); }
-// Outputs of a workgroup: of 16, 8, 4, and 32 for 33 and more rows, those with which a CU, in as many rounds as it has workgroups, reads the fewest
-// rows of weights and x.  One row of 4096 to 1024 takes 7.6 us with 16, 5.8 with 4; of 8192 to 2048 12.0 with 16, 10.4 with 8; hidden of 2048 to 5461 13.3
-// with 16, 11.4 with 8.  64 rows, hidden of 2048 to 8192 28.6 us with 16 and 23.8 with 32; of 1024 to 4096 9.6 and 13.1.  (24 rows, 2048 to 8192 and to 5461:
-// 17.3 and 17.0 with 16, 18.3 and 15.3 with 32, which were not worth an instance.)
-int cols_of(int64_t M, int64_t N, int parts) {
-  int best = 0;
-  int64_t least = 0;
-  for (int cols = groups_of(M) == 4 ? 32 : 16; cols >= 4; cols /= 2) {
-    const int64_t cost = ceil_div(ceil_div(N, cols), 256) * (cols * parts + rows_read(M, parts));
-    if (best == 0 || cost < least) {
-      best = cols;
-      least = cost;
-    }
-  }
-  return best;
-}
-// What a launch is expected to take, us: 2, 0.35 for each 16 x 16 outputs whose parts its waves add up, and for every CU the lines that come back to it
-// at 33 GB/s, or the weights at 4.6 TB/s.  Measured and so expected, hidden of 2048 to 8192 at 16, 24 and 64 rows: 15.1, 16.9   17.2, 17.3   23.8, 20.7;
-// outputs of 8192 to 2048: 14.2, 14.3   18.5, 18.6   35.7, 39.1.
-double few_us(int64_t M, int64_t N, int64_t K, int parts) {
-  const int cols = cols_of(M, N, parts);
-  const double pieces = (double)ceil_div(K, kDeep), wgs = (double)ceil_div(N, cols), rounds = wgs > 256.0 ? wgs / 256.0 : 1.0;
-  const double returned = rounds * pieces * 128.0 * (cols * parts + rows_read(M, parts)) / 33e3, weights = 2.0 * parts * (double)N * (double)K / 4.6e6;
-  return 2.0 + 0.35 * groups_of(M) * (cols > 16 ? 2 : 1) + (returned > weights ? returned : weights);
+// the parts' sums, always in one order
+template <typename T>
+__global__ __launch_bounds__(256) void few_sum_kernel(Few g, int shares) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)g.M * g.N;
+  if (at >= all) return;
+  float sum = 0.f;
+  for (int i = 0; i < shares; ++i) sum += g.parts[i * all + at];
+  g.y[at / g.N * g.ldy + at % g.N] = T::from_float(sum);
 }
 
-template <typename T, bool HIDDEN, bool ODD>
-void launch_few(const Few& f, hipStream_t stream) {
+int groups_of(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
+
+// A launch's outputs to a workgroup (4, 8, 16, for 17 and more rows 32), how many workgroups share out a reduction, and what it is expected to take, us:
+// 2.5, 0.16 for each 16 x 16 sums that the waves add up, and the longer of the weights at 5.4 TB/s and, for a CU in as many rounds as it has
+// workgroups, the lines that come back to it at 36 GB/s (lanes that load nothing take a quarter of it all the same); 2.8 for the sum of the parts, and those, written
+// and read, at 1.7 TB/s.  Within 7 % (root mean square) of 330 launches measured, 512 to 4096 wide, hidden of 1000 to 8192, and what it picks takes 0.1 %
+// longer than the best of them.  One row of 8192 to 2048: 16 outputs 12.3 us, 8 10.6, with two shares of 16 13.0; 24 rows 8 outputs 18.9,
+// four shares of 32 13.7; 64 rows 36.2, 19.7.  Hidden of 24 rows of 2048: 8192 with 16 17.6, with 32 15.8.
+struct FewPlan {
+  int cols = 0, shares = 0;
+  double us = 1e30;
+};
+FewPlan plan_few(int64_t M, int64_t N, int64_t K, int parts) {
+  const int groups = groups_of(M), rows = (int)(parts == 1 && M <= kTwice ? 2 * M : M);  // (either half of h for few of them)
+  const int64_t pieces = ceil_div(K, kDeep);
+  const double weights = 2.0 * parts * (double)N * (double)K / 5.4e6;
+  FewPlan best;
+  for (int shares = 1; shares <= (parts == 1 ? 8 : 1) && (shares == 1 || pieces >= 8 * shares); shares *= 2)
+    for (int cols = groups > 1 ? 32 : 16; cols >= 4; cols /= 2) {
+      const double rounds = (double)ceil_div(ceil_div(N, cols) * shares, 256), none = (cols < 16 ? 16 - cols : 0) * parts + 16 * groups - rows;
+      const double lines = rounds * (double)pieces / shares * 128.0 * (cols * parts + rows + 0.25 * none) / 36e3;
+      const double us = 2.5 + 0.16 * groups * (cols > 16 ? 2 : 1) * parts + (lines > weights ? lines + 0.05 * weights : weights + 0.05 * lines) +
+                        (shares > 1 ? 2.8 + 8.0 * shares * (double)M * (double)N / 1.7e6 : 0.0);
+      if (us < best.us) best = {cols, shares, us};
+    }
+  return best;
+}
+
+template <typename T, bool HIDDEN, bool ODD, bool SHARED>
+void launch_few(const Few& f, const FewPlan& plan, hipStream_t stream) {
   Few g = f;
-  const int groups = groups_of(g.M), cols = cols_of(g.M, g.N, HIDDEN ? 2 : 1);
-  g.cols = cols;
-  const dim3 grid((unsigned)ceil_div(g.N, cols)), block(512);
-  // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 15.0 us, with one 16.0), one for more (24 rows 17.2, with two 19.3)
-  if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2, ODD>), grid, block, 0, stream, g);
-  else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1, ODD>), grid, block, 0, stream, g);
-  else if (cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1, ODD>), grid, block, 0, stream, g);
-  else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1, ODD>), grid, block, 0, stream, g);
+  const int groups = groups_of(g.M);
+  g.cols = plan.cols;
+  g.share = (int)ceil_div(g.K / kDeep, plan.shares);
+  const dim3 grid((unsigned)ceil_div(g.N, plan.cols), (unsigned)plan.shares), block(512);
+  // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 13.4 us, with one 14.5), one for more (24 rows 17.0, with two 18.0)
+  if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2, ODD, SHARED>), grid, block, 0, stream, g);
+  else if (groups == 2 && plan.cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  else if (plan.cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  if constexpr (SHARED) hipLaunchKernelGGL((&few_sum_kernel<T>), dim3((unsigned)ceil_div((int64_t)g.M * g.N, 256)), dim3(256), 0, stream, g, plan.shares);
+}
+template <typename T, bool HIDDEN>
+void launch_few_type(const Few& g, const FewPlan& plan, bool odd, hipStream_t stream) {
+  if constexpr (!HIDDEN)
+    if (plan.shares > 1) return odd ? launch_few<T, HIDDEN, true, true>(g, plan, stream) : launch_few<T, HIDDEN, false, true>(g, plan, stream);
+  odd ? launch_few<T, HIDDEN, true, false>(g, plan, stream) : launch_few<T, HIDDEN, false, false>(g, plan, stream);
 }
 
 template <bool HIDDEN>
-void launch_few_of(const Few& g, int dtype, hipStream_t stream) {
+void launch_few_of(const Few& g, const FewPlan& plan, int dtype, hipStream_t stream) {
   const auto inside_dwords = [](const uint16_t* at, int64_t ld) { return (reinterpret_cast<uintptr_t>(at) & 2) != 0 || ld % 2 != 0; };
   const bool odd = inside_dwords(g.w, g.ldw) || (HIDDEN && inside_dwords(g.x, g.ldx));
-  if (dtype == SD_BF16) odd ? launch_few<BF16, HIDDEN, true>(g, stream) : launch_few<BF16, HIDDEN, false>(g, stream);
-  else odd ? launch_few<F16, HIDDEN, true>(g, stream) : launch_few<F16, HIDDEN, false>(g, stream);
+  if (dtype == SD_BF16) launch_few_type<BF16, HIDDEN>(g, plan, odd, stream);
+  else launch_few_type<F16, HIDDEN>(g, plan, odd, stream);
 }
 
 // Pitch of h: an odd number of whole pieces (rows a power of two apart lie in one channel of the L2).
 int64_t hidden_pitch(int64_t F) { return (ceil_div(F, kDeep) | 1) * kDeep; }
-int64_t hidden_rows(int64_t M) { return M <= kTwice ? 2 * kTwice : M; }
+int64_t hidden_bytes(int64_t M, int64_t F) { return 2 * (M <= kTwice ? 2 * kTwice : M) * hidden_pitch(F); }
+int64_t parts_bytes(const FewPlan& plan, int64_t M, int64_t N) { return plan.shares > 1 ? 4 * plan.shares * M * N : 0; }
 
 }  // namespace
 }  // namespace sd
@@ -283,8 +310,9 @@ using namespace sd;
 
 extern "C" {
 
-int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F) {
-  return M <= 0 || M > SD_GATED_FEW_ROWS || F <= 0 || F >= (1LL << 29) ? 0 : 2 * hidden_rows(M) * hidden_pitch(F);
+int64_t sd_gated_mlp_few_workspace_bytes(int64_t M, int64_t F, int64_t N) {
+  if (M <= 0 || M > SD_GATED_FEW_ROWS || F <= 0 || F >= (1LL << 29) || N <= 0 || N >= (1LL << 29)) return 0;
+  return hidden_bytes(M, F) + parts_bytes(plan_few(M, N, F, 1), M, N);
 }
 
 int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N) {
@@ -292,7 +320,7 @@ int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N) {
   if (M <= 16) return 1;
   // Rows that do not begin on 16 bytes are copied first on the other way: weights and activations at 3 TB/s, a launch each
   const double copied = (K % 8 ? 4.0 + 8.0 * F * K / 3e6 : 0.0) + (F % 8 ? 4.0 + 4.0 * N * F / 3e6 : 0.0);
-  return 1.1 * (few_us(M, F, K, 2) + few_us(M, N, F, 1)) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
+  return 1.05 * (plan_few(M, F, K, 2).us + plan_few(M, N, F, 1).us) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
 }
 
 int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi, const void* W_out, int64_t ldwo, void* Y, int64_t ldy, int64_t M,
@@ -305,7 +333,8 @@ int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi,
   if (M > SD_GATED_FEW_ROWS) return fail(SD_ERR_UNSUPPORTED, "gated_mlp_few: %lld rows, at most %d", (long long)M, SD_GATED_FEW_ROWS);
   SD_REQUIRE(X && W_in && W_out && Y, "gated_mlp_few: null pointer");
   SD_REQUIRE((M == 1 || (ldx >= K && ldy >= N)) && ldwi >= K && (N == 1 || ldwo >= F), "gated_mlp_few: a pitch is shorter than its row");
-  const int64_t need = sd_gated_mlp_few_workspace_bytes(M, F);
+  const FewPlan hidden = plan_few(M, F, K, 2), outputs = plan_few(M, N, F, 1);
+  const int64_t need = hidden_bytes(M, F) + parts_bytes(outputs, M, N);
   SD_REQUIRE(workspace && workspace_bytes >= need, "gated_mlp_few: workspace too small: need %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
   SD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "gated_mlp_few: workspace must be 16-byte aligned");
   Few g = {};
@@ -319,18 +348,19 @@ int sd_gated_mlp_few(const void* X, int64_t ldx, const void* W_in, int64_t ldwi,
   g.N = (int)F;
   g.K = (int)K;
   g.act = act;
-  launch_few_of<true>(g, dtype, (hipStream_t)stream);
+  launch_few_of<true>(g, hidden, dtype, (hipStream_t)stream);
   if (int rc = check_launch("gated_mlp_few")) return rc;
   g.x = g.h;
   g.w = static_cast<const uint16_t*>(W_out);
   g.y = static_cast<uint16_t*>(Y);
+  if (outputs.shares > 1) g.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + hidden_bytes(M, F));
   g.ldx = g.ldh;
   g.ldw = ldwo;
   g.ldy = ldy;
   g.N = (int)N;
   g.K = (int)F;
-  launch_few_of<false>(g, dtype, (hipStream_t)stream);
-  note_kernel("gated:few groups=%d cols=%d,%d", groups_of(M), cols_of(M, F, 2), cols_of(M, N, 1));
+  launch_few_of<false>(g, outputs, dtype, (hipStream_t)stream);
+  note_kernel("gated:few groups=%d cols=%d,%d shares=%d", groups_of(M), hidden.cols, outputs.cols, outputs.shares);
   return check_launch("gated_mlp_few");
 }
 

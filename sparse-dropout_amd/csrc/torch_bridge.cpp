@@ -823,7 +823,7 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
     } else if (!rec && !drops(0) && !drops(1) && row_major(wi) && row_major(wo) && sd_gated_mlp_few_taken(M, K, F, N)) {
       const Tensor rows = rows_of(x);
       y = new_matrix(x, M, N);
-      const Scratch ws(x, sd_gated_mlp_few_workspace_bytes(M, F));
+      const Scratch ws(x, sd_gated_mlp_few_workspace_bytes(M, F, N));
       const Mat xm(rows), im(wi), om(wo);
       c10::DeviceGuard device(x.device());
       check(sd_gated_mlp_few(xm.ptr, xm.sr, im.ptr, im.sr, om.ptr, om.sr, y.data_ptr(), N, M, K, F, N, act, dtype_of(x), ws.ptr, ws.bytes, stream_of(x)),

@@ -150,7 +150,7 @@ SIGNATURES = {
                                                 *([c_void_p] * 5), *([c_int64] * 4), c_int, c_int, c_void_p]),
     "sd_gated_matmul_gradient": (c_int, [*_mat, *_mat, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, *_mat, *_mat, *([c_void_p] * 4), *([c_int64] * 4),
                                          c_double, c_int, c_int, c_void_p, c_int64, c_void_p]),
-    "sd_gated_mlp_few_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "sd_gated_mlp_few_workspace_bytes": (c_int64, [c_int64] * 3),
     "sd_gated_mlp_few_taken": (c_int, [c_int64] * 4),
     "sd_gated_mlp_few": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
                                  c_void_p, c_int64, c_void_p]),

@@ -307,7 +307,7 @@ def few(x, w_in, w_out, act, pitches=(0, 0, 0, 0)):
 
     xs, ws, os_ = (wide(t, p) for t, p in zip((x, w_in, w_out), pitches))
     y = torch.full((m + 2, n + pitches[3]), guard, dtype=x.dtype, device="cuda")
-    need = lib.sd_gated_mlp_few_workspace_bytes(m, f)
+    need = lib.sd_gated_mlp_few_workspace_bytes(m, f, n)
     scratch = torch.full((need + 64,), 0x5a, dtype=torch.uint8, device="cuda")
     rc = lib.sd_gated_mlp_few(xs.data_ptr(), xs.stride(0), ws.data_ptr(), ws.stride(0), os_.data_ptr(), os_.stride(0), y[1:].data_ptr(), y.stride(0), m, k, f, n,
                               {"relu": 1, "gelu": 2, "silu": 3}[act], 1 if x.dtype == torch.bfloat16 else 0, scratch.data_ptr(), need,
@@ -325,6 +325,16 @@ def test_few_rows(m):
         ref = O.reference(*ops, act, DT[dtype])
         check({"y": few(*ops[:3], act)}, ref)
         check({"y": few(*ops[:3], act, (3, 1, 5, 2))}, ref)
+
+
+@pytest.mark.parametrize("m,k,f,n,plan", [(24, 1024, 4096, 1024, ",16 shares=4"), (48, 512, 8192, 2048, ",32 shares=4"), (16, 64, 8192, 2048, "shares=2"),
+                                          (8, 64, 8193, 2047, "shares=2"), (24, 64, 8255, 2040, "shares=4")])
+def test_few_rows_share_out_a_reduction(m, k, f, n, plan):
+    ops = operands(m, k, f, n, "bf16", seed=45)
+    got = few(*ops[:3], "silu", (0, 0, 1, 3))
+    assert plan in _loader.load().sd_last_kernel_detail().decode()
+    check({"y": got}, O.reference(*ops, "silu", torch.bfloat16))
+    assert torch.equal(few(*ops[:3], "silu"), few(*ops[:3], "silu"))
 
 
 def test_few_rows_keep_the_hidden_activations_to_more_than_their_type():

@@ -58,11 +58,12 @@ def test_gated_products_refuse_bad_arguments():
 
 def test_few_rows_refuse_bad_arguments():
     lib = _loader.load()
-    assert lib.sd_gated_mlp_few_workspace_bytes(1, 64) == 2 * 16 * 64 and lib.sd_gated_mlp_few_workspace_bytes(9, 65) == 2 * 9 * 192
-    assert [lib.sd_gated_mlp_few_workspace_bytes(*a) for a in ((0, 64), (65, 64), (4, 0), (4, 1 << 29))] == [0] * 4
+    assert lib.sd_gated_mlp_few_workspace_bytes(1, 64, 16) == 2 * 16 * 64 and lib.sd_gated_mlp_few_workspace_bytes(9, 65, 3) == 2 * 9 * 192
+    assert lib.sd_gated_mlp_few_workspace_bytes(24, 4096, 1024) == 2 * 24 * 65 * 64 + 4 * 4 * 24 * 1024  # a reduction in four shares
+    assert [lib.sd_gated_mlp_few_workspace_bytes(*a) for a in ((0, 64, 8), (65, 64, 8), (4, 0, 8), (4, 1 << 29, 8), (4, 64, 0), (4, 64, 1 << 29))] == [0] * 6
     assert lib.sd_gated_mlp_few_taken(1, 1024, 4096, 1024) == 1 and lib.sd_gated_mlp_few_taken(16, 8192, 8192, 8192) == 1
     assert [lib.sd_gated_mlp_few_taken(*a) for a in ((0, 64, 64, 64), (65, 64, 64, 64), (4, 0, 64, 64), (4, 64, 1 << 29, 64), (64, 2048, 8192, 2048))] == [0] * 5
-    need = lib.sd_gated_mlp_few_workspace_bytes(4, 64)
+    need = lib.sd_gated_mlp_few_workspace_bytes(4, 64, 16)
     ok = dict(X=fake, ldx=32, Wi=fake, ldwi=32, Wo=fake, ldwo=64, Y=fake, ldy=16, M=4, K=32, F=64, N=16, act=3, dtype=0, ws=fake, nbytes=need)
     call = lambda **kw: lib.sd_gated_mlp_few(*{**ok, **kw}.values(), None)
     for bad, message in ((dict(K=0), b"extents"), (dict(M=-1), b"extents"), (dict(F=1 << 29), b"extents"), (dict(dtype=2), b"dtype"), (dict(act=0), b"act"), (dict(X=None), b"null"),
