@@ -3,7 +3,7 @@
 //   h = act(x W_g^T) (x W_u^T)        y = h W_out^T
 //
 // Bound by the weights' bytes, 2 (2 F K + N F), and with few of them by a memory latency and a launch each.  So weights go from memory straight
-// into the matrix instruction's registers.  A workgroup owns 16 outputs (or 32; or 8 or 4 where there would be too few workgroups: the others' lanes load
+// into the matrix instruction's registers.  A workgroup owns 4 to 32 outputs, 16 to a matrix instruction (lanes of outputs that are not there load
 // nothing); its waves share out the 64-deep pieces of the reduction, which are whole 128-byte lines of its weight rows, wave w every piece
 // w + WAVES n, AHEAD of them on their way at a time, and meet once in LDS.  A lane takes 32 consecutive bytes of a line (two loads, four lanes to a
 // line); the order of the reduction within a piece is the same for both operands and shows in nothing but the last bits.  Rows come in groups of
@@ -12,6 +12,8 @@
 //
 // Up to 8 rows leave room for h twice in a group: h, which nothing but the second launch reads, is then held as the sum of two 16-bit numbers, the
 // low halves in rows 8 to 15, and its rounding, the largest of the path, is saved.
+#include <algorithm>
+
 #include "gated.h"
 
 namespace sd {
@@ -26,7 +28,7 @@ struct Few {
   uint16_t* y;
   int64_t ldx, ldw, ldh, ldy;
   int M, N, K, act;  // N: hidden columns or outputs
-  int cols;          // of a workgroup, where that owns 16 or fewer
+  int cols;          // of a workgroup
   float* parts;      // of the second launch's sums, [gridDim.y][M][N], where its reduction is shared out over more workgroups ...
   int share;         // ... of so many pieces each
 };
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
   constexpr bool ODD_X = ODD && HIDDEN;  // (h has rows of whole lines)
   __shared__ float sums[WAVES][WP][16][17];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15, q = lane >> 4;
-  const int per = COLS == 1 ? g.cols : 16 * COLS, n0 = (int)blockIdx.x * per;
+  const int per = g.cols, n0 = (int)blockIdx.x * per;
   const bool twice = g.M <= kTwice;
   const uint16_t* w[COLS][WP];
   uint32_t w_shift[COLS][WP], x_shift[GROUPS];
@@ -95,7 +97,8 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
       w[j][p] = g.w + (int64_t)(min(n0 + 16 * j + r, g.N - 1) + p * g.N) * g.ldw + 16 * q;
       w_shift[j][p] = shift_of<ODD>(w[j][p]);
     }
-  const bool reads_w = COLS > 1 || r < per;
+  // (a workgroup of a COLS of two or more fills all 16-column tiles but the last)
+  auto reads_w = [&](int j) { return j + 1 < COLS || 16 * j + r < per; };
   const uint16_t* x[GROUPS];
   bool reads_x[GROUPS];
 #pragma unroll
@@ -145,16 +148,16 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) a[u][i].none();
     }
-    if (reads_w) {
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (there(u)) {
+    for (int j = 0; j < COLS; ++j)
+      if (reads_w(j)) {
 #pragma unroll
-          for (int j = 0; j < COLS; ++j)
+        for (int u = 0; u < AHEAD; ++u)
+          if (there(u)) {
 #pragma unroll
             for (int p = 0; p < WP; ++p) b[u][j][p].load(w[j][p] + at(u));
-        }
-    }
+          }
+      }
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
       if (reads_x[i]) {
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
 #pragma unroll
       for (int j = 0; j < COLS; ++j)
 #pragma unroll
-        for (int p = 0; p < WP; ++p) b[0][j][p].load_some(w[j][p], reads_w ? g.K - 16 * q : 0, w_shift[j][p]);
+        for (int p = 0; p < WP; ++p) b[0][j][p].load_some(w[j][p], reads_w(j) ? g.K - 16 * q : 0, w_shift[j][p]);
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) a[0][i].load_some(x[i], reads_x[i] ? g.K - 16 * q : 0, x_shift[i]);
       multiply(a[0], b[0], 0, 0);
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
       __syncthreads();
       if (t < 256) {
         const int at = t >> 4, col = t & 15, n = n0 + 16 * j + col, m = 16 * i + at;
-        if (m < g.M && (COLS > 1 || col < per)) {
+        if (m < g.M && (j + 1 < COLS || 16 * j + col < per)) {
           float s[WP] = {};
 #pragma unroll
           for (int o = 0; o < WAVES; ++o)
@@ -242,12 +245,13 @@ __global__ __launch_bounds__(256) void few_sum_kernel(Few g, int shares) {
 
 int groups_of(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
 
-// A launch's outputs to a workgroup (4, 8, 16, for 17 and more rows 32), how many workgroups share out a reduction, and what it is expected to take, us:
-// 2.5, 0.16 for each 16 x 16 sums that the waves add up, and the longer of the weights at 5.4 TB/s and, for a CU in as many rounds as it has
-// workgroups, the lines that come back to it at 36 GB/s (lanes that load nothing take a quarter of it all the same); 2.8 for the sum of the parts, and those, written
-// and read, at 1.7 TB/s.  Within 7 % (root mean square) of 330 launches measured, 512 to 4096 wide, hidden of 1000 to 8192, and what it picks takes 0.1 %
-// longer than the best of them.  One row of 8192 to 2048: 16 outputs 12.3 us, 8 10.6, with two shares of 16 13.0; 24 rows 8 outputs 18.9,
-// four shares of 32 13.7; 64 rows 36.2, 19.7.  Hidden of 24 rows of 2048: 8192 with 16 17.6, with 32 15.8.
+// A launch's outputs to a workgroup (4 to 16, for 17 and more rows to 32: as many as leave one to four workgroups to a CU), how many workgroups share out a
+// reduction, and what it is expected to take, us: 2.5, 0.16 for each 16 x 16 sums that the waves add up, and the longer of the weights at 5.4 TB/s and, for a CU
+// in as many rounds as it has workgroups, the lines that come back to it at 36 GB/s (lanes that load nothing take a quarter of it all the same); 2.8 for the
+// sum of the parts, and those, written and read, at 1.7 TB/s.  Within 7 % (root mean square) of 330 launches measured, 512 to 4096 wide, hidden of 1000 to 8192;
+// of their shapes it picks such as take 0.1 % longer than the best.  One row of 8192 to 2048: 16 outputs 12.3 us, 8 10.6, two shares of 16 13.0; 24 rows 8
+// outputs 18.9, four shares of 32 13.4; 64 rows 36.2, 19.7.  Hidden of 24 rows of 2048: 8192 with 16 17.6, with 32 15.8.  The block of 2048 to 5464 and back, one
+// and 24 rows: with powers of two 20.2 and 28.4, with 11, 22 and 8, 32 18.1 and 24.8.
 struct FewPlan {
   int cols = 0, shares = 0;
   double us = 1e30;
@@ -257,13 +261,18 @@ FewPlan plan_few(int64_t M, int64_t N, int64_t K, int parts) {
   const int64_t pieces = ceil_div(K, kDeep);
   const double weights = 2.0 * parts * (double)N * (double)K / 5.4e6;
   FewPlan best;
-  for (int shares = 1; shares <= (parts == 1 ? 8 : 1) && (shares == 1 || pieces >= 8 * shares); shares *= 2)
-    for (int cols = groups > 1 ? 32 : 16; cols >= 4; cols /= 2) {
-      const double rounds = (double)ceil_div(ceil_div(N, cols) * shares, 256), none = (cols < 16 ? 16 - cols : 0) * parts + 16 * groups - rows;
+  const uint32_t n = (uint32_t)N;  // (under 2^29, as the kernels count)
+  for (uint32_t shares = 1; shares <= (parts == 1 ? 8 : 1) && (shares == 1 || pieces >= 8 * shares); shares *= 2)
+    for (uint32_t round = 1, last = 0; round <= 4; ++round) {  // as many outputs as leave so many workgroups to a CU
+      const uint32_t each = (n * shares - 1) / (256 * round) + 1;
+      const int cols = (int)std::min(std::max(each, 4u), groups > 1 ? 32u : 16u);
+      if ((uint32_t)cols == last) continue;
+      last = (uint32_t)cols;
+      const double rounds = (double)((((n - 1) / cols + 1) * shares + 255) / 256), none = (cols > 16 ? 32 - cols : 16 - cols) * parts + 16 * groups - rows;
       const double lines = rounds * (double)pieces / shares * 128.0 * (cols * parts + rows + 0.25 * none) / 36e3;
       const double us = 2.5 + 0.16 * groups * (cols > 16 ? 2 : 1) * parts + (lines > weights ? lines + 0.05 * weights : weights + 0.05 * lines) +
                         (shares > 1 ? 2.8 + 8.0 * shares * (double)M * (double)N / 1.7e6 : 0.0);
-      if (us < best.us) best = {cols, shares, us};
+      if (us < best.us) best = {cols, (int)shares, us};
     }
   return best;
 }
@@ -277,9 +286,9 @@ void launch_few(const Few& f, const FewPlan& plan, hipStream_t stream) {
   const dim3 grid((unsigned)ceil_div(g.N, plan.cols), (unsigned)plan.shares), block(512);
   // two pieces on their way at a time for 16 rows (one row, hidden of 2048 to 8192 cold: 13.4 us, with one 14.5), one for more (24 rows 17.0, with two 18.0)
   if (groups == 1) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 1, 1, 2, ODD, SHARED>), grid, block, 0, stream, g);
-  else if (groups == 2 && plan.cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  else if (groups == 2 && plan.cols > 16) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
   else if (groups == 2) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 2, 1, 1, ODD, SHARED>), grid, block, 0, stream, g);
-  else if (plan.cols == 32) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
+  else if (plan.cols > 16) hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 2, 1, ODD, SHARED>), grid, block, 0, stream, g);
   else hipLaunchKernelGGL((&gated_few_kernel<T, HIDDEN, 8, 4, 1, 1, ODD, SHARED>), grid, block, 0, stream, g);
   if constexpr (SHARED) hipLaunchKernelGGL((&few_sum_kernel<T>), dim3((unsigned)ceil_div((int64_t)g.M * g.N, 256)), dim3(256), 0, stream, g, plan.shares);
 }
