@@ -642,6 +642,7 @@ Tensor mlp(const Tensor& input, const std::vector<Tensor>& weights, int64_t bs, 
 // (see functional/gated_mlp.py for what is computed)
 int64_t up8(int64_t n) { return ceil_div(n, 8) * 8; }
 Tensor rows_of(const Tensor& t) { return row_major(t) ? t : t.contiguous(); }
+Tensor columns_of(const Tensor& t, int64_t n) { return t.size(1) == n ? t : t.narrow(1, 0, n); }  // (a view takes the host 1 us)
 // (of a layer's lists: none where nothing is dropped)
 struct ListArgs {
   const int32_t *row_ptr = nullptr, *col_idx = nullptr, *col_ptr = nullptr, *row_idx = nullptr;
@@ -720,7 +721,7 @@ Tensor gated_forward(const GatedOperands& o, int act, int64_t bs, double p, cons
 std::pair<Tensor, Tensor> gated_backward(const Tensor& dy, const Tensor& w_out, const Tensor& h, const Tensor& pre, int64_t F, int act, double p, const Lists& lists,
                                          bool need_da, bool need_dw) {
   const int64_t M = dy.size(0), N = dy.size(1), F8 = h.size(1), R8 = up8(2 * F);
-  const Tensor hf = h.narrow(1, 0, F), wf = w_out.narrow(1, 0, F);
+  const Tensor hf = columns_of(h, F), wf = columns_of(w_out, F);
   if (!need_da) return {Tensor(), layer_products(dy, wf, hf, lists, p, false, need_dw, SD_ACT_NONE, Tensor()).second};
   Tensor da = new_matrix(h, M, R8), dw;
   const bool masked = lists.buf.defined();
@@ -780,7 +781,7 @@ struct GatedMlpBackward : Node {
     if (need_out) out[2] = dw.size(0) != N ? dw.narrow(0, 0, N) : dw;
     if (!need_x && !need_in) return out;
     if (wir.size(0) != da.size(1)) wir = at::empty({da.size(1), K}, wir.options());  // dW_in alone: only its shape is looked at
-    std::tie(out[0], dw) = layer_products(da, wir.narrow(1, 0, K), xr.narrow(1, 0, K), lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
+    std::tie(out[0], dw) = layer_products(da, columns_of(wir, K), columns_of(xr, K), lists[0].get(), p[0], need_x, need_in, SD_ACT_NONE, Tensor());
     if (need_in) out[1] = dw.size(0) != 2 * F ? dw.narrow(0, 0, 2 * F) : dw;
     return out;
   }

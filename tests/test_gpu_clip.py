@@ -294,7 +294,7 @@ def test_clipping_keeps_the_arguments_of_torchs():
     for p, q in zip(ps[1:], qs[1:]):
         torch.testing.assert_close(p.grad, q.grad, rtol=1e-5, atol=1e-8)
     one = parameters(torch.float32, 6)[1]
-    assert float(clip_grad_norm_(one, 1.0)) > 1.0
+    assert float(clip_grad_norm_(one, 1.0, foreach=True)) > 1.0
     assert float(clip_grad_norm_([torch.nn.Parameter(torch.ones(3))], 1.0)) == 0.0
 
 
