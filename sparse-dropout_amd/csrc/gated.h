@@ -6,14 +6,14 @@
 // registers: 3 of the 4 bytes a passing gate would move.  gated_hidden, gated_up: which row of W_in column n of a tile is.
 //   8192 x 2048 to 8192 bf16: 415 us, 454 with G and U; the product alone, which writes both, 429, and a gate's pass 74 more
 //   4096 x 1024 to 4096 fp16:  66 us,  70;              67 and 16            1024 x 512 to 2048: 10.2, 12.7; 10.2 and 3.6
-// Bound by the matrix cores and the loads into LDS as the ungated product is; at the largest the store of 8 bytes an element adds to that (360 us
+// Bound by the matrix cores and the loads into LDS as the ungated product is; at the largest the store of 2 or 6 bytes an element adds to that (360 us
 // without one).  Workgroups of the first round started up to 13 us apart, so that no two CUs' stores meet, take the same: it is not that they come together.
 //
 // Backward.  dH = (dY W_out) . keep is a product whose store reads g and u of its place and writes dg and du instead of dh.
 //   8192 x 8192 from 2048 bf16: 361 us, the product and a pass 239 and 120; half dropped 227, 166 and 121
 //   4096 x 4096 from 1024 fp16: 59 us, 40 and 25           1024 x 2048 from 512: 9.1, 7.3 and 4.7
 // Bound by the product and behind it by the 8 bytes read and written for each of its results: the gate saves dH's way to memory and back and a
-// launch.  (Loads and stores past the caches, nontemporal ones, took 3 to 20 us more of a block's 372 and 1432.)
+// launch.  (With nontemporal loads or stores, in either direction, a block's 372 us were 373 to 395, another's 1432 1421 to 1442.)
 #pragma once
 #include "common.h"
 
