@@ -31,7 +31,8 @@ def _gate(activation) -> int:
 @traceable
 def gated_mlp(input: torch.Tensor, weight_in: torch.Tensor, weight_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """``(act(x W_g^T) * (x W_u^T)) W_out^T``: ``input`` [M, K], ``weight_in`` [2 F, K] (the rows of W_g, then those of W_u), ``weight_out``
-    [N, F], all float16 or bfloat16 (under autocast: cast to its dtype).  Differentiable in all three."""
+    [N, F], all float16 or bfloat16 (under autocast: cast to its dtype).  Differentiable in all three.  Where nothing is recorded up to 64 rows may
+    run in launches of their own, whose results differ in the last bits (up to 8 rows round the hidden activations to twice as many)."""
     return _loader.bridge().gated_mlp(input, weight_in, weight_out, 0, (0.0, 0.0), _gate(activation), None, None, None)
 
 
