@@ -262,7 +262,8 @@ FewPlan plan_few(int64_t M, int64_t N, int64_t K, int parts) {
   const double weights = 2.0 * parts * (double)N * (double)K / 5.4e6;
   FewPlan best;
   const uint32_t n = (uint32_t)N;  // (under 2^29, as the kernels count)
-  for (uint32_t shares = 1; shares <= (parts == 1 ? 8 : 1) && (shares == 1 || pieces >= 8 * shares); shares *= 2)
+  for (uint32_t shares = 1; shares <= (parts == 1 ? 8 : 1) && (shares == 1 || pieces >= 8 * shares); shares *= 2) {
+    if (shares > 1 && best.us <= 5.3 + weights) break;  // (no sum of parts takes less)
     for (uint32_t round = 1, last = 0; round <= 4; ++round) {  // as many outputs as leave so many workgroups to a CU
       const uint32_t each = (n * shares - 1) / (256 * round) + 1;
       const int cols = (int)std::min(std::max(each, 4u), groups > 1 ? 32u : 16u);
@@ -274,6 +275,7 @@ FewPlan plan_few(int64_t M, int64_t N, int64_t K, int parts) {
                         (shares > 1 ? 2.8 + 8.0 * shares * (double)M * (double)N / 1.7e6 : 0.0);
       if (us < best.us) best = {cols, (int)shares, us};
     }
+  }
   return best;
 }
 
