@@ -46,11 +46,16 @@ struct Sixteen {
     if constexpr (ODD) behind = 0u;
   }
   __device__ inline void load(const uint16_t* at) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(at);
-    const char* from = reinterpret_cast<const char*>(ODD ? a & ~uintptr_t(3) : a);
-    v[0] = *reinterpret_cast<const u32x4_dwords*>(from);
-    v[1] = *reinterpret_cast<const u32x4_dwords*>(from + 16);
-    if constexpr (ODD) behind = *reinterpret_cast<const uint32_t*>(from + 28 + (a & 2) * 2);
+    if constexpr (ODD) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+      const char* from = reinterpret_cast<const char*>(a & ~uintptr_t(3));
+      v[0] = *reinterpret_cast<const u32x4_dwords*>(from);
+      v[1] = *reinterpret_cast<const u32x4_dwords*>(from + 16);
+      behind = *reinterpret_cast<const uint32_t*>(from + 28 + (a & 2) * 2);
+    } else {  // (the last piece of an odd reduction begins inside a dword all the same)
+      v[0] = *reinterpret_cast<const u32x4_any*>(at);
+      v[1] = *reinterpret_cast<const u32x4_any*>(at + 8);
+    }
   }
   // those of `left` that are there, zeros behind them: the dwords in which one is wanted, the last one's upper half taken out where it is none
   __device__ inline void load_some(const uint16_t* at, int left, uint32_t shift) {
