@@ -20,12 +20,13 @@
 namespace sd {
 
 // act(g).  SILU: g / (1 + exp(-g)), one exponential and one reciprocal, 4 roundings and g's of the exponent: within 2^-21 of itself where |g| < 16.
-// An exponential of 2^126 and more gives 0 for a value under 2^-119.
+// An exponential of 2^126 and more gives 0 for a value under 2^-119.  NaN stays NaN in every gate (ReLU's comparison is the one that it fails).
 __device__ inline float gate_value(int act, float g) {
   if (act == SD_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+  if (act == SD_ACT_RELU) return g <= 0.f ? 0.f : g;
   return act_apply(act, g);
 }
-// act(g) and act'(g) together: they share what is dear.  GELU: Phi(g) from the root of its tail, phi(g) one exponential more.
+// act(g) and act'(g) together: they share what is dear.  GELU: Phi(g) from the root of its tail, phi(g) one exponential more.  ReLU': 0 or 1, or NaN.
 __device__ inline void gate_slope(int act, float g, float& value, float& slope) {
   if (act == SD_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
@@ -36,8 +37,8 @@ __device__ inline void gate_slope(int act, float g, float& value, float& slope) 
     value = g * below;
     slope = __builtin_fmaf(g * 0.39894228040143268f, __builtin_amdgcn_exp2f((g * -0.72134752044448170f) * g), below);
   } else {
-    value = act_apply(act, g);
-    slope = act_derivative(act, g);
+    value = gate_value(act, g);
+    slope = g > 0.f ? 1.f : value;
   }
 }
 
