@@ -226,7 +226,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(Few g) {
               float low = 0.f;
 #pragma unroll
               for (int o = 0; o < WAVES; ++o) low += sums[o][0][kTwice + (at & (kTwice - 1))][col];
-              s[0] += low;
+              if (__builtin_isfinite(s[0])) s[0] += low;  // (an infinite weight is one in the high halves' sum already; times a low half of 0 it is NaN)
             }
             if (n < g.N) {
               if constexpr (SHARED) g.parts[((int64_t)blockIdx.y * g.M + m) * g.N + n] = s[0];

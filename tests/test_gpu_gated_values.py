@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from oracle import gated_oracle as O
 from test_gpu_gated import DT, masks_of, operands, run
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,25 @@ def test_nan_in_a_gate_by_itself(f, act):
         assert torch.equal(h.isnan(), nan) and torch.equal(h[~nan], ref[0][~nan])
         twice = torch.cat((nan, nan), 1)
         assert torch.equal(da.isnan(), twice) and torch.equal(da[~twice], ref[1][~twice])
+
+
+# ---- infinite weights ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("m,k,f,n", [(1, 136, 200, 72), (5, 65, 99, 33), (8, 136, 200, 72), (8, 64, 8193, 2047), (9, 136, 200, 72), (24, 64, 4096, 1024), (200, 136, 200, 72)])
+def test_infinite_output_weights_give_infinite_outputs(m, k, f, n, dtype):
+    """An output with one infinite weight is an infinity of the sign of its product, with two NaN where the signs differ; others are as they were."""
+    x, w_in, w_out, _ = operands(m, k, f, n, dtype, seed=102)
+    h = (O.act((x.double() @ w_in.double().t())[:, :f], "silu")[0] * (x.double() @ w_in.double().t())[:, f:])
+    # (the hidden columns furthest from 0 in every row: 16 bits hold their signs)
+    one, two = h.abs().amin(0).topk(2).indices.tolist()
+    assert float(h[:, [one, two]].abs().min()) > 2.0 ** -20
+    with torch.no_grad():
+        ref = F.gated_mlp(x, w_in, w_out)
+        w_out[3, one], w_out[7, two], w_out[n - 1, one], w_out[n - 1, two] = math.inf, -math.inf, math.inf, math.inf
+        y = F.gated_mlp(x, w_in, w_out)
+    assert torch.equal(y[:, 3].double(), math.inf * h[:, one].sign()) and torch.equal(y[:, 7].double(), -math.inf * h[:, two].sign())
+    both = math.inf * h[:, one].sign() + math.inf * h[:, two].sign()
+    assert torch.equal(y[:, n - 1].isnan(), both.isnan()) and torch.equal(y[:, n - 1][~both.isnan()].double(), both[~both.isnan()])
+    others = torch.ones(n, dtype=torch.bool, device="cuda")
+    others[[3, 7, n - 1]] = False
+    assert torch.equal(y[:, others], ref[:, others])
