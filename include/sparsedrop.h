@@ -713,7 +713,8 @@ int sd_clip_grads(int count, void* const* grads, const int64_t* numels, const in
  * A[M, ..] = [G | U] (pitch lda): both projections' results, F columns each, U's `up` columns behind G's; act: relu, gelu or silu.
  * sd_gated_forward:  H = act(G) U                        (H [M, F], pitch ldh)
  * sd_gated_backward: dA = [dH U act'(G) | dH act(G)]     (dH [M, F], pitch ldd; dA [M, 2F], pitch ldda, side by side)
- *   where dH is 0 both gradients are 0, whatever stands in A: what was dropped has none.
+ *   where dH is 0 both gradients are 0, whatever stands in A: what was dropped has none.  An infinite G has act's limits, 0 below and a slope
+ *   of 1 above, and behind a slope of 0 an infinite U has no gradient: they stand for what 16 bits do not hold.
  * Computed in fp32, rounded once.  h_cols, da_cols (here and below): the columns behind the last, up to these, are filled with zeros, at most up to the
  * next multiple of 8: H and dA are the next product's operands, whose reduction comes in 16 bytes.
  *

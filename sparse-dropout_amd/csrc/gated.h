@@ -27,19 +27,30 @@ __device__ inline float gate_value(int act, float g) {
   return act_apply(act, g);
 }
 // act(g) and act'(g) together: they share what is dear.  GELU: Phi(g) from the root of its tail, phi(g) one exponential more.  ReLU': 0 or 1, or NaN.
+// A G that was beyond its type has been kept as an infinity: there they are their limits, 0 and 0 below, infinite and 1 above.
 __device__ inline void gate_slope(int act, float g, float& value, float& slope) {
   if (act == SD_ACT_SILU) {
-    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
-    value = g * s;
-    slope = __builtin_fmaf(value, 1.f - s, s);
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f)), rest = 1.f - s;
+    value = s != 0.f ? g * s : 0.f;
+    slope = rest != 0.f ? __builtin_fmaf(value, rest, s) : s;
   } else if (act == SD_ACT_GELU) {
     const float root = normal_tail_root(fabsf(g)), below = g >= 0.f ? __builtin_fmaf(-root, root, 1.f) : root * root;
-    value = g * below;
-    slope = __builtin_fmaf(g * 0.39894228040143268f, __builtin_amdgcn_exp2f((g * -0.72134752044448170f) * g), below);
+    const float bell = __builtin_amdgcn_exp2f((g * -0.72134752044448170f) * g);
+    value = below != 0.f ? g * below : 0.f;
+    slope = bell != 0.f ? __builtin_fmaf(g * 0.39894228040143268f, bell, below) : below;
   } else {
     value = gate_value(act, g);
     slope = g > 0.f ? 1.f : value;
   }
+}
+// dG = d U act'(G) and dU = d act(G) in the places of G and U; d: of H.  A U that was beyond its type is an infinity too, and nothing behind a slope of 0.
+// Where d is 0 so are both: what was dropped has no gradient, whatever stands there.
+__device__ inline void gate_gradient(int act, float d, float& gate, float& up) {
+  float value, slope;
+  gate_slope(act, gate, value, slope);
+  const float u = slope == 0.f && __builtin_isinf(up) ? 0.f : up;
+  gate = d != 0.f ? d * u * slope : 0.f;
+  up = d != 0.f ? d * value : 0.f;
 }
 
 // columns of the product's output as its tiles see them
@@ -139,7 +150,7 @@ struct GateAt {
 __device__ inline void fill_gradient(const GemmArgs& g, int64_t m) {
   for (int64_t i = 2 * g.gate; i < g.c_cols; ++i) g.c[m * g.c_sr + i] = 0;
 }
-// eight of dh, unscaled fp32 accumulators.  What was dropped has no gradient, whatever stands in g and u.
+// eight of dh, unscaled fp32 accumulators
 template <typename T>
 __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t c, float (&dh)[8], const GateAt& pre) {
   if (m >= g.M || c >= g.gate) return;
@@ -159,13 +170,7 @@ __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t
   }
   auto apply = [&](int act) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float value, slope;
-      gate_slope(act, gate[i], value, slope);
-      const float d = dh[i] * g.scale;
-      gate[i] = dh[i] != 0.f ? d * up[i] * slope : 0.f;
-      up[i] = dh[i] != 0.f ? d * value : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) gate_gradient(act, dh[i] * g.scale, gate[i], up[i]);
   };
   if (g.act == SD_ACT_SILU) apply(SD_ACT_SILU);
   else if (g.act == SD_ACT_GELU) apply(SD_ACT_GELU);

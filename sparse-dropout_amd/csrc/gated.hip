@@ -65,12 +65,7 @@ __global__ __launch_bounds__(kThreads) void gate_kernel(Gate g) {
       Eight d;
       d.load<T>(g.dh + m * g.ldd + c, left);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float value, slope;
-        gate_slope(ACT, gate.v[e], value, slope);
-        gate.v[e] = d.v[e] != 0.f ? d.v[e] * up.v[e] * slope : 0.f;  // (what was dropped has no gradient, whatever stands there)
-        up.v[e] = d.v[e] != 0.f ? d.v[e] * value : 0.f;
-      }
+      for (int e = 0; e < 8; ++e) gate_gradient(ACT, d.v[e], gate.v[e], up.v[e]);
       gate.store<T>(g.out + m * g.ldo + c, left);
       up.store<T>(g.out + m * g.ldo + g.F + c, left);
       if (c + 8 >= g.F) fill_row(g.out + m * g.ldo, 2 * g.F, g.cols);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import gated_oracle as O
-from test_gpu_gated import DT, masks_of, operands, run
+from test_gpu_gated import DT, NAMES, masks_of, operands, run
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,90 @@ def test_infinite_output_weights_give_infinite_outputs(m, k, f, n, dtype):
     others = torch.ones(n, dtype=torch.bool, device="cuda")
     others[[3, 7, n - 1]] = False
     assert torch.equal(y[:, others], ref[:, others])
+
+
+# ---- projections beyond fp16 ------------------------------------------------------------------------------------------------------
+# The forward's gate is computed from 32-bit sums and the backward's from G and U in 16 bits, where what lies beyond 65504 is infinite.  Where an
+# activation is flat (0 or 1 its slope, to the last of 32 bits) gradients do not depend on how far out G lies: calls with G inside of fp16 and beyond it
+# have equal ones, bit by bit.
+def far_operands(size, which, unit, value, seed=103):
+    """Hidden column `unit` of G (which 0) or of U (1) is about value, up to a few times that, in every row."""
+    m, k, f, n = size
+    x, w_in, w_out, dy = operands(*size, "fp16", seed=seed)
+    x = x.abs() + 0.5
+    w_in[which * f + unit] = value / (1.3 * k)
+    return x, w_in, w_out, dy
+
+
+def equal_gradients(a, b, unit, f, names=NAMES, halves=(0, 1)):
+    rows = torch.ones(2 * f, dtype=torch.bool, device="cuda")
+    for half in (0, 1):
+        rows[half * f + unit] = half in halves
+    for name in names:
+        x, y = (t[name][rows] if name == "dw_in" else t[name] for t in (a, b))
+        assert y.isfinite().all(), name
+        assert torch.equal(x, y), name
+
+
+@pytest.mark.parametrize("p", [0.0, 0.4])
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("size", [(70, 136, 200, 72), (130, 77, 99, 50), (320, 256, 512, 128)], ids=lambda s: "x".join(map(str, s)))
+def test_a_gate_far_below_zero_has_no_gradient(size, act, p, tiles):
+    f, unit = size[2], 21
+    masks = masks_of(*size[:3], 64, p) if p else None
+    got = []
+    for value in (-20000.0, -200000.0):
+        x, w_in, w_out, dy = far_operands(size, 0, unit, value)
+        assert (w_in[unit].isfinite().all()) and float((x.double() @ w_in[unit].double()).max()) < value / 3
+        got.append(run(x, w_in, w_out, dy, act, 64 if p else None, p, masks))
+    # dx sums products of gradients that are 0 with weights that differ
+    equal_gradients(*got, unit, f)
+    assert not got[1]["dw_in"][unit].any() and not got[1]["dw_in"][f + unit].any()
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("size", [(70, 136, 200, 72), (130, 77, 99, 50), (320, 256, 512, 128)], ids=lambda s: "x".join(map(str, s)))
+def test_a_gate_far_above_zero_has_a_slope_of_one(size, act, tiles):
+    """dG = dH U; act(G) itself, which dU is a multiple of, is not held."""
+    f, unit = size[2], 21
+    got = []
+    for value in (20000.0, 200000.0):
+        x, w_in, w_out, dy = far_operands(size, 0, unit, value)
+        w_in[f + unit] *= 2.0 ** -10
+        got.append(run(x, w_in, w_out, dy, act))
+    assert got[0]["dw_in"][unit].any()
+    equal_gradients(*got, unit, f, names=("dw_in",), halves=(0,))
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("size", [(70, 136, 200, 72), (130, 77, 99, 50), (320, 256, 512, 128)], ids=lambda s: "x".join(map(str, s)))
+def test_behind_a_closed_gate_the_other_projection_may_be_anything(size, act, tiles):
+    f, unit = size[2], 21
+    got = []
+    for value in (20000.0, 200000.0):
+        x, w_in, w_out, dy = far_operands(size, 1, unit, value)
+        w_in[unit] = -200.0 / size[1]  # the gate: under -100 in every row, where the slope is 0
+        assert float((x.double() @ w_in[unit].double()).max()) < -110
+        got.append(run(x, w_in, w_out, dy, act))
+    equal_gradients(*got, unit, f)
+    assert not got[1]["dw_in"][unit].any() and not got[1]["dw_in"][f + unit].any()
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("f", [40, 37])
+def test_infinite_projections_of_a_gate_by_itself(f, act):
+    for dtype in DT.values():
+        a = torch.randn(30, 2 * f, device="cuda").to(dtype)
+        dh = torch.randn(30, f, device="cuda").to(dtype)
+        dh[dh == 0] = 1
+        g, u = a[:, :f], a[:, f:]
+        g[0], g[1], g[2], g[3] = -math.inf, math.inf, -math.inf, -200.0
+        u[2], u[3], u[4] = math.inf, -math.inf, math.nan
+        g[4], g[5], u[5] = -200.0, 200.0, math.inf
+        da = gate_apart(a, act, dh)
+        dg, du = da[:, :f], da[:, f:]
+        assert not dg[[0, 2, 3]].any() and not du[[0, 2, 3]].any()
+        assert torch.equal(dg[1].double(), (dh[1].double() * u[1].double()).to(dtype).double()) and du[1].isinf().all()
+        assert dg[4].isnan().all() and not du[4].any()
+        assert dg[5].isinf().all() and torch.equal(du[5].double(), (dh[5].double() * 200).to(dtype).double())
+        assert da[6:].isfinite().all()
