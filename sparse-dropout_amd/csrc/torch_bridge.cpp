@@ -656,21 +656,16 @@ struct ListArgs {
 };
 
 // The block's operands with rows on 16-byte boundaries and whole 16 bytes of a reduction: copies, filled up with zeros, where they have none, made in one
-// launch.  W_in and W_out get as many rows as make 16 bytes too, since in the backward these are the reductions.
+// launch.  (The backward makes its own from what was saved: copies beside it would pass saved-tensor hooks by.)
 struct GatedOperands {
   Tensor x, w_in, w_out;
   int64_t M, K, F, N;
-  bool copied[3] = {false, false, false};
   GatedOperands(const Tensor& x_, const Tensor& w_in_, const Tensor& w_out_)
       : x(rows_of(x_)), w_in(rows_of(w_in_)), w_out(rows_of(w_out_)), M(x_.size(0)), K(x_.size(1)), F(w_out_.size(1)), N(w_out_.size(0)) {
     RowPadding pad;
-    auto copy = [&](int i, Tensor& t, int64_t rows) {
-      copied[i] = true;
-      t = pad.add(t, rows);
-    };
-    if (K % 8 || !rows_on_16_bytes(x)) copy(0, x, M);
-    if (K % 8 || !rows_on_16_bytes(w_in)) copy(1, w_in, up8(2 * F));
-    if (F % 8 || !rows_on_16_bytes(w_out)) copy(2, w_out, up8(N));
+    if (K % 8 || !rows_on_16_bytes(x)) x = pad.add(x, M);
+    if (K % 8 || !rows_on_16_bytes(w_in)) w_in = pad.add(w_in, 2 * F);
+    if (F % 8 || !rows_on_16_bytes(w_out)) w_out = pad.add(w_out, N);
     pad.launch();
   }
 };
@@ -747,7 +742,6 @@ std::pair<Tensor, Tensor> gated_backward(const Tensor& dy, const Tensor& w_out, 
 struct GatedMlpBackward : Node {
   Saved x, w_in, w_out, pre, h;  // pre: [G | U], h = act(G) U, both as gated_forward makes them
   SavedLists lists[2];           // nothing kept: nothing is dropped
-  Tensor copies[3];              // of the operands, where the forward took copies
   double p[2] = {0.0, 0.0};
   int act = SD_ACT_NONE;
   variable_list apply(variable_list&& grads) override {
@@ -765,10 +759,9 @@ struct GatedMlpBackward : Node {
     const int64_t M = xs.size(0), K = xs.size(1), N = wo.size(0), F = wo.size(1);
     Tensor dy = rows_of(grad_matrix(grads[0], xs));
     TORCH_CHECK_VALUE(dy.size(0) == M && dy.size(1) == N && dy.device() == xs.device(), "dy must be a [", M, ", ", N, "] tensor on ", xs.device());
-    Tensor xr = copies[0].defined() ? copies[0] : rows_of(xs), wir = copies[1].defined() ? copies[1] : rows_of(wi),
-           wor = copies[2].defined() ? copies[2] : rows_of(wo);
+    Tensor xr = rows_of(xs), wir = rows_of(wi), wor = rows_of(wo);
     {
-      // (saved-tensor hooks may have moved what was on 16 bytes)
+      // rows on 16 bytes, and W_in and W_out with as many as make 16 bytes: in here they are the reductions
       RowPadding pad;
       if (N % 8 || !rows_on_16_bytes(dy)) dy = pad.add(dy, M);
       if (wor.size(0) % 8 || !rows_on_16_bytes(wor)) wor = pad.add(wor, up8(N));
@@ -789,7 +782,6 @@ struct GatedMlpBackward : Node {
     std::lock_guard<std::mutex> lock(mutex_);
     for (Saved* s : {&x, &w_in, &w_out, &pre, &h}) s->drop();
     for (SavedLists& l : lists) l.drop();
-    for (Tensor& t : copies) t = Tensor();
   }
   std::string name() const override { return "GatedMLPHIPBackward"; }
 };
@@ -816,7 +808,7 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
     return Draw{masks ? (*masks)[i] : OptTensor(), seed ? std::optional<uint64_t>(*seed + (uint64_t)i) : std::nullopt, state};
   };
   Lists lists[2];
-  Tensor pre, h, y, copies[3];
+  Tensor pre, h, y;
   {
     NoRecord guard;
     if (M == 0) {
@@ -835,13 +827,7 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
       for (int i = 0; i < 2; ++i)
         if (drops(i)) d[i] = draw(i);
       h = gated_forward(o, act, bs, ps[0], drops(0) ? &d[0] : nullptr, lists[0], rec, pre);
-      const Tensor w = o.w_out.size(0) != N ? o.w_out.narrow(0, 0, N) : o.w_out;
-      y = drops(1) ? layer_forward(h, w, bs, ps[1], d[1], SD_ACT_NONE, false, lists[1], nullptr) : dense(h, w, SD_ACT_NONE, false, nullptr);
-      if (rec) {
-        const Tensor* from[3] = {&o.x, &o.w_in, &o.w_out};
-        for (int i = 0; i < 3; ++i)
-          if (o.copied[i]) copies[i] = *from[i];
-      }
+      y = drops(1) ? layer_forward(h, o.w_out, bs, ps[1], d[1], SD_ACT_NONE, false, lists[1], nullptr) : dense(h, o.w_out, SD_ACT_NONE, false, nullptr);
     }
   }
   if (rec) {
@@ -851,7 +837,6 @@ Tensor gated_mlp(const Tensor& input, const Tensor& weight_in, const Tensor& wei
     node->w_out.keep(wo);
     node->pre.keep(pre);
     node->h.keep(h);
-    for (int i = 0; i < 3; ++i) node->copies[i] = copies[i];
     for (int i = 0; i < 2; ++i) {
       if (lists[i].buf.defined()) node->lists[i].keep(std::move(lists[i]));
       node->p[i] = bs ? ps[i] : 0.0;

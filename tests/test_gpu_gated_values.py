@@ -1,4 +1,4 @@
-"""Values of the gated feed-forward block where they are not ordinary numbers."""
+"""Values of the gated feed-forward block where they are not ordinary numbers, and what saved-tensor hooks hand back."""
 import math
 
 import pytest
@@ -196,3 +196,38 @@ def test_infinite_projections_of_a_gate_by_itself(f, act):
         assert dg[4].isnan().all() and not du[4].any()
         assert dg[5].isinf().all() and torch.equal(du[5].double(), (dh[5].double() * 200).to(dtype).double())
         assert da[6:].isfinite().all()
+
+
+# ---- saved-tensor hooks ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("size", [(70, 136, 200, 72), (65, 130, 99, 33), (130, 77, 104, 56), (130, 80, 99, 50)], ids=lambda s: "x".join(map(str, s)))
+def test_what_a_hook_hands_back_is_used(size, p):
+    """Twice a saved operand gives twice the gradients that it is a factor of, whatever the widths."""
+    m, k, f, n = size
+    ops = operands(*size, "bf16", seed=104)
+    masks = masks_of(m, k, f, 64, p) if p else None
+    ref = run(*ops, "silu", 64 if p else None, p, masks)
+    for i, name in ((0, "dw_in"), (1, "dx")):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t * 2 if t.shape == ops[i].shape and t.dtype == torch.bfloat16 else t):
+            got = run(*ops, "silu", 64 if p else None, p, masks)
+        for other in NAMES:
+            assert torch.equal(got[other], ref[other] * 2 if other == name else ref[other]), (name, other)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t * 2 if t.shape == (n, f) and t.dtype == torch.bfloat16 else t):
+        got = run(*ops, "silu", 64 if p else None, p, masks)
+    assert torch.equal(got["dx"], ref["dx"] * 2) and torch.equal(got["dw_in"], ref["dw_in"] * 2) and torch.equal(got["dw_out"], ref["dw_out"])
+
+
+@pytest.mark.parametrize("size", [(4000, 1024, 1040, 520), (4000, 1025, 1041, 523)], ids=lambda s: "x".join(map(str, s)))
+def test_offloading_leaves_nothing_of_the_forward_on_the_gpu(size):
+    ops = operands(*size, "bf16", seed=105)
+    leaves = [t.requires_grad_() for t in ops[:3]]
+    with torch.no_grad():
+        F.gated_mlp(*leaves)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        y = F.gated_mlp(*leaves)
+    assert torch.cuda.memory_allocated() - before <= y.numel() * 2 + (1 << 16)
+    y.backward(ops[3])
+    ref = run(*ops, "silu")
+    assert all(torch.equal(t.grad, ref[name]) for t, name in zip(leaves, NAMES[1:]))
