@@ -1763,6 +1763,14 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     to.n.push_back(size);
   }
   check_apart(spans);
+  // (workgroups read these while others write)
+  for (const Tensor* t : {&step, lr_at ? &*lr_at : nullptr, grad_scale ? &*grad_scale : nullptr}) {
+    if (!t) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t->data_ptr()), end = at + t->element_size();
+    for (const Span& s : spans)
+      TORCH_CHECK_VALUE(s.end <= at || end <= s.begin || (t != &step && !s.written), "parameter ", s.parameter,
+                        ": the step, a learning rate or a factor of the gradients lies in its memory, its averages' or its gradient's");
+  }
   int last = 0;
   for (int i = 0; i < 3; ++i)
     if (!groups[i].n.empty()) last = i;

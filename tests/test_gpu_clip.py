@@ -331,3 +331,21 @@ def test_a_training_step_of_the_gated_block_with_clipping():
                          grad_scale=factor)
         assert torch.equal(norm, a.grad_norm) and float(factor) < 1.0
         assert all(torch.equal(p, q) for p, q in zip(one.parameters(), two.parameters()))
+
+
+def test_a_factor_or_a_rate_inside_what_a_step_writes_is_refused():
+    p, g = torch.randn(1000, device="cuda"), torch.randn(1000, device="cuda")
+    m, v, step = torch.zeros_like(p), torch.zeros_like(p), torch.zeros((), dtype=torch.int64, device="cuda")
+    before = p.clone()
+    for t in (p, m, v):
+        for kw in ({"grad_scale": t[990]}, {"lr": t[3:4]}):
+            with pytest.raises(ValueError, match="parameter 0.*factor of the gradients"):
+                F.adamw_step([p], [g], [m], [v], step, **kw)
+    for t in (p, m, v, g):
+        with pytest.raises(ValueError, match="parameter 0.*the step"):
+            F.adamw_step([p], [g], [m], [v], t[4:6].view(torch.int64)[0])
+    assert torch.equal(p, before) and not m.any() and not v.any() and int(step) == 0
+    factors = torch.tensor([0.0, 0.5], device="cuda")  # beside what is written, and in a gradient, which is read alone
+    F.adamw_step([p], [g], [m], [v], step, lr=factors[0], grad_scale=factors[1], weight_decay=0.0)
+    F.adamw_step([p], [g], [m], [v], step, lr=factors[0], grad_scale=g[5], weight_decay=0.0)
+    assert torch.equal(p, before) and int(step) == 2 and bool(m.any())
