@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import gated_oracle as O
-from test_gpu_gated import DT, NAMES, masks_of, operands, run
+from test_gpu_gated import DT, NAMES, check, masks_of, operands, run
 
 pytestmark = pytest.mark.gpu
 
@@ -231,3 +231,17 @@ def test_offloading_leaves_nothing_of_the_forward_on_the_gpu(size):
     y.backward(ops[3])
     ref = run(*ops, "silu")
     assert all(torch.equal(t.grad, ref[name]) for t, name in zip(leaves, NAMES[1:]))
+
+
+# ---- rows behind two to the 31 elements --------------------------------------------------------------------------------------------
+def test_weight_gradients_of_rows_behind_two_to_the_31_elements():
+    """Only the last rows have a gradient, so the weights' gradients are those of these rows alone."""
+    m, k, f, n, last = 66000, 64, 16384 + 320, 64, 200  # [G | U] has 2.2e9 elements
+    gen = torch.Generator("cuda").manual_seed(106)
+    make = lambda r, c, std: (torch.randn(r, c, generator=gen, device="cuda") * std).bfloat16()
+    x, w_in, w_out, dy = make(m, k, 1.0), make(2 * f, k, k ** -0.5), make(n, f, f ** -0.5), make(m, n, 0.1)
+    dy[:-last] = 0
+    got = run(x, w_in, w_out, dy, "silu")
+    assert not got["dx"][:-last].any()
+    ref = O.reference(x[-last:], w_in, w_out, dy[-last:], "silu", torch.bfloat16)
+    check({"y": got["y"][-last:], "dx": got["dx"][-last:], "dw_in": got["dw_in"], "dw_out": got["dw_out"]}, ref)
