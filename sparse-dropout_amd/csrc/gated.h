@@ -19,8 +19,8 @@
 
 namespace sd {
 
-// act(g).  SILU: g / (1 + exp(-g)), one exponential and one reciprocal, 4 roundings and g's of the exponent: within 2^-21 of itself where |g| < 16.
-// An exponential of 2^126 and more gives 0 for a value under 2^-119.  NaN stays NaN in every gate (ReLU's comparison is the one that it fails).
+// act(g).  SILU: g / (1 + exp(-g)), one exponential and one reciprocal.  Within 2^-19 of itself where |g| < 16: what rounds g / ln 2, by up to 2^-20 there,
+// moves the exponential by 0.7 times that, the constant by |g| 2^-26, and each of the other steps by 2^-24 or 2^-23; beyond it grows with -g.  An exponential of 2^126 and more gives 0 for a value under 2^-119.  NaN stays NaN in every gate (ReLU's comparison is the one that it fails).
 __device__ inline float gate_value(int act, float g) {
   if (act == SD_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
   if (act == SD_ACT_RELU) return g <= 0.f ? 0.f : g;
@@ -188,21 +188,24 @@ __device__ inline void store_gate_gradient(const GemmArgs& g, int64_t m, int64_t
     fill_gradient(g, m);
   }
 }
-// a wave's 64 x 64 tile of dh staged in LDS with a pitch of 68 floats
+// A wave's 64 x 64 tile of dh staged in LDS with a pitch of 68 floats.  In two turns: all eight passes side by side are 96 KB of instructions in the
+// 256 x 256 kernel, more than a CU's instruction cache holds.
 template <typename T>
 __device__ inline void store_staged_gate_gradient(const GemmArgs& g, const float* stg, int lane, int64_t m0, int64_t c0) {
   constexpr int PITCH = 68, AHEAD = 4;
-  GateAt pre[AHEAD];
+#pragma unroll 1
+  for (int first = 0; first < 8; first += AHEAD) {
+    const int row0 = first * 8 + lane / 8, ch = lane % 8;
+    GateAt pre[AHEAD];
 #pragma unroll
-  for (int pass = 0; pass < 8; ++pass) {
-    const int row = pass * 8 + lane / 8, ch = lane % 8;
-    if (pass % AHEAD == 0) {
+    for (int i = 0; i < AHEAD; ++i) pre[i].load(g, m0 + row0 + 8 * i, c0 + ch * 8);
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) pre[i].load(g, m0 + row + 8 * i, c0 + ch * 8);
+    for (int i = 0; i < AHEAD; ++i) {
+      const float* at = stg + (row0 + 8 * i) * PITCH + ch * 8;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 4);
+      float dh[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      store_gate_gradient<T>(g, m0 + row0 + 8 * i, c0 + ch * 8, dh, pre[i]);
     }
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(stg + row * PITCH + ch * 8), hi = *reinterpret_cast<const f32x4*>(stg + row * PITCH + ch * 8 + 4);
-    float dh[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    store_gate_gradient<T>(g, m0 + row, c0 + ch * 8, dh, pre[pass % AHEAD]);
   }
 }
 
