@@ -222,8 +222,10 @@ __global__ __launch_bounds__(kThreads) void norm_finish_kernel(const double* par
 }
 
 // A factor of one leaves every gradient as it is, so nothing more is read then; the first chunk is on its way while the partial sums are added up.
-// The chunks are taken from the last eight on, for what the norm read last is still in the last cache (168 M bf16 elements, norm and all: 151 us, from
-// the first on 165), and each on the XCD that read it for the norm, whose L2 may hold it (10 M: 12.7 us, on another XCD 19).
+// A table's chunks are taken from the last eight on, for what the norm read last is still in the last cache (168 M bf16 elements, norm and all: 151 us,
+// from the first on 165), and each on the XCD that read it for the norm, whose L2 may hold it (10 M: 12.7 us, on another XCD 19).  So it is with
+// one table, up to kTensors tensors.  Several are scaled from the first on; and where the norm's workgroups of a launch (1024 shared out to the tables, 64 at
+// least) are no multiple of eight, as with three tables, chunks behind a launch's first round were read on other XCDs.
 template <typename T>
 __device__ inline bool scale_first(const ScaleArgs& a, const Place& at, float& by, double* waves) {
   Chunk<T> c;

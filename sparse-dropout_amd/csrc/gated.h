@@ -4,14 +4,15 @@
 // projection at a time: 16-column tile 2 q of its output is g, tile 2 q + 1 is u of the hidden columns 16 q .. + 15.  Either tile of a pair is
 // in the same registers of the same lanes, so H needs nothing from another wave, and where nothing will be differentiated G and U never leave the
 // registers: 3 of the 4 bytes a passing gate would move.  gated_hidden, gated_up: which row of W_in column n of a tile is.
-//   8192 x 2048 to 8192 bf16: 415 us, 454 with G and U; the product alone, which writes both, 429, and a gate's pass 74 more
-//   4096 x 1024 to 4096 fp16:  66 us,  70;              67 and 16            1024 x 512 to 2048: 10.2, 12.7; 10.2 and 3.6
+//   8192 x 2048 to 8192 bf16: 408 us, 447 with G and U; the product alone, which writes both, 419 to 425, and a gate's pass 73 more (with the clock
+//   settled; 415 to 437 in a block, card by card)
+//   4096 x 1024 to 4096 fp16:  66 us,  69;              66 and 16            1024 x 512 to 2048: 10.8, 12.7; 10.8 and 3.6
 // Bound by the matrix cores and the loads into LDS as the ungated product is; at the largest the store of 2 or 6 bytes an element adds to that (360 us
 // without one).  Workgroups of the first round started up to 13 us apart, so that no two CUs' stores meet, take the same: it is not that they come together.
 //
 // Backward.  dH = (dY W_out) . keep is a product whose store reads g and u of its place and writes dg and du instead of dh.
-//   8192 x 8192 from 2048 bf16: 361 us, the product and a pass 239 and 120; half dropped 227, 166 and 121
-//   4096 x 4096 from 1024 fp16: 59 us, 40 and 25           1024 x 2048 from 512: 9.1, 7.3 and 4.7
+//   8192 x 8192 from 2048 bf16: 336 us, the product and a pass 233 and 120; half dropped 235, 163 and 121 (243 in a block)
+//   4096 x 4096 from 1024 fp16: 55 us, 37 and 26           1024 x 2048 from 512: 9.3, 7.3 and 4.9
 // Bound by the product and behind it by the 8 bytes read and written for each of its results: the gate saves dH's way to memory and back and a
 // launch.  (With nontemporal loads or stores, in either direction, a block's 372 us were 373 to 395, another's 1432 1421 to 1442.)
 #pragma once
@@ -20,7 +21,8 @@
 namespace sd {
 
 // act(g).  SILU: g / (1 + exp(-g)), one exponential and one reciprocal.  Within 2^-19 of itself where |g| < 16: what rounds g / ln 2, by up to 2^-20 there,
-// moves the exponential by 0.7 times that, the constant by |g| 2^-26, and each of the other steps by 2^-24 or 2^-23; beyond it grows with -g.  An exponential of 2^126 and more gives 0 for a value under 2^-119.  NaN stays NaN in every gate (ReLU's comparison is the one that it fails).
+// moves the exponential by 0.7 times that, the constant by |g| 2^-26, and each of the other steps by 2^-24 or 2^-23; beyond it grows with -g.  An exponential
+// of 2^126 and more gives 0 for a value under 2^-119.  NaN stays NaN in every gate (ReLU's comparison is the one that it fails).
 __device__ inline float gate_value(int act, float g) {
   if (act == SD_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
   if (act == SD_ACT_RELU) return g <= 0.f ? 0.f : g;

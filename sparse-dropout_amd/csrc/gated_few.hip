@@ -336,7 +336,8 @@ int sd_gated_mlp_few_taken(int64_t M, int64_t K, int64_t F, int64_t N) {
   if (M <= 16) return 1;  // (6 to 58 % less time on ten layers, 256 to 4096 wide, 1 to 16 rows)
   // Of 60 calls with 17 to 64 rows on those layers 12 are sent the slower way, one by 17 %, the others by up to 7: 2048 to 8192 and back 24 rows 29.4 us
   // against 31.0, 64 rows 41.3 and 33.5; 1024 to 4096 and back 15.2 and 17.2, 21.5 and 18.4.
-  // Rows that do not begin on 16 bytes are copied first on the other way: weights and activations at 3 TB/s, a launch each
+  // Rows that do not begin on 16 bytes are copied first on the other way: weights and activations at 3 TB/s, a launch each.  (By widths alone: that rows of
+  // whole widths lie at odd pitches, and are copied too, is not asked, and goes against this way.)
   const double copied = (K % 8 ? 4.0 + 8.0 * F * K / 3e6 : 0.0) + (F % 8 ? 4.0 + 4.0 * N * F / 3e6 : 0.0);
   return 1.05 * (plan_few(M, F, K, 2).us + plan_few(M, N, F, 1).us) <= gated_expected_us(M, F, K) + dense_expected_us(M, N, F) + copied ? 1 : 0;
 }

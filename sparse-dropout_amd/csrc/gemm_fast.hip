@@ -2300,9 +2300,10 @@ int launch_gated(const GemmArgs& g_, int dtype, hipStream_t stream) {
 
 // The shape of a gradient behind a gate.  Its store reads two and writes two results for every one of the product, so that what a tile takes beside its
 // steps (sdd_work's) is counted anew: us for a launch, steps at the ungated product's rate, and for a thousand kept 64 x 64 tiles, of those all that are there,
-// and with GELU.  Picked so 596 drawn gradients (256 to 16384 rows, 0 to 0.75 dropped, their operands cold) take 1.7 % longer than on the best shape, by
-// the product's own plan 5.6 %: 4096 x 4096 from 1024 with GELU 98.7 us on strips of two, 84.0 on the big shape; 2048 x 4096, half dropped, 50.0 on strips
-// of four, 38.7 on those of two.
+// and with GELU.  Picked so 656 drawn gradients (256 to 16384 rows, 0 to 0.75 dropped, their operands cold) take 1.4 % longer than on the best shape, one in
+// ten 5 % or more, by the product's own plan 5.6 % on average.  Where it is furthest off it expects two shapes to take the same: 4096 x 4096 from 1024 with
+// GELU goes to strips of two, 101 us (the big shape 78), 2048 x 4096 half dropped to strips of four, 48 (those of two 40).  A fit made again on these
+// gradients picks no better (1.5 %).
 struct GateCost {
   double start, step, kept, tile, gelu;
 };

@@ -45,7 +45,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     tensors laid out like their parameters or ``(codes, scales)`` pairs of uint8 tensors, the codes laid out like their parameters too or in one
     run.  ``step``: one int64 on the GPU, the number of steps so far, moved on by the call itself: a captured graph counts its replays.
     ``lr`` may be a float32 tensor on the GPU, which a captured graph reads at every replay, and so may ``grad_scale``, which gradients are
-    multiplied by as they are read (:func:`grad_norm` gives the one that clips).  One launch for each 56 tensors of a dtype.
+    multiplied by as they are read (:func:`grad_norm` gives the one that clips).  None of these lies in what is written.  One launch for each 56 tensors of a dtype.
     ``torch.jit.trace`` is refused."""
     beta1, beta2 = (float(b) for b in betas)
     firsts, first_scales = _split(exp_avgs, "exp_avgs")

@@ -35,6 +35,6 @@ def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, max_norm: f
 
 @refused_under_trace
 def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-    """Scales ``grads`` in place so that their norm is ``max_norm`` at most, and returns the norm they had.  They must fill their memory and share
-    none of it."""
+    """Scales ``grads`` (types as in :func:`grad_norm`, on one GPU) in place so that their norm is ``max_norm`` at most, and returns the norm they had.
+    They must fill their memory and share none of it."""
     return _loader.bridge().clip_grads(list(grads), float(max_norm), _norm_type(norm_type))

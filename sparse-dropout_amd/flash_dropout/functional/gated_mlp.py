@@ -9,7 +9,8 @@ GELU (erf form) or ReLU.  Sums and the gate are in 32 bits; G, U, H and dG, dU a
 whose operands they are.  G, U and H are kept for the backward; a forward that nothing is recorded of keeps none.
 H is computed before G and U are rounded, so it may be finite where they are beyond their type (65504 in fp16) and kept as infinities.
 Gradients then take the activation's limits: dG and dU are 0 behind a gate that is closed for all 32 bits, dG is dH U behind an open one;
-dU is infinite where act(G) is not held, and dG where U is not.
+dU is infinite where act(G) is not held, and dG where U is not.  (Where product and gate run apart, behind more than 131072 features, H is made
+from G and U as they are kept.)
 
 The reference has no gated block; arguments are those of the stack of layers (functional/blockwise_dropout_mlp_hip.py).
 """

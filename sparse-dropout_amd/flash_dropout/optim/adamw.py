@@ -22,7 +22,7 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_norm``: gradients are clipped to that joint norm (of all groups) as the step reads them; ``p.grad`` stays as it is, and ``grad_norm`` is
     the norm that the last step found, a float32 on the GPU (of a captured step: of its last replay).  It belongs to the optimizer, not to its
-    state, and may be changed between steps."""
+    state, and may be changed between steps.  The gradients must be on one GPU then; without it parameters may be on several."""
 
     max_norm: float | None = None
     grad_norm: torch.Tensor | None = None
